@@ -244,6 +244,44 @@ npu_status fused_llama_rmsnorm_swiglu(const npu_memref *h, const npu_memref *g2,
                                       const npu_memref *act, float eps,
                                       npu_stream stream);
 
+/* ---- serving a Llama decoder from a paged cache ---------------------------
+ * The layer's groups above take a whole prompt; the entry points below keep
+ * its keys and values from step to step, attend to them, and choose tokens.
+ * Beyond the conventions at the top:
+ *  - Row operands (Q, K, V, Qo, A) may have any row stride that keeps rows
+ *    16-byte aligned (slices of one [T, (H + 2 Hkv) Dh] buffer), and Qo may be
+ *    Q.  1-D operands and tables need contiguous rows, 4-byte aligned.
+ *  - A cache is bf16 [P, Hkv, page, Dh], Dh = 64 or 128, page a power of two
+ *    of at least 16, each page contiguous, pages at any stride; it may hold
+ *    more than 2^31 elements.
+ *  - The batch: B sequences (the rows of page_table i32 [B, max_pages]).
+ *    Sequence b has the new tokens q_start[b] .. q_start[b+1]-1 of the T rows
+ *    (q_start i32 [B+1], not decreasing; absent: T = B, token b is b's), and
+ *    kv_len[b] own keys, the new tokens' included, 0 allowed.  Own key j lies
+ *    in page page_table[b][j / page] at slot j % page.  All sequences share
+ *    prefix_len keys before their own (0: none).  New token i of n is own key
+ *    j = kv_len[b] - n + i, at position prefix_len + j.
+ *  - These arrays live on the device and are read by the kernels, so a
+ *    captured call serves every step.  Kernels check them: a page number
+ *    outside [0, P) stands for no page (nothing is stored there, its keys count
+ *    as masked), keys past the table do not exist, and rows of T outside every
+ *    sequence give zeros. */
+#define NPU_PAIRS_INTERLEAVED 0 /* rotated pairs (2t, 2t+1), as fused_llama_qkv_rope */
+#define NPU_PAIRS_HALVES 1      /* rotated pairs (t, t + width)                      */
+/* Qo = rotate(Q); K rotated and V as it is go to the new tokens' places in the
+ * cache.  Q, Qo bf16 [T, H Dh]; K, V bf16 [T, Hkv Dh]; cos_t, sin_t f32
+ * [positions, width], width a multiple of 8 up to Dh / 2: the first 2 width
+ * entries of a head are rotated, the others pass.  The tables cover every
+ * position: positions >= prefix_len + max_pages * page.  f32 arithmetic, one
+ * rounding.  A token outside its table (own key j < 0 or past it) is not
+ * stored and its Qo row is 0. */
+npu_status fused_llama_rope_append(const npu_memref *Q, const npu_memref *K, const npu_memref *V,
+                                   const npu_memref *cos_t, const npu_memref *sin_t,
+                                   const npu_memref *k_pages, const npu_memref *v_pages,
+                                   const npu_memref *page_table, const npu_memref *kv_len,
+                                   const npu_memref *q_start, const npu_memref *Qo,
+                                   int32_t prefix_len, int32_t pairs, npu_stream stream);
+
 /* ---- the reference's SRAM plan as the LDS layout --------------------------
  * The group `fill -> matmul -> generic(bias add, act)` run as the tile loop
  * that npu-temporal-tiling and npu-bufferize make of it (per output tile of

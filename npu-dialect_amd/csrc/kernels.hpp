@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "serve_batch.hpp"
+
 namespace npu {
 
 struct MatmulArgs {
@@ -93,5 +95,16 @@ struct LlamaGemmArgs {
 hipError_t launch_llama_gemm(const LlamaGemmArgs &a, int pro, int epi, hipStream_t s);
 hipError_t launch_llama_attention(const uint16_t *Q, const uint16_t *K, const uint16_t *V,
                                   uint16_t *O, int S, int H, int dh, float scale, hipStream_t s);
+
+// Serving from a paged cache (serve_batch.hpp: the batch).
+struct RopeAppendArgs {
+  const uint16_t *Q, *K, *V;
+  const float *cos_t, *sin_t;
+  uint16_t *k_pages, *v_pages, *Qo;
+  long long q_stride, k_stride, v_stride, o_stride, kpage_stride, vpage_stride;  // elements
+  int H, Hkv, dh, width, pairs;
+  ServeBatch b;
+};
+hipError_t launch_llama_rope_append(const RopeAppendArgs &a, hipStream_t s);
 
 }  // namespace npu

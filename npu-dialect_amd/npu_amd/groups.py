@@ -204,6 +204,36 @@ def fused_llama_rmsnorm_swiglu(h, g2, wg, wu, act, eps=1e-5, stream=None):
     return act
 
 
+PAIRS = {"interleaved": 0, "halves": 1}
+
+
+def _device_ref(name, t):
+    """Descriptor of a serving operand: a tensor on the GPU (a host pointer
+    would fault in the kernel)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a tensor on the GPU, got one on {t.device}")
+    return from_tensor(t)
+
+
+def _device_refs(**ts):
+    return [absent() if t is None else _device_ref(n, t) for n, t in ts.items()]
+
+
+def fused_llama_rope_append(Q, K, V, cos_t, sin_t, k_pages, v_pages, page_table, kv_len, Qo,
+                            q_start=None, prefix_len=0, pairs="interleaved", stream=None):
+    """Qo = rope(Q); rope(K) and V stored at the new tokens' places of the
+    paged cache k_pages, v_pages [P, Hkv, page, Dh]; bf16.  Own key j of
+    sequence b lies in page page_table[b, j // page]; kv_len counts the new
+    tokens; q_start [B + 1] are their first rows (None: one token each).
+    Positions count the shared prefix: prefix_len + j."""
+    ms = _device_refs(Q=Q, K=K, V=V, cos_t=cos_t, sin_t=sin_t, k_pages=k_pages, v_pages=v_pages,
+                      page_table=page_table, kv_len=kv_len, q_start=q_start, Qo=Qo)
+    st = _lib.lib().fused_llama_rope_append(*[ref(m) for m in ms], int(prefix_len), PAIRS[pairs],
+                                            _stream(stream))
+    _check(st, "fused_llama_rope_append")
+    return Qo, k_pages, v_pages
+
+
 class Empty:
     """A tensor.empty argument of an outlined group: a shape and element type,
     and optionally the tensor that holds it (None: no data; the group never
