@@ -282,6 +282,28 @@ npu_status fused_llama_rope_append(const npu_memref *Q, const npu_memref *K, con
                                    const npu_memref *q_start, const npu_memref *Qo,
                                    int32_t prefix_len, int32_t pairs, npu_stream stream);
 
+/* A = softmax over the keys a token sees of Q K^T * scale, times V, per query
+ * head; query head h uses key head h / (H / Hkv).  New token i of n sees the
+ * prefix's keys and own keys j <= kv_len[b] - n + i; a token that sees none
+ * gives 0.  What masked places of the cache hold, NaN and Inf too, does not
+ * count, except that a value of a later new token of the same sequence must be
+ * finite.  Q, A bf16 [T, H Dh]; prefix_table i32 [>= ceil(prefix_len / page)],
+ * absent iff prefix_len is 0: key j of the prefix lies in page
+ * prefix_table[j / page], and is read once for all sequences where each has
+ * few rows.  f32 sums; the probabilities are rounded to bf16.
+ * workspace f32 [n], n >= npu_paged_attention_workspace: scratch that only
+ * this call uses while it runs; its contents need not be kept. */
+npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_pages,
+                                       const npu_memref *v_pages, const npu_memref *page_table,
+                                       const npu_memref *kv_len, const npu_memref *q_start,
+                                       const npu_memref *prefix_table, const npu_memref *A,
+                                       const npu_memref *workspace, int32_t prefix_len,
+                                       float scale, npu_stream stream);
+/* f32 elements of the workspace for T rows of B sequences on the current
+ * device; -1: not a call that the entry point takes. */
+int64_t npu_paged_attention_workspace(int64_t T, int64_t B, int32_t n_heads, int32_t n_kv_heads,
+                                      int32_t head_dim, int32_t prefix_len);
+
 /* ---- the reference's SRAM plan as the LDS layout --------------------------
  * The group `fill -> matmul -> generic(bias add, act)` run as the tile loop
  * that npu-temporal-tiling and npu-bufferize make of it (per output tile of

@@ -106,5 +106,18 @@ struct RopeAppendArgs {
   ServeBatch b;
 };
 hipError_t launch_llama_rope_append(const RopeAppendArgs &a, hipStream_t s);
+struct PagedAttentionArgs {
+  const uint16_t *Q, *k_pages, *v_pages;
+  const int *prefix_table;  // pages of the shared prefix (null: none)
+  uint16_t *out;
+  void *workspace;
+  long long q_stride, o_stride, kpage_stride, vpage_stride;  // elements
+  int H, Hkv, dh;
+  float scale;
+  ServeBatch b;
+};
+// Bytes of the workspace a call needs; of the batch T, B, prefix_len are used.
+size_t paged_attention_workspace(const ServeBatch &b, int H, int Hkv, int dh);
+hipError_t launch_llama_paged_attention(const PagedAttentionArgs &a, hipStream_t s);
 
 }  // namespace npu

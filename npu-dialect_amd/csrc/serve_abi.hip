@@ -140,6 +140,7 @@ npu_status check_batch(const npu_memref *k_pages, const npu_memref *v_pages, con
   const void *pt, *kl, *qs = nullptr;
   NPU_TRY(check_rows(page_table, "page_table", NPU_I32, 4, &pt, &b->table_stride));
   const long long B = page_table->sizes[0];
+  if (B > 1 << 24) return fail(NPU_ERR_UNSUPPORTED, "%lld sequences, at most 2^24", B);
   NPU_TRY(check_vec(kv_len, "kv_len", NPU_I32, B, &kl));
   if (!absent(q_start)) {
     NPU_TRY(check_vec(q_start, "q_start", NPU_I32, B + 1, &qs));
@@ -220,6 +221,61 @@ npu_status fused_llama_rope_append(const npu_memref *Q, const npu_memref *K, con
   a.Hkv = c.Hkv; a.dh = c.dh; a.width = (int)width; a.pairs = pairs;
   return launched("fused_llama_rope_append launch",
                   [&] { return npu::launch_llama_rope_append(a, static_cast<hipStream_t>(stream)); });
+}
+
+int64_t npu_paged_attention_workspace(int64_t T, int64_t B, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                      int32_t prefix_len) {
+  if (T <= 0 || B <= 0 || T > kMaxInt || B > 1 << 24 || n_heads <= 0 || n_heads > 1024 || n_kv_heads <= 0 ||
+      n_heads % n_kv_heads != 0 || (head_dim != 64 && head_dim != 128) || prefix_len < 0 || T * n_heads > kMaxInt)
+    return -1;
+  npu::ServeBatch b{};
+  b.T = (int)T;
+  b.B = (int)B;
+  b.prefix_len = prefix_len;
+  return (int64_t)(npu::paged_attention_workspace(b, n_heads, n_kv_heads, head_dim) / sizeof(float));
+}
+
+npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_pages, const npu_memref *v_pages,
+                                       const npu_memref *page_table, const npu_memref *kv_len,
+                                       const npu_memref *q_start, const npu_memref *prefix_table, const npu_memref *A,
+                                       const npu_memref *workspace, int32_t prefix_len, float scale,
+                                       npu_stream stream) {
+  npu::plans_reset();
+  npu::PagedAttentionArgs a{};
+  Cache c;
+  const void *pq, *po, *pp = nullptr, *pw;
+  NPU_TRY(check_rows(Q, "Q", NPU_BF16, 16, &pq, &a.q_stride));
+  const long long T = Q->sizes[0];
+  NPU_TRY(check_batch(k_pages, v_pages, page_table, kv_len, q_start, T, prefix_len, &c, &a.b));
+  NPU_TRY(check_heads("Q", Q->sizes[1], c, &a.H));
+  NPU_TRY(check_rows(A, "A", NPU_BF16, 16, &po, &a.o_stride));
+  NPU_TRY(expect_cols(A, "A", T, Q->sizes[1]));
+  if (T * a.H > kMaxInt) return fail(NPU_ERR_UNSUPPORTED, "T * H = %lld is 2^31 or more", T * a.H);
+  if (prefix_len > 0) {
+    if (absent(prefix_table)) return fail(NPU_ERR_INVALID_ARG, "prefix_table: absent, prefix_len is %d", prefix_len);
+    NPU_TRY(check_vec(prefix_table, "prefix_table", NPU_I32, -1, &pp));
+    const long long page = k_pages->sizes[2], need = (prefix_len + page - 1) / page;
+    if (prefix_table->sizes[0] < need)
+      return fail(NPU_ERR_INVALID_ARG, "prefix_table: %lld pages, the prefix needs %lld",
+                  (long long)prefix_table->sizes[0], need);
+  } else if (!absent(prefix_table)) {
+    return fail(NPU_ERR_INVALID_ARG, "prefix_table: given, prefix_len is 0");
+  }
+  if (!(scale > 0.0f) || scale > 3e38f) return fail(NPU_ERR_INVALID_ARG, "scale must be positive and finite");
+  NPU_TRY(check_base(workspace, "workspace", 1, NPU_F32, 16, &pw));
+  if (workspace->sizes[0] > 1 && workspace->strides[0] != 1)
+    return fail(NPU_ERR_UNSUPPORTED, "workspace: must be contiguous");
+  const long long need = npu_paged_attention_workspace(T, a.b.B, a.H, c.Hkv, c.dh, prefix_len);
+  if (workspace->sizes[0] < need)
+    return fail(NPU_ERR_INVALID_ARG, "workspace: %lld elements, %lld needed", (long long)workspace->sizes[0], need);
+  a.Q = u16(pq); a.k_pages = u16(c.k); a.v_pages = u16(c.v);
+  a.prefix_table = static_cast<const int *>(pp);
+  a.out = u16w(po);
+  a.workspace = const_cast<void *>(pw);
+  a.kpage_stride = c.k_stride; a.vpage_stride = c.v_stride;
+  a.Hkv = c.Hkv; a.dh = c.dh; a.scale = scale;
+  return launched("fused_llama_paged_attention launch",
+                  [&] { return npu::launch_llama_paged_attention(a, static_cast<hipStream_t>(stream)); });
 }
 
 }  // extern "C"

@@ -76,7 +76,9 @@ NPU_HD Place place_of_token(const ServeBatch &b, int t) {
 // least, so that rows without keys are written too.  Units are numbered by
 // sequence, tile, key head, block; workgroup w of W takes the units
 // [U w / W, U (w + 1) / W): equal shares whatever the lengths, a group cut at
-// most at the workgroups' borders.
+// most at the workgroups' borders.  W is at most U (split_workgroups), so that
+// every one of them has work and a cut group's parts are those of consecutive
+// workgroups.
 struct AttnSplit {
   ServeBatch b;
   int G, Hkv;
@@ -109,6 +111,7 @@ NPU_HD long long seq_units(const AttnSplit &a, int seq) {
   for (int t = 0; t < tiles; ++t) sum += tile_blocks(a, seq, n, t);
   return sum * a.Hkv;
 }
+NPU_HD int split_workgroups(long long U, int launched) { return U < launched ? (int)U : launched; }
 NPU_HD long long first_unit(long long U, int W, int w) { return U * w / W; }
 NPU_HD int unit_owner(long long U, int W, long long u) { return (int)(((u + 1) * W - 1) / U); }
 

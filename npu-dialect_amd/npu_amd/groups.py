@@ -234,6 +234,31 @@ def fused_llama_rope_append(Q, K, V, cos_t, sin_t, k_pages, v_pages, page_table,
     return Qo, k_pages, v_pages
 
 
+def paged_attention_workspace(Q, k_pages, page_table, prefix_len=0):
+    """A workspace for fused_llama_paged_attention calls of these shapes, to be
+    kept beside the cache; one for each call that may run at the same time."""
+    import torch
+    _, hkv, _, dh = k_pages.shape
+    n = _lib.lib().npu_paged_attention_workspace(Q.shape[0], page_table.shape[0], Q.shape[1] // dh,
+                                                 hkv, dh, int(prefix_len))
+    if n < 0:
+        raise ValueError(f"no paged attention of rows {tuple(Q.shape)} over pages {tuple(k_pages.shape)}")
+    return torch.empty(n, dtype=torch.float32, device=Q.device)
+
+
+def fused_llama_paged_attention(Q, k_pages, v_pages, page_table, kv_len, A, scale, workspace,
+                                q_start=None, prefix_table=None, prefix_len=0, stream=None):
+    """A = softmax(Q K^T * scale) V over the paged cache; bf16.  A token sees
+    the shared prefix's prefix_len keys (pages prefix_table) and its sequence's
+    own keys up to its own; the other arrays as in fused_llama_rope_append."""
+    ms = _device_refs(Q=Q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, kv_len=kv_len,
+                      q_start=q_start, prefix_table=prefix_table, A=A, workspace=workspace)
+    st = _lib.lib().fused_llama_paged_attention(*[ref(m) for m in ms], int(prefix_len), float(scale),
+                                                _stream(stream))
+    _check(st, "fused_llama_paged_attention")
+    return A
+
+
 class Empty:
     """A tensor.empty argument of an outlined group: a shape and element type,
     and optionally the tensor that holds it (None: no data; the group never

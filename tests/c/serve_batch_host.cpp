@@ -36,19 +36,20 @@ int serve_visible(const HostBatch *h, int seq, int i) {
   return visible_keys(a, seq, seq_span(b, seq).n, i);
 }
 
-// The segments of all W workgroups in order, eight ints each: workgroup, seq,
+// The segments of all workgroups of a launch in order, eight ints each: workgroup, seq,
 // tile, head, first block, one past its last, blocks of the group, first token
 // of the sequence.  Returns their number, or -1 if a cursor found by seeking
 // differs from the one reached by walking, or the owners disagree.
-long long serve_segments(const HostBatch *h, int G, int Hkv, int rows, int keys, int pre_blocks, int stacked, int W,
-                         int *out, long long most) {
+long long serve_segments(const HostBatch *h, int G, int Hkv, int rows, int keys, int pre_blocks, int stacked,
+                         int launched, int *out, long long most) {
   const AttnSplit a{batch(h), G, Hkv, rows, keys, pre_blocks, stacked};
   long long U = 0, n = 0;
   for (int s = 0; s < split_seqs(a); ++s) U += seq_units(a, s);
-  for (int w = 0; w < W && U > 0; ++w) {
+  const int W = split_workgroups(U, launched);
+  for (int w = 0; w < W; ++w) {
     long long u = first_unit(U, W, w);
     const long long end = first_unit(U, W, w + 1);
-    if (u >= end) continue;
+    if (u >= end) return -3;
     UnitCursor c = seek_unit(a, 0, 0, u);
     while (u < end) {
       const long long left = end - u;

@@ -111,8 +111,9 @@ def test_every_block_of_every_tile_is_one_workgroups(host, news, lens, G, Hkv, r
         seen[(s, tile, h)] = b1
     assert seen == want
     # equal shares, at most one cut at each end of a workgroup
-    per = np.bincount(segs[:, 0], (segs[:, 5] - segs[:, 4]).astype(float), minlength=W)
+    per = np.bincount(segs[:, 0], (segs[:, 5] - segs[:, 4]).astype(float), minlength=segs[:, 0].max() + 1)
     assert per.max() - per.min() <= 1
+    assert (np.unique(segs[:, 0]) == np.arange(min(W, int(per.sum())))).all()
     for w in np.unique(segs[:, 0]):
         mine = segs[segs[:, 0] == w]
         assert (mine[1:, 4] == 0).all() and (mine[:-1, 5] == mine[:-1, 6]).all()
@@ -171,6 +172,38 @@ APPEND_REFUSALS = [
     (dict(lens=_mr([3], I32)), 1, "kv_len: size 3"), (dict(start=_mr([2], I32)), 1, "q_start: size 2"),
     (dict(lens=_mr([2], I32, strides=[2])), 2, "contiguous"), (dict(lens=_mr([2], I32, ptr=0x10002)), 2, "4-byte"),
 ]
+
+
+def _attend(prefix=0, scale=0.1, **over):
+    a = {"Q": _mr([2, 512], BF16), "kp": _mr([5, 2, 16, 128], BF16), "vp": _mr([5, 2, 16, 128], BF16),
+         "table": _mr([2, 4], I32), "lens": _mr([2], I32), "start": None, "pre": None, "A": _mr([2, 512], BF16),
+         "ws": _mr([1 << 27])}
+    a.update(over)
+    return _call("fused_llama_paged_attention", a.values(), prefix, C.c_float(scale))
+
+
+ATTEND_REFUSALS = [
+    (dict(A=_mr([2, 256], BF16)), 1, "A: [2,256]"), (dict(A=_mr([2, 512])), 1, "element type"),
+    (dict(Q=_mr([2, 640], BF16)), 1, "multiple of 2"), (dict(prefix=17), 1, "prefix_table: absent"),
+    (dict(prefix=17, pre=_mr([1], I32)), 1, "needs 2"), (dict(pre=_mr([1], I32)), 1, "prefix_len is 0"),
+    (dict(scale=0.0), 1, "scale"), (dict(scale=float("nan")), 1, "scale"), (dict(scale=float("inf")), 1, "scale"),
+    (dict(ws=_mr([64])), 1, "workspace: 64"), (dict(ws=None), 1, "workspace"), (dict(ws=_mr([1 << 27], ptr=0x10008)), 2, "16-byte"),
+    (dict(vp=_mr([4, 2, 16, 128], BF16)), 1, "v_pages"), (dict(table=_mr([2, 4], I32, strides=[3, 1])), 2, "overlap"),
+]
+
+
+@pytest.mark.parametrize("over,status,text", ATTEND_REFUSALS)
+def test_attention_refuses(over, status, text):
+    over = dict(over)
+    assert _attend(over.pop("prefix", 0), over.pop("scale", 0.1), **over) == status and text in _err(), _err()
+
+
+def test_attention_workspace_sizes():
+    f = npu_amd.lib().npu_paged_attention_workspace
+    assert f(2, 2, 4, 2, 128, 0) > 0 and f(64, 64, 32, 8, 128, 6000) > 0
+    for bad in ((0, 1, 4, 2, 128, 0), (1, 1, 4, 3, 128, 0), (1, 1, 4, 2, 96, 0), (1, 1, 4, 2, 64, -1), (1, 0, 4, 2, 64, 0),
+                (2 ** 30, 1, 4, 4, 64, 0), (1, 1, 2048, 1, 64, 0)):
+        assert f(*bad) == -1, bad
 
 
 @pytest.mark.parametrize("over,status,text", APPEND_REFUSALS)
