@@ -304,6 +304,34 @@ npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_
 int64_t npu_paged_attention_workspace(int64_t T, int64_t B, int32_t n_heads, int32_t n_kv_heads,
                                       int32_t head_dim, int32_t prefix_len);
 
+/* The next token of each row of logits, from a given random number u.
+ * Entries are ordered by logit, descending, then by index; with weights
+ * w = exp((logit - max) / temperature):
+ *   top_k > 0: the first top_k entries stay;
+ *   top_p < 1: of those, the ones before which less than top_p of their mass
+ *              lies (top_p <= 0: the first);
+ *   min_p > 0: of those, the ones with w >= min_p, the first in any case;
+ *   tokens[b] = the first one whose running mass exceeds u times the mass of
+ *   what stayed (u in [0, 1); beyond, the first or the last), probs[b] its
+ *   share of that mass.
+ * temperature <= 0 (or NaN): the first entry, probability 1.  NaN and -Inf are
+ * no candidates; if there is +Inf, only +Inf is.  A row without candidates
+ * gives -1 and probability 0.
+ *   logits f32 or bf16 [B, V], V <= 2^20, rows at any stride; u, temperature,
+ *   top_p, min_p f32 [B], top_k i32 [B] (each but u may be absent: off,
+ *   temperature 1); tokens i32 [B]; probs f32 [B], may be absent; workspace
+ *   f32 [n], n >= npu_sample_workspace.
+ * Weights are f64 rounded to 2^-42, their sums exact: the same input gives the
+ * same token every time. */
+npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u,
+                               const npu_memref *temperature, const npu_memref *top_k,
+                               const npu_memref *top_p, const npu_memref *min_p,
+                               const npu_memref *tokens, const npu_memref *probs,
+                               const npu_memref *workspace, npu_stream stream);
+/* f32 elements of the workspace for B rows of V logits; -1: not a call that
+ * the entry point takes. */
+int64_t npu_sample_workspace(int64_t B, int64_t V);
+
 /* ---- the reference's SRAM plan as the LDS layout --------------------------
  * The group `fill -> matmul -> generic(bias add, act)` run as the tile loop
  * that npu-temporal-tiling and npu-bufferize make of it (per output tile of

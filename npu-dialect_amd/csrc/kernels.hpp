@@ -119,5 +119,18 @@ struct PagedAttentionArgs {
 // Bytes of the workspace a call needs; of the batch T, B, prefix_len are used.
 size_t paged_attention_workspace(const ServeBatch &b, int H, int Hkv, int dh);
 hipError_t launch_llama_paged_attention(const PagedAttentionArgs &a, hipStream_t s);
+struct SampleArgs {
+  const void *logits;  // f32, or bf16 bits
+  bool bf16;
+  long long row_stride;  // elements
+  int B, V;
+  const float *temperature, *top_p, *min_p, *u;  // all but u may be null
+  const int *top_k;                              // may be null
+  int *tokens;
+  float *probs;  // may be null
+  void *workspace;
+};
+size_t sample_workspace(int B, int V);  // bytes
+hipError_t launch_sample_tokens(const SampleArgs &a, hipStream_t s);
 
 }  // namespace npu

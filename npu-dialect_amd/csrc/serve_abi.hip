@@ -99,6 +99,16 @@ npu_status expect_cols(const npu_memref *m, const char *name, long long rows, lo
   return NPU_OK;
 }
 
+npu_status check_workspace(const npu_memref *m, long long need, void **ptr) {
+  const void *p;
+  NPU_TRY(check_base(m, "workspace", 1, NPU_F32, 16, &p));
+  if (m->sizes[0] > 1 && m->strides[0] != 1) return fail(NPU_ERR_UNSUPPORTED, "workspace: must be contiguous");
+  if (m->sizes[0] < need)
+    return fail(NPU_ERR_INVALID_ARG, "workspace: %lld elements, %lld needed", (long long)m->sizes[0], need);
+  *ptr = const_cast<void *>(p);
+  return NPU_OK;
+}
+
 // One half of the cache: bf16 [P, Hkv, page, Dh], each page contiguous.
 npu_status check_pages(const npu_memref *m, const char *name, const void **ptr, long long *stride) {
   NPU_TRY(check_base(m, name, 4, NPU_BF16, 16, ptr));
@@ -243,7 +253,7 @@ npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_
   npu::plans_reset();
   npu::PagedAttentionArgs a{};
   Cache c;
-  const void *pq, *po, *pp = nullptr, *pw;
+  const void *pq, *po, *pp = nullptr;
   NPU_TRY(check_rows(Q, "Q", NPU_BF16, 16, &pq, &a.q_stride));
   const long long T = Q->sizes[0];
   NPU_TRY(check_batch(k_pages, v_pages, page_table, kv_len, q_start, T, prefix_len, &c, &a.b));
@@ -262,20 +272,54 @@ npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_
     return fail(NPU_ERR_INVALID_ARG, "prefix_table: given, prefix_len is 0");
   }
   if (!(scale > 0.0f) || scale > 3e38f) return fail(NPU_ERR_INVALID_ARG, "scale must be positive and finite");
-  NPU_TRY(check_base(workspace, "workspace", 1, NPU_F32, 16, &pw));
-  if (workspace->sizes[0] > 1 && workspace->strides[0] != 1)
-    return fail(NPU_ERR_UNSUPPORTED, "workspace: must be contiguous");
-  const long long need = npu_paged_attention_workspace(T, a.b.B, a.H, c.Hkv, c.dh, prefix_len);
-  if (workspace->sizes[0] < need)
-    return fail(NPU_ERR_INVALID_ARG, "workspace: %lld elements, %lld needed", (long long)workspace->sizes[0], need);
+  NPU_TRY(check_workspace(workspace, npu_paged_attention_workspace(T, a.b.B, a.H, c.Hkv, c.dh, prefix_len),
+                          &a.workspace));
   a.Q = u16(pq); a.k_pages = u16(c.k); a.v_pages = u16(c.v);
   a.prefix_table = static_cast<const int *>(pp);
   a.out = u16w(po);
-  a.workspace = const_cast<void *>(pw);
   a.kpage_stride = c.k_stride; a.vpage_stride = c.v_stride;
   a.Hkv = c.Hkv; a.dh = c.dh; a.scale = scale;
   return launched("fused_llama_paged_attention launch",
                   [&] { return npu::launch_llama_paged_attention(a, static_cast<hipStream_t>(stream)); });
+}
+
+int64_t npu_sample_workspace(int64_t B, int64_t V) {
+  if (B <= 0 || B > kMaxInt || V <= 0 || V > 1 << 20) return -1;
+  return (int64_t)((npu::sample_workspace((int)B, (int)V) + sizeof(float) - 1) / sizeof(float));
+}
+
+npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u, const npu_memref *temperature,
+                               const npu_memref *top_k, const npu_memref *top_p, const npu_memref *min_p,
+                               const npu_memref *tokens, const npu_memref *probs, const npu_memref *workspace,
+                               npu_stream stream) {
+  npu::plans_reset();
+  npu::SampleArgs a{};
+  if (!logits) return fail(NPU_ERR_INVALID_ARG, "logits: null descriptor");
+  a.bf16 = logits->dtype == NPU_BF16;
+  const void *pl, *p[7] = {};
+  NPU_TRY(check_rows(logits, "logits", a.bf16 ? NPU_BF16 : NPU_F32, a.bf16 ? 2 : 4, &pl, &a.row_stride));
+  const long long B = logits->sizes[0], V = logits->sizes[1];
+  if (V > 1 << 20) return fail(NPU_ERR_UNSUPPORTED, "logits: %lld columns, at most 2^20", V);
+  NPU_TRY(check_vec(u, "u", NPU_F32, B, &p[0]));
+  if (!absent(temperature)) NPU_TRY(check_vec(temperature, "temperature", NPU_F32, B, &p[1]));
+  if (!absent(top_k)) NPU_TRY(check_vec(top_k, "top_k", NPU_I32, B, &p[2]));
+  if (!absent(top_p)) NPU_TRY(check_vec(top_p, "top_p", NPU_F32, B, &p[3]));
+  if (!absent(min_p)) NPU_TRY(check_vec(min_p, "min_p", NPU_F32, B, &p[4]));
+  NPU_TRY(check_vec(tokens, "tokens", NPU_I32, B, &p[5]));
+  if (!absent(probs)) NPU_TRY(check_vec(probs, "probs", NPU_F32, B, &p[6]));
+  NPU_TRY(check_workspace(workspace, npu_sample_workspace(B, V), &a.workspace));
+  a.logits = pl;
+  a.B = (int)B;
+  a.V = (int)V;
+  a.u = static_cast<const float *>(p[0]);
+  a.temperature = static_cast<const float *>(p[1]);
+  a.top_k = static_cast<const int *>(p[2]);
+  a.top_p = static_cast<const float *>(p[3]);
+  a.min_p = static_cast<const float *>(p[4]);
+  a.tokens = const_cast<int *>(static_cast<const int *>(p[5]));
+  a.probs = const_cast<float *>(static_cast<const float *>(p[6]));
+  return launched("fused_sample_tokens launch",
+                  [&] { return npu::launch_sample_tokens(a, static_cast<hipStream_t>(stream)); });
 }
 
 }  // extern "C"

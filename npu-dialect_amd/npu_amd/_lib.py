@@ -147,6 +147,8 @@ SIGNATURES = {
     "fused_llama_rope_append": (_I32, [_MR] * 11 + [_I32, _I32, _P]),
     "fused_llama_paged_attention": (_I32, [_MR] * 9 + [_I32, C.c_float, _P]),
     "npu_paged_attention_workspace": (_I64, [_I64, _I64, _I32, _I32, _I32, _I32]),
+    "fused_sample_tokens": (_I32, [_MR] * 9 + [_P]),
+    "npu_sample_workspace": (_I64, [_I64, _I64]),
     "npu_group_launch": (_I32, [C.c_char_p, C.POINTER(NpuGroupAttrs), _ARG, _I32, _ARG, _I32,
                                 _P]),
     "npu_last_launch_plans": (_I32, [C.POINTER(NpuLaunchPlan), _I32]),

@@ -259,6 +259,28 @@ def fused_llama_paged_attention(Q, k_pages, v_pages, page_table, kv_len, A, scal
     return A
 
 
+def sample_workspace(logits):
+    """A workspace for fused_sample_tokens calls on logits of this shape; one
+    for each call that may run at the same time."""
+    import torch
+    n = _lib.lib().npu_sample_workspace(*logits.shape)
+    if n < 0:
+        raise ValueError(f"no sampling from logits of shape {tuple(logits.shape)}")
+    return torch.empty(n, dtype=torch.float32, device=logits.device)
+
+
+def fused_sample_tokens(logits, u, tokens, workspace, temperature=None, top_k=None, top_p=None,
+                        min_p=None, probs=None, stream=None):
+    """tokens[b] = a token of row b of logits (f32 or bf16), drawn with the
+    random number u[b] in [0, 1) from what temperature, top-k, top-p and min-p
+    (one value a row, None: off) leave; probs[b] its probability there."""
+    ms = _device_refs(logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p,
+                      min_p=min_p, tokens=tokens, probs=probs, workspace=workspace)
+    st = _lib.lib().fused_sample_tokens(*[ref(m) for m in ms], _stream(stream))
+    _check(st, "fused_sample_tokens")
+    return tokens
+
+
 class Empty:
     """A tensor.empty argument of an outlined group: a shape and element type,
     and optionally the tensor that holds it (None: no data; the group never

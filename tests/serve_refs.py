@@ -126,3 +126,28 @@ def attend64(bt, Q, scale):
             clean = torch.nan_to_num(vs[h // G], nan=0.0, posinf=0.0, neginf=0.0)
             out[rows, c], mag[rows, c] = p @ clean, p @ clean.abs()
     return out, mag, seen
+
+
+def sample64(x, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """(token, probability) of one row, numpy f64: the operator's definition."""
+    x = np.asarray(x, np.float64)
+    cand = np.isposinf(x) if np.isposinf(x).any() else np.isfinite(x)
+    idx = np.nonzero(cand)[0]
+    if not idx.size:
+        return -1, 0.0
+    order = idx[np.argsort(-x[idx], kind="stable")]
+    t = 1.0 if temperature is None else float(temperature)
+    if not t > 0:
+        return int(order[0]), 1.0
+    top = x[order[0]]
+    w = np.ones(order.size) if np.isposinf(top) else np.exp((x[order] - top) / t)
+    n = order.size
+    if top_k is not None and top_k > 0:
+        n = min(n, int(top_k))
+    cum = np.concatenate([[0.0], np.cumsum(w)])
+    if top_p is not None and top_p < 1:
+        n = min(n, max(1, int((cum[:n] < float(top_p) * cum[n]).sum())))
+    if min_p is not None and min_p > 0:
+        n = min(n, max(1, int((w >= float(min_p)).sum())))
+    pick = min(n - 1, int((cum[1:n + 1] <= float(u) * cum[n]).sum()))
+    return int(order[pick]), float(w[pick] / cum[n])

@@ -298,3 +298,165 @@ def test_attention_captured(cuda, prefix):
         bt.table = bt.page_table.cpu().numpy()
         exact, mag, seen = R.attend64(bt, Q, 0.125)
         assert ((A.cpu().double() - exact).abs() <= _attend_bound(bt, Q, 0.125, exact, mag, seen)).all(), step
+
+
+# ---- sampling ------------------------------------------------------------------------
+def _sample(x, u, temperature=None, top_k=None, top_p=None, min_p=None, probs=True, stream=None):
+    from npu_amd import groups
+    B = x.shape[0]
+    f = lambda v: None if v is None else torch.tensor(v, dtype=torch.float32, device="cuda")
+    i = None if top_k is None else torch.tensor(top_k, dtype=torch.int32, device="cuda")
+    tokens = torch.full((B,), -7, dtype=torch.int32, device="cuda")
+    pr = torch.full((B,), -7.0, device="cuda") if probs else None
+    ws = groups.sample_workspace(x)
+    ws.fill_(float("nan"))
+    if stream is not None:
+        stream.wait_stream(torch.cuda.current_stream())
+    groups.fused_sample_tokens(x, f(u), tokens, ws, temperature=f(temperature), top_k=i, top_p=f(top_p),
+                               min_p=f(min_p), probs=pr, stream=stream)
+    torch.cuda.synchronize()
+    return tokens.cpu().numpy(), None if pr is None else pr.cpu().double().numpy()
+
+
+def _check_sample(x, u, **kw):
+    """Tokens equal; probabilities within f32's rounding (2^-24) and the
+    weights' (2^-43 of the largest weight each, above and below the line)."""
+    u = np.asarray(u, np.float32)
+    kw = {n: None if v is None else np.asarray(v, np.int32 if n == "top_k" else np.float32) for n, v in kw.items()}
+    tokens, probs = _sample(x, u, **kw)
+    host = x.double().cpu().numpy()
+    for b in range(x.shape[0]):
+        row = {n: None if v is None else v[b] for n, v in kw.items()}
+        tok, pr = R.sample64(host[b], u[b], **row)
+        assert tokens[b] == tok, (b, tokens[b], tok, row)
+        assert abs(probs[b] - pr) <= 2.0 ** -24 * pr + (x.shape[1] + 1) * 2.0 ** -42, (b, probs[b], pr)
+
+
+def _logits(B, V, seed, spread=2.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((B, V), generator=g) * spread
+    x.scatter_add_(1, torch.randint(0, V, (B, 6), generator=g), torch.rand((B, 6), generator=g) * 8)
+    return x.to(dtype).cuda()
+
+
+SETTINGS = {
+    "none": lambda r, B: {},
+    "temperature": lambda r, B: {"temperature": r.uniform(0.1, 3, B)},
+    "top_k": lambda r, B: {"top_k": r.integers(1, 200, B)},
+    "top_p": lambda r, B: {"top_p": r.uniform(0.05, 1, B)},
+    "min_p": lambda r, B: {"min_p": r.uniform(0.001, 0.9, B)},
+    "all": lambda r, B: {"temperature": r.uniform(0.1, 3, B), "top_k": r.integers(-1, 3000, B),
+                         "top_p": r.uniform(0.3, 1.2, B), "min_p": r.uniform(-0.1, 0.1, B)},
+}
+
+
+@pytest.mark.parametrize("setting", SETTINGS)
+@pytest.mark.parametrize("B,V,dtype", [(3, 1, "f32"), (4, 2, "bf16"), (5, 7, "f32"), (9, 100, "bf16"), (6, 1023, "f32"),
+                                       (7, 2049, "f32"), (5, 32000, "f32"), (4, 50257, "bf16"), (3, 128000, "f32"),
+                                       (2, 300001, "bf16"), (300, 517, "f32")])
+def test_sample(cuda, B, V, dtype, setting):
+    r = np.random.default_rng(B * V)
+    x = _logits(B, V, B + V, dtype=torch.bfloat16 if dtype == "bf16" else torch.float32)
+    _check_sample(x, r.random(B, np.float32), **SETTINGS[setting](r, B))
+
+
+def test_sample_flat_and_steep(cuda):
+    """Spreads from almost equal logits to one that has all the mass."""
+    r = np.random.default_rng(1)
+    for spread in (1e-6, 0.01, 0.3, 30.0, 1e4, 1e30):
+        x = _logits(4, 40000, 3, spread)
+        _check_sample(x, r.random(4, np.float32), temperature=[1, 1, 0.3, 2])
+        _check_sample(x, r.random(4, np.float32), top_p=[0.9, 0.5, 0.999, 0.1], top_k=[0, 30000, 5, 0])
+
+
+@pytest.mark.parametrize("V", [5, 4096, 100000])
+def test_sample_ties_go_to_the_lowest_index(cuda, V):
+    """Equal logits, and logits of few values: more in one bin than are ranked
+    at once."""
+    u = np.linspace(0, 0.999, 8, dtype=np.float32)
+    same = torch.full((8, V), 1.5, device="cuda")
+    same[1::2] = -0.0
+    same[1::4, ::2] = 0.0
+    _check_sample(same, u)
+    _check_sample(same, u, top_k=[1, 2, 3, V // 2, V - 1, V, 0, V + 7])
+    _check_sample(same, u, top_p=[0.5, 0.25, 1e-6, 0.75, 0.125, 1.0, 2.0, 0.0])
+    few = torch.from_numpy(np.random.default_rng(2).integers(-3, 3, (8, V)).astype(np.float32)).cuda()
+    _check_sample(few, u, top_k=[0, 1, 2, V // 3, V // 2, V, 0, 7], top_p=[0.9] * 8)
+    _check_sample(few, u, min_p=[np.exp(np.float32(-1)) * 1.001, 0.5, 1.0, 3.0, 1e-30, 0.0, 0.3, 0.01])
+
+
+def test_sample_at_the_borders_of_u(cuda):
+    """Eight equal weights: u = i / 8 is the first number of entry i."""
+    x = torch.zeros((8, 8), device="cuda")
+    tokens, _ = _sample(x, [i / 8 for i in range(8)])
+    assert tokens.tolist() == list(range(8))
+    tokens, _ = _sample(x, [float(np.nextafter(np.float32(i / 8), np.float32(0))) for i in range(1, 9)])
+    assert tokens.tolist() == list(range(8))
+    tokens, _ = _sample(x, [-1.0, 0.0, 1.0, 2.0, float("inf"), -float("inf"), float("nan"), 0.99])
+    assert tokens.tolist() == [0, 0, 7, 7, 7, 0, 0, 7]
+
+
+def test_sample_masked_and_infinite_logits(cuda):
+    inf, nan = float("inf"), float("nan")
+    low = torch.finfo(torch.float32).min
+    rows = [[-inf] * 6, [nan] * 6, [-inf, nan, -inf, 2.0, -inf, nan], [inf, 1, inf, nan, -inf, inf],
+            [low] * 6, [low, low, -3.0, low, -3.0, low], [nan, 1.0, 1.0, -inf, 0.5, inf], [3e38, -3e38, 3e38, 0, low, 1]]
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.tensor(rows, device="cuda").to(dtype)
+        for u in (0.0, 0.4, 0.7, 0.999):
+            _check_sample(x, [u] * 8)
+            _check_sample(x, [u] * 8, top_k=[2] * 8, top_p=[0.8] * 8, min_p=[0.1] * 8)
+            _check_sample(x, [u] * 8, temperature=[1e-44] * 8)
+            _check_sample(x, [u] * 8, temperature=[1e30] * 8)
+    wide = torch.full((2, 70000), -inf, device="cuda")
+    wide[0, 69999] = -50.0
+    _check_sample(wide, [0.5, 0.5], top_p=[0.9, 0.9])
+
+
+def test_sample_greedy(cuda):
+    x = _logits(6, 3000, 4)
+    x[0, 7] = x[0, 2900] = 50.0
+    tokens, probs = _sample(x, [0.9] * 6, temperature=[0.0, -1.0, float("nan"), 0.0, 1.0, 1.0],
+                            top_k=[0, 0, 0, 5, 1, 0], top_p=[1, 1, 1, 1, 1, -0.5])
+    assert tokens.tolist() == x.argmax(1).tolist() and tokens[0] == 7 and (probs == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_strided_rows(cuda, dtype):
+    """Rows at every alignment, inside a wider buffer whose other columns would
+    win; without probs; on another stream; the same call gives the same answer."""
+    buf = torch.full((9, 5021), 100.0, device="cuda", dtype=dtype)
+    x = buf[:, 3:4999]
+    x.copy_(_logits(9, 4996, 5))
+    u = np.random.default_rng(3).random(9, np.float32)
+    _check_sample(x, u, top_p=[0.9] * 9)
+    want, _ = _sample(x, u, top_p=[0.9] * 9)
+    got, _ = _sample(x, u, top_p=[0.9] * 9, probs=False, stream=torch.cuda.Stream())
+    assert (got == want).all()
+
+
+def test_sample_captured(cuda):
+    from npu_amd import groups
+    x = _logits(4, 9000, 6)
+    u = torch.rand(4, device="cuda")
+    tokens, probs = torch.empty(4, dtype=torch.int32, device="cuda"), torch.empty(4, device="cuda")
+    ws = groups.sample_workspace(x)
+    p = torch.full((4,), 0.9, device="cuda")
+    call = lambda: groups.fused_sample_tokens(x, u, tokens, ws, top_p=p, probs=probs, stream=torch.cuda.current_stream())
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for step in range(4):
+        x.copy_(_logits(4, 9000, 60 + step))
+        u.copy_(torch.rand(4))
+        g.replay()
+        torch.cuda.synchronize()
+        got = tokens.clone(), probs.clone()
+        tokens.zero_()
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(tokens, got[0]) and torch.equal(probs, got[1]), step
+        host = x.double().cpu().numpy()
+        assert tokens.tolist() == [R.sample64(host[b], float(u[b]), top_p=np.float32(0.9))[0] for b in range(4)], step

@@ -212,6 +212,35 @@ def test_append_refuses(over, status, text):
     assert _append(over.pop("prefix", 0), over.pop("pairs", 0), **over) == status and text in _err(), _err()
 
 
+def _sample(**over):
+    a = {"logits": _mr([3, 100]), "u": _mr([3]), "temperature": _mr([3]), "top_k": _mr([3], I32), "top_p": _mr([3]),
+         "min_p": _mr([3]), "tokens": _mr([3], I32), "probs": _mr([3]), "ws": _mr([1 << 27])}
+    a.update(over)
+    return _call("fused_sample_tokens", a.values())
+
+
+SAMPLE_REFUSALS = [
+    (dict(logits=None), 1, "logits: null"), (dict(logits=_mr([3, 100], I32)), 1, "element type"),
+    (dict(logits=_mr([300])), 1, "rank"), (dict(logits=_mr([3, (1 << 20) + 1])), 2, "2^20"),
+    (dict(logits=_mr([3, 100], strides=[1, 3])), 2, "contiguous"), (dict(logits=_mr([3, 100], strides=[90, 1])), 2, "overlap"),
+    (dict(logits=_mr([3, 100], ptr=0x10002)), 2, "4-byte"), (dict(u=None), 1, "u: null"), (dict(u=_mr([4])), 1, "u: size 4"),
+    (dict(temperature=_mr([1])), 1, "temperature"), (dict(top_k=_mr([3])), 1, "top_k"), (dict(top_p=_mr([3], BF16)), 1, "top_p"),
+    (dict(min_p=_mr([3], strides=[2])), 2, "min_p"), (dict(tokens=None), 1, "tokens"), (dict(tokens=_mr([3])), 1, "tokens"),
+    (dict(probs=_mr([2])), 1, "probs"), (dict(ws=None), 1, "workspace"), (dict(ws=_mr([1])), 1, "workspace: 1"),
+]
+
+
+@pytest.mark.parametrize("over,status,text", SAMPLE_REFUSALS)
+def test_sampling_refuses(over, status, text):
+    assert _sample(**over) == status and text in _err(), _err()
+
+
+def test_sampling_workspace_sizes():
+    f = npu_amd.lib().npu_sample_workspace
+    assert f(1, 1) > 0 and f(256, 1 << 20) > 0
+    assert [f(0, 5), f(5, 0), f(1, (1 << 20) + 1), f(-1, 5)] == [-1] * 4
+
+
 def test_wrappers_refuse_host_tensors():
     import torch
     from npu_amd import groups
