@@ -178,6 +178,19 @@ def lib():
     return _lib
 
 
+@functools.lru_cache(maxsize=None)
+def serve():
+    """The serving entry points' binding (bind/serve_bind.cpp), which takes
+    torch tensors; built with the library, and as it without a fallback."""
+    lib()
+    import torch  # noqa: F401  (the binding's own libraries)
+    try:
+        from . import _serve
+    except ImportError as e:
+        raise RuntimeError(f"npu_amd._serve not built: build it with `make -C {SRC_DIR}`") from e
+    return _serve
+
+
 def last_launch_plans():
     """Launch plans of this thread's most recent fused_* call (a list of NpuLaunchPlan)."""
     n = lib().npu_last_launch_plans(None, 0)

@@ -207,16 +207,9 @@ def fused_llama_rmsnorm_swiglu(h, g2, wg, wu, act, eps=1e-5, stream=None):
 PAIRS = {"interleaved": 0, "halves": 1}
 
 
-def _device_ref(name, t):
-    """Descriptor of a serving operand: a tensor on the GPU (a host pointer
-    would fault in the kernel)."""
-    if not t.is_cuda:
-        raise ValueError(f"{name}: expected a tensor on the GPU, got one on {t.device}")
-    return from_tensor(t)
-
-
-def _device_refs(**ts):
-    return [absent() if t is None else _device_ref(n, t) for n, t in ts.items()]
+def _raw(stream):
+    """A stream's raw handle; None stays None, torch's current stream."""
+    return getattr(stream, "cuda_stream", stream)
 
 
 def fused_llama_rope_append(Q, K, V, cos_t, sin_t, k_pages, v_pages, page_table, kv_len, Qo,
@@ -226,10 +219,8 @@ def fused_llama_rope_append(Q, K, V, cos_t, sin_t, k_pages, v_pages, page_table,
     sequence b lies in page page_table[b, j // page]; kv_len counts the new
     tokens; q_start [B + 1] are their first rows (None: one token each).
     Positions count the shared prefix: prefix_len + j."""
-    ms = _device_refs(Q=Q, K=K, V=V, cos_t=cos_t, sin_t=sin_t, k_pages=k_pages, v_pages=v_pages,
-                      page_table=page_table, kv_len=kv_len, q_start=q_start, Qo=Qo)
-    st = _lib.lib().fused_llama_rope_append(*[ref(m) for m in ms], int(prefix_len), PAIRS[pairs],
-                                            _stream(stream))
+    st = _lib.serve().rope_append(Q, K, V, cos_t, sin_t, k_pages, v_pages, page_table, kv_len,
+                                  q_start, Qo, prefix_len, PAIRS[pairs], _raw(stream))
     _check(st, "fused_llama_rope_append")
     return Qo, k_pages, v_pages
 
@@ -251,10 +242,9 @@ def fused_llama_paged_attention(Q, k_pages, v_pages, page_table, kv_len, A, scal
     """A = softmax(Q K^T * scale) V over the paged cache; bf16.  A token sees
     the shared prefix's prefix_len keys (pages prefix_table) and its sequence's
     own keys up to its own; the other arrays as in fused_llama_rope_append."""
-    ms = _device_refs(Q=Q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, kv_len=kv_len,
-                      q_start=q_start, prefix_table=prefix_table, A=A, workspace=workspace)
-    st = _lib.lib().fused_llama_paged_attention(*[ref(m) for m in ms], int(prefix_len), float(scale),
-                                                _stream(stream))
+    st = _lib.serve().paged_attention(Q, k_pages, v_pages, page_table, kv_len, q_start,
+                                      prefix_table, A, workspace, prefix_len, scale,
+                                      _raw(stream))
     _check(st, "fused_llama_paged_attention")
     return A
 
@@ -274,9 +264,8 @@ def fused_sample_tokens(logits, u, tokens, workspace, temperature=None, top_k=No
     """tokens[b] = a token of row b of logits (f32 or bf16), drawn with the
     random number u[b] in [0, 1) from what temperature, top-k, top-p and min-p
     (one value a row, None: off) leave; probs[b] its probability there."""
-    ms = _device_refs(logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p,
-                      min_p=min_p, tokens=tokens, probs=probs, workspace=workspace)
-    st = _lib.lib().fused_sample_tokens(*[ref(m) for m in ms], _stream(stream))
+    st = _lib.serve().sample_tokens(logits, u, temperature, top_k, top_p, min_p, tokens, probs,
+                                    workspace, _raw(stream))
     _check(st, "fused_sample_tokens")
     return tokens
 
