@@ -60,9 +60,9 @@ struct PartInfo {
   int pad[3];
 };
 
-// The workspace's regions.  Plain: info[W], first parts [W][ROWS], later parts
-// [W][ROWS].  Stacked prefix: own and prefix first parts [T][H] each, later parts
-// [W][ROWS] each.
+// The workspace's regions.  Plain: info[W], first parts [W][rows of a tile],
+// later parts the same.  Stacked prefix, for the own keys and for the prefix:
+// first parts [T][H], later parts [W][rows of a tile].
 template <int DH>
 struct Parts {
   PartInfo *info;
@@ -101,49 +101,68 @@ __device__ __forceinline__ void load_block(KeyBlock<DH> &b, const uint16_t *k0, 
   }
 }
 
+// A workgroup's share of the units, [u0, u1) of U, and the group its first lies
+// in; false: none (the launch has more workgroups than units).  Each lane sums
+// the units of some sequences, a scan over the lanes finds the one that holds u0.
+struct Share {
+  long long sum[NT];
+  UnitCursor cur;
+};
+__device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long long &U, int &W, long long &u0,
+                                           long long &u1, UnitCursor &c) {
+  const int tid = threadIdx.x;
+  const int seqs = split_seqs(sp), per = (seqs + NT - 1) / NT;
+  long long mine = 0;
+  for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) mine += seq_units(sp, i);
+  s.sum[tid] = mine;
+  __syncthreads();
+  for (int off = 1; off < NT; off <<= 1) {
+    const long long v = tid >= off ? s.sum[tid - off] : 0;
+    __syncthreads();
+    s.sum[tid] += v;
+    __syncthreads();
+  }
+  U = s.sum[NT - 1];
+  W = split_workgroups(U, gridDim.x);
+  if ((int)blockIdx.x >= W) return false;
+  u0 = first_unit(U, W, blockIdx.x);
+  u1 = first_unit(U, W, blockIdx.x + 1);
+  const long long before = s.sum[tid] - mine;
+  if (u0 >= before && u0 < s.sum[tid]) s.cur = seek_unit(sp, tid * per, before, u0);
+  __syncthreads();
+  c = s.cur;
+  return true;
+}
+
+// Rows of no sequence give zeros.
+template <int DH>
+__device__ __forceinline__ void zero_spare_rows(const PagedAttentionArgs &a, const AttnSplit &sp) {
+  if (sp.stacked || !sp.b.q_start) return;
+  const int lo = clamp_int(sp.b.q_start[0], 0, sp.b.T), hi = clamp_int(sp.b.q_start[sp.b.B], lo, sp.b.T);
+  const int spare = lo + (sp.b.T - hi), cols = sp.Hkv * sp.G * DH / 8;
+  for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < (long long)spare * cols; i += (long long)gridDim.x * NT) {
+    const int t = (int)(i / cols), c = (int)(i - (long long)t * cols);
+    *reinterpret_cast<u32x4 *>(a.out + (long long)(t < lo ? t : hi + t - lo) * a.o_stride + c * 8) = u32x4{0, 0, 0, 0};
+  }
+}
+
 template <int DH>
 __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
                                                                 Parts<DH> parts) {
   constexpr int E = DH / 16;  // entries of a lane's output run, MFMAs of the second product
-  __shared__ long long s_sum[NT];
-  __shared__ UnitCursor s_cur;
+  __shared__ Share share;
   __shared__ float s_m[4][ROWS], s_l[4][ROWS];
   __shared__ __attribute__((aligned(16))) float s_o[4][ROWS][DH + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int w = blockIdx.x;
 
-  // rows of no sequence give zeros
-  if (!sp.stacked && sp.b.q_start) {
-    const int lo = clamp_int(sp.b.q_start[0], 0, sp.b.T), hi = clamp_int(sp.b.q_start[sp.b.B], lo, sp.b.T);
-    const int spare = lo + (sp.b.T - hi), cols = sp.Hkv * sp.G * DH / 8;
-    for (long long i = (long long)w * NT + tid; i < (long long)spare * cols; i += (long long)gridDim.x * NT) {
-      const int t = (int)(i / cols), c = (int)(i - (long long)t * cols);
-      *reinterpret_cast<u32x4 *>(a.out + (long long)(t < lo ? t : hi + t - lo) * a.o_stride + c * 8) = u32x4{0, 0, 0, 0};
-    }
-  }
-
-  // this workgroup's share: the units of every sequence, summed over the lanes
-  const int seqs = split_seqs(sp), per = (seqs + NT - 1) / NT;
-  long long mine = 0;
-  for (int s = tid * per; s < min(seqs, (tid + 1) * per); ++s) mine += seq_units(sp, s);
-  s_sum[tid] = mine;
-  __syncthreads();
-  for (int off = 1; off < NT; off <<= 1) {
-    const long long v = tid >= off ? s_sum[tid - off] : 0;
-    __syncthreads();
-    s_sum[tid] += v;
-    __syncthreads();
-  }
-  const long long U = s_sum[NT - 1];
-  const int W = split_workgroups(U, gridDim.x);
+  zero_spare_rows<DH>(a, sp);
   if (!dense && tid == 0) parts.info[w].rows = 0;
-  if (w >= W) return;
-  const long long u0 = first_unit(U, W, w), u1 = first_unit(U, W, w + 1);
-  const long long before = s_sum[tid] - mine;
-  if (u0 >= before && u0 < s_sum[tid]) s_cur = seek_unit(sp, tid * per, before, u0);
-  __syncthreads();
-  UnitCursor c = s_cur;
+  long long U, u0, u1;
+  UnitCursor c;
+  int W;
+  if (!take_share(sp, share, U, W, u0, u1, c)) return;
 
   const float scale = a.scale * 1.44269504088896340736f;  // exponentials in base 2
   for (long long u = u0; u < u1;) {
@@ -276,14 +295,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
     __syncthreads();
     const bool starts = b0 == 0, ends = b1 == c.nb;
     const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
-    if (!dense && starts && !ends && tid == 0) {
-      PartInfo &in = parts.info[w];
-      in.rows = rows;
-      in.token = c.start;
-      in.row0 = row0;
-      in.head = c.head;
-      in.more = more;
-    }
+    if (!dense && starts && !ends && tid == 0) parts.info[w] = PartInfo{rows, c.start, row0, c.head, more, {0, 0, 0}};
     // lane (jr, jc): entries 8 jc .. of row jr
     for (int i = tid; i < rows * (DH / 8); i += NT) {
       const int jr = i / (DH / 8), jc = i % (DH / 8);
@@ -326,12 +338,262 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
   }
 }
 
-// Joins the parts of one output row: 8 lanes' worth of parts at a time, each
-// lane 4 (Dh 128) entries.  The order of the sums is the parts', whatever ran
-// first.
+// ---- many rows: prompts, and a shared prefix under the rows of a batch --------
+// A tile of 128 rows, 32 a wave, over blocks of 64 keys that the four waves share
+// through LDS: with enough rows per key the matrix instructions and the
+// exponentials bound it, not the cache's bytes.  32x32x16 MFMAs in the same two
+// products as above: S^T = K Q^T leaves a lane sixteen keys (8 j + 4 h + i of each
+// 32, h its half of the wave) of one row, so the row's maximum is one exchange
+// between the halves away, and keys 8 j + 4 h + i, j = 2 g and 2 g + 1, are the
+// k slots of its half in the g-th MFMA of O^T = V^T P^T.
+//  - K lies in LDS by keys, 16-byte chunks exchanged by the key's number so that
+//    the 32 keys of an operand read fall into different banks; V by keys as it is:
+//    a lane reads Dh / 32 entries of eight keys and turns them with v_perm.
+//  - Two buffers: while block i is computed, block i + 1, fetched a step ago, is
+//    written to the other, and block i + 2 is on its way; one barrier a block.
+//  - The running maximum is only a reference: it is raised, and the sums scaled,
+//    when a row's maximum passes it by more than 2^8 (a uniform branch), so that
+//    p <= 2^8 and most blocks scale nothing.
+constexpr int TROWS = 128, TKEYS = 64;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
 template <int DH>
+__global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
+                                                                     Parts<DH> parts) {
+  constexpr int CH = DH / 8;             // 16-byte chunks of a key
+  constexpr int NL = TKEYS * CH / NT;    // chunks a lane fetches, of K and of V
+  constexpr int KPL = NT / CH;           // keys that one fetch of all lanes covers
+  constexpr int E = DH / 32;             // entries of a lane's output run, MFMAs of the second product a k step
+  __shared__ __attribute__((aligned(16))) uint16_t sk[2][TKEYS * DH], sv[2][TKEYS * DH];
+  __shared__ Share share;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int w = blockIdx.x;
+  zero_spare_rows<DH>(a, sp);
+  if (!dense && tid == 0) parts.info[w].rows = 0;
+  long long U, u0, u1;
+  UnitCursor c;
+  int W;
+  if (!take_share(sp, share, U, W, u0, u1, c)) return;
+
+  const float scale = a.scale * 1.44269504088896340736f;
+  // where key `k` of a block keeps its chunk `ch`
+  auto k_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? k & 15 : (k >> 1) & 7)); };
+  const int fk = tid / CH, fc = tid % CH;  // the key and chunk this lane fetches
+
+  for (long long u = u0; u < u1;) {
+    const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
+    const int row0 = c.tile * TROWS, rows = min(TROWS, c.n * sp.G - row0);
+    const int wrow = wave * 32;  // this wave's first row in the tile
+    const bool busy = wrow < rows;
+    const int row = row0 + min(wrow + r, rows - 1), tok = row / sp.G;
+    Frag16 qf[DH / 16];
+    {
+      const uint16_t *p = a.Q + (long long)(c.start + tok) * a.q_stride + (c.head * sp.G + row - tok * sp.G) * DH + h * 8;
+#pragma unroll
+      for (int d = 0; d < DH / 16; ++d) qf[d] = load16(p + d * 16);
+    }
+    const int lim = visible_keys(sp, c.seq, c.n, tok);
+    const int lim_first = visible_keys(sp, c.seq, c.n, (row0 + min(wrow, rows - 1)) / sp.G);
+    const int lim_last = visible_keys(sp, c.seq, c.n, (row0 + min(wrow + 31, rows - 1)) / sp.G);
+    const int tile_lim = visible_keys(sp, c.seq, c.n, (row0 + rows - 1) / sp.G);
+    const int *table = sp.b.page_table + (sp.stacked ? 0 : c.seq * sp.b.table_stride);
+    const uint16_t *kh = a.k_pages + ((long long)c.head << sp.b.page_log2) * DH;
+    const uint16_t *vh = a.v_pages + ((long long)c.head << sp.b.page_log2) * DH;
+
+    f32x16 o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[e][i] = 0.f;
+    float m = -__builtin_inff(), l = 0.f;  // l: this lane's keys only
+
+    u32x4 kr[NL], vr[NL];
+    uint32_t live = 0;  // of the block in kr, vr: bit g, its keys 16 g ..
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
+      const bool pre = blk < sp.pre_blocks;
+      const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS, all = pre ? sp.b.prefix_len : tile_lim;
+      const int *t = pre ? a.prefix_table : table;
+      int page[TKEYS / 16];
+      live = 0;
+#pragma unroll
+      for (int g = 0; g < TKEYS / 16; ++g) {
+        const int j = j0 + 16 * g;
+        int pg = -1;
+        if (j < all) pg = checked_page(t[j >> sp.b.page_log2], sp.b.n_pages);
+        pg = __builtin_amdgcn_readfirstlane(pg);
+        live |= (pg >= 0 ? 1u : 0u) << g;
+        page[g] = max(pg, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        // the sixteen keys this wave's lanes fetch from
+        const int g = KPL == 16 ? i : 2 * i + (wave >> 1);
+        const int pg = KPL == 16 ? page[i] : wave >> 1 ? page[2 * i + 1] : page[2 * i];
+        const int j = j0 + 16 * g, in = ((j & ((1 << sp.b.page_log2) - 1)) + (fk & 15)) * DH + fc * 8;
+        const bool keep = j + (fk & 15) < all && (live >> g & 1);
+        kr[i] = *reinterpret_cast<const u32x4 *>(kh + pg * a.kpage_stride + in);
+        // values that no row may see must not meet p = 0
+        vr[i] = masked(*reinterpret_cast<const u32x4 *>(vh + pg * a.vpage_stride + in), keep);
+      }
+    };
+    auto commit = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int k = i * KPL + fk;
+        *reinterpret_cast<u32x4 *>(&sk[buf][k_chunk(k, fc) * 8]) = kr[i];
+        *reinterpret_cast<u32x4 *>(&sv[buf][k * DH + fc * 8]) = vr[i];
+      }
+    };
+    fetch(b0);
+    commit(0);
+    uint32_t here = live;
+    if (b0 + 1 < b1) fetch(b0 + 1);
+    __syncthreads();
+    for (int blk = b0; blk < b1; ++blk) {
+      const int buf = (blk - b0) & 1;
+      const uint32_t lv = here;
+      if (blk + 1 < b1) {
+        commit(buf ^ 1);
+        here = live;
+        if (blk + 2 < b1) fetch(blk + 2);
+      }
+      const bool pre = blk < sp.pre_blocks;
+      const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS;
+      const int my_lim = pre ? sp.b.prefix_len : lim;
+      const int first_lim = pre ? sp.b.prefix_len : lim_first, last_lim = pre ? sp.b.prefix_len : lim_last;
+      if (busy && j0 < last_lim) {
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+          for (int d = 0; d < DH / 16; ++d) {
+            const Frag16 kf = load16(&sk[buf][k_chunk(32 * t + r, 2 * d + h) * 8]);
+            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.h, qf[d].h, s[t], 0, 0, 0);
+          }
+        }
+        if (j0 + TKEYS > first_lim || lv != (1u << TKEYS / 16) - 1) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+              if (j0 + k >= my_lim || !(lv >> (k >> 4) & 1)) s[t][i] = -__builtin_inff();
+            }
+        }
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+        const LanePair tp = lane_pair32(top);
+        top = fmaxf(tp.lo, tp.hi) * scale;
+        if (__any(top > m + 8.0f)) {
+          const float mn = fmaxf(m, top);
+          const float alpha = mn == -__builtin_inff() ? 1.f : exp2_(m - mn);
+          m = mn;
+          l *= alpha;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[e][i] *= alpha;
+        }
+        const float base = m == -__builtin_inff() ? 0.f : m;
+        Frag16 pf[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            p[i] = exp2_(fmaf(s[t][i], scale, -base));
+            l += p[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            pf[2 * t].u[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
+            pf[2 * t + 1].u[i] = cvt_pk_bf16(p[8 + 2 * i], p[8 + 2 * i + 1]);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {  // sixteen keys
+          uint32_t v[8][E / 2];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint16_t *p = &sv[buf][(16 * g + 8 * (e >> 2) + 4 * h + (e & 3)) * DH + r * E];
+            if constexpr (DH == 128) {
+              const uint2 f = *reinterpret_cast<const uint2 *>(p);
+              v[e][0] = f.x;
+              v[e][1] = f.y;
+            } else {
+              v[e][0] = *reinterpret_cast<const uint32_t *>(p);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            Frag16 vf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              vf.u[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+            o[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.h, pf[g].h, o[e], 0, 0, 0);
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    const LanePair lp = lane_pair32(l);
+    l = lp.lo + lp.hi;
+    const bool starts = b0 == 0, ends = b1 == c.nb;
+    const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
+    if (!dense && starts && !ends && tid == 0) parts.info[w] = PartInfo{rows, c.start, row0, c.head, more, {0, 0, 0}};
+    const int jr = wrow + r;
+    if (jr < rows) {
+      const int head = c.head * sp.G + row - tok * sp.G;
+      const long long token = c.start + tok;
+      // this lane's entries: E at (8 j + 4 h + i) E
+      if (!dense && starts && ends) {
+        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+        uint16_t *to = a.out + token * a.o_stride + head * DH + 4 * h * E;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          uint16_t *t = to + (8 * (i >> 2) + (i & 3)) * E;
+          if constexpr (DH == 128)
+            *reinterpret_cast<uint2 *>(t) = make_uint2(cvt_pk_bf16(o[0][i] * inv, o[1][i] * inv), cvt_pk_bf16(o[2][i] * inv, o[3][i] * inv));
+          else
+            *reinterpret_cast<uint32_t *>(t) = cvt_pk_bf16(o[0][i] * inv, o[1][i] * inv);
+        }
+      } else {
+        PartRow<DH> *to = !starts ? parts.later + (long long)w * TROWS + jr
+                          : dense ? parts.first + token * (sp.G * sp.Hkv) + head
+                                  : parts.first + (long long)w * TROWS + jr;
+        float *t = to->o + 4 * h * E;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) t[(8 * (i >> 2) + (i & 3)) * E + e] = o[e][i];
+        if (h == 0) {
+          to->m = m;
+          to->l = l;
+          to->first = w;
+          to->more = more | (jr << 16);
+        }
+      }
+    }
+    u += b1 - b0;
+    if (u < u1) next_group(sp, c);
+  }
+}
+
+// ---- the joins ------------------------------------------------------------------
+// A row's parts, SPLIT of them at a time, 4 entries a lane; a workgroup takes
+// NT / (DH / 4) / SPLIT rows.  The order of the sums is the parts', whatever ran
+// first.
+template <int DH, int SPLIT>
 struct RowJoin {
-  static constexpr int CH = DH / 4, SPLIT = NT / CH;
+  static constexpr int CH = DH / 4, PER = NT / CH / SPLIT;  // PER: rows of a workgroup
   float m, l;
   f32x4 o;
   __device__ __forceinline__ void clear() {
@@ -351,13 +613,16 @@ struct RowJoin {
     add(p->m, p->l, *reinterpret_cast<const f32x4 *>(p->o + ch * 4));
   }
   // over the lanes' splits, to split 0
-  __device__ __forceinline__ void gather(f32x4 *so, float *sm, float *sl, int split, int ch) {
-    so[split * CH + ch] = o;
-    sm[split * CH + ch] = m;
-    sl[split * CH + ch] = l;
-    __syncthreads();
-    if (split == 0)
-      for (int s = 1; s < SPLIT; ++s) add(sm[s * CH + ch], sl[s * CH + ch], so[s * CH + ch]);
+  __device__ __forceinline__ void gather(f32x4 *so, float *sm, float *sl, int split) {
+    if constexpr (SPLIT > 1) {
+      const int tid = threadIdx.x, at = tid % (NT / SPLIT);
+      so[tid] = o;
+      sm[tid] = m;
+      sl[tid] = l;
+      __syncthreads();
+      if (split == 0)
+        for (int s = 1; s < SPLIT; ++s) add(sm[s * (NT / SPLIT) + at], sl[s * (NT / SPLIT) + at], so[s * (NT / SPLIT) + at]);
+    }
   }
   __device__ __forceinline__ void store(uint16_t *out, int ch) const {
     const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
@@ -366,102 +631,133 @@ struct RowJoin {
   }
 };
 
-// Workgroup (w, jr): row jr of the group whose first part workgroup w left.
-template <int DH>
-__global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttentionArgs a, int G, Parts<DH> parts) {
-  using J = RowJoin<DH>;
-  __shared__ f32x4 so[NT];
-  __shared__ float sm[NT], sl[NT];
-  const int w = blockIdx.x, jr = blockIdx.y;
+// Workgroup (w, y): rows of the group whose first part workgroup w left in its
+// slot of `slot_rows`.
+template <int DH, int SPLIT>
+__global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttentionArgs a, int G, int slot_rows,
+                                                                  Parts<DH> parts) {
+  using J = RowJoin<DH, SPLIT>;
+  __shared__ f32x4 so[SPLIT > 1 ? NT : 1];
+  __shared__ float sm[SPLIT > 1 ? NT : 1], sl[SPLIT > 1 ? NT : 1];
+  const int w = blockIdx.x, ch = threadIdx.x % J::CH, sub = threadIdx.x / J::CH % J::PER;
+  const int split = threadIdx.x / (J::CH * J::PER), jr = blockIdx.y * J::PER + sub;
   const PartInfo in = parts.info[w];
-  if (jr >= in.rows) return;
-  const int ch = threadIdx.x % J::CH, split = threadIdx.x / J::CH;
+  if ((int)blockIdx.y * J::PER >= in.rows) return;
   J j;
   j.clear();
-  for (int i = split; i <= in.more; i += J::SPLIT)
-    j.add(i == 0 ? parts.first + w * ROWS + jr : parts.later + (w + i) * ROWS + jr, ch);
-  j.gather(so, sm, sl, split, ch);
-  if (split == 0) {
+  if (jr < in.rows)
+    for (int i = split; i <= in.more; i += SPLIT)
+      j.add(i == 0 ? parts.first + (long long)w * slot_rows + jr : parts.later + (long long)(w + i) * slot_rows + jr, ch);
+  j.gather(so, sm, sl, split);
+  if (split == 0 && jr < in.rows) {
     const int row = in.row0 + jr, tok = row / G;
     j.store(a.out + (long long)(in.token + tok) * a.o_stride + (in.head * G + row - tok * G) * DH, ch);
   }
 }
 
-// Workgroup i: row i = token * H + head, its own parts and the prefix's.
-template <int DH>
-__global__ __launch_bounds__(NT) void paged_attention_join2_kernel(PagedAttentionArgs a, ServeBatch b, int H,
-                                                                   int W, Parts<DH> own, Parts<DH> pre) {
-  using J = RowJoin<DH>;
-  __shared__ f32x4 so[NT];
-  __shared__ float sm[NT], sl[NT];
-  const long long i = blockIdx.x;
+// Row i = token * H + head: its own parts and the prefix's.
+template <int DH, int SPLIT>
+__global__ __launch_bounds__(NT) void paged_attention_join2_kernel(PagedAttentionArgs a, ServeBatch b, int H, int W,
+                                                                   Parts<DH> own, int own_rows, Parts<DH> pre, int pre_rows) {
+  using J = RowJoin<DH, SPLIT>;
+  __shared__ f32x4 so[SPLIT > 1 ? NT : 1];
+  __shared__ float sm[SPLIT > 1 ? NT : 1], sl[SPLIT > 1 ? NT : 1];
+  const int ch = threadIdx.x % J::CH, sub = threadIdx.x / J::CH % J::PER, split = threadIdx.x / (J::CH * J::PER);
+  const long long i = (long long)blockIdx.x * J::PER + sub;
   const int tok = (int)(i / H), head = (int)(i - (long long)tok * H);
-  if (seq_of_token(b, tok) < 0) return;  // zeroed already
-  const int ch = threadIdx.x % J::CH, split = threadIdx.x / J::CH;
+  const bool in = tok < b.T && seq_of_token(b, tok) >= 0;  // else zeroed already
   J j;
   j.clear();
+  if (in) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const Parts<DH> &p = k ? pre : own;
-    const PartRow<DH> *f = p.first + i;
-    // (clamped: sequences that overlap, which q_start must not make, would mix two groups' words)
-    const int first = clamp_int(f->first, 0, W - 1), more = min(f->more & 0xffff, W - 1 - first);
-    const int jr = (f->more >> 16) & (ROWS - 1);
-    for (int n = split; n <= more; n += J::SPLIT) j.add(n == 0 ? f : p.later + (first + n) * ROWS + jr, ch);
+    for (int k = 0; k < 2; ++k) {
+      const Parts<DH> &p = k ? pre : own;
+      const int slot_rows = k ? pre_rows : own_rows;
+      const PartRow<DH> *f = p.first + i;
+      // (clamped: sequences that overlap, which q_start must not make, would mix two groups' words)
+      const int first = clamp_int(f->first, 0, W - 1), more = min(f->more & 0xffff, W - 1 - first);
+      const int jr = (f->more >> 16) & (slot_rows - 1);
+      for (int n = split; n <= more; n += SPLIT)
+        j.add(n == 0 ? f : p.later + (long long)(first + n) * slot_rows + jr, ch);
+    }
   }
-  j.gather(so, sm, sl, split, ch);
-  if (split == 0) j.store(a.out + (long long)tok * a.o_stride + head * DH, ch);
+  j.gather(so, sm, sl, split);
+  if (split == 0 && in) j.store(a.out + (long long)tok * a.o_stride + head * DH, ch);
 }
 
-// How a call is divided: the workgroups of a launch, and whether the prefix is
-// computed once for the rows of all sequences.
+// ---- the division of a call --------------------------------------------------------
 struct Division {
-  int W;
-  bool stacked;
+  int W;          // workgroups of a launch
+  bool stacked;   // the prefix once for the rows of all sequences
+  bool own_tiles, pre_tiles;  // 128-row tiles for the own keys' part, the prefix's
 };
-// A prefix is shared by a product of its own where it saves reading it per
-// sequence: more than one sequence, each with less than a tile of rows.
 Division divide(const ServeBatch &b, int H, int Hkv) {
-  const int G = H / Hkv;
-  const bool stacked = b.prefix_len > 0 && b.B > 1 && (long long)b.T * G < (long long)b.B * ROWS;
-  return Division{2 * device_cus(), stacked};
+  const long long G = H / Hkv, rows = b.T * G;
+  Division d;
+  d.W = 2 * device_cus();
+  // A prefix is shared by a product of its own where it saves reading it per
+  // sequence: more than one sequence, each with less than a tile of rows.
+  d.stacked = b.prefix_len > 0 && b.B > 1 && rows < (long long)b.B * TROWS;
+  d.own_tiles = rows >= (long long)b.B * 4 * ROWS;
+  d.pre_tiles = rows >= 4 * ROWS;
+  return d;
+}
+
+template <int DH>
+size_t slot_bytes(const Division &d, bool tiles) {
+  return (size_t)d.W * (tiles ? TROWS : ROWS) * sizeof(PartRow<DH>);
+}
+
+template <int DH>
+size_t workspace_of(const ServeBatch &b, int H, int Hkv) {
+  const Division d = divide(b, H, Hkv);
+  const size_t own = slot_bytes<DH>(d, d.own_tiles);
+  if (!d.stacked) return d.W * sizeof(PartInfo) + 2 * own;
+  return 2 * (size_t)b.T * H * sizeof(PartRow<DH>) + own + slot_bytes<DH>(d, d.pre_tiles);
 }
 
 template <int DH>
 hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
   const Division d = divide(a.b, a.H, a.Hkv);
-  const int G = a.H / a.Hkv, rows = a.b.T * a.H;
-  const int pre_blocks = (a.b.prefix_len + KEYS - 1) / KEYS;
-  AttnSplit sp{a.b, G, a.Hkv, ROWS, KEYS, d.stacked ? 0 : pre_blocks, 0};
+  const int G = a.H / a.Hkv;
   char *ws = static_cast<char *>(a.workspace);
-  const size_t slots = (size_t)d.W * ROWS * sizeof(PartRow<DH>);
-  auto plan = [&](const char *name, int grid) {
-    npu_launch_plan p = make_plan(name, grid, wg_per_cu(paged_attention_kernel<DH>, NT), grid, 16);
-    plans_add(p);
+  auto plan = [&](const char *name, int grid, int per_cu) {
+    plans_add(make_plan(name, grid, per_cu, grid, 16));
   };
-  auto kern = paged_attention_kernel<DH>;
+  // the own keys' part or, stacked, the prefix's
+  auto attend = [&](bool tiles, bool stacked, int dense, const Parts<DH> &parts) {
+    const int keys = tiles ? TKEYS : KEYS, pre_blocks = (a.b.prefix_len + keys - 1) / keys;
+    const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, keys, d.stacked && !stacked ? 0 : pre_blocks, stacked};
+    auto kern = tiles ? paged_attention_tile_kernel<DH> : paged_attention_kernel<DH>;
+    static const char *const names[2][2] = {{"llama_paged_attention", "llama_paged_attention_tiles"},
+                                            {"llama_paged_attention_prefix", "llama_paged_attention_prefix_tiles"}};
+    plan(names[stacked][tiles], d.W, wg_per_cu(kern, NT));
+    hipLaunchKernelGGL(kern, dim3(d.W), dim3(NT), 0, s, a, sp, dense, parts);
+  };
+  const int own_rows = d.own_tiles ? TROWS : ROWS, pre_rows = d.pre_tiles ? TROWS : ROWS;
   if (!d.stacked) {
     Parts<DH> parts;
     parts.info = reinterpret_cast<PartInfo *>(ws);
     parts.first = reinterpret_cast<PartRow<DH> *>(ws + d.W * sizeof(PartInfo));
-    parts.later = parts.first + (size_t)d.W * ROWS;
-    plan("llama_paged_attention", d.W);
-    hipLaunchKernelGGL(kern, dim3(d.W), dim3(NT), 0, s, a, sp, 0, parts);
-    plan("llama_paged_attention_join", d.W);
-    const int most = a.b.q_start ? ROWS : std::min(ROWS, G);
-    hipLaunchKernelGGL(paged_attention_join_kernel<DH>, dim3(d.W, most), dim3(NT), 0, s, a, G, parts);
+    parts.later = parts.first + (size_t)d.W * own_rows;
+    attend(d.own_tiles, false, 0, parts);
+    auto join = d.own_tiles ? paged_attention_join_kernel<DH, 1> : paged_attention_join_kernel<DH, NT * 4 / DH>;
+    const int per = d.own_tiles ? RowJoin<DH, 1>::PER : 1, most = a.b.q_start || d.own_tiles ? own_rows : std::min(ROWS, G);
+    plan("llama_paged_attention_join", d.W * ((most + per - 1) / per), wg_per_cu(join, NT));
+    hipLaunchKernelGGL(join, dim3(d.W, (most + per - 1) / per), dim3(NT), 0, s, a, G, own_rows, parts);
   } else {
-    const size_t dense = (size_t)rows * sizeof(PartRow<DH>);
-    Parts<DH> own{nullptr, reinterpret_cast<PartRow<DH> *>(ws), reinterpret_cast<PartRow<DH> *>(ws + dense)};
-    ws += dense + slots;
-    Parts<DH> pre{nullptr, reinterpret_cast<PartRow<DH> *>(ws), reinterpret_cast<PartRow<DH> *>(ws + dense)};
-    AttnSplit sq{a.b, G, a.Hkv, ROWS, KEYS, pre_blocks, 1};
-    plan("llama_paged_attention_prefix", d.W);
-    hipLaunchKernelGGL(kern, dim3(d.W), dim3(NT), 0, s, a, sq, 1, pre);
-    plan("llama_paged_attention", d.W);
-    hipLaunchKernelGGL(kern, dim3(d.W), dim3(NT), 0, s, a, sp, 1, own);
-    plan("llama_paged_attention_join", rows);
-    hipLaunchKernelGGL(paged_attention_join2_kernel<DH>, dim3(rows), dim3(NT), 0, s, a, a.b, a.H, d.W, own, pre);
+    const size_t dense = (size_t)a.b.T * a.H * sizeof(PartRow<DH>);
+    auto take = [&](size_t later) {
+      Parts<DH> p{nullptr, reinterpret_cast<PartRow<DH> *>(ws), reinterpret_cast<PartRow<DH> *>(ws + dense)};
+      ws += dense + later;
+      return p;
+    };
+    const Parts<DH> own = take(slot_bytes<DH>(d, d.own_tiles)), pre = take(slot_bytes<DH>(d, d.pre_tiles));
+    attend(d.pre_tiles, true, 1, pre);
+    attend(d.own_tiles, false, 1, own);
+    auto join = paged_attention_join2_kernel<DH, NT * 4 / DH>;
+    plan("llama_paged_attention_join", a.b.T * a.H, wg_per_cu(join, NT));
+    hipLaunchKernelGGL(join, dim3(a.b.T * a.H), dim3(NT), 0, s, a, a.b, a.H, d.W, own, own_rows, pre, pre_rows);
   }
   return hipGetLastError();
 }
@@ -469,9 +765,7 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t paged_attention_workspace(const ServeBatch &b, int H, int Hkv, int dh) {
-  const Division d = divide(b, H, Hkv);
-  const size_t row = dh == 128 ? sizeof(PartRow<128>) : sizeof(PartRow<64>), slots = (size_t)d.W * ROWS * row;
-  return d.stacked ? 2 * ((size_t)b.T * H * row + slots) : d.W * sizeof(PartInfo) + 2 * slots;
+  return dh == 128 ? workspace_of<128>(b, H, Hkv) : workspace_of<64>(b, H, Hkv);
 }
 
 hipError_t launch_llama_paged_attention(const PagedAttentionArgs &a, hipStream_t s) {

@@ -74,7 +74,7 @@ NPU_HD Place place_of_token(const ServeBatch &b, int t) {
 // `pre_blocks` blocks and its own up to what its last token sees, are cut into
 // blocks of `keys`; a (tile, key head)'s blocks are a group of units, one at
 // least, so that rows without keys are written too.  Units are numbered by
-// sequence, tile, key head, block; workgroup w of W takes the units
+// sequence, key head, tile, block (tiles that stand together read the same keys); workgroup w of W takes the units
 // [U w / W, U (w + 1) / W): equal shares whatever the lengths, a group cut at
 // most at the workgroups' borders.  W is at most U (split_workgroups), so that
 // every one of them has work and a cut group's parts are those of consecutive
@@ -105,11 +105,15 @@ NPU_HD int tile_blocks(const AttnSplit &a, int seq, int n, int tile) {
   const int nb = a.pre_blocks + (int)(((long long)v + a.keys - 1) / a.keys);
   return nb > 0 ? nb : 1;
 }
-NPU_HD long long seq_units(const AttnSplit &a, int seq) {
-  const int n = split_span(a, seq).n, tiles = split_tiles(a, n);
+// Units of one key head of a sequence of n new tokens.
+NPU_HD long long head_units(const AttnSplit &a, int seq, int n) {
+  const int tiles = split_tiles(a, n);
   long long sum = 0;
   for (int t = 0; t < tiles; ++t) sum += tile_blocks(a, seq, n, t);
-  return sum * a.Hkv;
+  return sum;
+}
+NPU_HD long long seq_units(const AttnSplit &a, int seq) {
+  return head_units(a, seq, split_span(a, seq).n) * a.Hkv;
 }
 NPU_HD int split_workgroups(long long U, int launched) { return U < launched ? (int)U : launched; }
 NPU_HD long long first_unit(long long U, int W, int w) { return U * w / W; }
@@ -129,18 +133,20 @@ NPU_HD UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long lo
     const SeqSpan sp = split_span(a, c.seq);
     c.n = sp.n;
     c.start = sp.start;
-    const int tiles = split_tiles(a, sp.n);
-    for (c.tile = 0; c.tile < tiles; ++c.tile) {
-      c.nb = tile_blocks(a, c.seq, c.n, c.tile);
-      const long long here = (long long)c.nb * a.Hkv;
-      if (u < c.base + here) {
-        c.head = (int)((u - c.base) / c.nb);
-        c.base += (long long)c.head * c.nb;
-        c.blk = (int)(u - c.base);
-        return c;
-      }
-      c.base += here;
+    const long long per = head_units(a, c.seq, c.n);
+    if (u >= c.base + per * a.Hkv) {
+      c.base += per * a.Hkv;
+      continue;
     }
+    c.head = (int)((u - c.base) / per);
+    c.base += per * c.head;
+    for (;; ++c.tile) {
+      c.nb = tile_blocks(a, c.seq, c.n, c.tile);
+      if (u < c.base + c.nb) break;
+      c.base += c.nb;
+    }
+    c.blk = (int)(u - c.base);
+    return c;
   }
   return c;  // u is past the last unit
 }
@@ -148,15 +154,17 @@ NPU_HD UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long lo
 NPU_HD void next_group(const AttnSplit &a, UnitCursor &c) {
   c.base += c.nb;
   c.blk = 0;
-  if (++c.head < a.Hkv) return;
-  c.head = 0;
-  ++c.tile;
-  while (c.tile >= split_tiles(a, c.n)) {
-    if (++c.seq >= split_seqs(a)) return;
-    const SeqSpan sp = split_span(a, c.seq);
-    c.n = sp.n;
-    c.start = sp.start;
+  if (++c.tile >= split_tiles(a, c.n)) {
     c.tile = 0;
+    if (++c.head >= a.Hkv) {
+      c.head = 0;
+      do {
+        if (++c.seq >= split_seqs(a)) return;
+        const SeqSpan sp = split_span(a, c.seq);
+        c.n = sp.n;
+        c.start = sp.start;
+      } while (c.n == 0);
+    }
   }
   c.nb = tile_blocks(a, c.seq, c.n, c.tile);
 }

@@ -194,6 +194,13 @@ ATTEND = [
     ([6, 1], [50, 1], 4, 2, 64, 16, 0, {"max_pages": 3}),  # keys past the table
     ([3, 2], [9, 20], 4, 2, 64, 16, 0, {"extra": 4}),      # rows of no sequence
     ([1, 2], [9, 20], 4, 2, 64, 16, 40, {"extra": 4}),
+    ([257, 0, 90], [300, 7, 90], 4, 1, 64, 64, 33, {"extra": 3}),
+    ([128], [128], 1, 1, 128, 16, 0, {}),
+    ([129], [2], 2, 1, 128, 16, 65, {}),                   # most tokens see the prefix alone
+    ([200], [50], 1, 1, 64, 16, 0, {}),                    # most tokens see nothing
+    ([64], [2000], 3, 3, 128, 32, 0, {}),
+    ([1] * 90, [i % 7 for i in range(90)], 6, 2, 128, 16, 500, {"ragged": False}),
+    ([3] * 30, [3 + i for i in range(30)], 4, 4, 64, 16, 257, {}),
 ]
 
 
@@ -205,6 +212,21 @@ def test_attention(cuda, news, lens, H, Hkv, Dh, page, prefix, kind):
     assert not spare or not A[-spare:].any()
 
 
+@pytest.mark.parametrize("news,H,Hkv,prefix,names", [
+    ([1] * 8, 8, 2, 0, ["", "_join"]), ([1] * 8, 8, 2, 20, ["_prefix", "", "_join"]),
+    ([1] * 16, 8, 2, 20, ["_prefix_tiles", "", "_join"]), ([200], 4, 2, 20, ["_tiles", "_join"]),
+    ([40] * 2, 4, 2, 20, ["_prefix_tiles", "_tiles", "_join"]), ([31] * 2, 4, 2, 0, ["", "_join"]),
+])
+def test_attention_kernels_by_rows(cuda, news, H, Hkv, prefix, names):
+    """Few rows a sequence: the kernel that divides keys over waves; many, or a
+    prefix under many rows of a batch: the one that divides rows."""
+    from npu_amd import groups
+    bt = R.Batch(news, [n + 3 for n in news], Hkv, 64, 16, prefix, ragged=set(news) != {1})
+    with groups.collect_plans() as cp:
+        _attend(bt, bt.rnd(bt.T, H * 64))
+    assert [p.kernel.decode() for p in cp.plans] == ["llama_paged_attention" + n for n in names]
+
+
 def test_attention_large_logits(cuda):
     """Logits of hundreds, rising and falling along the keys: maxima that move
     in every block."""
@@ -212,6 +234,9 @@ def test_attention_large_logits(cuda):
     ramp = torch.linspace(-8, 8, bt.P, device="cuda").to(torch.bfloat16)
     bt.k_pages *= ramp[:, None, None, None]
     _check_attend(bt, bt.rnd(bt.T, 4 * 64) * 6)
+    bt = R.Batch([90, 130], [900, 130], 2, 128, 16, 50, seed=3)
+    bt.k_pages *= torch.linspace(-8, 8, bt.P, device="cuda").to(torch.bfloat16)[:, None, None, None]
+    _check_attend(bt, bt.rnd(bt.T, 4 * 128) * 4)
 
 
 @pytest.mark.parametrize("prefix", [0, 70])
@@ -238,6 +263,10 @@ def test_attention_bad_pages_are_masked(cuda):
     bt.page_table[2, 0] = bt.page_table[2, 1] = -2 ** 31
     bt.prefix_table[1] = bt.P + 7
     _check_attend(bt, bt.rnd(3, 8 * 128))
+    bt = R.Batch([70], [200], 2, 64, 16, 40, seed=7)
+    bt.page_table[0, 2], bt.page_table[0, 9], bt.prefix_table[0] = -1, bt.P, -7
+    bt.table = bt.page_table.cpu().numpy()
+    _check_attend(bt, bt.rnd(70, 4 * 64))
 
 
 def test_attention_strides_streams_and_repeats(cuda):
