@@ -347,8 +347,9 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
 // between the halves away, and keys 8 j + 4 h + i, j = 2 g and 2 g + 1, are the
 // k slots of its half in the g-th MFMA of O^T = V^T P^T.
 //  - K lies in LDS by keys, 16-byte chunks exchanged by the key's number so that
-//    the 32 keys of an operand read fall into different banks; V by keys as it is:
-//    a lane reads Dh / 32 entries of eight keys and turns them with v_perm.
+//    the 32 keys of an operand read fall into different banks; V by keys with its
+//    64-byte runs exchanged, for gfx950's transposing reads: sixteen lanes read four
+//    keys of sixteen entries, each gets four keys of its entry.
 //  - Two buffers: while block i is computed, block i + 1, fetched a step ago, is
 //    written to the other, and block i + 2 is on its way; one barrier a block.
 //  - The running maximum is only a reference: it is raised, and the sums scaled,
@@ -358,13 +359,17 @@ constexpr int TROWS = 128, TKEYS = 64;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+__device__ __forceinline__ uint2 read_tr(const uint16_t *p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+}
+
 template <int DH>
 __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
                                                                      Parts<DH> parts) {
   constexpr int CH = DH / 8;             // 16-byte chunks of a key
   constexpr int NL = TKEYS * CH / NT;    // chunks a lane fetches, of K and of V
   constexpr int KPL = NT / CH;           // keys that one fetch of all lanes covers
-  constexpr int E = DH / 32;             // entries of a lane's output run, MFMAs of the second product a k step
+  constexpr int E = DH / 32;             // MFMAs of the second product a k step
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][TKEYS * DH], sv[2][TKEYS * DH];
   __shared__ Share share;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -380,6 +385,16 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   const float scale = a.scale * 1.44269504088896340736f;
   // where key `k` of a block keeps its chunk `ch`
   auto k_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? k & 15 : (k >> 1) & 7)); };
+  // the same of V: 64-byte runs exchanged, which a transposing read takes whole
+  auto v_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? (k & 3) << 2 : (k & 2) << 1)); };
+  constexpr uint32_t kAllLive = (1u << TKEYS / 16) - 1;
+  // this lane's operand addresses in a buffer: K's chunks of key r, V's runs
+  int ka[DH / 16], va[E];
+#pragma unroll
+  for (int d = 0; d < DH / 16; ++d) ka[d] = k_chunk(r, 2 * d + h) * 8;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    va[e] = v_chunk(4 * h + (lane >> 2 & 3), 4 * e + (r >> 4) * 2 + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
   const int fk = tid / CH, fc = tid % CH;  // the key and chunk this lane fetches
 
   for (long long u = u0; u < u1;) {
@@ -410,7 +425,10 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     float m = -__builtin_inff(), l = 0.f;  // l: this lane's keys only
 
     u32x4 kr[NL], vr[NL];
-    uint32_t live = 0;  // of the block in kr, vr: bit g, its keys 16 g ..
+    // of the block in kr, vr: bit g, whether its keys 16 g .. have a page; its
+    // keys that a row of the tile may see
+    uint32_t live = 0;
+    int seen = 0;
     auto fetch = [&](int blk) __attribute__((always_inline)) {
       const bool pre = blk < sp.pre_blocks;
       const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS, all = pre ? sp.b.prefix_len : tile_lim;
@@ -432,18 +450,25 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
         const int g = KPL == 16 ? i : 2 * i + (wave >> 1);
         const int pg = KPL == 16 ? page[i] : wave >> 1 ? page[2 * i + 1] : page[2 * i];
         const int j = j0 + 16 * g, in = ((j & ((1 << sp.b.page_log2) - 1)) + (fk & 15)) * DH + fc * 8;
-        const bool keep = j + (fk & 15) < all && (live >> g & 1);
         kr[i] = *reinterpret_cast<const u32x4 *>(kh + pg * a.kpage_stride + in);
-        // values that no row may see must not meet p = 0
-        vr[i] = masked(*reinterpret_cast<const u32x4 *>(vh + pg * a.vpage_stride + in), keep);
+        vr[i] = *reinterpret_cast<const u32x4 *>(vh + pg * a.vpage_stride + in);
       }
+      seen = all - j0;
     };
     auto commit = [&](int buf) __attribute__((always_inline)) {
+      if (seen < TKEYS || live != kAllLive) {  // values that no row may see must not meet p = 0
+        __builtin_amdgcn_sched_barrier(0);     // (keeps the branch)
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int k = i * KPL + fk;
+          vr[i] = masked(vr[i], k < seen && (live >> (k >> 4) & 1));
+        }
+      }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int k = i * KPL + fk;
         *reinterpret_cast<u32x4 *>(&sk[buf][k_chunk(k, fc) * 8]) = kr[i];
-        *reinterpret_cast<u32x4 *>(&sv[buf][k * DH + fc * 8]) = vr[i];
+        *reinterpret_cast<u32x4 *>(&sv[buf][v_chunk(k, fc) * 8]) = vr[i];
       }
     };
     fetch(b0);
@@ -471,11 +496,12 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
           for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
 #pragma unroll
           for (int d = 0; d < DH / 16; ++d) {
-            const Frag16 kf = load16(&sk[buf][k_chunk(32 * t + r, 2 * d + h) * 8]);
+            const Frag16 kf = load16(sk[buf] + ka[d] + 32 * t * DH);
             s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.h, qf[d].h, s[t], 0, 0, 0);
           }
         }
-        if (j0 + TKEYS > first_lim || lv != (1u << TKEYS / 16) - 1) {
+        if (j0 + TKEYS > first_lim || lv != kAllLive) {
+          __builtin_amdgcn_sched_barrier(0);  // (keeps the branch: 100 instructions that few blocks need)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -505,12 +531,13 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
         Frag16 pf[4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          float p[16];
+          float p[16], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             p[i] = exp2_(fmaf(s[t][i], scale, -base));
-            l += p[i];
+            sum[i & 3] += p[i];
           }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             pf[2 * t].u[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
@@ -519,24 +546,12 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {  // sixteen keys
-          uint32_t v[8][E / 2];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint16_t *p = &sv[buf][(16 * g + 8 * (e >> 2) + 4 * h + (e & 3)) * DH + r * E];
-            if constexpr (DH == 128) {
-              const uint2 f = *reinterpret_cast<const uint2 *>(p);
-              v[e][0] = f.x;
-              v[e][1] = f.y;
-            } else {
-              v[e][0] = *reinterpret_cast<const uint32_t *>(p);
-            }
-          }
 #pragma unroll
           for (int e = 0; e < E; ++e) {
+            // four keys of sixteen entries a 16-lane group and read: lane r gets entry 32 e + r
+            const uint2 lo = read_tr(sv[buf] + va[e] + 16 * g * DH), hi = read_tr(sv[buf] + va[e] + (16 * g + 8) * DH);
             Frag16 vf;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              vf.u[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+            vf.u = u32x4{lo.x, lo.y, hi.x, hi.y};
             o[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.h, pf[g].h, o[e], 0, 0, 0);
           }
         }
@@ -553,27 +568,27 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     if (jr < rows) {
       const int head = c.head * sp.G + row - tok * sp.G;
       const long long token = c.start + tok;
-      // this lane's entries: E at (8 j + 4 h + i) E
+      // this lane's entries: 32 e + 8 j + 4 h + i
       if (!dense && starts && ends) {
         const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-        uint16_t *to = a.out + token * a.o_stride + head * DH + 4 * h * E;
+        uint16_t *to = a.out + token * a.o_stride + head * DH + 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          uint16_t *t = to + (8 * (i >> 2) + (i & 3)) * E;
-          if constexpr (DH == 128)
-            *reinterpret_cast<uint2 *>(t) = make_uint2(cvt_pk_bf16(o[0][i] * inv, o[1][i] * inv), cvt_pk_bf16(o[2][i] * inv, o[3][i] * inv));
-          else
-            *reinterpret_cast<uint32_t *>(t) = cvt_pk_bf16(o[0][i] * inv, o[1][i] * inv);
-        }
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint2 *>(to + 32 * e + 8 * j) =
+                make_uint2(cvt_pk_bf16(o[e][4 * j] * inv, o[e][4 * j + 1] * inv),
+                           cvt_pk_bf16(o[e][4 * j + 2] * inv, o[e][4 * j + 3] * inv));
       } else {
         PartRow<DH> *to = !starts ? parts.later + (long long)w * TROWS + jr
                           : dense ? parts.first + token * (sp.G * sp.Hkv) + head
                                   : parts.first + (long long)w * TROWS + jr;
-        float *t = to->o + 4 * h * E;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int e = 0; e < E; ++e) t[(8 * (i >> 2) + (i & 3)) * E + e] = o[e][i];
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f32x4 *>(to->o + 32 * e + 8 * j + 4 * h) =
+                f32x4{o[e][4 * j], o[e][4 * j + 1], o[e][4 * j + 2], o[e][4 * j + 3]};
         if (h == 0) {
           to->m = m;
           to->l = l;
