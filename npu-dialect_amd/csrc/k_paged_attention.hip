@@ -101,15 +101,17 @@ __device__ __forceinline__ void load_block(KeyBlock<DH> &b, const uint16_t *k0, 
   }
 }
 
-// A workgroup's share of the units, [u0, u1) of U, and the group its first lies
-// in; false: none (the launch has more workgroups than units).  Each lane sums
-// the units of some sequences, a scan over the lanes finds the one that holds u0.
+// A workgroup's number w in the division, its share of the units, [u0, u1) of U,
+// and the group its first lies in; false: none (the launch has more workgroups
+// than units).  Each lane sums the units of some sequences, a scan over the lanes
+// finds the one that holds u0.  by_xcd: workgroups that the dispatcher puts on one
+// XCD (every eighth) take neighbouring shares, whose tiles read the same keys.
 struct Share {
   long long sum[NT];
   UnitCursor cur;
 };
 __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long long &U, int &W, long long &u0,
-                                           long long &u1, UnitCursor &c) {
+                                           long long &u1, UnitCursor &c, int &w, bool by_xcd) {
   const int tid = threadIdx.x;
   const int seqs = split_seqs(sp), per = (seqs + NT - 1) / NT;
   long long mine = 0;
@@ -124,9 +126,11 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
   }
   U = s.sum[NT - 1];
   W = split_workgroups(U, gridDim.x);
-  if ((int)blockIdx.x >= W) return false;
-  u0 = first_unit(U, W, blockIdx.x);
-  u1 = first_unit(U, W, blockIdx.x + 1);
+  w = blockIdx.x;
+  if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
+  if (w >= W) return false;
+  u0 = first_unit(U, W, w);
+  u1 = first_unit(U, W, w + 1);
   const long long before = s.sum[tid] - mine;
   if (u0 >= before && u0 < s.sum[tid]) s.cur = seek_unit(sp, tid * per, before, u0);
   __syncthreads();
@@ -155,14 +159,13 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
   __shared__ __attribute__((aligned(16))) float s_o[4][ROWS][DH + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int w = blockIdx.x;
-
   zero_spare_rows<DH>(a, sp);
-  if (!dense && tid == 0) parts.info[w].rows = 0;
   long long U, u0, u1;
   UnitCursor c;
-  int W;
-  if (!take_share(sp, share, U, W, u0, u1, c)) return;
+  int W, w;
+  const bool some = take_share(sp, share, U, W, u0, u1, c, w, false);
+  if (!dense && tid == 0) parts.info[w].rows = 0;
+  if (!some) return;
 
   const float scale = a.scale * 1.44269504088896340736f;  // exponentials in base 2
   for (long long u = u0; u < u1;) {
@@ -374,13 +377,13 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   __shared__ Share share;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int w = blockIdx.x;
   zero_spare_rows<DH>(a, sp);
-  if (!dense && tid == 0) parts.info[w].rows = 0;
   long long U, u0, u1;
   UnitCursor c;
-  int W;
-  if (!take_share(sp, share, U, W, u0, u1, c)) return;
+  int W, w;
+  const bool some = take_share(sp, share, U, W, u0, u1, c, w, true);
+  if (!dense && tid == 0) parts.info[w].rows = 0;
+  if (!some) return;
 
   const float scale = a.scale * 1.44269504088896340736f;
   // where key `k` of a block keeps its chunk `ch`
