@@ -101,40 +101,100 @@ __device__ __forceinline__ void load_block(KeyBlock<DH> &b, const uint16_t *k0, 
   }
 }
 
+// Inclusive sum over the lanes of a wave.
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  const int lane = threadIdx.x & 63;
+  for (int off = 1; off < 64; off <<= 1) {
+    const T u = __shfl_up(v, off);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+
 // A workgroup's number w in the division, its share of the units, [u0, u1) of U,
 // and the group its first lies in; false: none (the launch has more workgroups
-// than units).  Each lane sums the units of some sequences, a scan over the lanes
-// finds the one that holds u0.  by_xcd: workgroups that the dispatcher puts on one
-// XCD (every eighth) take neighbouring shares, whose tiles read the same keys.
+// than units).  by_xcd: workgroups that the dispatcher puts on one XCD (every
+// eighth) take neighbouring shares, whose tiles read the same keys.
+// Every workgroup finds its own: the units of each sequence (by a lane each or,
+// where they have many tiles, by a wave each), a scan over the lanes, and in the
+// sequence that holds u0 a scan over its tiles.
 struct Share {
-  long long sum[NT];
-  UnitCursor cur;
+  long long sum[NT], wave[NT / 64];
+  long long base, per;  // of the sequence: its first unit, the units of a key head
+  int seq;
 };
 __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long long &U, int &W, long long &u0,
                                            long long &u1, UnitCursor &c, int &w, bool by_xcd) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int seqs = split_seqs(sp), per = (seqs + NT - 1) / NT;
   long long mine = 0;
-  for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) mine += seq_units(sp, i);
-  s.sum[tid] = mine;
-  __syncthreads();
-  for (int off = 1; off < NT; off <<= 1) {
-    const long long v = tid >= off ? s.sum[tid - off] : 0;
+  if (seqs <= NT && (unsigned)sp.b.T * sp.G / (unsigned)sp.rows >= 16u * seqs) {
+    for (int q = wave; q < seqs; q += NT / 64) {
+      const int n = split_span(sp, q).n, tiles = split_tiles(sp, n);
+      long long sum = 0;
+      for (int t = lane; t < tiles; t += 64) sum += tile_blocks(sp, q, n, t);
+      sum = wave_scan(sum);
+      if (lane == 63) s.sum[q] = sum * sp.Hkv;
+    }
     __syncthreads();
-    s.sum[tid] += v;
-    __syncthreads();
+    if (tid < seqs) mine = s.sum[tid];
+  } else {
+    for (int q = tid * per; q < min(seqs, (tid + 1) * per); ++q) mine += seq_units(sp, q);
   }
-  U = s.sum[NT - 1];
+  const long long in_wave = wave_scan(mine);
+  if (lane == 63) s.wave[wave] = in_wave;
+  __syncthreads();
+  long long before = in_wave - mine;
+  U = 0;
+  for (int v = 0; v < NT / 64; ++v) {
+    if (v < wave) before += s.wave[v];
+    U += s.wave[v];
+  }
+  U = (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(U >> 32)) << 32 |
+                  (unsigned)__builtin_amdgcn_readfirstlane((int)U));
   W = split_workgroups(U, gridDim.x);
   w = blockIdx.x;
   if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
   if (w >= W) return false;
   u0 = first_unit(U, W, w);
   u1 = first_unit(U, W, w + 1);
-  const long long before = s.sum[tid] - mine;
-  if (u0 >= before && u0 < s.sum[tid]) s.cur = seek_unit(sp, tid * per, before, u0);
+  if (u0 >= before && u0 < before + mine) {  // one lane's sequences hold u0
+    int q = tid * per;
+    long long units = mine;
+    for (; per > 1; ++q) {
+      units = seq_units(sp, q);
+      if (u0 < before + units) break;
+      before += units;
+    }
+    s.seq = q;
+    s.base = before;
+    s.per = units / sp.Hkv;
+  }
   __syncthreads();
-  c = s.cur;
+  c.seq = __builtin_amdgcn_readfirstlane(s.seq);
+  const SeqSpan span = split_span(sp, c.seq);
+  c.n = span.n;
+  c.start = span.start;
+  c.head = __builtin_amdgcn_readfirstlane((int)((u0 - s.base) / s.per));
+  c.base = s.base + c.head * s.per;
+  int rest = (int)min(u0 - c.base, (long long)0x7fffffff);  // units before u0 in the tiles from c.tile on
+  for (c.tile = 0;; c.tile += 64) {
+    const int tiles = split_tiles(sp, c.n);
+    const int nb = c.tile + lane < tiles ? tile_blocks(sp, c.seq, c.n, c.tile + lane) : 0;
+    const int up_to = wave_scan(nb), all = __builtin_amdgcn_readlane(up_to, 63);
+    if (rest < all) {
+      const int at = __builtin_ctzll(__ballot(up_to > rest));
+      c.tile += at;
+      c.nb = __builtin_amdgcn_readlane(nb, at);
+      const int skipped = __builtin_amdgcn_readlane(up_to, at) - c.nb;
+      c.base += skipped;
+      c.blk = rest - skipped;
+      break;
+    }
+    c.base += all;
+    rest -= all;
+  }
   return true;
 }
 
@@ -358,7 +418,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
 //  - The running maximum is only a reference: it is raised, and the sums scaled,
 //    when a row's maximum passes it by more than 2^8 (a uniform branch), so that
 //    p <= 2^8 and most blocks scale nothing.
-constexpr int TROWS = 128, TKEYS = 64;
+constexpr int TROWS = 128, TKEYS = 64;  // sixteen keys a wave fetches
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -371,9 +431,10 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
                                                                      Parts<DH> parts) {
   constexpr int CH = DH / 8;             // 16-byte chunks of a key
   constexpr int NL = TKEYS * CH / NT;    // chunks a lane fetches, of K and of V
-  constexpr int KPL = NT / CH;           // keys that one fetch of all lanes covers
+  constexpr int KPL = 64 / CH;           // keys that one load of a wave covers
   constexpr int E = DH / 32;             // MFMAs of the second product a k step
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][TKEYS * DH], sv[2][TKEYS * DH];
+  __shared__ __attribute__((aligned(16))) int s_live[2][TKEYS / 16];  // whether a buffer's sixteen keys have a page
   __shared__ Share share;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
@@ -390,7 +451,6 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   auto k_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? k & 15 : (k >> 1) & 7)); };
   // the same of V: 64-byte runs exchanged, which a transposing read takes whole
   auto v_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? (k & 3) << 2 : (k & 2) << 1)); };
-  constexpr uint32_t kAllLive = (1u << TKEYS / 16) - 1;
   // this lane's operand addresses in a buffer: K's chunks of key r, V's runs
   int ka[DH / 16], va[E];
 #pragma unroll
@@ -398,7 +458,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
 #pragma unroll
   for (int e = 0; e < E; ++e)
     va[e] = v_chunk(4 * h + (lane >> 2 & 3), 4 * e + (r >> 4) * 2 + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
-  const int fk = tid / CH, fc = tid % CH;  // the key and chunk this lane fetches
+  const int fk = lane / CH, fc = lane % CH;  // the key and chunk of this lane in a load of its wave
 
   for (long long u = u0; u < u1;) {
     const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
@@ -427,90 +487,87 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
       for (int i = 0; i < 16; ++i) o[e][i] = 0.f;
     float m = -__builtin_inff(), l = 0.f;  // l: this lane's keys only
 
+    // A wave fetches sixteen keys of a block, which lie in one page; the page's
+    // number is read a block ahead of its keys.
     u32x4 kr[NL], vr[NL];
-    // of the block in kr, vr: bit g, whether its keys 16 g .. have a page; its
-    // keys that a row of the tile may see
-    uint32_t live = 0;
-    int seen = 0;
+    int page = -1, seen = 0;  // of the block to be fetched next; of the one in vr
+    bool live = false;
+    auto find = [&](int blk) __attribute__((always_inline)) {
+      const bool pre = blk < sp.pre_blocks;
+      const int j = (pre ? blk : blk - sp.pre_blocks) * TKEYS + 16 * wave;
+      page = -1;
+      if (j < (pre ? sp.b.prefix_len : tile_lim)) page = (pre ? a.prefix_table : table)[j >> sp.b.page_log2];
+    };
     auto fetch = [&](int blk) __attribute__((always_inline)) {
       const bool pre = blk < sp.pre_blocks;
-      const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS, all = pre ? sp.b.prefix_len : tile_lim;
-      const int *t = pre ? a.prefix_table : table;
-      int page[TKEYS / 16];
-      live = 0;
-#pragma unroll
-      for (int g = 0; g < TKEYS / 16; ++g) {
-        const int j = j0 + 16 * g;
-        int pg = -1;
-        if (j < all) pg = checked_page(t[j >> sp.b.page_log2], sp.b.n_pages);
-        pg = __builtin_amdgcn_readfirstlane(pg);
-        live |= (pg >= 0 ? 1u : 0u) << g;
-        page[g] = max(pg, 0);
-      }
+      const int j = (pre ? blk : blk - sp.pre_blocks) * TKEYS + 16 * wave;
+      const int pg = __builtin_amdgcn_readfirstlane(checked_page(page, sp.b.n_pages));
+      live = pg >= 0;
+      seen = live ? (pre ? sp.b.prefix_len : tile_lim) - j : 0;
+      const int in = (j & ((1 << sp.b.page_log2) - 1)) * DH;
+      const uint16_t *kp = kh + max(pg, 0) * a.kpage_stride + in, *vp = vh + max(pg, 0) * a.vpage_stride + in;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        // the sixteen keys this wave's lanes fetch from
-        const int g = KPL == 16 ? i : 2 * i + (wave >> 1);
-        const int pg = KPL == 16 ? page[i] : wave >> 1 ? page[2 * i + 1] : page[2 * i];
-        const int j = j0 + 16 * g, in = ((j & ((1 << sp.b.page_log2) - 1)) + (fk & 15)) * DH + fc * 8;
-        kr[i] = *reinterpret_cast<const u32x4 *>(kh + pg * a.kpage_stride + in);
-        vr[i] = *reinterpret_cast<const u32x4 *>(vh + pg * a.vpage_stride + in);
+        kr[i] = *reinterpret_cast<const u32x4 *>(kp + i * 512 + lane * 8);
+        vr[i] = *reinterpret_cast<const u32x4 *>(vp + i * 512 + lane * 8);
       }
-      seen = all - j0;
     };
     auto commit = [&](int buf) __attribute__((always_inline)) {
-      if (seen < TKEYS || live != kAllLive) {  // values that no row may see must not meet p = 0
-        __builtin_amdgcn_sched_barrier(0);     // (keeps the branch)
+      if (lane == 0) s_live[buf][wave] = live;
+      if (seen < 16) {  // values that no row may see must not meet p = 0
+        __builtin_amdgcn_sched_barrier(0);  // (keeps the branch)
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int k = i * KPL + fk;
-          vr[i] = masked(vr[i], k < seen && (live >> (k >> 4) & 1));
-        }
+        for (int i = 0; i < NL; ++i) vr[i] = masked(vr[i], i * KPL + fk < seen);
       }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int k = i * KPL + fk;
+        const int k = 16 * wave + i * KPL + fk;
         *reinterpret_cast<u32x4 *>(&sk[buf][k_chunk(k, fc) * 8]) = kr[i];
         *reinterpret_cast<u32x4 *>(&sv[buf][v_chunk(k, fc) * 8]) = vr[i];
       }
     };
+    find(b0);
     fetch(b0);
+    if (b0 + 1 < b1) find(b0 + 1);
     commit(0);
-    uint32_t here = live;
     if (b0 + 1 < b1) fetch(b0 + 1);
+    if (b0 + 2 < b1) find(b0 + 2);
     __syncthreads();
     for (int blk = b0; blk < b1; ++blk) {
       const int buf = (blk - b0) & 1;
-      const uint32_t lv = here;
       if (blk + 1 < b1) {
         commit(buf ^ 1);
-        here = live;
         if (blk + 2 < b1) fetch(blk + 2);
+        if (blk + 3 < b1) find(blk + 3);
       }
+      const int4 lv = *reinterpret_cast<const int4 *>(s_live[buf]);
       const bool pre = blk < sp.pre_blocks;
       const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS;
       const int my_lim = pre ? sp.b.prefix_len : lim;
       const int first_lim = pre ? sp.b.prefix_len : lim_first, last_lim = pre ? sp.b.prefix_len : lim_last;
       if (busy && j0 < last_lim) {
+        const bool all_live = __builtin_amdgcn_readfirstlane(lv.x & lv.y & lv.z & lv.w);
         f32x16 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
 #pragma unroll
-          for (int d = 0; d < DH / 16; ++d) {
+        for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
             const Frag16 kf = load16(sk[buf] + ka[d] + 32 * t * DH);
             s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.h, qf[d].h, s[t], 0, 0, 0);
           }
-        }
-        if (j0 + TKEYS > first_lim || lv != kAllLive) {
+        if (j0 + TKEYS > first_lim || !all_live) {
           __builtin_amdgcn_sched_barrier(0);  // (keeps the branch: 100 instructions that few blocks need)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int k = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-              if (j0 + k >= my_lim || !(lv >> (k >> 4) & 1)) s[t][i] = -__builtin_inff();
+              const int has = (k >> 4) == 0 ? lv.x : (k >> 4) == 1 ? lv.y : (k >> 4) == 2 ? lv.z : lv.w;
+              if (j0 + k >= my_lim || !has) s[t][i] = -__builtin_inff();
             }
         }
         float top = -__builtin_inff();
@@ -745,7 +802,7 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
   // the own keys' part or, stacked, the prefix's
   auto attend = [&](bool tiles, bool stacked, int dense, const Parts<DH> &parts) {
     const int keys = tiles ? TKEYS : KEYS, pre_blocks = (a.b.prefix_len + keys - 1) / keys;
-    const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, keys, d.stacked && !stacked ? 0 : pre_blocks, stacked};
+    const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, tiles ? 6 : 7, d.stacked && !stacked ? 0 : pre_blocks, stacked};
     auto kern = tiles ? paged_attention_tile_kernel<DH> : paged_attention_kernel<DH>;
     static const char *const names[2][2] = {{"llama_paged_attention", "llama_paged_attention_tiles"},
                                             {"llama_paged_attention_prefix", "llama_paged_attention_prefix_tiles"}};

@@ -72,7 +72,7 @@ NPU_HD Place place_of_token(const ServeBatch &b, int t) {
 // head stand together, so the rows of a sequence's key head are numbered
 // token * G + g and cut into tiles of `rows`.  A tile's keys, the prefix's
 // `pre_blocks` blocks and its own up to what its last token sees, are cut into
-// blocks of `keys`; a (tile, key head)'s blocks are a group of units, one at
+// blocks of 2^keys_log2; a (tile, key head)'s blocks are a group of units, one at
 // least, so that rows without keys are written too.  Units are numbered by
 // sequence, key head, tile, block (tiles that stand together read the same keys); workgroup w of W takes the units
 // [U w / W, U (w + 1) / W): equal shares whatever the lengths, a group cut at
@@ -82,7 +82,7 @@ NPU_HD Place place_of_token(const ServeBatch &b, int t) {
 struct AttnSplit {
   ServeBatch b;
   int G, Hkv;
-  int rows, keys;
+  int rows, keys_log2;
   int pre_blocks;  // prefix blocks before each tile's own keys
   int stacked;     // the prefix alone: the rows of all tokens as one sequence
 };
@@ -98,11 +98,14 @@ NPU_HD int visible_keys(const AttnSplit &a, int seq, int n, int i) {
   return clamp_int((long long)a.b.kv_len[seq] - n + i + 1, 0,
                    clamp_int(a.b.kv_len[seq], 0, (int)cap));
 }
-NPU_HD int split_tiles(const AttnSplit &a, int n) { return (int)(((long long)n * a.G + a.rows - 1) / a.rows); }
+NPU_HD int split_tiles(const AttnSplit &a, int n) {
+  return (int)(((unsigned)n * (unsigned)a.G + (unsigned)a.rows - 1) / (unsigned)a.rows);
+}
 NPU_HD int tile_blocks(const AttnSplit &a, int seq, int n, int tile) {
-  const long long last = (((long long)tile + 1) * a.rows - 1) / a.G;
-  const int v = visible_keys(a, seq, n, last < n ? (int)last : n - 1);
-  const int nb = a.pre_blocks + (int)(((long long)v + a.keys - 1) / a.keys);
+  // (n G < 2^31, and a tile is at most 128 rows)
+  const unsigned last = (((unsigned)tile + 1) * (unsigned)a.rows - 1) / (unsigned)a.G;
+  const int v = visible_keys(a, seq, n, last < (unsigned)n ? (int)last : n - 1);
+  const int nb = a.pre_blocks + (int)(((unsigned)v + (1u << a.keys_log2) - 1) >> a.keys_log2);
   return nb > 0 ? nb : 1;
 }
 // Units of one key head of a sequence of n new tokens.

@@ -32,7 +32,7 @@ void serve_places(const HostBatch *h, int *out) {
 
 int serve_visible(const HostBatch *h, int seq, int i) {
   const ServeBatch b = batch(h);
-  const AttnSplit a{b, 1, 1, 16, 128, 0, 0};
+  const AttnSplit a{b, 1, 1, 16, 7, 0, 0};
   return visible_keys(a, seq, seq_span(b, seq).n, i);
 }
 
@@ -42,7 +42,7 @@ int serve_visible(const HostBatch *h, int seq, int i) {
 // differs from the one reached by walking, or the owners disagree.
 long long serve_segments(const HostBatch *h, int G, int Hkv, int rows, int keys, int pre_blocks, int stacked,
                          int launched, int *out, long long most) {
-  const AttnSplit a{batch(h), G, Hkv, rows, keys, pre_blocks, stacked};
+  const AttnSplit a{batch(h), G, Hkv, rows, __builtin_ctz(keys), pre_blocks, stacked};
   long long U = 0, n = 0;
   for (int s = 0; s < split_seqs(a); ++s) U += seq_units(a, s);
   const int W = split_workgroups(U, launched);
