@@ -210,29 +210,22 @@ __device__ __forceinline__ void zero_spare_rows(const PagedAttentionArgs &a, con
   }
 }
 
-template <int DH>
-__global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
-                                                                Parts<DH> parts) {
-  constexpr int E = DH / 16;  // entries of a lane's output run, MFMAs of the second product
-  __shared__ Share share;
-  __shared__ float s_m[4][ROWS], s_l[4][ROWS];
-  __shared__ __attribute__((aligned(16))) float s_o[4][ROWS][DH + 4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, q = lane >> 4;
-  zero_spare_rows<DH>(a, sp);
-  long long U, u0, u1;
-  UnitCursor c;
-  int W, w;
-  const bool some = take_share(sp, share, U, W, u0, u1, c, w, false);
-  if (!dense && tid == 0) parts.info[w].rows = 0;
-  if (!some) return;
+// The rows of one tile over the key blocks [b0, b1) of their group, 32 keys of
+// each block a wave: this wave's sums o, maximum m (base 2) and, by lane, l.
+template <int DH, int NW>
+struct TileWalk {
+  static constexpr int E = DH / 16;  // MFMAs of the second product, entries of a lane's output run
+  f32x4 o[E];
+  float m, l;
 
-  const float scale = a.scale * 1.44269504088896340736f;  // exponentials in base 2
-  for (long long u = u0; u < u1;) {
-    const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
+  __device__ __forceinline__ void run(const PagedAttentionArgs &a, const AttnSplit &sp, const UnitCursor &c, int b0,
+                                      int b1) {
+    constexpr int BLOCK = 32 * NW;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    const float scale = a.scale * 1.44269504088896340736f;  // exponentials in base 2
     const int row0 = c.tile * ROWS, rows = min(ROWS, c.n * sp.G - row0);
-    // the tile's queries: row `r` of this lane
-    const int row = row0 + min(r, rows - 1), tok = row / sp.G;
+    const int row = row0 + min(r, rows - 1), tok = row / sp.G;  // this lane's query
     Frag16 qf[DH / 32];
     {
       const uint16_t *p = a.Q + (long long)(c.start + tok) * a.q_stride + (c.head * sp.G + row - tok * sp.G) * DH + q * 8;
@@ -245,46 +238,55 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
     const uint16_t *kh = a.k_pages + ((long long)c.head << sp.b.page_log2) * DH;
     const uint16_t *vh = a.v_pages + ((long long)c.head << sp.b.page_log2) * DH;
 
-    f32x4 o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -__builtin_inff(), l = 0.f;
+    m = -__builtin_inff();
+    l = 0.f;
 
-    // Block blk of the group: its keys' places, the limit of this lane's row and
-    // of the whole tile, and the loads of this wave's 32 keys.
+    // A block's first key of this wave, the keys that this lane's row sees and any
+    // row of the tile, whether each half has a page.
     struct Where {
       int j, lim, all;
       bool live[2];
     };
     KeyBlock<DH> kb;
-    auto fetch = [&](int blk, KeyBlock<DH> &to) {
+    int page[2];  // of the block to be fetched next, read a block ahead of its keys
+    auto find = [&](int blk) __attribute__((always_inline)) {
+      const bool pre = blk < sp.pre_blocks;
+      const int *t = pre ? a.prefix_table : table;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = (pre ? blk : blk - sp.pre_blocks) * BLOCK + wave * 32 + 16 * h;
+        page[h] = -1;
+        if (j < (pre ? sp.b.prefix_len : tile_lim)) page[h] = t[j >> sp.b.page_log2];
+      }
+    };
+    auto fetch = [&](int blk) __attribute__((always_inline)) {
       Where x;
       const bool pre = blk < sp.pre_blocks;
-      x.j = (pre ? blk : blk - sp.pre_blocks) * KEYS + wave * 32;
+      x.j = (pre ? blk : blk - sp.pre_blocks) * BLOCK + wave * 32;
       x.lim = pre ? sp.b.prefix_len : lim;
       x.all = pre ? sp.b.prefix_len : tile_lim;
-      const int *t = pre ? a.prefix_table : table;
       const uint16_t *kp[2], *vp[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int j = x.j + 16 * h;
-        int page = -1;
-        if (j < x.all) page = checked_page(t[j >> sp.b.page_log2], sp.b.n_pages);
-        page = __builtin_amdgcn_readfirstlane(page);
-        x.live[h] = page >= 0;
-        const long long pg = max(page, 0);
-        const int in = (j & ((1 << sp.b.page_log2) - 1)) * DH;
-        kp[h] = kh + pg * a.kpage_stride + in;
-        vp[h] = vh + pg * a.vpage_stride + in;
+        const int pg = __builtin_amdgcn_readfirstlane(checked_page(page[h], sp.b.n_pages));
+        x.live[h] = pg >= 0;
+        const int in = ((x.j + 16 * h) & ((1 << sp.b.page_log2) - 1)) * DH;
+        kp[h] = kh + max(pg, 0) * a.kpage_stride + in;
+        vp[h] = vh + max(pg, 0) * a.vpage_stride + in;
       }
-      load_block<DH>(to, kp[0], kp[1], vp[0], vp[1], lane);
+      load_block<DH>(kb, kp[0], kp[1], vp[0], vp[1], lane);
       return x;
     };
-    Where at = fetch(b0, kb);
+    find(b0);
+    Where at = fetch(b0);
+    if (b0 + 1 < b1) find(b0 + 1);
     for (int blk = b0; blk < b1; ++blk) {
       KeyBlock<DH> cur = kb;
       const Where x = at;
-      if (blk + 1 < b1) at = fetch(blk + 1, kb);
+      if (blk + 1 < b1) at = fetch(blk + 1);
+      if (blk + 2 < b1) find(blk + 2);
       if (!x.live[0] && !x.live[1]) continue;
       // logits in base 2, keys x.j + 16 h + 4 q + i of row r
       f32x4 s[2];
@@ -340,47 +342,96 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
         MfmaBF16::mma(o[e], vf, pf);
       }
     }
+    l = sum_of_rows(l);
+  }
 
-    // join the four waves' sums
-    LanePair l16 = lane_pair16(l);
-    l = l16.lo + l16.hi;
-    LanePair l32 = lane_pair32(l);
-    l = l32.lo + l32.hi;
+  // over the wave's four 16-lane rows
+  static __device__ __forceinline__ float sum_of_rows(float v) {
+    const LanePair a = lane_pair16(v);
+    const LanePair b = lane_pair32(a.lo + a.hi);
+    return b.lo + b.hi;
+  }
+};
+
+// The waves' sums in LDS, one slot each, and their join.
+template <int DH, int SLOTS>
+struct WaveSums {
+  float m[SLOTS][ROWS], l[SLOTS][ROWS];
+  __attribute__((aligned(16))) float o[SLOTS][ROWS][DH + 4];
+
+  template <int NW>
+  __device__ __forceinline__ void put(int slot, const TileWalk<DH, NW> &t) {
+    constexpr int E = DH / 16;
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     if (q == 0) {
-      s_m[wave][r] = m;
-      s_l[wave][r] = l;
+      m[slot][r] = t.m;
+      l[slot][r] = t.l;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < E; e += 4)
-        *reinterpret_cast<f32x4 *>(&s_o[wave][r][(q * 4 + i) * E + e]) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+        *reinterpret_cast<f32x4 *>(&o[slot][r][(q * 4 + i) * E + e]) =
+            f32x4{t.o[e][i], t.o[e + 1][i], t.o[e + 2][i], t.o[e + 3][i]};
+  }
+  // entries 8 jc .. of row jr over the first n slots
+  __device__ __forceinline__ void join(int n, int jr, int jc, float &mm, float &ll, float (&acc)[8]) const {
+    mm = -__builtin_inff();
+    ll = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int v = 0; v < n; ++v) mm = fmaxf(mm, m[v][jr]);
+    const float base = mm == -__builtin_inff() ? 0.f : mm;
+    for (int v = 0; v < n; ++v) {
+      const float f = exp2_(m[v][jr] - base);
+      ll += f * l[v][jr];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += f * o[v][jr][jc * 8 + e];
+    }
+  }
+};
+
+// o / l as a row's eight entries; no key: 0.
+__device__ __forceinline__ void store_row8(uint16_t *to, const float (&acc)[8], float l) {
+  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+  u32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = cvt_pk_bf16(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  *reinterpret_cast<u32x4 *>(to) = v;
+}
+
+template <int DH>
+__global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
+                                                                Parts<DH> parts) {
+  __shared__ Share share;
+  __shared__ WaveSums<DH, 4> sums;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  zero_spare_rows<DH>(a, sp);
+  long long U, u0, u1;
+  UnitCursor c;
+  int W, w;
+  const bool some = take_share(sp, share, U, W, u0, u1, c, w, false);
+  if (!dense && tid == 0) parts.info[w].rows = 0;
+  if (!some) return;
+
+  for (long long u = u0; u < u1;) {
+    const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
+    const int row0 = c.tile * ROWS, rows = min(ROWS, c.n * sp.G - row0);
+    TileWalk<DH, 4> t;
+    t.run(a, sp, c, b0, b1);
+    sums.put(wave, t);
     __syncthreads();
     const bool starts = b0 == 0, ends = b1 == c.nb;
     const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
     if (!dense && starts && !ends && tid == 0) parts.info[w] = PartInfo{rows, c.start, row0, c.head, more, {0, 0, 0}};
-    // lane (jr, jc): entries 8 jc .. of row jr
     for (int i = tid; i < rows * (DH / 8); i += NT) {
       const int jr = i / (DH / 8), jc = i % (DH / 8);
-      float mm = -__builtin_inff(), ll = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int v = 0; v < 4; ++v) mm = fmaxf(mm, s_m[v][jr]);
-      const float base = mm == -__builtin_inff() ? 0.f : mm;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float f = exp2_(s_m[v][jr] - base);
-        ll += f * s_l[v][jr];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += f * s_o[v][jr][jc * 8 + e];
-      }
+      float mm, ll, acc[8];
+      sums.join(4, jr, jc, mm, ll, acc);
       const int orow = row0 + jr, ot = orow / sp.G, head = c.head * sp.G + orow - ot * sp.G;
       const long long token = c.start + ot;
       if (!dense && starts && ends) {
-        const float inv = ll > 0.f ? 1.0f / ll : ll == 0.f ? 0.f : ll;
-        u32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = cvt_pk_bf16(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-        *reinterpret_cast<u32x4 *>(a.out + token * a.o_stride + head * DH + jc * 8) = v;
+        store_row8(a.out + token * a.o_stride + head * DH + jc * 8, acc, ll);
       } else {
         PartRow<DH> *to = !starts ? parts.later + w * ROWS + jr
                           : dense ? parts.first + token * (sp.G * sp.Hkv) + head
@@ -398,6 +449,52 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
     u += b1 - b0;
     if (u < u1) next_group(sp, c);
     __syncthreads();
+  }
+}
+
+// Short histories, one token a sequence: a workgroup takes a whole group, so that
+// nothing is left to join, but for the parts of a shared prefix (pre, `pre_rows` to
+// a slot), which it takes in itself.
+template <int DH, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(PagedAttentionArgs a, AttnSplit sp, int tiles,
+                                                                           int W, Parts<DH> pre, int pre_rows) {
+  constexpr int N = 64 * NW;
+  __shared__ WaveSums<DH, NW> sums;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = blockIdx.x / tiles;
+  UnitCursor c{group / sp.Hkv, (int)blockIdx.x % tiles, group % sp.Hkv, 0, 0, 1, group / sp.Hkv, 0};
+  const int row0 = c.tile * ROWS, rows = min(ROWS, sp.G - row0);
+  const int nb = tile_blocks(sp, c.seq, 1, c.tile);
+  TileWalk<DH, NW> t;
+  t.run(a, sp, c, 0, nb);
+  sums.put(wave, t);
+  __syncthreads();
+  for (int i = tid; i < rows * (DH / 8); i += N) {
+    const int jr = i / (DH / 8), jc = i % (DH / 8), head = c.head * sp.G + row0 + jr;
+    float mm, ll, acc[8];
+    sums.join(NW, jr, jc, mm, ll, acc);
+    if (pre.first) {
+      const PartRow<DH> *f = pre.first + (long long)c.start * (sp.G * sp.Hkv) + head;
+      const int first = clamp_int(f->first, 0, W - 1), more = min(f->more & 0xffff, W - 1 - first);
+      const int pr = (f->more >> 16) & (pre_rows - 1);
+      auto part = [&](int n) { return n == 0 ? f : pre.later + (long long)(first + n) * pre_rows + pr; };
+      float top = mm;
+      for (int n = 0; n <= more; ++n) top = fmaxf(top, part(n)->m);
+      const float base = top == -__builtin_inff() ? 0.f : top, own = exp2_(mm - base);
+      ll *= own;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= own;
+#pragma unroll 4
+      for (int n = 0; n <= more; ++n) {
+        const PartRow<DH> *p = part(n);
+        const float g = exp2_(p->m - base);
+        ll += g * p->l;
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(p->o + jc * 8), y = *reinterpret_cast<const f32x4 *>(p->o + jc * 8 + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += g * x[e], acc[4 + e] += g * y[e];
+      }
+    }
+    store_row8(a.out + (long long)c.start * a.o_stride + head * DH + jc * 8, acc, ll);
   }
 }
 
@@ -765,6 +862,7 @@ struct Division {
   int W;          // workgroups of a launch
   bool stacked;   // the prefix once for the rows of all sequences
   bool own_tiles, pre_tiles;  // 128-row tiles for the own keys' part, the prefix's
+  bool whole;     // a workgroup for each group of the own keys' part
 };
 Division divide(const ServeBatch &b, int H, int Hkv) {
   const long long G = H / Hkv, rows = b.T * G;
@@ -775,6 +873,9 @@ Division divide(const ServeBatch &b, int H, int Hkv) {
   d.stacked = b.prefix_len > 0 && b.B > 1 && rows < (long long)b.B * TROWS;
   d.own_tiles = rows >= (long long)b.B * 4 * ROWS;
   d.pre_tiles = rows >= 4 * ROWS;
+  // Up to 1024 keys a group takes no longer than its cut parts and their join.
+  d.whole = !b.q_start && !d.own_tiles &&
+            ((long long)b.max_pages << b.page_log2) + (d.stacked ? 0 : b.prefix_len) <= 1024;
   return d;
 }
 
@@ -810,7 +911,30 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
     hipLaunchKernelGGL(kern, dim3(d.W), dim3(NT), 0, s, a, sp, dense, parts);
   };
   const int own_rows = d.own_tiles ? TROWS : ROWS, pre_rows = d.pre_tiles ? TROWS : ROWS;
-  if (!d.stacked) {
+  const size_t dense = (size_t)a.b.T * a.H * sizeof(PartRow<DH>);
+  auto take = [&](size_t later) {  // a stacked call's regions
+    Parts<DH> p{nullptr, reinterpret_cast<PartRow<DH> *>(ws), reinterpret_cast<PartRow<DH> *>(ws + dense)};
+    ws += dense + later;
+    return p;
+  };
+  Parts<DH> pre{nullptr, nullptr, nullptr};
+  if (d.stacked) {
+    pre = take(slot_bytes<DH>(d, d.pre_tiles));
+    attend(d.pre_tiles, true, 1, pre);
+  }
+  if (d.whole) {
+    const int tiles = (G + ROWS - 1) / ROWS, groups = a.b.B * a.Hkv * tiles;
+    auto launch = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      const int pre_blocks = d.stacked ? 0 : (a.b.prefix_len + 32 * NW - 1) / (32 * NW);
+      const AttnSplit sp{a.b, G, a.Hkv, ROWS, __builtin_ctz(32 * NW), pre_blocks, 0};
+      auto kern = paged_attention_whole_kernel<DH, NW>;
+      plan("llama_paged_attention_whole", groups, wg_per_cu(kern, 64 * NW));
+      hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * NW), 0, s, a, sp, tiles, d.W, pre, pre_rows);
+    };
+    if (groups > device_cus()) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 8>{});
+  } else if (!d.stacked) {
     Parts<DH> parts;
     parts.info = reinterpret_cast<PartInfo *>(ws);
     parts.first = reinterpret_cast<PartRow<DH> *>(ws + d.W * sizeof(PartInfo));
@@ -821,14 +945,7 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
     plan("llama_paged_attention_join", d.W * ((most + per - 1) / per), wg_per_cu(join, NT));
     hipLaunchKernelGGL(join, dim3(d.W, (most + per - 1) / per), dim3(NT), 0, s, a, G, own_rows, parts);
   } else {
-    const size_t dense = (size_t)a.b.T * a.H * sizeof(PartRow<DH>);
-    auto take = [&](size_t later) {
-      Parts<DH> p{nullptr, reinterpret_cast<PartRow<DH> *>(ws), reinterpret_cast<PartRow<DH> *>(ws + dense)};
-      ws += dense + later;
-      return p;
-    };
-    const Parts<DH> own = take(slot_bytes<DH>(d, d.own_tiles)), pre = take(slot_bytes<DH>(d, d.pre_tiles));
-    attend(d.pre_tiles, true, 1, pre);
+    const Parts<DH> own = take(slot_bytes<DH>(d, d.own_tiles));
     attend(d.own_tiles, false, 1, own);
     auto join = paged_attention_join2_kernel<DH, NT * 4 / DH>;
     plan("llama_paged_attention_join", a.b.T * a.H, wg_per_cu(join, NT));

@@ -201,6 +201,17 @@ ATTEND = [
     ([64], [2000], 3, 3, 128, 32, 0, {}),
     ([1] * 90, [i % 7 for i in range(90)], 6, 2, 128, 16, 500, {"ragged": False}),
     ([3] * 30, [3 + i for i in range(30)], 4, 4, 64, 16, 257, {}),
+    # tables that reach past 1024 keys, whatever the lengths: divided over workgroups
+    ([1] * 12, [0, 1, 15, 16, 17, 31, 32, 33, 127, 128, 129, 700], 6, 2, 128, 16, 0, {"ragged": False, "max_pages": 70}),
+    ([1] * 5, [3, 40, 0, 1, 90], 34, 2, 64, 16, 0, {"ragged": False, "max_pages": 70}),
+    ([1] * 300, [(37 * i) % 90 for i in range(300)], 4, 2, 64, 16, 0, {"ragged": False, "max_pages": 70}),
+    ([1] * 6, [0, 1, 100, 30, 0, 3], 8, 2, 128, 16, 1, {"ragged": False, "max_pages": 70}),
+    ([1] * 40, [(13 * i) % 70 for i in range(40)], 8, 2, 64, 32, 333, {"ragged": False, "max_pages": 70}),
+    # and ones that do not: whole groups to a workgroup, of four waves and of eight
+    ([1] * 5, [1024, 1023, 0, 513, 257], 8, 4, 128, 32, 0, {"ragged": False}),
+    ([1] * 70, [(97 * i) % 1025 for i in range(70)], 8, 4, 64, 256, 0, {"ragged": False}),
+    ([1] * 70, [(97 * i) % 1025 for i in range(70)], 12, 4, 128, 32, 700, {"ragged": False}),
+    ([1], [900], 5, 5, 64, 16, 100, {"ragged": False}),
 ]
 
 
@@ -213,13 +224,16 @@ def test_attention(cuda, news, lens, H, Hkv, Dh, page, prefix, kind):
 
 
 @pytest.mark.parametrize("news,H,Hkv,prefix,names", [
-    ([1] * 8, 8, 2, 0, ["", "_join"]), ([1] * 8, 8, 2, 20, ["_prefix", "", "_join"]),
-    ([1] * 16, 8, 2, 20, ["_prefix_tiles", "", "_join"]), ([200], 4, 2, 20, ["_tiles", "_join"]),
+    ([1] * 8, 8, 2, 0, ["_whole"]), ([1] * 8, 8, 2, 20, ["_prefix", "_whole"]),
+    ([1] * 16, 8, 2, 20, ["_prefix_tiles", "_whole"]), ([200], 4, 2, 20, ["_tiles", "_join"]),
+    ([1] * 8, 8, 2, 1025, ["_prefix", "_whole"]), ([1], 8, 2, 1025, ["", "_join"]), ([1, 2], 8, 2, 0, ["", "_join"]),
+    ([1, 2], 8, 2, 20, ["_prefix", "", "_join"]),
     ([40] * 2, 4, 2, 20, ["_prefix_tiles", "_tiles", "_join"]), ([31] * 2, 4, 2, 0, ["", "_join"]),
 ])
 def test_attention_kernels_by_rows(cuda, news, H, Hkv, prefix, names):
-    """Few rows a sequence: the kernel that divides keys over waves; many, or a
-    prefix under many rows of a batch: the one that divides rows."""
+    """Few rows a sequence: the kernel that divides keys over waves, whole groups
+    to a workgroup where histories are short; many rows, or a prefix under many
+    rows of a batch: the kernel that divides rows."""
     from npu_amd import groups
     bt = R.Batch(news, [n + 3 for n in news], Hkv, 64, 16, prefix, ragged=set(news) != {1})
     with groups.collect_plans() as cp:
