@@ -211,7 +211,9 @@ __device__ __forceinline__ void zero_spare_rows(const PagedAttentionArgs &a, con
 }
 
 // The rows of one tile over the key blocks [b0, b1) of their group, 32 keys of
-// each block a wave: this wave's sums o, maximum m (base 2) and, by lane, l.
+// each block a wave: this wave's sums o, maximum m (base 2) and l.  b1 < 0: to the
+// group's last block; then the first block's loads do not wait for kv_len (a block
+// past the end is read from what pages the table names there, and masked).
 template <int DH, int NW>
 struct TileWalk {
   static constexpr int E = DH / 16;  // MFMAs of the second product, entries of a lane's output run
@@ -232,8 +234,11 @@ struct TileWalk {
 #pragma unroll
       for (int d = 0; d < DH / 32; ++d) qf[d] = load16(p + d * 32);
     }
-    const int lim = visible_keys(sp, c.seq, c.n, tok);
-    const int tile_lim = visible_keys(sp, c.seq, c.n, (row0 + rows - 1) / sp.G);
+    int lim = 0, tile_lim = 0;
+    auto limits = [&]() __attribute__((always_inline)) {
+      lim = visible_keys(sp, c.seq, c.n, tok);
+      tile_lim = visible_keys(sp, c.seq, c.n, (row0 + rows - 1) / sp.G);
+    };
     const int *table = sp.b.page_table + (sp.stacked ? 0 : c.seq * sp.b.table_stride);
     const uint16_t *kh = a.k_pages + ((long long)c.head << sp.b.page_log2) * DH;
     const uint16_t *vh = a.v_pages + ((long long)c.head << sp.b.page_log2) * DH;
@@ -246,27 +251,25 @@ struct TileWalk {
     // A block's first key of this wave, the keys that this lane's row sees and any
     // row of the tile, whether each half has a page.
     struct Where {
-      int j, lim, all;
-      bool live[2];
+      int j;
+      bool pre, live[2];
     };
     KeyBlock<DH> kb;
     int page[2];  // of the block to be fetched next, read a block ahead of its keys
-    auto find = [&](int blk) __attribute__((always_inline)) {
+    auto find = [&](int blk, int end) __attribute__((always_inline)) {  // end: own keys
       const bool pre = blk < sp.pre_blocks;
       const int *t = pre ? a.prefix_table : table;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int j = (pre ? blk : blk - sp.pre_blocks) * BLOCK + wave * 32 + 16 * h;
         page[h] = -1;
-        if (j < (pre ? sp.b.prefix_len : tile_lim)) page[h] = t[j >> sp.b.page_log2];
+        if (j < (pre ? sp.b.prefix_len : end)) page[h] = t[j >> sp.b.page_log2];
       }
     };
     auto fetch = [&](int blk) __attribute__((always_inline)) {
       Where x;
-      const bool pre = blk < sp.pre_blocks;
-      x.j = (pre ? blk : blk - sp.pre_blocks) * BLOCK + wave * 32;
-      x.lim = pre ? sp.b.prefix_len : lim;
-      x.all = pre ? sp.b.prefix_len : tile_lim;
+      x.pre = blk < sp.pre_blocks;
+      x.j = (x.pre ? blk : blk - sp.pre_blocks) * BLOCK + wave * 32;
       const uint16_t *kp[2], *vp[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -279,15 +282,25 @@ struct TileWalk {
       load_block<DH>(kb, kp[0], kp[1], vp[0], vp[1], lane);
       return x;
     };
-    find(b0);
-    Where at = fetch(b0);
-    if (b0 + 1 < b1) find(b0 + 1);
+    Where at;
+    if (b1 < 0) {
+      find(b0, sp.b.max_pages << sp.b.page_log2);
+      at = fetch(b0);
+      limits();
+      b1 = tile_blocks(sp, c.seq, c.n, c.tile);
+    } else {
+      limits();
+      find(b0, tile_lim);
+      at = fetch(b0);
+    }
+    if (b0 + 1 < b1) find(b0 + 1, tile_lim);
     for (int blk = b0; blk < b1; ++blk) {
       KeyBlock<DH> cur = kb;
       const Where x = at;
       if (blk + 1 < b1) at = fetch(blk + 1);
-      if (blk + 2 < b1) find(blk + 2);
-      if (!x.live[0] && !x.live[1]) continue;
+      if (blk + 2 < b1) find(blk + 2, tile_lim);
+      const int row_end = x.pre ? sp.b.prefix_len : lim, end = x.pre ? sp.b.prefix_len : tile_lim;
+      if (x.j >= end || (!x.live[0] && !x.live[1])) continue;
       // logits in base 2, keys x.j + 16 h + 4 q + i of row r
       f32x4 s[2];
 #pragma unroll
@@ -302,7 +315,7 @@ struct TileWalk {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float v = s[h][i] * scale;
-          s[h][i] = x.live[h] && x.j + 16 * h + 4 * q + i < x.lim ? v : -__builtin_inff();
+          s[h][i] = x.live[h] && x.j + 16 * h + 4 * q + i < row_end ? v : -__builtin_inff();
           top = fmaxf(top, s[h][i]);
         }
       LanePair t16 = lane_pair16(top);
@@ -323,10 +336,10 @@ struct TileWalk {
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf.u[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
       // values that no row may see: whatever lies there must not meet p = 0
-      if (x.j + 32 > x.all || !x.live[0] || !x.live[1]) {
+      if (x.j + 32 > end || !x.live[0] || !x.live[1]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const bool keep = x.live[e >> 2] && x.j + 16 * (e >> 2) + 4 * q + (e & 3) < x.all;
+          const bool keep = x.live[e >> 2] && x.j + 16 * (e >> 2) + 4 * q + (e & 3) < end;
 #pragma unroll
           for (int i = 0; i < DH / 32; ++i) cur.v[e][i] = keep ? cur.v[e][i] : 0u;
         }
@@ -459,41 +472,46 @@ template <int DH, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(PagedAttentionArgs a, AttnSplit sp, int tiles,
                                                                            int W, Parts<DH> pre, int pre_rows) {
   constexpr int N = 64 * NW;
-  __shared__ WaveSums<DH, NW> sums;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ WaveSums<DH, 2 * NW> sums;  // the waves' sums; theirs of the prefix's parts
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = blockIdx.x / tiles;
   UnitCursor c{group / sp.Hkv, (int)blockIdx.x % tiles, group % sp.Hkv, 0, 0, 1, group / sp.Hkv, 0};
   const int row0 = c.tile * ROWS, rows = min(ROWS, sp.G - row0);
-  const int nb = tile_blocks(sp, c.seq, 1, c.tile);
   TileWalk<DH, NW> t;
-  t.run(a, sp, c, 0, nb);
+  t.run(a, sp, c, 0, -1);
   sums.put(wave, t);
+  if (pre.first) {  // every NW-th part of each row a wave
+    for (int i = lane; i < rows * (DH / 8); i += 64) {
+      const int jr = i / (DH / 8), jc = i % (DH / 8), head = c.head * sp.G + row0 + jr;
+      const PartRow<DH> *f = pre.first + (long long)c.start * (sp.G * sp.Hkv) + head;
+      const int first = clamp_int(f->first, 0, W - 1), more = min(f->more & 0xffff, W - 1 - first);
+      const int pr = (f->more >> 16) & (pre_rows - 1);
+      float mm = -__builtin_inff(), ll = 0.f;
+      f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+      for (int n = wave; n <= more; n += NW) {
+        const PartRow<DH> *p = n == 0 ? f : pre.later + (long long)(first + n) * pre_rows + pr;
+        const float pm = p->m, pl = p->l, mn = fmaxf(mm, pm), base = mn == -__builtin_inff() ? 0.f : mn;
+        const float g = exp2_(mm - base), k = exp2_(pm - base);
+        const f32x4 px = *reinterpret_cast<const f32x4 *>(p->o + jc * 8), py = *reinterpret_cast<const f32x4 *>(p->o + jc * 8 + 4);
+        mm = mn;
+        ll = ll * g + pl * k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = x[e] * g + px[e] * k, y[e] = y[e] * g + py[e] * k;
+      }
+      if (jc == 0) {
+        sums.m[NW + wave][jr] = mm;
+        sums.l[NW + wave][jr] = ll;
+      }
+      *reinterpret_cast<f32x4 *>(&sums.o[NW + wave][jr][jc * 8]) = x;
+      *reinterpret_cast<f32x4 *>(&sums.o[NW + wave][jr][jc * 8 + 4]) = y;
+    }
+  }
   __syncthreads();
   for (int i = tid; i < rows * (DH / 8); i += N) {
     const int jr = i / (DH / 8), jc = i % (DH / 8), head = c.head * sp.G + row0 + jr;
     float mm, ll, acc[8];
-    sums.join(NW, jr, jc, mm, ll, acc);
-    if (pre.first) {
-      const PartRow<DH> *f = pre.first + (long long)c.start * (sp.G * sp.Hkv) + head;
-      const int first = clamp_int(f->first, 0, W - 1), more = min(f->more & 0xffff, W - 1 - first);
-      const int pr = (f->more >> 16) & (pre_rows - 1);
-      auto part = [&](int n) { return n == 0 ? f : pre.later + (long long)(first + n) * pre_rows + pr; };
-      float top = mm;
-      for (int n = 0; n <= more; ++n) top = fmaxf(top, part(n)->m);
-      const float base = top == -__builtin_inff() ? 0.f : top, own = exp2_(mm - base);
-      ll *= own;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= own;
-#pragma unroll 4
-      for (int n = 0; n <= more; ++n) {
-        const PartRow<DH> *p = part(n);
-        const float g = exp2_(p->m - base);
-        ll += g * p->l;
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(p->o + jc * 8), y = *reinterpret_cast<const f32x4 *>(p->o + jc * 8 + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += g * x[e], acc[4 + e] += g * y[e];
-      }
-    }
+    sums.join(pre.first ? 2 * NW : NW, jr, jc, mm, ll, acc);
     store_row8(a.out + (long long)c.start * a.o_stride + head * DH + jc * 8, acc, ll);
   }
 }
