@@ -71,6 +71,15 @@ struct Parts {
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// 16 bytes of the cache; ONCE: past the caches.
+template <bool ONCE>
+__device__ __forceinline__ Frag16 load_cache(const uint16_t *p) {
+  if constexpr (!ONCE) return load16(p);
+  Frag16 f;
+  f.u = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+  return f;
+}
+
 // One 32-key step's loads of a wave.
 template <int DH>
 struct KeyBlock {
@@ -78,20 +87,20 @@ struct KeyBlock {
   uint32_t v[8][DH / 32];  // [key][dword]: DH / 16 bf16 of the lane's entries
 };
 
-template <int DH>
+template <int DH, bool ONCE>
 __device__ __forceinline__ void load_block(KeyBlock<DH> &b, const uint16_t *k0, const uint16_t *k1,
                                            const uint16_t *v0, const uint16_t *v1, int lane) {
   const int r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int d = 0; d < DH / 32; ++d) {
-    b.k[0][d] = load16(k0 + r * DH + d * 32 + q * 8);
-    b.k[1][d] = load16(k1 + r * DH + d * 32 + q * 8);
+    b.k[0][d] = load_cache<ONCE>(k0 + r * DH + d * 32 + q * 8);
+    b.k[1][d] = load_cache<ONCE>(k1 + r * DH + d * 32 + q * 8);
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const uint16_t *p = (e < 4 ? v0 : v1) + (q * 4 + (e & 3)) * DH + r * (DH / 16);
     if constexpr (DH == 128) {
-      const Frag16 f = load16(p);
+      const Frag16 f = load_cache<ONCE>(p);
       for (int i = 0; i < 4; ++i) b.v[e][i] = f.u[i];
     } else {
       const uint2 f = *reinterpret_cast<const uint2 *>(p);
@@ -214,7 +223,9 @@ __device__ __forceinline__ void zero_spare_rows(const PagedAttentionArgs &a, con
 // each block a wave: this wave's sums o, maximum m (base 2) and l.  b1 < 0: to the
 // group's last block; then the first block's loads do not wait for kv_len (a block
 // past the end is read from what pages the table names there, and masked).
-template <int DH, int NW>
+// ONCE: keys and values are loaded past the caches (48 sequences of up to 8000 keys
+// 147 -> 137 us, one of 131 000 96 -> 91; not for the short ones below, 16.8 -> 21).
+template <int DH, int NW, bool ONCE>
 struct TileWalk {
   static constexpr int E = DH / 16;  // MFMAs of the second product, entries of a lane's output run
   f32x4 o[E];
@@ -279,7 +290,7 @@ struct TileWalk {
         kp[h] = kh + max(pg, 0) * a.kpage_stride + in;
         vp[h] = vh + max(pg, 0) * a.vpage_stride + in;
       }
-      load_block<DH>(kb, kp[0], kp[1], vp[0], vp[1], lane);
+      load_block<DH, ONCE>(kb, kp[0], kp[1], vp[0], vp[1], lane);
       return x;
     };
     Where at;
@@ -372,8 +383,8 @@ struct WaveSums {
   float m[SLOTS][ROWS], l[SLOTS][ROWS];
   __attribute__((aligned(16))) float o[SLOTS][ROWS][DH + 4];
 
-  template <int NW>
-  __device__ __forceinline__ void put(int slot, const TileWalk<DH, NW> &t) {
+  template <class Walk>
+  __device__ __forceinline__ void put(int slot, const Walk &t) {
     constexpr int E = DH / 16;
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     if (q == 0) {
@@ -430,7 +441,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
   for (long long u = u0; u < u1;) {
     const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
     const int row0 = c.tile * ROWS, rows = min(ROWS, c.n * sp.G - row0);
-    TileWalk<DH, 4> t;
+    TileWalk<DH, 4, true> t;
     t.run(a, sp, c, b0, b1);
     sums.put(wave, t);
     __syncthreads();
@@ -477,7 +488,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(Paged
   const int group = blockIdx.x / tiles;
   UnitCursor c{group / sp.Hkv, (int)blockIdx.x % tiles, group % sp.Hkv, 0, 0, 1, group / sp.Hkv, 0};
   const int row0 = c.tile * ROWS, rows = min(ROWS, sp.G - row0);
-  TileWalk<DH, NW> t;
+  TileWalk<DH, NW, false> t;
   t.run(a, sp, c, 0, -1);
   sums.put(wave, t);
   if (pre.first) {  // every NW-th part of each row a wave
@@ -821,11 +832,9 @@ struct RowJoin {
   }
 };
 
-// Workgroup (w, y): rows of the group whose first part workgroup w left in its
-// slot of `slot_rows`.
+// Workgroup (w, y): rows of the group whose first part workgroup w left in its slot.
 template <int DH, int SPLIT>
-__global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttentionArgs a, int G, int slot_rows,
-                                                                  Parts<DH> parts) {
+__global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttentionArgs a, int G, Parts<DH> parts) {
   using J = RowJoin<DH, SPLIT>;
   __shared__ f32x4 so[SPLIT > 1 ? NT : 1];
   __shared__ float sm[SPLIT > 1 ? NT : 1], sl[SPLIT > 1 ? NT : 1];
@@ -836,12 +845,48 @@ __global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttention
   J j;
   j.clear();
   if (jr < in.rows)
+#pragma unroll 4
     for (int i = split; i <= in.more; i += SPLIT)
-      j.add(i == 0 ? parts.first + (long long)w * slot_rows + jr : parts.later + (long long)(w + i) * slot_rows + jr, ch);
+      j.add(i == 0 ? parts.first + w * ROWS + jr : parts.later + (w + i) * ROWS + jr, ch);
   j.gather(so, sm, sl, split);
   if (split == 0 && jr < in.rows) {
     const int row = in.row0 + jr, tok = row / G;
     j.store(a.out + (long long)(in.token + tok) * a.o_stride + (in.head * G + row - tok * G) * DH, ch);
+  }
+}
+
+// The same for 128-row tiles, few parts a row: a lane's four rows at once, so that
+// one round of the workgroups has all loads in flight (15.5 -> 14.0 us for the 1024
+// slots of a prompt call).
+template <int DH>
+__global__ __launch_bounds__(NT) void paged_attention_tile_join_kernel(PagedAttentionArgs a, int G, Parts<DH> parts) {
+  using J = RowJoin<DH, 1>;
+  constexpr int R = 4;
+  const int w = blockIdx.x, ch = threadIdx.x % J::CH, jr0 = blockIdx.y * J::PER * R + threadIdx.x / J::CH;
+  const PartInfo in = parts.info[w];
+  if ((int)blockIdx.y * J::PER * R >= in.rows) return;
+  J j[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) j[k].clear();
+  for (int i = 0; i <= in.more; ++i) {
+    const PartRow<DH> *p = i == 0 ? parts.first + (long long)w * TROWS : parts.later + (long long)(w + i) * TROWS;
+    f32x4 o[R];
+    float m[R], l[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const PartRow<DH> *row = p + min(jr0 + k * J::PER, in.rows - 1);
+      o[k] = *reinterpret_cast<const f32x4 *>(row->o + ch * 4);
+      m[k] = row->m;
+      l[k] = row->l;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) j[k].add(m[k], l[k], o[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int row = in.row0 + jr0 + k * J::PER, tok = row / G;
+    if (jr0 + k * J::PER < in.rows)
+      j[k].store(a.out + (long long)(in.token + tok) * a.o_stride + (in.head * G + row - tok * G) * DH, ch);
   }
 }
 
@@ -867,6 +912,7 @@ __global__ __launch_bounds__(NT) void paged_attention_join2_kernel(PagedAttentio
       // (clamped: sequences that overlap, which q_start must not make, would mix two groups' words)
       const int first = clamp_int(f->first, 0, W - 1), more = min(f->more & 0xffff, W - 1 - first);
       const int jr = (f->more >> 16) & (slot_rows - 1);
+#pragma unroll 4
       for (int n = split; n <= more; n += SPLIT)
         j.add(n == 0 ? f : p.later + (long long)(first + n) * slot_rows + jr, ch);
     }
@@ -958,10 +1004,17 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
     parts.first = reinterpret_cast<PartRow<DH> *>(ws + d.W * sizeof(PartInfo));
     parts.later = parts.first + (size_t)d.W * own_rows;
     attend(d.own_tiles, false, 0, parts);
-    auto join = d.own_tiles ? paged_attention_join_kernel<DH, 1> : paged_attention_join_kernel<DH, NT * 4 / DH>;
-    const int per = d.own_tiles ? RowJoin<DH, 1>::PER : 1, most = a.b.q_start || d.own_tiles ? own_rows : std::min(ROWS, G);
-    plan("llama_paged_attention_join", d.W * ((most + per - 1) / per), wg_per_cu(join, NT));
-    hipLaunchKernelGGL(join, dim3(d.W, (most + per - 1) / per), dim3(NT), 0, s, a, G, own_rows, parts);
+    if (d.own_tiles) {
+      auto join = paged_attention_tile_join_kernel<DH>;
+      const int y = TROWS / (4 * RowJoin<DH, 1>::PER);
+      plan("llama_paged_attention_join", d.W * y, wg_per_cu(join, NT));
+      hipLaunchKernelGGL(join, dim3(d.W, y), dim3(NT), 0, s, a, G, parts);
+    } else {
+      auto join = paged_attention_join_kernel<DH, NT * 4 / DH>;
+      const int y = a.b.q_start ? ROWS : std::min(ROWS, G);
+      plan("llama_paged_attention_join", d.W * y, wg_per_cu(join, NT));
+      hipLaunchKernelGGL(join, dim3(d.W, y), dim3(NT), 0, s, a, G, parts);
+    }
   } else {
     const Parts<DH> own = take(slot_bytes<DH>(d, d.own_tiles));
     attend(d.own_tiles, false, 1, own);
