@@ -110,6 +110,12 @@ __device__ __forceinline__ void load_block(KeyBlock<DH> &b, const uint16_t *k0, 
   }
 }
 
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ long long uniform(long long v) {
+  return (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                     (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 // Inclusive sum over the lanes of a wave.
 template <class T>
 __device__ __forceinline__ T wave_scan(T v) {
@@ -160,8 +166,7 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     if (v < wave) before += s.wave[v];
     U += s.wave[v];
   }
-  U = (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(U >> 32)) << 32 |
-                  (unsigned)__builtin_amdgcn_readfirstlane((int)U));
+  U = uniform(U);
   W = split_workgroups(U, gridDim.x);
   w = blockIdx.x;
   if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
@@ -204,6 +209,9 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     c.base += all;
     rest -= all;
   }
+  c.blk = __builtin_amdgcn_readfirstlane(c.blk);
+  c.tile = __builtin_amdgcn_readfirstlane(c.tile);
+  c.base = uniform(c.base);
   return true;
 }
 
@@ -535,12 +543,14 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(Paged
 // 32, h its half of the wave) of one row, so the row's maximum is one exchange
 // between the halves away, and keys 8 j + 4 h + i, j = 2 g and 2 g + 1, are the
 // k slots of its half in the g-th MFMA of O^T = V^T P^T.
+//  - Two buffers: the next block is fetched, sixteen keys a wave, while one is
+//    computed, and then written to the other; one barrier a block.
 //  - K lies in LDS by keys, 16-byte chunks exchanged by the key's number so that
 //    the 32 keys of an operand read fall into different banks; V by keys with its
 //    64-byte runs exchanged, for gfx950's transposing reads: sixteen lanes read four
 //    keys of sixteen entries, each gets four keys of its entry.
-//  - Two buffers: while block i is computed, block i + 1, fetched a step ago, is
-//    written to the other, and block i + 2 is on its way; one barrier a block.
+//  - Blocks follow each other across groups: a group's last block is computed with
+//    the next one's first on its way.
 //  - The running maximum is only a reference: it is raised, and the sums scaled,
 //    when a row's maximum passes it by more than 2^8 (a uniform branch), so that
 //    p <= 2^8 and most blocks scale nothing.
@@ -556,8 +566,8 @@ template <int DH>
 __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
                                                                      Parts<DH> parts) {
   constexpr int CH = DH / 8;             // 16-byte chunks of a key
-  constexpr int NL = TKEYS * CH / NT;    // chunks a lane fetches, of K and of V
-  constexpr int KPL = 64 / CH;           // keys that one load of a wave covers
+  constexpr int NL = TKEYS * CH / NT;    // loads of a wave a block, of K and of V
+  constexpr int KPL = 64 / CH;           // keys that one of them covers
   constexpr int E = DH / 32;             // MFMAs of the second product a k step
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][TKEYS * DH], sv[2][TKEYS * DH];
   __shared__ __attribute__((aligned(16))) int s_live[2][TKEYS / 16];  // whether a buffer's sixteen keys have a page
@@ -573,218 +583,285 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   if (!some) return;
 
   const float scale = a.scale * 1.44269504088896340736f;
-  // where key `k` of a block keeps its chunk `ch`
-  auto k_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? k & 15 : (k >> 1) & 7)); };
-  // the same of V: 64-byte runs exchanged, which a transposing read takes whole
-  auto v_chunk = [](int k, int ch) { return k * CH + (ch ^ (CH == 16 ? (k & 3) << 2 : (k & 2) << 1)); };
-  // this lane's operand addresses in a buffer: K's chunks of key r, V's runs
-  int ka[DH / 16], va[E];
-#pragma unroll
-  for (int d = 0; d < DH / 16; ++d) ka[d] = k_chunk(r, 2 * d + h) * 8;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    va[e] = v_chunk(4 * h + (lane >> 2 & 3), 4 * e + (r >> 4) * 2 + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
-  const int fk = lane / CH, fc = lane % CH;  // the key and chunk of this lane in a load of its wave
+  // the chunk exchanges: of key k's chunk ch
+  auto k_swap = [](int k) { return CH == 16 ? k & 15 : (k >> 1) & 7; };
+  auto v_swap = [](int k) { return CH == 16 ? (k & 3) << 2 : (k & 2) << 1; };
+  // This lane's addresses in a buffer, of chunk h of key r, its first run of V, and
+  // where it writes its first chunks of its wave's sixteen keys; the others differ by
+  // an exclusive or of the chunk and by whole keys.
+  const int ka = r * DH + (h ^ k_swap(r)) * 8;
+  const int vk = 4 * h + (lane >> 2 & 3);
+  const int va = vk * DH + (((r >> 4) * 2 + (lane >> 1 & 1)) ^ v_swap(vk)) * 8 + (lane & 1) * 4;
+  const int wk = 16 * wave + lane / CH;
+  const int ks = wk * DH + (lane % CH ^ k_swap(wk)) * 8, vs = wk * DH + (lane % CH ^ v_swap(wk)) * 8;
+  const int wrow = wave * 32;  // this wave's first row in a tile
 
-  for (long long u = u0; u < u1;) {
-    const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
-    const int row0 = c.tile * TROWS, rows = min(TROWS, c.n * sp.G - row0);
-    const int wrow = wave * 32;  // this wave's first row in the tile
-    const bool busy = wrow < rows;
-    const int row = row0 + min(wrow + r, rows - 1), tok = row / sp.G;
-    Frag16 qf[DH / 16];
-    {
-      const uint16_t *p = a.Q + (long long)(c.start + tok) * a.q_stride + (c.head * sp.G + row - tok * sp.G) * DH + h * 8;
+  // The group whose blocks are computed: its rows, and the own keys that this
+  // lane's row, the wave's first and last rows and any row of the tile see.
+  struct Group {
+    int row0, rows, row, tok;
+    int lim, lim_first, lim_last, end;
+  };
+  auto tile_end = [&](const UnitCursor &u) __attribute__((always_inline)) {
+    const unsigned last = min((u.tile + 1) * TROWS, u.n * sp.G) - 1;
+    return visible_keys(sp, u.seq, u.n, last / (unsigned)sp.G);
+  };
+  auto group_of = [&](const UnitCursor &u) __attribute__((always_inline)) {
+    Group g;
+    g.row0 = u.tile * TROWS;
+    g.rows = min(TROWS, u.n * sp.G - g.row0);
+    g.row = g.row0 + min(wrow + r, g.rows - 1);
+    g.tok = (unsigned)g.row / (unsigned)sp.G;
+    const int first = (unsigned)(g.row0 + min(wrow, g.rows - 1)) / (unsigned)sp.G;
+    const int last = (unsigned)(g.row0 + min(wrow + 31, g.rows - 1)) / (unsigned)sp.G;
+    g.lim = visible_keys(sp, u.seq, u.n, g.tok);
+    g.lim_first = visible_keys(sp, u.seq, u.n, first);
+    g.lim_last = visible_keys(sp, u.seq, u.n, last);
+    g.end = tile_end(u);
+    return g;
+  };
+  Frag16 qf[DH / 16];
+  auto load_queries = [&](const UnitCursor &u) __attribute__((always_inline)) {
+    const int row = min(u.tile * TROWS + wrow + r, u.n * sp.G - 1), tok = (unsigned)row / (unsigned)sp.G;
+    const uint16_t *p = a.Q + (long long)(u.start + tok) * a.q_stride + (u.head * sp.G + row - tok * sp.G) * DH + h * 8;
 #pragma unroll
-      for (int d = 0; d < DH / 16; ++d) qf[d] = load16(p + d * 16);
+    for (int d = 0; d < DH / 16; ++d) qf[d] = load16(p + d * 16);
+  };
+  // Waits for the queries where they are loaded: at their use the next block's loads,
+  // issued after them, would be waited for too.
+  auto touch_queries = [&]() __attribute__((always_inline)) {
+    uint32_t zero;
+    asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+#pragma unroll
+    for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[d].u[i] |= zero;
+  };
+  // The pages of this wave's sixteen keys of 64 blocks from blk on, one a lane (-1: none
+  // of the keys is seen, or the table names no page).  One load for many blocks: a load
+  // a block, carried to the next, was waited for behind the block's keys (158 -> XX us).
+  auto find = [&](const UnitCursor &u, int end, int blk) __attribute__((always_inline)) {
+    const int b = blk + lane;
+    const bool pre = b < sp.pre_blocks;
+    const long long j = (long long)(pre ? b : b - sp.pre_blocks) * TKEYS + 16 * wave;
+    if (j >= (pre ? sp.b.prefix_len : end)) return -1;
+    const int *t = pre ? a.prefix_table : sp.b.page_table + u.seq * (sp.stacked ? 0 : sp.b.table_stride);
+    return checked_page(t[j >> sp.b.page_log2], sp.b.n_pages);
+  };
+  u32x4 kr[NL], vr[NL];  // the next block's sixteen keys of this wave
+  int seen = 0;          // of these, the ones that a row may see
+  auto fetch = [&](const UnitCursor &u, int end, int blk, int page) __attribute__((always_inline)) {
+    const bool pre = blk < sp.pre_blocks;
+    const int j = (pre ? blk : blk - sp.pre_blocks) * TKEYS + 16 * wave;
+    seen = page >= 0 ? (pre ? sp.b.prefix_len : end) - j : 0;
+    const int in = ((u.head << sp.b.page_log2) + (j & ((1 << sp.b.page_log2) - 1))) * DH;
+    const uint16_t *kp = a.k_pages + max(page, 0) * a.kpage_stride + in, *vp = a.v_pages + max(page, 0) * a.vpage_stride + in;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      kr[i] = *reinterpret_cast<const u32x4 *>(kp + i * 512 + lane * 8);
+      vr[i] = *reinterpret_cast<const u32x4 *>(vp + i * 512 + lane * 8);
     }
-    const int lim = visible_keys(sp, c.seq, c.n, tok);
-    const int lim_first = visible_keys(sp, c.seq, c.n, (row0 + min(wrow, rows - 1)) / sp.G);
-    const int lim_last = visible_keys(sp, c.seq, c.n, (row0 + min(wrow + 31, rows - 1)) / sp.G);
-    const int tile_lim = visible_keys(sp, c.seq, c.n, (row0 + rows - 1) / sp.G);
-    const int *table = sp.b.page_table + (sp.stacked ? 0 : c.seq * sp.b.table_stride);
-    const uint16_t *kh = a.k_pages + ((long long)c.head << sp.b.page_log2) * DH;
-    const uint16_t *vh = a.v_pages + ((long long)c.head << sp.b.page_log2) * DH;
+  };
+  auto commit = [&](int to) __attribute__((always_inline)) {
+    if (lane == 0) s_live[to][wave] = seen > 0;
+    if (seen < 16) {  // values that no row may see must not meet p = 0
+      __builtin_amdgcn_sched_barrier(0);  // (keeps the branch)
+#pragma unroll
+      for (int i = 0; i < NL; ++i) vr[i] = masked(vr[i], i * KPL + lane / CH < seen);
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      *reinterpret_cast<u32x4 *>(sk[to] + (ks ^ i * 32) + i * KPL * DH) = kr[i];
+      *reinterpret_cast<u32x4 *>(sv[to] + vs + i * KPL * DH) = vr[i];
+    }
+  };
 
-    f32x16 o[E];
+  Group g = group_of(c);
+  f32x16 o[E];
+  float m, l;  // l: this lane's keys only
+  auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[e][i] = 0.f;
-    float m = -__builtin_inff(), l = 0.f;  // l: this lane's keys only
+    m = -__builtin_inff();
+    l = 0.f;
+  };
+  clear();
+  long long left = u1 - u0;  // blocks, the one computed included
+  int b0 = c.blk, pages0 = c.blk, pages = find(c, g.end, pages0);
+  load_queries(c);
+  fetch(c, g.end, c.blk, __builtin_amdgcn_readlane(pages, 0));
+  commit(0);
+  touch_queries();
+  __syncthreads();
 
-    // A wave fetches sixteen keys of a block, which lie in one page; the page's
-    // number is read a block ahead of its keys.
-    u32x4 kr[NL], vr[NL];
-    int page = -1, seen = 0;  // of the block to be fetched next; of the one in vr
-    bool live = false;
-    auto find = [&](int blk) __attribute__((always_inline)) {
-      const bool pre = blk < sp.pre_blocks;
-      const int j = (pre ? blk : blk - sp.pre_blocks) * TKEYS + 16 * wave;
-      page = -1;
-      if (j < (pre ? sp.b.prefix_len : tile_lim)) page = (pre ? a.prefix_table : table)[j >> sp.b.page_log2];
-    };
-    auto fetch = [&](int blk) __attribute__((always_inline)) {
-      const bool pre = blk < sp.pre_blocks;
-      const int j = (pre ? blk : blk - sp.pre_blocks) * TKEYS + 16 * wave;
-      const int pg = __builtin_amdgcn_readfirstlane(checked_page(page, sp.b.n_pages));
-      live = pg >= 0;
-      seen = live ? (pre ? sp.b.prefix_len : tile_lim) - j : 0;
-      const int in = (j & ((1 << sp.b.page_log2) - 1)) * DH;
-      const uint16_t *kp = kh + max(pg, 0) * a.kpage_stride + in, *vp = vh + max(pg, 0) * a.vpage_stride + in;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        kr[i] = *reinterpret_cast<const u32x4 *>(kp + i * 512 + lane * 8);
-        vr[i] = *reinterpret_cast<const u32x4 *>(vp + i * 512 + lane * 8);
-      }
-    };
-    auto commit = [&](int buf) __attribute__((always_inline)) {
-      if (lane == 0) s_live[buf][wave] = live;
-      if (seen < 16) {  // values that no row may see must not meet p = 0
-        __builtin_amdgcn_sched_barrier(0);  // (keeps the branch)
-#pragma unroll
-        for (int i = 0; i < NL; ++i) vr[i] = masked(vr[i], i * KPL + fk < seen);
-      }
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int k = 16 * wave + i * KPL + fk;
-        *reinterpret_cast<u32x4 *>(&sk[buf][k_chunk(k, fc) * 8]) = kr[i];
-        *reinterpret_cast<u32x4 *>(&sv[buf][v_chunk(k, fc) * 8]) = vr[i];
-      }
-    };
-    find(b0);
-    fetch(b0);
-    if (b0 + 1 < b1) find(b0 + 1);
-    commit(0);
-    if (b0 + 1 < b1) fetch(b0 + 1);
-    if (b0 + 2 < b1) find(b0 + 2);
-    __syncthreads();
-    for (int blk = b0; blk < b1; ++blk) {
-      const int buf = (blk - b0) & 1;
-      if (blk + 1 < b1) {
-        commit(buf ^ 1);
-        if (blk + 2 < b1) fetch(blk + 2);
-        if (blk + 3 < b1) find(blk + 3);
-      }
-      const int4 lv = *reinterpret_cast<const int4 *>(s_live[buf]);
-      const bool pre = blk < sp.pre_blocks;
-      const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS;
-      const int my_lim = pre ? sp.b.prefix_len : lim;
-      const int first_lim = pre ? sp.b.prefix_len : lim_first, last_lim = pre ? sp.b.prefix_len : lim_last;
-      if (busy && j0 < last_lim) {
-        const bool all_live = __builtin_amdgcn_readfirstlane(lv.x & lv.y & lv.z & lv.w);
-        f32x16 s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DH / 16; ++d)
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const Frag16 kf = load16(sk[buf] + ka[d] + 32 * t * DH);
-            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf.h, qf[d].h, s[t], 0, 0, 0);
-          }
-        if (j0 + TKEYS > first_lim || !all_live) {
-          __builtin_amdgcn_sched_barrier(0);  // (keeps the branch: 100 instructions that few blocks need)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-              const int has = (k >> 4) == 0 ? lv.x : (k >> 4) == 1 ? lv.y : (k >> 4) == 2 ? lv.z : lv.w;
-              if (j0 + k >= my_lim || !has) s[t][i] = -__builtin_inff();
-            }
+  for (int buf = 0;; buf ^= 1) {
+    const uint16_t *const kb = sk[buf], *const vb = sv[buf];
+    const int blk = c.blk;
+    const bool same = blk + 1 < c.nb, more_blocks = left > 1;
+    // the next block's loads: of the next group the pages are to be found first
+    UnitCursor c2 = c;
+    int end2 = 0;
+    if (more_blocks) {
+      if (same) {
+        if (blk + 1 >= pages0 + 64) {
+          pages0 = blk + 1;
+          pages = find(c, g.end, pages0);
         }
-        float top = -__builtin_inff();
+        fetch(c, g.end, blk + 1, __builtin_amdgcn_readlane(pages, blk + 1 - pages0));
+      } else {
+        next_group(sp, c2);
+        end2 = tile_end(c2);
+        pages0 = 0;
+        pages = find(c2, end2, 0);
+      }
+    }
+    const bool pre = blk < sp.pre_blocks;
+    const int j0 = (pre ? blk : blk - sp.pre_blocks) * TKEYS;
+    const int my_lim = pre ? sp.b.prefix_len : g.lim;
+    const int first_lim = pre ? sp.b.prefix_len : g.lim_first, last_lim = pre ? sp.b.prefix_len : g.lim_last;
+    const bool busy = wrow < g.rows && j0 < last_lim;
+    f32x16 s[2];
+    if (busy) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+      // operands a few MFMAs ahead of their use: a read's latency is four of them
+      constexpr int N = 2 * (DH / 16), AHEAD = 6;
+      Frag16 kf[N];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) kf[i] = load16(kb + (ka ^ (i >> 1) * 16) + 32 * (i & 1) * DH);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + AHEAD < N) kf[i + AHEAD] = load16(kb + (ka ^ ((i + AHEAD) >> 1) * 16) + 32 * (i & 1) * DH);
+        __builtin_amdgcn_sched_barrier(0);
+        s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i].h, qf[i >> 1].h, s[i & 1], 0, 0, 0);
+      }
+    }
+    if (more_blocks && !same) {
+      fetch(c2, end2, 0, __builtin_amdgcn_readlane(pages, 0));
+    }
+    if (busy) {
+      const int4 lv = *reinterpret_cast<const int4 *>(s_live[buf]);
+      const bool all_live = __builtin_amdgcn_readfirstlane(lv.x & lv.y & lv.z & lv.w);
+      if (j0 + TKEYS > first_lim || !all_live) {
+        __builtin_amdgcn_sched_barrier(0);  // (keeps the branch: 100 instructions that few blocks need)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-        const LanePair tp = lane_pair32(top);
-        top = fmaxf(tp.lo, tp.hi) * scale;
-        if (__any(top > m + 8.0f)) {
-          const float mn = fmaxf(m, top);
-          const float alpha = mn == -__builtin_inff() ? 1.f : exp2_(m - mn);
-          m = mn;
-          l *= alpha;
+          for (int i = 0; i < 16; ++i) {
+            const int k = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+            const int has = t == 0 ? (i < 8 ? lv.x : lv.y) : (i < 8 ? lv.z : lv.w);
+            if (j0 + k >= my_lim || !has) s[t][i] = -__builtin_inff();
+          }
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+      const LanePair tp = lane_pair32(top);
+      top = fmaxf(tp.lo, tp.hi) * scale;
+      if (__any(top > m + 8.0f)) {
+        const float mn = fmaxf(m, top);
+        const float alpha = mn == -__builtin_inff() ? 1.f : exp2_(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[e][i] *= alpha;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
+      Frag16 pf[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float p[16], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[i] = exp2_(fmaf(s[t][i], scale, -base));
+          sum[i & 3] += p[i];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pf[2 * t].u[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
+          pf[2 * t + 1].u[i] = cvt_pk_bf16(p[8 + 2 * i], p[8 + 2 * i + 1]);
+        }
+      }
+      // MFMA i: sixteen keys k = i / E, entries 32 e + r; four keys of sixteen
+      // entries a 16-lane group and read
+      constexpr int N = 4 * E, AHEAD = 4;
+      Frag16 vf[N];
+      auto operand = [&](int i) __attribute__((always_inline)) {
+        const uint16_t *from = vb + (va ^ (i % E) * 32) + 16 * (i / E) * DH;
+        const uint2 lo = read_tr(from), hi = read_tr(from + 8 * DH);
+        vf[i].u = u32x4{lo.x, lo.y, hi.x, hi.y};
+      };
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) operand(i);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + AHEAD < N) operand(i + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+        o[i % E] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i].h, pf[i / E].h, o[i % E], 0, 0, 0);
+      }
+    }
+    if (!same || !more_blocks) {  // the end of the group, or of the share
+      load_queries(c2);  // (the old ones again after the last block)
+      const LanePair lp = lane_pair32(l);
+      l = lp.lo + lp.hi;
+      const bool starts = b0 == 0, ends = !same;
+      const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
+      if (!dense && starts && !ends && tid == 0)
+        parts.info[w] = PartInfo{g.rows, c.start, g.row0, c.head, more, {0, 0, 0}};
+      const int jr = wrow + r;
+      if (jr < g.rows) {
+        const int head = c.head * sp.G + g.row - g.tok * sp.G;
+        const long long token = c.start + g.tok;
+        // this lane's entries: 32 e + 8 j + 4 h + i
+        if (!dense && starts && ends) {
+          const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+          uint16_t *to = a.out + token * a.o_stride + head * DH + 4 * h;
 #pragma unroll
           for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[e][i] *= alpha;
-        }
-        const float base = m == -__builtin_inff() ? 0.f : m;
-        Frag16 pf[4];
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint2 *>(to + 32 * e + 8 * j) =
+                  make_uint2(cvt_pk_bf16(o[e][4 * j] * inv, o[e][4 * j + 1] * inv),
+                             cvt_pk_bf16(o[e][4 * j + 2] * inv, o[e][4 * j + 3] * inv));
+        } else {
+          PartRow<DH> *to = !starts ? parts.later + (long long)w * TROWS + jr
+                            : dense ? parts.first + token * (sp.G * sp.Hkv) + head
+                                    : parts.first + (long long)w * TROWS + jr;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float p[16], sum[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            p[i] = exp2_(fmaf(s[t][i], scale, -base));
-            sum[i & 3] += p[i];
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            pf[2 * t].u[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
-            pf[2 * t + 1].u[i] = cvt_pk_bf16(p[8 + 2 * i], p[8 + 2 * i + 1]);
-          }
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {  // sixteen keys
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            // four keys of sixteen entries a 16-lane group and read: lane r gets entry 32 e + r
-            const uint2 lo = read_tr(sv[buf] + va[e] + 16 * g * DH), hi = read_tr(sv[buf] + va[e] + (16 * g + 8) * DH);
-            Frag16 vf;
-            vf.u = u32x4{lo.x, lo.y, hi.x, hi.y};
-            o[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf.h, pf[g].h, o[e], 0, 0, 0);
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<f32x4 *>(to->o + 32 * e + 8 * j + 4 * h) =
+                  f32x4{o[e][4 * j], o[e][4 * j + 1], o[e][4 * j + 2], o[e][4 * j + 3]};
+          if (h == 0) {
+            to->m = m;
+            to->l = l;
+            to->first = w;
+            to->more = more | (jr << 16);
           }
         }
       }
-      __syncthreads();
+      touch_queries();
+      if (!more_blocks) break;
+      clear();
+      c = c2;
+      g = group_of(c);
+      b0 = 0;
+    } else {
+      ++c.blk;
     }
-
-    const LanePair lp = lane_pair32(l);
-    l = lp.lo + lp.hi;
-    const bool starts = b0 == 0, ends = b1 == c.nb;
-    const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
-    if (!dense && starts && !ends && tid == 0) parts.info[w] = PartInfo{rows, c.start, row0, c.head, more, {0, 0, 0}};
-    const int jr = wrow + r;
-    if (jr < rows) {
-      const int head = c.head * sp.G + row - tok * sp.G;
-      const long long token = c.start + tok;
-      // this lane's entries: 32 e + 8 j + 4 h + i
-      if (!dense && starts && ends) {
-        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-        uint16_t *to = a.out + token * a.o_stride + head * DH + 4 * h;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint2 *>(to + 32 * e + 8 * j) =
-                make_uint2(cvt_pk_bf16(o[e][4 * j] * inv, o[e][4 * j + 1] * inv),
-                           cvt_pk_bf16(o[e][4 * j + 2] * inv, o[e][4 * j + 3] * inv));
-      } else {
-        PartRow<DH> *to = !starts ? parts.later + (long long)w * TROWS + jr
-                          : dense ? parts.first + token * (sp.G * sp.Hkv) + head
-                                  : parts.first + (long long)w * TROWS + jr;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<f32x4 *>(to->o + 32 * e + 8 * j + 4 * h) =
-                f32x4{o[e][4 * j], o[e][4 * j + 1], o[e][4 * j + 2], o[e][4 * j + 3]};
-        if (h == 0) {
-          to->m = m;
-          to->l = l;
-          to->first = w;
-          to->more = more | (jr << 16);
-        }
-      }
-    }
-    u += b1 - b0;
-    if (u < u1) next_group(sp, c);
+    --left;
+    commit(buf ^ 1);
+    __syncthreads();
   }
 }
 
