@@ -146,9 +146,9 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
   long long mine = 0;
   if (seqs <= NT && (unsigned)sp.b.T * sp.G / (unsigned)sp.rows >= 16u * seqs) {
     for (int q = wave; q < seqs; q += NT / 64) {
-      const int n = split_span(sp, q).n, tiles = split_tiles(sp, n);
+      const int n = split_span(sp, q).n, kv = split_kv(sp, q), tiles = split_tiles(sp, n);
       long long sum = 0;
-      for (int t = lane; t < tiles; t += 64) sum += tile_blocks(sp, q, n, t);
+      for (int t = lane; t < tiles; t += 64) sum += tile_blocks(sp, kv, n, t);
       sum = wave_scan(sum);
       if (lane == 63) s.sum[q] = sum * sp.Hkv;
     }
@@ -190,12 +190,13 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
   const SeqSpan span = split_span(sp, c.seq);
   c.n = span.n;
   c.start = span.start;
+  c.kv = split_kv(sp, c.seq);
   c.head = __builtin_amdgcn_readfirstlane((int)((u0 - s.base) / s.per));
   c.base = s.base + c.head * s.per;
   int rest = (int)min(u0 - c.base, (long long)0x7fffffff);  // units before u0 in the tiles from c.tile on
   for (c.tile = 0;; c.tile += 64) {
     const int tiles = split_tiles(sp, c.n);
-    const int nb = c.tile + lane < tiles ? tile_blocks(sp, c.seq, c.n, c.tile + lane) : 0;
+    const int nb = c.tile + lane < tiles ? tile_blocks(sp, c.kv, c.n, c.tile + lane) : 0;
     const int up_to = wave_scan(nb), all = __builtin_amdgcn_readlane(up_to, 63);
     if (rest < all) {
       const int at = __builtin_ctzll(__ballot(up_to > rest));
@@ -255,8 +256,8 @@ struct TileWalk {
     }
     int lim = 0, tile_lim = 0;
     auto limits = [&]() __attribute__((always_inline)) {
-      lim = visible_keys(sp, c.seq, c.n, tok);
-      tile_lim = visible_keys(sp, c.seq, c.n, (row0 + rows - 1) / sp.G);
+      lim = visible_keys(sp, c.kv, c.n, tok);
+      tile_lim = visible_keys(sp, c.kv, c.n, (row0 + rows - 1) / sp.G);
     };
     const int *table = sp.b.page_table + (sp.stacked ? 0 : c.seq * sp.b.table_stride);
     const uint16_t *kh = a.k_pages + ((long long)c.head << sp.b.page_log2) * DH;
@@ -306,7 +307,7 @@ struct TileWalk {
       find(b0, sp.b.max_pages << sp.b.page_log2);
       at = fetch(b0);
       limits();
-      b1 = tile_blocks(sp, c.seq, c.n, c.tile);
+      b1 = tile_blocks(sp, c.kv, c.n, c.tile);
     } else {
       limits();
       find(b0, tile_lim);
@@ -494,7 +495,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(Paged
   __shared__ WaveSums<DH, 2 * NW> sums;  // the waves' sums; theirs of the prefix's parts
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = blockIdx.x / tiles;
-  UnitCursor c{group / sp.Hkv, (int)blockIdx.x % tiles, group % sp.Hkv, 0, 0, 1, group / sp.Hkv, 0};
+  UnitCursor c{group / sp.Hkv, (int)blockIdx.x % tiles, group % sp.Hkv, 0, 0, 1, group / sp.Hkv, 0, 0};
+  c.kv = split_kv(sp, c.seq);
   const int row0 = c.tile * ROWS, rows = min(ROWS, sp.G - row0);
   TileWalk<DH, NW, false> t;
   t.run(a, sp, c, 0, -1);
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   };
   auto tile_end = [&](const UnitCursor &u) __attribute__((always_inline)) {
     const unsigned last = min((u.tile + 1) * TROWS, u.n * sp.G) - 1;
-    return visible_keys(sp, u.seq, u.n, last / (unsigned)sp.G);
+    return visible_keys(sp, u.kv, u.n, last / (unsigned)sp.G);
   };
   auto group_of = [&](const UnitCursor &u) __attribute__((always_inline)) {
     Group g;
@@ -614,9 +616,9 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     g.tok = (unsigned)g.row / (unsigned)sp.G;
     const int first = (unsigned)(g.row0 + min(wrow, g.rows - 1)) / (unsigned)sp.G;
     const int last = (unsigned)(g.row0 + min(wrow + 31, g.rows - 1)) / (unsigned)sp.G;
-    g.lim = visible_keys(sp, u.seq, u.n, g.tok);
-    g.lim_first = visible_keys(sp, u.seq, u.n, first);
-    g.lim_last = visible_keys(sp, u.seq, u.n, last);
+    g.lim = visible_keys(sp, u.kv, u.n, g.tok);
+    g.lim_first = visible_keys(sp, u.kv, u.n, first);
+    g.lim_last = visible_keys(sp, u.kv, u.n, last);
     g.end = tile_end(u);
     return g;
   };

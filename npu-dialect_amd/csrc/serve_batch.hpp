@@ -91,52 +91,53 @@ NPU_HD int split_seqs(const AttnSplit &a) { return a.stacked ? 1 : a.b.B; }
 NPU_HD SeqSpan split_span(const AttnSplit &a, int seq) {
   return a.stacked ? SeqSpan{0, a.b.T} : seq_span(a.b, seq);
 }
-// Own keys of a sequence that new token i of n sees.
-NPU_HD int visible_keys(const AttnSplit &a, int seq, int n, int i) {
+NPU_HD int split_kv(const AttnSplit &a, int seq) { return a.stacked ? 0 : a.b.kv_len[seq]; }
+// Own keys that new token i of n sees in a sequence of kv_len `kv`.
+NPU_HD int visible_keys(const AttnSplit &a, int kv, int n, int i) {
   if (a.stacked) return 0;
   const long long cap = (long long)a.b.max_pages << a.b.page_log2;
-  return clamp_int((long long)a.b.kv_len[seq] - n + i + 1, 0,
-                   clamp_int(a.b.kv_len[seq], 0, (int)cap));
+  return clamp_int((long long)kv - n + i + 1, 0, clamp_int(kv, 0, (int)cap));
 }
 NPU_HD int split_tiles(const AttnSplit &a, int n) {
   return (int)(((unsigned)n * (unsigned)a.G + (unsigned)a.rows - 1) / (unsigned)a.rows);
 }
-NPU_HD int tile_blocks(const AttnSplit &a, int seq, int n, int tile) {
+NPU_HD int tile_blocks(const AttnSplit &a, int kv, int n, int tile) {
   // (n G < 2^31, and a tile is at most 128 rows)
   const unsigned last = (((unsigned)tile + 1) * (unsigned)a.rows - 1) / (unsigned)a.G;
-  const int v = visible_keys(a, seq, n, last < (unsigned)n ? (int)last : n - 1);
+  const int v = visible_keys(a, kv, n, last < (unsigned)n ? (int)last : n - 1);
   const int nb = a.pre_blocks + (int)(((unsigned)v + (1u << a.keys_log2) - 1) >> a.keys_log2);
   return nb > 0 ? nb : 1;
 }
 // Units of one key head of a sequence of n new tokens.
-NPU_HD long long head_units(const AttnSplit &a, int seq, int n) {
+NPU_HD long long head_units(const AttnSplit &a, int kv, int n) {
   const int tiles = split_tiles(a, n);
   long long sum = 0;
-  for (int t = 0; t < tiles; ++t) sum += tile_blocks(a, seq, n, t);
+  for (int t = 0; t < tiles; ++t) sum += tile_blocks(a, kv, n, t);
   return sum;
 }
 NPU_HD long long seq_units(const AttnSplit &a, int seq) {
-  return head_units(a, seq, split_span(a, seq).n) * a.Hkv;
+  return head_units(a, split_kv(a, seq), split_span(a, seq).n) * a.Hkv;
 }
 NPU_HD int split_workgroups(long long U, int launched) { return U < launched ? (int)U : launched; }
 NPU_HD long long first_unit(long long U, int W, int w) { return U * w / W; }
 NPU_HD int unit_owner(long long U, int W, long long u) { return (int)(((u + 1) * W - 1) / U); }
 
 // A place in the order of the units: block blk of the nb of group (seq, tile,
-// head), whose first unit is `base`.
+// head), whose first unit is `base`; n, start, kv: the sequence's.
 struct UnitCursor {
-  int seq, tile, head, blk, nb, n, start;
+  int seq, tile, head, blk, nb, n, start, kv;
   long long base;
 };
 // The group of unit u, from sequence seq on, whose first unit is `base`.
 NPU_HD UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long long u) {
-  UnitCursor c{seq, 0, 0, 0, 1, 0, 0, base};
+  UnitCursor c{seq, 0, 0, 0, 1, 0, 0, 0, base};
   const int seqs = split_seqs(a);
   for (; c.seq < seqs; ++c.seq) {
     const SeqSpan sp = split_span(a, c.seq);
     c.n = sp.n;
     c.start = sp.start;
-    const long long per = head_units(a, c.seq, c.n);
+    c.kv = split_kv(a, c.seq);
+    const long long per = head_units(a, c.kv, c.n);
     if (u >= c.base + per * a.Hkv) {
       c.base += per * a.Hkv;
       continue;
@@ -144,7 +145,7 @@ NPU_HD UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long lo
     c.head = (int)((u - c.base) / per);
     c.base += per * c.head;
     for (;; ++c.tile) {
-      c.nb = tile_blocks(a, c.seq, c.n, c.tile);
+      c.nb = tile_blocks(a, c.kv, c.n, c.tile);
       if (u < c.base + c.nb) break;
       c.base += c.nb;
     }
@@ -167,9 +168,10 @@ NPU_HD void next_group(const AttnSplit &a, UnitCursor &c) {
         c.n = sp.n;
         c.start = sp.start;
       } while (c.n == 0);
+      c.kv = split_kv(a, c.seq);
     }
   }
-  c.nb = tile_blocks(a, c.seq, c.n, c.tile);
+  c.nb = tile_blocks(a, c.kv, c.n, c.tile);
 }
 
 }  // namespace npu

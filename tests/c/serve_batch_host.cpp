@@ -33,7 +33,7 @@ void serve_places(const HostBatch *h, int *out) {
 int serve_visible(const HostBatch *h, int seq, int i) {
   const ServeBatch b = batch(h);
   const AttnSplit a{b, 1, 1, 16, 7, 0, 0};
-  return visible_keys(a, seq, seq_span(b, seq).n, i);
+  return visible_keys(a, split_kv(a, seq), seq_span(b, seq).n, i);
 }
 
 // The segments of all workgroups of a launch in order, eight ints each: workgroup, seq,
