@@ -15,9 +15,18 @@
 // would not do: their rounding, 2^-24 of a mass, is of the order of the
 // distance of u from the nearest of 10^5 borders.
 //
-// A workgroup takes a row.  A bin of more than LIST entries (equal logits, or
-// all of them far below the maximum) is divided further by the order's own key,
-// the logit's bits and then the index, eleven bits at a time.
+// A workgroup takes a row.  What bounds it: each pass over a long row is at the rate
+// of the memory behind the L2 (256 rows of 128000 f32: 19 us), and the weights' f64
+// arithmetic, so passes are saved:
+//  - the maximum, always;
+//  - with top-k, the entries that can be among the k: at least k of the lanes' own
+//    maxima are in the bins up to the k-th's, so all entries up to that bin are
+//    copied to LDS, and the rest of the row is not looked at again;
+//  - else the histogram, with every entry's weight, and then the entries of the
+//    bins that the searches end in, in one pass for all of them: the bin that one
+//    search ends in bounds the mass that the next one starts from.
+// A bin of more than LIST entries (equal logits, say) is divided further by the
+// order's own key, the logit's bits and then the index, eleven bits at a time.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -30,10 +39,10 @@ namespace npu {
 
 namespace {
 
-constexpr int ST = 1024;     // lanes of a workgroup
+constexpr int ST = 512;      // lanes of a workgroup: 1024 would leave a lane 128 registers
 constexpr int BINS = 2048;
 constexpr int LIST = 2048;   // entries of a bin that are ranked at once
-constexpr float BINS_PER_NAT = 64.0f;
+constexpr int CAND = 4096;   // entries that are kept from one pass over the row
 constexpr double ONE = 4398046511104.0;  // 2^42: weight 1
 
 typedef unsigned long long u64;
@@ -51,15 +60,15 @@ __device__ __forceinline__ u64 uniform(u64 v) {
          (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(uniform(__float_as_int(v))); }
 __device__ __forceinline__ double uniform(double v) {
   return __longlong_as_double((long long)uniform((u64)__double_as_longlong(v)));
 }
 
-// 2^y for y <= 0: the nearest whole power times the Taylor polynomial of
-// exp(f ln 2), |f| <= 1/2, to degree 11 (the next term is below 7e-15).
-__device__ __forceinline__ double exp2_64(double y) {
-  y = fmax(y, -1000.0);
-  const double whole = rint(y), r = (y - whole) * 0.69314718055994530942;
+// 2^y, |y| <= 1/2, by the Taylor polynomial of exp(y ln 2) to degree 11 (the next term
+// is below 7e-15): for the table below.
+__device__ __forceinline__ double exp2_small(double y) {
+  const double r = y * 0.69314718055994530942;
   double p = 1.0 / 39916800;
   p = fma(p, r, 1.0 / 3628800);
   p = fma(p, r, 1.0 / 362880);
@@ -71,17 +80,42 @@ __device__ __forceinline__ double exp2_64(double y) {
   p = fma(p, r, 1.0 / 6);
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return ldexp(p, (int)whole);
-}
-// A weight's whole number, rounded to nearest: the significand of w 2^42 + 2^52.
-__device__ __forceinline__ u64 fixed(double w) {
-  const double big = 4503599627370496.0;  // 2^52
-  return (u64)__double_as_longlong(fma(w, ONE, big)) - (u64)__double_as_longlong(big);
+  return fma(p, r, 1.0);
 }
 
-// The row's entries, each once, as f(x, index): 16-byte loads of the aligned part.
-template <bool BF, class F>
+// The weights of a row: 2^42 2^y, y = (x - top) rate, as a whole power, a table of
+// 64ths and the Taylor polynomial of what is left, |r| <= 1/128, to degree 4 (the next
+// term is 4e-14, a third of the last bit of a weight's whole number).
+constexpr int TABLE = 64;
+struct Weights {
+  const double *table;  // 2^42 2^(j / 64), in LDS
+  double top, rate;
+  bool infinite;        // the maximum is +Inf: its like weigh 1, nothing else is a candidate
+  __device__ __forceinline__ double operator()(float x) const {
+    if (infinite) return ONE;
+    const double y = fmax(((double)x - top) * rate, -1000.0);
+    const double magic = 6755399441055744.0;  // 1.5 2^52: y 64 rounded to nearest in the low bits
+    const double t = fma(y, 64.0, magic);
+    const int k = (int)__double_as_longlong(t);
+    const double r = fma(t - magic, -1.0 / 64, y);
+    constexpr double L = 0.69314718055994530942;
+    double p = L * L * L * L / 24;
+    p = fma(p, r, L * L * L / 6);
+    p = fma(p, r, L * L / 2);
+    p = fma(p, r, L);
+    p = fma(p, r, 1.0);
+    return ldexp(table[k & (TABLE - 1)] * p, k >> 6);
+  }
+};
+// A weight's whole number, rounded to nearest: the significand of w + 2^52.
+__device__ __forceinline__ u64 whole(double w) {
+  const double big = 4503599627370496.0;  // 2^52
+  return (u64)__double_as_longlong(w + big) - (u64)__double_as_longlong(big);
+}
+
+// The row's entries, each once, as f(x, index): 16-byte loads of the aligned part,
+// DEEP of them ahead of the one that is worked on.
+template <bool BF, int DEEP, class F>
 __device__ __forceinline__ void each_entry(const void *row, int V, F f) {
   constexpr int PER = BF ? 8 : 4, ES = BF ? 2 : 4;
   const char *p = static_cast<const char *>(row);
@@ -90,12 +124,20 @@ __device__ __forceinline__ void each_entry(const void *row, int V, F f) {
     f(BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]) : reinterpret_cast<const float *>(p)[i], i);
   };
   const int head = min(V, (int)((16 - ((uintptr_t)p & 15)) & 15) / ES);
-  if (tid < head) one(tid);
   const int chunks = (V - head) / PER;
   const u32x4 *body = reinterpret_cast<const u32x4 *>(p + head * ES);
+  u32x4 ahead[DEEP];
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d)
+    if (tid + d * ST < chunks) ahead[d] = body[tid + d * ST];
+  if (tid < head) one(tid);
+  for (int i = head + chunks * PER + tid; i < V; i += ST) one(i);
 #pragma unroll 1
   for (int c = tid; c < chunks; c += ST) {
-    const u32x4 v = body[c];
+    const u32x4 v = ahead[0];
+#pragma unroll
+    for (int d = 0; d + 1 < DEEP; ++d) ahead[d] = ahead[d + 1];
+    if (c + DEEP * ST < chunks) ahead[DEEP - 1] = body[c + DEEP * ST];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = head + c * PER + e * (PER / 4);
@@ -107,101 +149,124 @@ __device__ __forceinline__ void each_entry(const void *row, int V, F f) {
       }
     }
   }
-  for (int i = head + chunks * PER + tid; i < V; i += ST) one(i);
 }
 
 struct Shared {
   u64 mass[BINS];
   uint32_t count[BINS];
-  float lx[LIST];
-  int li[LIST];
-  u64 lw[LIST];
+  double table[TABLE];
+  float cx[CAND];        // candidates kept from a pass
+  int ci[CAND];
+  u64 lk[LIST], lw[LIST];  // a bin's order keys and weights
   u64 wave_m[ST / 64], wave_c[ST / 64];
   u64 key;               // the maximum's order key
-  int n_list, bin, pos;
+  int n_cand, n_list, pos;
   u64 rank, cum, own;    // the entry found: entries and mass up to it (inclusive), its mass
 };
 
 // Exclusive prefix sums of the histogram in place; the totals to all lanes.
 __device__ __forceinline__ void scan_bins(Shared &s, u64 &mass, u64 &count) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const u64 m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
-  const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-  u64 m = m0 + m1, c = (u64)c0 + c1;
+  constexpr int PL = BINS / ST;  // bins of a lane
+  u64 bin_m[PL], m = 0;
+  uint32_t bin_c[PL], c = 0;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) m += bin_m[i] = s.mass[PL * tid + i], c += bin_c[i] = s.count[PL * tid + i];
+  const u64 lane_m = m;
+  const uint32_t lane_c = c;
   for (int off = 1; off < 64; off <<= 1) {
-    const u64 pm = __shfl_up(m, off), pc = __shfl_up(c, off);
+    const u64 pm = __shfl_up(m, off);
+    const uint32_t pc = __shfl_up(c, off);
     if (lane >= off) m += pm, c += pc;
   }
   if (lane == 63) s.wave_m[wave] = m, s.wave_c[wave] = c;
   __syncthreads();
-  u64 bm = 0, bc = 0;
-  u64 am = 0, ac = 0;
-#pragma unroll 2
-  for (int v = 0; v < ST / 64; ++v) {
-    if (v < wave) bm += s.wave_m[v], bc += s.wave_c[v];
-    am += s.wave_m[v], ac += s.wave_c[v];
+  // every wave scans the waves' totals
+  constexpr int NW = ST / 64;
+  u64 tm = lane < NW ? s.wave_m[lane] : 0;
+  uint32_t tc = lane < NW ? s.wave_c[lane] : 0;
+  for (int off = 1; off < NW; off <<= 1) {
+    const u64 pm = __shfl_up(tm, off);
+    const uint32_t pc = __shfl_up(tc, off);
+    if (lane >= off) tm += pm, tc += pc;
   }
-  mass = uniform(am);
-  count = uniform(ac);
-  m += bm - m0 - m1;
-  c += bc - c0 - c1;
-  s.mass[2 * tid] = m;
-  s.mass[2 * tid + 1] = m + m0;
-  s.count[2 * tid] = (uint32_t)c;
-  s.count[2 * tid + 1] = (uint32_t)c + c0;
+  const u64 bm = wave > 0 ? __shfl(tm, wave - 1) : 0;
+  const uint32_t bc = wave > 0 ? __shfl(tc, wave - 1) : 0;
+  mass = uniform(__shfl(tm, NW - 1));
+  count = (u64)(uint32_t)uniform((int)__shfl(tc, NW - 1));
+  m += bm - lane_m;
+  c += bc - lane_c;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    s.mass[PL * tid + i] = m;
+    s.count[PL * tid + i] = c;
+    m += bin_m[i];
+    c += bin_c[i];
+  }
   __syncthreads();
 }
-static_assert(BINS == 2 * ST, "two bins a lane");
+static_assert(BINS % ST == 0, "whole bins a lane");
 
 __device__ __forceinline__ void clear_bins(Shared &s) {
   for (int b = threadIdx.x; b < BINS; b += ST) s.mass[b] = 0, s.count[b] = 0;
   __syncthreads();
 }
 
-// The bin whose running count (by_count) or mass passes t: t is below the total.
-// Every lane gets the bin, its entries, and what comes before it.
-struct Found {
-  int bin, entries;
-  u64 count, mass;
-};
-__device__ __forceinline__ Found find_bin(Shared &s, bool by_count, u64 t, u64 all_mass, u64 all_count) {
-  for (int b = threadIdx.x; b < BINS; b += ST) {
-    const u64 lo = by_count ? s.count[b] : s.mass[b];
-    const u64 hi = b + 1 < BINS ? (by_count ? s.count[b + 1] : s.mass[b + 1]) : (by_count ? all_count : all_mass);
-    if (lo <= t && t < hi) s.bin = b;
-  }
-  __syncthreads();
-  const int b = uniform(s.bin);
-  Found f;
-  f.bin = b;
-  f.count = (u64)(uint32_t)uniform((int)s.count[b]);
-  f.mass = uniform(s.mass[b]);
-  f.entries = uniform((int)((b + 1 < BINS ? s.count[b + 1] : (uint32_t)all_count) - (uint32_t)f.count));
-  __syncthreads();
-  return f;
+// The bin whose running count (by_count) or mass passes t, which is below the total:
+// the last one before which no more than t lies, of empty ones among it the last.
+// Every wave looks for itself: one of 64 runs of bins, then one of its 32.
+__device__ __forceinline__ int bin_of_total(const Shared &s, bool by_count, u64 t) {
+  const int lane = threadIdx.x & 63;
+  const u64 a = by_count ? (u64)s.count[lane * (BINS / 64)] : s.mass[lane * (BINS / 64)];
+  const int run = 63 - __builtin_clzll(__ballot(a <= t));  // (bin 0's is 0)
+  const int at = run * (BINS / 64) + (lane & (BINS / 64 - 1));
+  const u64 b = by_count ? (u64)s.count[at] : s.mass[at];
+  const uint32_t in = (uint32_t)__ballot(b <= t);
+  return uniform(run * (BINS / 64) + 31 - __builtin_clz(in));
+}
+static_assert(BINS / 64 == 32, "a run's bins in half a wave");
+// What comes before a bin.
+__device__ __forceinline__ u64 mass_before(const Shared &s, int b, u64 all) { return b < BINS ? uniform(s.mass[b]) : all; }
+__device__ __forceinline__ int count_before(const Shared &s, int b, u64 all) {
+  return b < BINS ? uniform((int)s.count[b]) : (int)all;
 }
 
+// What a histogram divides: the row by the distance from the maximum (kNear: 128 bins
+// a nat of weight for 16 nats, the rest in the last bin; kFar: that bin, 32 a nat), or
+// a bin by the order key's bits from `shift` down to `next`.
+enum { kNear = 0, kFar = 1, kKeys = 2 };
+struct Range {
+  int level, bin, shift, next;  // bin: of level `from`, that kKeys divides
+  int from;
+  u64 prefix, mass, count;      // mass, count: what comes before the range
+};
+constexpr float PER_NAT = 128.0f;
+
 template <bool BF>
-__global__ __launch_bounds__(ST) void sample_tokens_kernel(SampleArgs a) {
+__global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   __shared__ Shared s;
-  const int tid = threadIdx.x, row = blockIdx.x, V = a.V;
+  const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x, V = a.V;
   const char *x0 = static_cast<const char *>(a.logits) + (long long)row * a.row_stride * (BF ? 2 : 4);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
   const int k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
 
   // the maximum and its first index
-  if (tid == 0) s.key = ~0ull;
+  if (tid == 0) s.key = ~0ull, s.n_cand = 0;
+  if (tid < TABLE) s.table[tid] = ONE * (tid < TABLE / 2 ? exp2_small(tid / 64.0) : 2.0 * exp2_small(tid / 64.0 - 1.0));
   __syncthreads();
-  u64 best = ~0ull;
-  each_entry<BF>(x0, V, [&](float x, int i) {
-    x += 0.0f;  // -0 is 0
-    if (x > -__builtin_inff()) best = min(best, order_key(x, i));
-  });
-  for (int off = 32; off; off >>= 1) best = min(best, (u64)__shfl_xor(best, off));
-  if ((tid & 63) == 0) atomicMin(&s.key, best);
-  __syncthreads();
-  best = uniform(s.key);
+  float mine = -__builtin_inff();  // this lane's maximum
+  {
+    int at = 0;
+    each_entry<BF, 8>(x0, V, [&](float x, int i) {
+      if (x > mine || (x == mine && i < at)) mine = x, at = i;
+    });
+    u64 key = mine > -__builtin_inff() ? order_key(mine + 0.0f, at) : ~0ull;  // -0 is 0
+    for (int off = 32; off; off >>= 1) key = min(key, (u64)__shfl_xor(key, off));
+    if (lane == 0) atomicMin(&s.key, key);
+  }
+  clear_bins(s);
+  const u64 best = uniform(s.key);
   const int first = (int)(uint32_t)best;
   // no candidate, or one that every setting leaves
   const bool greedy = !(temp > 0.0f) || k == 1 || top_p <= 0.0f;
@@ -214,51 +279,131 @@ __global__ __launch_bounds__(ST) void sample_tokens_kernel(SampleArgs a) {
   }
   const uint32_t ob = (uint32_t)(best >> 32);
   const float top = __uint_as_float(ob & 0x80000000u ? ob : ~ob & 0x7fffffffu);
-  const bool infinite = top == __builtin_inff();  // then only the infinite logits are candidates
-  const double rate = uniform(1.4426950408889634074 / (double)temp);
-  auto weight = [&](float x) { return infinite ? 1.0 : exp2_64(((double)x - (double)top) * rate); };
-  auto is_candidate = [&](float x) { return infinite ? x == top : x > -__builtin_inff(); };
-  const float per = BINS_PER_NAT / temp;
-  auto bin_of = [&](float x) {
-    const float d = infinite ? 0.0f : (top - x) * per;
-    return d < (float)(BINS - 1) ? (int)d : BINS - 1;
+  Weights weight;
+  weight.table = s.table;
+  weight.infinite = top == __builtin_inff();
+  weight.rate = uniform(1.4426950408889634074 / (double)temp);
+  weight.top = uniform((double)top);
+  const float floor_x = weight.infinite ? 3.402823466e38f : -__builtin_inff();  // candidates are above
+  auto candidate = [&](float x) { return x > floor_x; };
+  const float per = uniform(PER_NAT / temp);
+  // a bin is the whole part of this (monotone in x, a NaN of 0 Inf included: then
+  // everything is in the last bin)
+  auto distance = [&](float x) { return fminf(weight.infinite ? 0.0f : (top - x) * per, (float)(BINS - 1)); };
+  auto near_bin = [&](float x) { return (int)distance(x); };
+  auto far_bin = [&](float x) {
+    return (int)fminf(fmaxf((top - x) * per * 0.25f - (float)(BINS / 4), 0.0f), (float)(BINS - 1));
+  };
+  auto keep = [&](float x, int i) {  // to the list in LDS
+    const int at = atomicAdd(&s.n_cand, 1);
+    if (at < CAND) s.cx[at] = x, s.ci[at] = i;
   };
 
-  // The histogram's range: the whole row by bins, or, where a bin is divided, the
-  // entries of bin `in_bin` whose key starts with `prefix`, by the key's next bits.
-  int in_bin = -1, shift = 64, next = 64;
-  u64 prefix = 0, base_m = 0, base_n = 0;
-  auto inside = [&](float x, int i) {
-    if (!is_candidate(x)) return false;
-    if (in_bin < 0) return true;
-    return bin_of(x) == in_bin && (shift == 64 || order_key(x, i) >> shift == prefix);
+  // The entries that the searches look at: the row's, or the list's where it holds
+  // all that can be drawn.
+  bool listed_all = false;
+  u64 range_m = 0, range_n = 0;
+  if (V <= CAND || (k > 0 && k <= ST / 2)) {
+    int last = BINS - 1;  // the list's last bin
+    if (V > CAND) {
+      if (candidate(mine)) atomicAdd(&s.count[near_bin(mine + 0.0f)], 1u);
+      __syncthreads();
+      scan_bins(s, range_m, range_n);
+      last = range_n >= (u64)k ? bin_of_total(s, true, (u64)k - 1) : BINS;
+    }
+    if (last < (V > CAND ? BINS - 1 : BINS)) {
+      each_entry<BF, 4>(x0, V, [&](float x, int i) {
+        x += 0.0f;
+        if (candidate(x) && near_bin(x) <= last) keep(x, i);
+      });
+      __syncthreads();
+      listed_all = uniform(s.n_cand) <= CAND;
+    }
+    __syncthreads();
+    if (!listed_all && tid == 0) s.n_cand = 0;
+  }
+  const int n_all = listed_all ? uniform(s.n_cand) : 0;
+  auto each_listed = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int e = tid; e < n_all; e += ST) f(s.cx[e], s.ci[e]);
+  };
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if (listed_all) {
+      each_listed(f);
+    } else {
+      each_entry<BF, 4>(x0, V, [&](float x, int i) {
+        x += 0.0f;
+        if (candidate(x)) f(x, i);
+      });
+    }
+  };
+
+  Range g{kNear, 0, 64, 64, kNear, 0, 0, 0};
+  auto inside = [&](float x, int i) {  // of the range
+    if (near_bin(x) != (g.from == kNear && g.level == kKeys ? g.bin : BINS - 1)) return false;
+    if (g.level == kFar) return true;
+    if (g.from == kFar && far_bin(x) != g.bin) return false;
+    return g.shift == 64 || order_key(x, i) >> g.shift == g.prefix;
   };
 
   // The searches in turn: 0 for top-k's count, 1 for top-p's mass, 2 for the draw.
-  u64 n = 0, m = 0, range_m = 0, range_n = 0, all_n = 0, all_m = 0, keep_n = 0, keep_m = 0, t = 0;
+  u64 n = 0, m = 0, all_n = 0, all_m = 0, keep_n = 0, keep_m = 0, t = 0;
+  const double u = uniform((double)a.u[row]);
+  auto bound_p = [&](u64 mass) {
+    const double v = uniform(ceil((double)top_p * (double)mass));
+    return v >= 1.0 ? min((u64)v, mass) - 1 : (u64)0;
+  };
+  auto bound_u = [&](u64 mass) {
+    const double v = uniform(floor(u * (double)mass));
+    return v >= 0.0 ? min((u64)v, mass - 1) : (u64)0;
+  };
   bool by_count = false, have = false, known = false;
+  int iv[3][2] = {{0, 0}, {0, 0}, {0, 0}};  // the near bins whose entries are in the list: [first, past the last)
   for (int step = -1;;) {
     if (!have) {
+      if (tid == 0) s.rank = 0, s.cum = 0;
       clear_bins(s);
-      u64 kn = 0, km = 0;
-      each_entry<BF>(x0, V, [&](float x, int i) {
-        x += 0.0f;
-        if (!inside(x, i)) return;
-        const double w = weight(x);
-        const u64 f = fixed(w);
-        const int b = in_bin < 0 ? bin_of(x) : (int)(order_key(x, i) >> next & ((1ull << (shift - next)) - 1));
-        atomicAdd(&s.mass[b], f);
-        atomicAdd(&s.count[b], 1u);
-        if (w >= (double)min_p) ++kn, km += f;
-      });
-      if (step < 0) {  // what min-p keeps, counted on the way
-        if (tid == 0) s.rank = 0, s.cum = 0;
-        __syncthreads();
-        for (int off = 32; off; off >>= 1) kn += __shfl_xor(kn, off), km += __shfl_xor(km, off);
-        if ((tid & 63) == 0) {
+      if (g.level == kNear) {
+        // what min-p keeps is counted on the way; the last bin, without atomics, by lane
+        u64 kn = 0, km = 0, om = 0, oc = 0;
+        const bool count_min = min_p > 0.0f;
+        const double least = uniform((double)min_p * ONE);
+        auto add = [&](float x, int) __attribute__((always_inline)) {
+          const bool counts = candidate(x);
+          const double w = counts ? weight(x) : 0.0;
+          const u64 f = whole(w);
+          const int b = counts ? near_bin(x) : BINS - 1;
+          if (b < BINS - 1) {
+            atomicAdd(&s.mass[b], f);
+            atomicAdd(&s.count[b], 1u);
+          } else {
+            om += f;
+            oc += counts;
+          }
+          if (count_min && counts && w >= least) ++kn, km += f;
+        };
+        if (listed_all)
+          each_listed(add);
+        else
+          each_entry<BF, 4>(x0, V, add);
+        for (int off = 32; off; off >>= 1) {
+          kn += __shfl_xor(kn, off), km += __shfl_xor(km, off);
+          om += __shfl_xor(om, off), oc += __shfl_xor(oc, off);
+        }
+        if (lane == 0) {
+          atomicAdd(&s.mass[BINS - 1], om);
+          atomicAdd(&s.count[BINS - 1], (uint32_t)oc);
           atomicAdd(&s.rank, kn);
           atomicAdd(&s.cum, km);
         }
+      } else {
+        each([&](float x, int i) {
+          if (!inside(x, i)) return;
+          const int b = g.level == kFar ? far_bin(x)
+                                        : (int)(order_key(x, i) >> g.next & ((1ull << (g.shift - g.next)) - 1));
+          atomicAdd(&s.mass[b], whole(weight(x)));
+          atomicAdd(&s.count[b], 1u);
+        });
       }
       __syncthreads();
       scan_bins(s, range_m, range_n);
@@ -284,9 +429,8 @@ __global__ __launch_bounds__(ST) void sample_tokens_kernel(SampleArgs a) {
       }
       if (step == 1) {
         if (top_p < 1.0f) {
-          const double v = uniform(ceil((double)top_p * (double)m));
           by_count = false;
-          t = v >= 1.0 ? min((u64)v, m) - 1 : 0;
+          t = bound_p(m);
           known = true;
         } else {
           step = 2;
@@ -294,58 +438,116 @@ __global__ __launch_bounds__(ST) void sample_tokens_kernel(SampleArgs a) {
       }
       if (step == 2) {
         if (min_p > 0.0f && keep_n < n) n = keep_n > 0 ? keep_n : 1, m = keep_n > 0 ? keep_m : (u64)ONE;
-        const double v = uniform(floor((double)a.u[row] * (double)m));
         by_count = false;
-        t = v >= 0.0 ? min((u64)v, m - 1) : 0;
+        t = bound_u(m);
         known = true;
       }
     }
-    const Found f = find_bin(s, by_count, t - (by_count ? base_n : base_m), range_m, range_n);
-    if (in_bin < 0) {
-      in_bin = f.bin;
-    } else {
-      prefix = (shift == 64 ? 0 : prefix << (shift - next)) | (u64)f.bin;
-      shift = next;
+    const int bin = bin_of_total(s, by_count, t - (by_count ? g.count : g.mass));
+    const u64 before_m = mass_before(s, bin, range_m);
+    const int before_n = count_before(s, bin, range_n), entries = count_before(s, bin + 1, range_n) - before_n;
+    g.mass += before_m;
+    g.count += (u64)before_n;
+    const bool near = g.level == kNear;
+    if (g.level == kKeys) {
+      g.prefix = (g.shift == 64 ? 0 : g.prefix << (g.shift - g.next)) | (u64)bin;
+      g.shift = g.next;
     }
-    base_m += f.mass;
-    base_n += f.count;
-    if (f.entries > LIST) {
-      next = shift > 11 ? shift - 11 : 0;
+    if (entries > LIST) {  // divide the bin
+      if (near && bin == BINS - 1 && !weight.infinite) {
+        g.level = kFar;
+      } else {
+        if (g.level != kKeys) g.from = g.level, g.bin = bin, g.level = kKeys;
+        g.next = g.shift > 11 ? g.shift - 11 : 0;
+      }
+      __syncthreads();
       have = false;
       continue;
     }
-    // the entries that are left, ranked by comparing each with all
+    // The bin's entries, from the list or, to the list, from the row.
+    const auto in_list = [&](int b) {
+      return (b >= iv[0][0] && b < iv[0][1]) || (b >= iv[1][0] && b < iv[1][1]) || (b >= iv[2][0] && b < iv[2][1]);
+    };
+    if (!listed_all && !(near && in_list(bin))) {
+      iv[0][0] = bin, iv[0][1] = bin + 1;
+      iv[1][0] = iv[1][1] = iv[2][0] = iv[2][1] = 0;
+      if (near) {
+        // where the searches that follow can end, from the mass that this one leaves
+        u64 lo = mass_before(s, bin, range_m), hi = mass_before(s, bin + 1, range_m);
+        auto follow = [&](int w, u64 t_lo, u64 t_hi) {
+          iv[w][0] = bin_of_total(s, false, t_lo);
+          iv[w][1] = bin_of_total(s, false, t_hi) + 1;
+          lo = mass_before(s, iv[w][0], range_m);
+          hi = mass_before(s, iv[w][1], range_m);
+        };
+        if (lo == 0) lo = 1;  // (a search leaves at least an entry)
+        if (step == 0 && top_p < 1.0f) follow(1, bound_p(lo), bound_p(hi));
+        if (step < 2) {
+          if (lo == 0) lo = 1;
+          if (min_p > 0.0f && keep_n > 0) lo = min(lo, keep_m), hi = min(hi, keep_m);
+          follow(2, bound_u(lo), bound_u(hi));
+        }
+        int total = entries;
+        for (int w = 1; w < 3; ++w)
+          if (iv[w][1] > iv[w][0]) total += count_before(s, iv[w][1], range_n) - count_before(s, iv[w][0], range_n);
+        if (total > CAND || iv[1][1] >= BINS || iv[2][1] >= BINS || bin == BINS - 1)
+          iv[1][0] = iv[1][1] = iv[2][0] = iv[2][1] = 0;
+      }
+      if (tid == 0) s.n_cand = 0;
+      __syncthreads();
+      if (near && bin < BINS - 1) {
+        float f0[3], f1[3];
+        for (int w = 0; w < 3; ++w) f0[w] = (float)iv[w][0], f1[w] = (float)iv[w][1];
+        each_entry<BF, 4>(x0, V, [&](float x, int i) {
+          if (!candidate(x)) return;
+          const float d = distance(x);
+          if ((d >= f0[0] && d < f1[0]) || (d >= f0[1] && d < f1[1]) || (d >= f0[2] && d < f1[2])) keep(x + 0.0f, i);
+        });
+      } else {
+        const int level = g.level;
+        if (level != kKeys) g.from = level, g.bin = bin, g.level = kKeys;  // inside(): this bin
+        each([&](float x, int i) {
+          if (inside(x, i)) keep(x, i);
+        });
+        g.level = level;
+      }
+    }
     if (tid == 0) s.n_list = 0;
     __syncthreads();
-    each_entry<BF>(x0, V, [&](float x, int i) {
-      x += 0.0f;
-      if (!inside(x, i)) return;
-      const int at = atomicAdd(&s.n_list, 1);
-      if (at < LIST) s.lx[at] = x, s.li[at] = i;
-    });
+    const int kept = uniform(min(s.n_cand, CAND));
+    {
+      const int level = g.level;
+      if (level != kKeys) g.from = level, g.bin = bin, g.level = kKeys;
+      for (int e = tid; e < kept; e += ST) {
+        const float x = s.cx[e];
+        if (!inside(x, s.ci[e])) continue;
+        const int at = atomicAdd(&s.n_list, 1);
+        if (at < LIST) s.lk[at] = order_key(x, s.ci[e]), s.lw[at] = whole(weight(x));
+      }
+      g.level = level;
+    }
     __syncthreads();
+    // ranked by comparing each with all
     const int listed = uniform(min(s.n_list, LIST));
-    for (int e = tid; e < listed; e += ST) s.lw[e] = fixed(weight(s.lx[e]));
-    __syncthreads();
     for (int e = tid; e < listed; e += ST) {
-      const u64 key = order_key(s.lx[e], s.li[e]), w = s.lw[e];
-      u64 rank = base_n, cum = base_m;
+      const u64 key = s.lk[e], w = s.lw[e];
+      u64 rank = g.count, cum = g.mass;
 #pragma unroll 4
       for (int j = 0; j < listed; ++j)
-        if (order_key(s.lx[j], s.li[j]) < key) ++rank, cum += s.lw[j];
+        if (s.lk[j] < key) ++rank, cum += s.lw[j];
       const u64 lo = by_count ? rank : cum, hi = by_count ? rank + 1 : cum + w;
-      if (lo <= t && t < hi) s.rank = rank + 1, s.cum = cum + w, s.own = w, s.pos = s.li[e];
+      if (lo <= t && t < hi) s.rank = rank + 1, s.cum = cum + w, s.own = w, s.pos = (int)(uint32_t)key;
     }
     __syncthreads();
     if (step == 2) break;
     if (uniform(s.rank) < n) n = uniform(s.rank), m = uniform(s.cum);
     __syncthreads();
     // a divided bin's histogram is of no use for the next search
-    if (shift != 64) have = false;
-    if (have) range_m = all_m, range_n = all_n;
-    in_bin = -1;
-    shift = next = 64;
-    prefix = base_m = base_n = 0;
+    if (!near) {
+      have = false;
+      iv[0][1] = iv[1][1] = iv[2][1] = 0;
+    }
+    g = Range{kNear, 0, 64, 64, kNear, 0, 0, 0};
     known = false;
     ++step;
   }
