@@ -90,9 +90,8 @@ constexpr int TABLE = 64;
 struct Weights {
   const double *table;  // 2^42 2^(j / 64), in LDS
   double top, rate;
-  bool infinite;        // the maximum is +Inf: its like weigh 1, nothing else is a candidate
+  // (-Inf and NaN, which are no candidates, weigh 0)
   __device__ __forceinline__ double operator()(float x) const {
-    if (infinite) return ONE;
     const double y = fmax(((double)x - top) * rate, -1000.0);
     const double magic = 6755399441055744.0;  // 1.5 2^52: y 64 rounded to nearest in the low bits
     const double t = fma(y, 64.0, magic);
@@ -113,40 +112,49 @@ __device__ __forceinline__ u64 whole(double w) {
   return (u64)__double_as_longlong(w + big) - (u64)__double_as_longlong(big);
 }
 
-// The row's entries, each once, as f(x, index): 16-byte loads of the aligned part,
-// DEEP of them ahead of the one that is worked on.
+// The row's entries, each once, as f(x, i): x four entries from index i on, in rising
+// order for a lane, NaN past the row's ends.  16-byte loads of the aligned part, DEEP
+// of them ahead of the one that is worked on; the ends are chunks of their own.
 template <bool BF, int DEEP, class F>
-__device__ __forceinline__ void each_entry(const void *row, int V, F f) {
+__device__ __forceinline__ void each_four(const void *row, int V, F f) {
   constexpr int PER = BF ? 8 : 4, ES = BF ? 2 : 4;
   const char *p = static_cast<const char *>(row);
-  const int tid = threadIdx.x;
-  auto one = [&](int i) {
-    f(BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]) : reinterpret_cast<const float *>(p)[i], i);
-  };
-  const int head = min(V, (int)((16 - ((uintptr_t)p & 15)) & 15) / ES);
-  const int chunks = (V - head) / PER;
-  const u32x4 *body = reinterpret_cast<const u32x4 *>(p + head * ES);
+  const int head = min(V, (int)((16 - ((uintptr_t)p & 15)) & 15) / ES), chunks = (V - head) / PER;
+  const u32x4 *body = reinterpret_cast<const u32x4 *>(p + head * ES) - 1;  // chunk 0 is the head
   u32x4 ahead[DEEP];
+  auto load = [&](int c) { return c > 0 && c <= chunks ? body[c] : u32x4{0, 0, 0, 0}; };
 #pragma unroll
-  for (int d = 0; d < DEEP; ++d)
-    if (tid + d * ST < chunks) ahead[d] = body[tid + d * ST];
-  if (tid < head) one(tid);
-  for (int i = head + chunks * PER + tid; i < V; i += ST) one(i);
+  for (int d = 0; d < DEEP; ++d) ahead[d] = load(threadIdx.x + d * ST);
 #pragma unroll 1
-  for (int c = tid; c < chunks; c += ST) {
+  for (int c = threadIdx.x; c < chunks + 2; c += ST) {
     const u32x4 v = ahead[0];
 #pragma unroll
     for (int d = 0; d + 1 < DEEP; ++d) ahead[d] = ahead[d + 1];
-    if (c + DEEP * ST < chunks) ahead[DEEP - 1] = body[c + DEEP * ST];
+    ahead[DEEP - 1] = load(c + DEEP * ST);
+    const int i = c == 0 ? 0 : head + (c - 1) * PER;
+    float x[PER];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int i = head + c * PER + e * (PER / 4);
       if constexpr (BF) {
-        f(__uint_as_float(v[e] << 16), i);
-        f(__uint_as_float(v[e] & 0xffff0000u), i + 1);
+        x[2 * e] = __uint_as_float(v[e] << 16);
+        x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
       } else {
-        f(__uint_as_float(v[e]), i);
+        x[e] = __uint_as_float(v[e]);
       }
+    }
+    if (c == 0 || c > chunks) {
+      const int end = c == 0 ? head : V;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        x[e] = __builtin_nanf("");
+        if (i + e < end)
+          x[e] = BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i + e]) : reinterpret_cast<const float *>(p)[i + e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < PER; e += 4) {
+      const float y[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]};
+      f(y, i + e);
     }
   }
 }
@@ -157,7 +165,7 @@ struct Shared {
   double table[TABLE];
   float cx[CAND];        // candidates kept from a pass
   int ci[CAND];
-  u64 lk[LIST], lw[LIST];  // a bin's order keys and weights
+  ulonglong2 list[LIST];  // a bin's order keys and weights
   u64 wave_m[ST / 64], wave_c[ST / 64];
   u64 key;               // the maximum's order key
   int n_cand, n_list, pos;
@@ -242,6 +250,67 @@ struct Range {
 };
 constexpr float PER_NAT = 128.0f;
 
+// The smallest x whose bin is at most b, for a bin that does not rise with x: 64 lanes
+// try 64 places of the order, six bits at a time.
+template <class B>
+__device__ __forceinline__ float least_in(B bin_of, int b) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t first = 0;  // the order's numbers up to `first` are in
+  for (int shift = 26;; shift = shift > 6 ? shift - 6 : 0) {
+    const u64 at = (u64)first + ((u64)lane << shift);
+    const uint32_t o = at > 0xff800000ull ? 0xff800000u : (uint32_t)at;  // (past -Inf: NaN)
+    const float x = __uint_as_float(o & 0x80000000u ? o : ~o & 0x7fffffffu);
+    // the order begins with NaNs, which no entry is: they count as in
+    const u64 in = __ballot(at <= 0xff800000ull && (x != x || bin_of(x) <= b));
+    first += (uint32_t)(63 - __builtin_clzll(in | 1)) << shift;
+    if (shift == 0) break;
+  }
+  return uniform(__uint_as_float(first & 0x80000000u ? first : ~first & 0x7fffffffu));
+}
+
+// A row with +Inf: its like weigh 1 and nothing else is a candidate, so each setting
+// leaves a number of them, by index.
+template <bool BF>
+__device__ void sample_infinite(const SampleArgs &a, Shared &s, const char *row, int r, int k, float top_p, float min_p) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto is_inf = [&](int i) {
+    return i < a.V && (BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(row)[i]) : reinterpret_cast<const float *>(row)[i]) ==
+                          __builtin_inff();
+  };
+  if (tid == 0) s.n_list = 0;
+  __syncthreads();
+  int mine = 0;
+  for (int i = tid; i < a.V; i += ST) mine += is_inf(i);
+  atomicAdd(&s.n_list, mine);
+  __syncthreads();
+  int n = s.n_list;
+  if (k > 0) n = min(n, k);
+  if (top_p < 1.0f) n = min(n, max(1, (int)ceil((double)top_p * n)));
+  if (min_p > 1.0f) n = 1;
+  const double at = floor((double)a.u[r] * n);
+  const int pick = at >= 0.0 ? min(n - 1, (int)fmin(at, 2e9)) : 0;
+  // the pick-th of them, a tile of lanes at a time
+  int before = 0;
+  for (int i0 = 0; i0 < a.V; i0 += ST) {
+    const bool in = is_inf(i0 + tid);
+    const u64 votes = __ballot(in);
+    if (lane == 0) s.wave_c[wave] = __popcll(votes);
+    __syncthreads();
+    int total = 0, place = before + __popcll(votes & ((1ull << lane) - 1));
+    for (int v = 0; v < ST / 64; ++v) {
+      if (v < wave) place += (int)s.wave_c[v];
+      total += (int)s.wave_c[v];
+    }
+    if (in && place == pick) {
+      a.tokens[r] = i0 + tid;
+      if (a.probs) a.probs[r] = (float)(1.0 / n);
+    }
+    before += total;
+    __syncthreads();
+    if (before > pick) break;
+  }
+}
+
 template <bool BF>
 __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   __shared__ Shared s;
@@ -258,8 +327,13 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   float mine = -__builtin_inff();  // this lane's maximum
   {
     int at = 0;
-    each_entry<BF, 8>(x0, V, [&](float x, int i) {
-      if (x > mine || (x == mine && i < at)) mine = x, at = i;
+    each_four<BF, 8>(x0, V, [&](const float (&x)[4], int i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool more = x[e] > mine;
+        mine = more ? x[e] : mine;
+        at = more ? i + e : at;
+      }
     });
     u64 key = mine > -__builtin_inff() ? order_key(mine + 0.0f, at) : ~0ull;  // -0 is 0
     for (int off = 32; off; off >>= 1) key = min(key, (u64)__shfl_xor(key, off));
@@ -279,24 +353,24 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   }
   const uint32_t ob = (uint32_t)(best >> 32);
   const float top = __uint_as_float(ob & 0x80000000u ? ob : ~ob & 0x7fffffffu);
+  if (top == __builtin_inff()) {
+    sample_infinite<BF>(a, s, x0, row, k, top_p, min_p);
+    return;
+  }
   Weights weight;
   weight.table = s.table;
-  weight.infinite = top == __builtin_inff();
   weight.rate = uniform(1.4426950408889634074 / (double)temp);
   weight.top = uniform((double)top);
-  const float floor_x = weight.infinite ? 3.402823466e38f : -__builtin_inff();  // candidates are above
-  auto candidate = [&](float x) { return x > floor_x; };
   const float per = uniform(PER_NAT / temp);
-  // a bin is the whole part of this (monotone in x, a NaN of 0 Inf included: then
-  // everything is in the last bin)
-  auto distance = [&](float x) { return fminf(weight.infinite ? 0.0f : (top - x) * per, (float)(BINS - 1)); };
-  auto near_bin = [&](float x) { return (int)distance(x); };
+  // a bin is the whole part of this (it does not rise with x, a NaN of 0 Inf included:
+  // then everything is in the last bin)
+  auto near_bin = [&](float x) { return (int)fminf((top - x) * per, (float)(BINS - 1)); };
   auto far_bin = [&](float x) {
     return (int)fminf(fmaxf((top - x) * per * 0.25f - (float)(BINS / 4), 0.0f), (float)(BINS - 1));
   };
   auto keep = [&](float x, int i) {  // to the list in LDS
     const int at = atomicAdd(&s.n_cand, 1);
-    if (at < CAND) s.cx[at] = x, s.ci[at] = i;
+    if (at < CAND) s.cx[at] = x + 0.0f, s.ci[at] = i;
   };
 
   // The entries that the searches look at: the row's, or the list's where it holds
@@ -304,17 +378,22 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   bool listed_all = false;
   u64 range_m = 0, range_n = 0;
   if (V <= CAND || (k > 0 && k <= ST / 2)) {
-    int last = BINS - 1;  // the list's last bin
+    float least = -3.402823466e38f;  // the list's last entry
+    bool small = true;
     if (V > CAND) {
-      if (candidate(mine)) atomicAdd(&s.count[near_bin(mine + 0.0f)], 1u);
+      if (mine > -__builtin_inff()) atomicAdd(&s.count[near_bin(mine)], 1u);
       __syncthreads();
       scan_bins(s, range_m, range_n);
-      last = range_n >= (u64)k ? bin_of_total(s, true, (u64)k - 1) : BINS;
+      const int last = range_n >= (u64)k ? bin_of_total(s, true, (u64)k - 1) : BINS - 1;
+      small = last < BINS - 1;
+      if (small) least = least_in(near_bin, last);
     }
-    if (last < (V > CAND ? BINS - 1 : BINS)) {
-      each_entry<BF, 4>(x0, V, [&](float x, int i) {
-        x += 0.0f;
-        if (candidate(x) && near_bin(x) <= last) keep(x, i);
+    if (small) {
+      each_four<BF, 4>(x0, V, [&](const float (&x)[4], int i) {
+        if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= least)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (x[e] >= least) keep(x[e], i + e);
       });
       __syncthreads();
       listed_all = uniform(s.n_cand) <= CAND;
@@ -323,17 +402,15 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
     if (!listed_all && tid == 0) s.n_cand = 0;
   }
   const int n_all = listed_all ? uniform(s.n_cand) : 0;
-  auto each_listed = [&](auto f) __attribute__((always_inline)) {
-#pragma unroll 1
-    for (int e = tid; e < n_all; e += ST) f(s.cx[e], s.ci[e]);
-  };
   auto each = [&](auto f) __attribute__((always_inline)) {
     if (listed_all) {
-      each_listed(f);
+#pragma unroll 1
+      for (int e = tid; e < n_all; e += ST) f(s.cx[e], s.ci[e]);
     } else {
-      each_entry<BF, 4>(x0, V, [&](float x, int i) {
-        x += 0.0f;
-        if (candidate(x)) f(x, i);
+      each_four<BF, 4>(x0, V, [&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x[e] > -__builtin_inff()) f(x[e] + 0.0f, i + e);
       });
     }
   };
@@ -368,24 +445,39 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
         u64 kn = 0, km = 0, om = 0, oc = 0;
         const bool count_min = min_p > 0.0f;
         const double least = uniform((double)min_p * ONE);
-        auto add = [&](float x, int) __attribute__((always_inline)) {
-          const bool counts = candidate(x);
-          const double w = counts ? weight(x) : 0.0;
-          const u64 f = whole(w);
-          const int b = counts ? near_bin(x) : BINS - 1;
-          if (b < BINS - 1) {
-            atomicAdd(&s.mass[b], f);
-            atomicAdd(&s.count[b], 1u);
-          } else {
-            om += f;
-            oc += counts;
+        auto add = [&](const float (&x)[4], int) __attribute__((always_inline)) {
+          double w[4];
+          u64 f[4];
+          int b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[e] = weight(x[e]);
+            f[e] = whole(w[e]);
+            b[e] = near_bin(x[e]);
+            om += b[e] < BINS - 1 ? 0 : f[e];
+            oc += b[e] == BINS - 1 && x[e] > -__builtin_inff();
           }
-          if (count_min && counts && w >= least) ++kn, km += f;
+          if (count_min)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (w[e] >= least) ++kn, km += f[e];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (b[e] < BINS - 1) {
+              atomicAdd(&s.mass[b[e]], f[e]);
+              atomicAdd(&s.count[b[e]], 1u);
+            }
         };
-        if (listed_all)
-          each_listed(add);
-        else
-          each_entry<BF, 4>(x0, V, add);
+        if (listed_all) {
+          const float none = __builtin_nanf("");
+#pragma unroll 1
+          for (int e = tid; e < n_all; e += ST) {
+            const float x[4] = {s.cx[e], none, none, none};
+            add(x, 0);
+          }
+        } else {
+          each_four<BF, 4>(x0, V, add);
+        }
         for (int off = 32; off; off >>= 1) {
           kn += __shfl_xor(kn, off), km += __shfl_xor(km, off);
           om += __shfl_xor(om, off), oc += __shfl_xor(oc, off);
@@ -454,7 +546,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
       g.shift = g.next;
     }
     if (entries > LIST) {  // divide the bin
-      if (near && bin == BINS - 1 && !weight.infinite) {
+      if (near && bin == BINS - 1) {
         g.level = kFar;
       } else {
         if (g.level != kKeys) g.from = g.level, g.bin = bin, g.level = kKeys;
@@ -496,12 +588,23 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
       if (tid == 0) s.n_cand = 0;
       __syncthreads();
       if (near && bin < BINS - 1) {
-        float f0[3], f1[3];
-        for (int w = 0; w < 3; ++w) f0[w] = (float)iv[w][0], f1[w] = (float)iv[w][1];
-        each_entry<BF, 4>(x0, V, [&](float x, int i) {
-          if (!candidate(x)) return;
-          const float d = distance(x);
-          if ((d >= f0[0] && d < f1[0]) || (d >= f0[1] && d < f1[1]) || (d >= f0[2] && d < f1[2])) keep(x + 0.0f, i);
+        float lo[3], hi[3];  // the intervals as logits: [lo, hi)
+        for (int w = 0; w < 3; ++w) {
+          const bool any = iv[w][1] > iv[w][0];
+          lo[w] = any ? least_in(near_bin, iv[w][1] - 1) : __builtin_inff();
+          hi[w] = any && iv[w][0] > 0 ? least_in(near_bin, iv[w][0] - 1) : __builtin_inff();
+        }
+        each_four<BF, 4>(x0, V, [&](const float (&x)[4], int i) {
+          bool in[4], any = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            in[e] = (x[e] >= lo[0] && x[e] < hi[0]) | (x[e] >= lo[1] && x[e] < hi[1]) | (x[e] >= lo[2] && x[e] < hi[2]);
+            any |= in[e];
+          }
+          if (any)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (in[e]) keep(x[e], i + e);
         });
       } else {
         const int level = g.level;
@@ -522,7 +625,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
         const float x = s.cx[e];
         if (!inside(x, s.ci[e])) continue;
         const int at = atomicAdd(&s.n_list, 1);
-        if (at < LIST) s.lk[at] = order_key(x, s.ci[e]), s.lw[at] = whole(weight(x));
+        if (at < LIST) s.list[at] = make_ulonglong2(order_key(x, s.ci[e]), whole(weight(x)));
       }
       g.level = level;
     }
@@ -530,11 +633,16 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
     // ranked by comparing each with all
     const int listed = uniform(min(s.n_list, LIST));
     for (int e = tid; e < listed; e += ST) {
-      const u64 key = s.lk[e], w = s.lw[e];
-      u64 rank = g.count, cum = g.mass;
-#pragma unroll 4
-      for (int j = 0; j < listed; ++j)
-        if (s.lk[j] < key) ++rank, cum += s.lw[j];
+      const u64 key = s.list[e].x, w = s.list[e].y;
+      uint32_t ahead = 0;
+      u64 cum = g.mass;
+#pragma unroll 8
+      for (int j = 0; j < listed; ++j) {
+        const ulonglong2 v = s.list[j];
+        ahead += v.x < key;
+        cum += v.x < key ? v.y : 0;
+      }
+      const u64 rank = g.count + ahead;
       const u64 lo = by_count ? rank : cum, hi = by_count ? rank + 1 : cum + w;
       if (lo <= t && t < hi) s.rank = rank + 1, s.cum = cum + w, s.own = w, s.pos = (int)(uint32_t)key;
     }
