@@ -16,8 +16,9 @@
 // distance of u from the nearest of 10^5 borders.
 //
 // A workgroup takes a row.  What bounds it: each pass over a long row is at the rate
-// of the memory behind the L2 (256 rows of 128000 f32: 19 us), and the weights' f64
-// arithmetic, so passes are saved:
+// of the memory behind the L2 (256 rows of 128000 f32, 131 MB: 18 us), and in the
+// histogram's pass the f64 arithmetic and the LDS atomics (46 us of those rows' 125), so
+// passes and work in them are saved:
 //  - the maximum, always;
 //  - with top-k, the entries that can be among the k: at least k of the lanes' own
 //    maxima are in the bins up to the k-th's, so all entries up to that bin are
@@ -25,6 +26,8 @@
 //  - else the histogram, with every entry's weight, and then the entries of the
 //    bins that the searches end in, in one pass for all of them: the bin that one
 //    search ends in bounds the mass that the next one starts from.
+// A row alone (one of 32000: 19 us, of which 5 are a call of nothing) is a chain of
+// such steps, each with a barrier and an LDS or memory latency.
 // A bin of more than LIST entries (equal logits, say) is divided further by the
 // order's own key, the logit's bits and then the index, eleven bits at a time.
 #include <hip/hip_runtime.h>
@@ -85,78 +88,113 @@ __device__ __forceinline__ double exp2_small(double y) {
 
 // The weights of a row: 2^42 2^y, y = (x - top) rate, as a whole power, a table of
 // 64ths and the Taylor polynomial of what is left, |r| <= 1/128, to degree 4 (the next
-// term is 4e-14, a third of the last bit of a weight's whole number).
+// term is 4e-14, a third of the last bit of a weight's whole number).  A polynomial of
+// degree 9 in place of the table took 133 us for 256 rows of 128000 f32 to this one's 125.
 constexpr int TABLE = 64;
 struct Weights {
   const double *table;  // 2^42 2^(j / 64), in LDS
   double top, rate;
   // (-Inf and NaN, which are no candidates, weigh 0)
-  __device__ __forceinline__ double operator()(float x) const {
-    const double y = fmax(((double)x - top) * rate, -1000.0);
-    const double magic = 6755399441055744.0;  // 1.5 2^52: y 64 rounded to nearest in the low bits
-    const double t = fma(y, 64.0, magic);
+  __device__ __forceinline__ double power(float x) const { return fmax(((double)x - top) * rate, -1000.0); }
+  static constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: a sum's low bits are the other's nearest whole number
+  // The weight as a whole number, rounded to nearest (the significand of w + 2^52), and
+  // -k, the 64ths of y.
+  __device__ __forceinline__ u64 operator()(float x, int &bin) const {
+    const double y = power(x), t = fma(y, 64.0, MAGIC);
     const int k = (int)__double_as_longlong(t);
-    const double r = fma(t - magic, -1.0 / 64, y);
+    bin = -k;
+    const double r = fma(t - MAGIC, -1.0 / 64, y);
     constexpr double L = 0.69314718055994530942;
     double p = L * L * L * L / 24;
     p = fma(p, r, L * L * L / 6);
     p = fma(p, r, L * L / 2);
     p = fma(p, r, L);
     p = fma(p, r, 1.0);
-    return ldexp(table[k & (TABLE - 1)] * p, k >> 6);
+    // (k is above -2^16: the exponent's field cannot underflow)
+    const double big = 4503599627370496.0;  // 2^52
+    const double scale = __longlong_as_double(__double_as_longlong(table[k & (TABLE - 1)]) + ((long long)(k & -TABLE) << 46));
+    return (u64)__double_as_longlong(fma(scale, p, big)) - (u64)__double_as_longlong(big);
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    int bin;
+    return (*this)(x, bin);
+  }
+  // -k alone, for any x that is not NaN.
+  __device__ __forceinline__ int steps(float x) const {
+    return -(int)__double_as_longlong(fma(fmin(power(x), 0.0), 64.0, MAGIC));
   }
 };
-// A weight's whole number, rounded to nearest: the significand of w + 2^52.
-__device__ __forceinline__ u64 whole(double w) {
-  const double big = 4503599627370496.0;  // 2^52
-  return (u64)__double_as_longlong(w + big) - (u64)__double_as_longlong(big);
-}
 
 // The row's entries, each once, as f(x, i): x four entries from index i on, in rising
-// order for a lane, NaN past the row's ends.  16-byte loads of the aligned part, DEEP
-// of them ahead of the one that is worked on; the ends are chunks of their own.
-template <bool BF, int DEEP, class F>
-__device__ __forceinline__ void each_four(const void *row, int V, F f) {
-  constexpr int PER = BF ? 8 : 4, ES = BF ? 2 : 4;
+// order for a lane, NaN past the row's ends.  After a round of n entries done(i0, n): the
+// j-th of them has index i0 + j / PER ST PER + j % PER.  16-byte loads of the aligned
+// part, UN of them together a round ahead (a longer queue costs a move each step for
+// every register in it); the ends are chunks of their own.  f32 rows take 4 or 8 copies of f
+// for 4 entries each, which hides the loads' latency; a bf16 row's load has 8 entries,
+// and more copies only make the code longer (96 rows of 50257: 49 us, with 4 and 2 58).
+template <bool BF>
+constexpr int PER = BF ? 8 : 4;
+template <bool BF, int UN, class F, class D>
+__device__ __forceinline__ void each_four(const void *row, int V, F f, D done) {
+  constexpr int PER = npu::PER<BF>, ES = BF ? 2 : 4;
   const char *p = static_cast<const char *>(row);
   const int head = min(V, (int)((16 - ((uintptr_t)p & 15)) & 15) / ES), chunks = (V - head) / PER;
-  const u32x4 *body = reinterpret_cast<const u32x4 *>(p + head * ES) - 1;  // chunk 0 is the head
-  u32x4 ahead[DEEP];
-  auto load = [&](int c) { return c > 0 && c <= chunks ? body[c] : u32x4{0, 0, 0, 0}; };
-#pragma unroll
-  for (int d = 0; d < DEEP; ++d) ahead[d] = load(threadIdx.x + d * ST);
-#pragma unroll 1
-  for (int c = threadIdx.x; c < chunks + 2; c += ST) {
-    const u32x4 v = ahead[0];
-#pragma unroll
-    for (int d = 0; d + 1 < DEEP; ++d) ahead[d] = ahead[d + 1];
-    ahead[DEEP - 1] = load(c + DEEP * ST);
-    const int i = c == 0 ? 0 : head + (c - 1) * PER;
-    float x[PER];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (BF) {
-        x[2 * e] = __uint_as_float(v[e] << 16);
-        x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
-      } else {
-        x[e] = __uint_as_float(v[e]);
-      }
-    }
-    if (c == 0 || c > chunks) {
-      const int end = c == 0 ? head : V;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        x[e] = __builtin_nanf("");
-        if (i + e < end)
-          x[e] = BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i + e]) : reinterpret_cast<const float *>(p)[i + e];
-      }
-    }
+  const u32x4 *body = reinterpret_cast<const u32x4 *>(p + head * ES);
+  auto give = [&](const float (&x)[PER], int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < PER; e += 4) {
       const float y[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]};
       f(y, i + e);
     }
+  };
+  u32x4 v[UN], next[UN] = {};
+#pragma unroll 1
+  for (int c0 = -1;; c0 = c0 < 0 ? 0 : c0 + UN * ST) {  // -1: the ends, a lane each
+    if (c0 >= chunks) break;
+#pragma unroll
+    for (int d = 0; d < UN; ++d) {
+      const int c = (c0 < 0 ? 0 : c0 + UN * ST) + d * ST + (int)threadIdx.x;
+      v[d] = next[d];
+      next[d] = u32x4{0, 0, 0, 0};
+      if (c < chunks) next[d] = body[c];
+    }
+    int i0 = 0;
+#pragma unroll
+    for (int d = 0; d < UN; ++d) {
+      const int c = c0 + d * ST + (int)threadIdx.x;
+      float x[PER];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (BF) {
+          x[2 * e] = __uint_as_float(v[d][e] << 16);
+          x[2 * e + 1] = __uint_as_float(v[d][e] & 0xffff0000u);
+        } else {
+          x[e] = __uint_as_float(v[d][e]);
+        }
+      }
+      int i = head + c * PER;
+      if (c0 < 0 || c >= chunks) {
+        // (the first two lanes of the first round: the head, the tail)
+        const bool tail = threadIdx.x == 1;
+        i = tail ? head + chunks * PER : 0;
+        const int end = c0 < 0 && d == 0 && threadIdx.x < 2 ? (tail ? V : head) : 0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          x[e] = __builtin_nanf("");
+          if (i + e < end)
+            x[e] = BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i + e]) : reinterpret_cast<const float *>(p)[i + e];
+        }
+        if (c0 < 0 && d > 0) break;
+      }
+      if (d == 0) i0 = i;
+      give(x, i);
+    }
+    done(i0, c0 < 0 ? PER : UN * PER);
   }
+}
+template <bool BF, int UN, class F>
+__device__ __forceinline__ void each_four(const void *row, int V, F f) {
+  each_four<BF, UN>(row, V, f, [](int, int) {});
 }
 
 struct Shared {
@@ -167,9 +205,10 @@ struct Shared {
   int ci[CAND];
   ulonglong2 list[LIST];  // a bin's order keys and weights
   u64 wave_m[ST / 64], wave_c[ST / 64];
-  u64 key;               // the maximum's order key
-  int n_cand, n_list, pos;
-  u64 rank, cum, own;    // the entry found: entries and mass up to it (inclusive), its mass
+  u64 key;               // the first index of the maximum
+  u64 total;             // the mass of all
+  int n_cand, n_list, pos, candidates;
+  u64 cum, own;          // the entry found: the mass up to it (inclusive), its own
 };
 
 // Exclusive prefix sums of the histogram in place; the totals to all lanes.
@@ -239,17 +278,15 @@ __device__ __forceinline__ int count_before(const Shared &s, int b, u64 all) {
   return b < BINS ? uniform((int)s.count[b]) : (int)all;
 }
 
-// What a histogram divides: the row by the distance from the maximum (kNear: 128 bins
-// a nat of weight for 16 nats, the rest in the last bin; kFar: that bin, 32 a nat), or
-// a bin by the order key's bits from `shift` down to `next`.
+// What a histogram divides: the row by the distance from the maximum (kNear: by 64ths of
+// the weight's power of two, for 32 powers, the rest in the last bin; kFar: that bin, by
+// 16ths), or a bin by the order key's bits from `shift` down to `next`.
 enum { kNear = 0, kFar = 1, kKeys = 2 };
 struct Range {
   int level, bin, shift, next;  // bin: of level `from`, that kKeys divides
   int from;
   u64 prefix, mass, count;      // mass, count: what comes before the range
 };
-constexpr float PER_NAT = 128.0f;
-
 // The smallest x whose bin is at most b, for a bin that does not rise with x: 64 lanes
 // try 64 places of the order, six bits at a time.
 template <class B>
@@ -268,10 +305,16 @@ __device__ __forceinline__ float least_in(B bin_of, int b) {
   return uniform(__uint_as_float(first & 0x80000000u ? first : ~first & 0x7fffffffu));
 }
 
+// The next float below a finite one.
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return x == 0.0f ? __uint_as_float(0x80000001u) : __uint_as_float(x > 0.0f ? b - 1 : b + 1);
+}
+
 // A row with +Inf: its like weigh 1 and nothing else is a candidate, so each setting
 // leaves a number of them, by index.
 template <bool BF>
-__device__ void sample_infinite(const SampleArgs &a, Shared &s, const char *row, int r, int k, float top_p, float min_p) {
+__device__ __forceinline__ void sample_infinite(const SampleArgs &a, Shared &s, const char *row, int r, int k, float top_p, float min_p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto is_inf = [&](int i) {
     return i < a.V && (BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(row)[i]) : reinterpret_cast<const float *>(row)[i]) ==
@@ -321,38 +364,45 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
 
   // the maximum and its first index
-  if (tid == 0) s.key = ~0ull, s.n_cand = 0;
+  if (tid == 0) s.key = ~0ull, s.n_cand = 0, s.candidates = 0;
   if (tid < TABLE) s.table[tid] = ONE * (tid < TABLE / 2 ? exp2_small(tid / 64.0) : 2.0 * exp2_small(tid / 64.0 - 1.0));
   __syncthreads();
   float mine = -__builtin_inff();  // this lane's maximum
-  {
-    int at = 0;
-    each_four<BF, 8>(x0, V, [&](const float (&x)[4], int i) {
+  int finite = 0;                  // its candidates
+  each_four<BF, BF ? 1 : 8>(x0, V, [&](const float (&x)[4], int) __attribute__((always_inline)) {
+    mine = fmaxf(fmaxf(fmaxf(mine, x[0]), fmaxf(x[1], x[2])), x[3]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool more = x[e] > mine;
-        mine = more ? x[e] : mine;
-        at = more ? i + e : at;
-      }
-    });
-    u64 key = mine > -__builtin_inff() ? order_key(mine + 0.0f, at) : ~0ull;  // -0 is 0
-    for (int off = 32; off; off >>= 1) key = min(key, (u64)__shfl_xor(key, off));
-    if (lane == 0) atomicMin(&s.key, key);
+    for (int e = 0; e < 4; ++e) finite += x[e] > -__builtin_inff();
+  });
+  {
+    float m = mine;
+    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off)), finite += __shfl_xor(finite, off);
+    if (lane == 0) s.wave_m[tid >> 6] = (u64)__float_as_uint(m), atomicAdd(&s.candidates, finite);
   }
   clear_bins(s);
-  const u64 best = uniform(s.key);
-  const int first = (int)(uint32_t)best;
-  // no candidate, or one that every setting leaves
-  const bool greedy = !(temp > 0.0f) || k == 1 || top_p <= 0.0f;
-  if (best == ~0ull || greedy) {
+  float top = -__builtin_inff();
+  for (int v = 0; v < ST / 64; ++v) top = fmaxf(top, __uint_as_float((uint32_t)s.wave_m[v]));
+  top = uniform(top) + 0.0f;  // -0 is 0
+  if (!(top > -__builtin_inff())) {
     if (tid == 0) {
-      a.tokens[row] = best == ~0ull ? -1 : first;
-      if (a.probs) a.probs[row] = best == ~0ull ? 0.0f : 1.0f;
+      a.tokens[row] = -1;
+      if (a.probs) a.probs[row] = 0.0f;
     }
     return;
   }
-  const uint32_t ob = (uint32_t)(best >> 32);
-  const float top = __uint_as_float(ob & 0x80000000u ? ob : ~ob & 0x7fffffffu);
+  if (!(temp > 0.0f) || k == 1 || top_p <= 0.0f) {  // the first of the largest
+    each_four<BF, BF ? 1 : 8>(x0, V, [&](const float (&x)[4], int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (x[e] == top) atomicMin(&s.key, (u64)(i + e));
+    });
+    __syncthreads();
+    if (tid == 0) {
+      a.tokens[row] = (int)s.key;
+      if (a.probs) a.probs[row] = 1.0f;
+    }
+    return;
+  }
   if (top == __builtin_inff()) {
     sample_infinite<BF>(a, s, x0, row, k, top_p, min_p);
     return;
@@ -361,16 +411,42 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   weight.table = s.table;
   weight.rate = uniform(1.4426950408889634074 / (double)temp);
   weight.top = uniform((double)top);
-  const float per = uniform(PER_NAT / temp);
-  // a bin is the whole part of this (it does not rise with x, a NaN of 0 Inf included:
-  // then everything is in the last bin)
-  auto near_bin = [&](float x) { return (int)fminf((top - x) * per, (float)(BINS - 1)); };
-  auto far_bin = [&](float x) {
-    return (int)fminf(fmaxf((top - x) * per * 0.25f - (float)(BINS / 4), 0.0f), (float)(BINS - 1));
-  };
-  auto keep = [&](float x, int i) {  // to the list in LDS
+  const int candidates = uniform(s.candidates);
+  auto near_bin = [&](float x) { return min(weight.steps(x), BINS - 1); };
+  auto far_bin = [&](float x) { return min((weight.steps(x) - (BINS - 1)) >> 2, BINS - 1); };  // of a last near bin's
+  auto keep = [&](float x, int i) __attribute__((always_inline)) {  // to the list in LDS
     const int at = atomicAdd(&s.n_cand, 1);
     if (at < CAND) s.cx[at] = x + 0.0f, s.ci[at] = i;
+  };
+
+  // All entries of the row for which in(x) to the list: a round's are marked in a bit
+  // each and then kept, by index, with one atomic addition a lane; their logits are read
+  // again at the end.  (Kept one by one the atomic's latency was most of the pass.)
+  auto keep_all = [&](auto in) __attribute__((always_inline)) {
+    uint32_t hits = 0;
+    auto mark = [&](const float (&x)[4], int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hits = hits * 2 + (in(x[e]) ? 1 : 0);
+    };
+    auto keep_marked = [&](int i0, int n) __attribute__((always_inline)) {
+      if (hits == 0) return;
+      int at = atomicAdd(&s.n_cand, __popc(hits));
+      while (hits) {
+        const int bit = 31 - __clz(hits), j = n - 1 - bit;
+        hits ^= 1u << bit;
+        if (at < CAND) s.ci[at] = i0 + j / PER<BF> * (ST * PER<BF>) + j % PER<BF>;
+        ++at;
+      }
+    };
+    each_four<BF, BF ? 1 : 8>(x0, V, mark, keep_marked);
+    __syncthreads();
+    const int kept = uniform(min(s.n_cand, CAND));
+#pragma unroll 4
+    for (int e = tid; e < kept; e += ST) {
+      const int i = s.ci[e];
+      s.cx[e] = (BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(x0)[i]) : reinterpret_cast<const float *>(x0)[i]) + 0.0f;
+    }
+    __syncthreads();
   };
 
   // The entries that the searches look at: the row's, or the list's where it holds
@@ -389,13 +465,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
       if (small) least = least_in(near_bin, last);
     }
     if (small) {
-      each_four<BF, 4>(x0, V, [&](const float (&x)[4], int i) {
-        if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= least)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (x[e] >= least) keep(x[e], i + e);
-      });
-      __syncthreads();
+      keep_all([&](float x) __attribute__((always_inline)) { return x >= least; });
       listed_all = uniform(s.n_cand) <= CAND;
     }
     __syncthreads();
@@ -407,7 +477,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
 #pragma unroll 1
       for (int e = tid; e < n_all; e += ST) f(s.cx[e], s.ci[e]);
     } else {
-      each_four<BF, 4>(x0, V, [&](const float (&x)[4], int i) {
+      each_four<BF, BF ? 1 : 4>(x0, V, [&](const float (&x)[4], int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (x[e] > -__builtin_inff()) f(x[e] + 0.0f, i + e);
@@ -416,7 +486,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   };
 
   Range g{kNear, 0, 64, 64, kNear, 0, 0, 0};
-  auto inside = [&](float x, int i) {  // of the range
+  auto inside = [&](float x, int i) __attribute__((always_inline)) {  // of the range
     if (near_bin(x) != (g.from == kNear && g.level == kKeys ? g.bin : BINS - 1)) return false;
     if (g.level == kFar) return true;
     if (g.from == kFar && far_bin(x) != g.bin) return false;
@@ -424,7 +494,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
   };
 
   // The searches in turn: 0 for top-k's count, 1 for top-p's mass, 2 for the draw.
-  u64 n = 0, m = 0, all_n = 0, all_m = 0, keep_n = 0, keep_m = 0, t = 0;
+  u64 m = 0, keep_m = 0, t = 0;
   const double u = uniform((double)a.u[row]);
   auto bound_p = [&](u64 mass) {
     const double v = uniform(ceil((double)top_p * (double)mass));
@@ -434,39 +504,41 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
     const double v = uniform(floor(u * (double)mass));
     return v >= 0.0 ? min((u64)v, mass - 1) : (u64)0;
   };
+  // min-p's bound lies in the bin of its power of two or, by rounding, one next to it;
+  // past the last bin but one, in any bin from there on
+  const u64 min_mass = min_p > 0.0f ? (u64)uniform(ceil(fmin((double)min_p, 2.0) * ONE)) : 0;
+  const int min_at = min_p > 0.0f ? (int)fminf(fmaxf(-64.0f * log2f(min_p), 0.0f), (float)(BINS - 2)) : 0;
+  const int min_bin = uniform(max(min_at - 1, 0));
+  const uint32_t min_bins = min_p > 0.0f ? (min_at < BINS - 2 ? 4u : 0x7fffffffu) : 0u;
+  // The entries of bins are counted where top-k needs it.  Elsewhere the bins' masses
+  // say it, from above, as all weights of a bin are alike: half of the atomics.
+  const bool counted = listed_all || k > 0;
   bool by_count = false, have = false, known = false;
   int iv[3][2] = {{0, 0}, {0, 0}, {0, 0}};  // the near bins whose entries are in the list: [first, past the last)
   for (int step = -1;;) {
     if (!have) {
-      if (tid == 0) s.rank = 0, s.cum = 0;
+      if (tid == 0) s.cum = 0, s.total = 0;
       clear_bins(s);
       if (g.level == kNear) {
-        // what min-p keeps is counted on the way; the last bin, without atomics, by lane
-        u64 kn = 0, km = 0, om = 0, oc = 0;
-        const bool count_min = min_p > 0.0f;
-        const double least = uniform((double)min_p * ONE);
+        // what min-p keeps of the bins that its bound can be in is counted on the way; the
+        // last bin, which most entries may be in, is what the others leave of the total
+        u64 km = 0, total = 0;
         auto add = [&](const float (&x)[4], int) __attribute__((always_inline)) {
-          double w[4];
           u64 f[4];
           int b[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            w[e] = weight(x[e]);
-            f[e] = whole(w[e]);
-            b[e] = near_bin(x[e]);
-            om += b[e] < BINS - 1 ? 0 : f[e];
-            oc += b[e] == BINS - 1 && x[e] > -__builtin_inff();
+            f[e] = weight(x[e], b[e]);
+            total += f[e];
           }
-          if (count_min)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (w[e] >= least) ++kn, km += f[e];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 4; ++e) {
             if (b[e] < BINS - 1) {
               atomicAdd(&s.mass[b[e]], f[e]);
-              atomicAdd(&s.count[b[e]], 1u);
+              if (counted) atomicAdd(&s.count[b[e]], 1u);
             }
+            if ((uint32_t)(b[e] - min_bin) < min_bins && f[e] >= min_mass) km += f[e];
+          }
         };
         if (listed_all) {
           const float none = __builtin_nanf("");
@@ -476,42 +548,39 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
             add(x, 0);
           }
         } else {
-          each_four<BF, 4>(x0, V, add);
+          each_four<BF, BF ? 1 : 4>(x0, V, add);
         }
         for (int off = 32; off; off >>= 1) {
-          kn += __shfl_xor(kn, off), km += __shfl_xor(km, off);
-          om += __shfl_xor(om, off), oc += __shfl_xor(oc, off);
+          km += __shfl_xor(km, off);
+          total += __shfl_xor(total, off);
         }
         if (lane == 0) {
-          atomicAdd(&s.mass[BINS - 1], om);
-          atomicAdd(&s.count[BINS - 1], (uint32_t)oc);
-          atomicAdd(&s.rank, kn);
+          atomicAdd(&s.total, total);
           atomicAdd(&s.cum, km);
         }
       } else {
-        each([&](float x, int i) {
+        each([&](float x, int i) __attribute__((always_inline)) {
           if (!inside(x, i)) return;
           const int b = g.level == kFar ? far_bin(x)
                                         : (int)(order_key(x, i) >> g.next & ((1ull << (g.shift - g.next)) - 1));
-          atomicAdd(&s.mass[b], whole(weight(x)));
+          atomicAdd(&s.mass[b], weight(x));
           atomicAdd(&s.count[b], 1u);
         });
       }
       __syncthreads();
       scan_bins(s, range_m, range_n);
+      if (g.level == kNear) range_m = uniform(s.total), range_n = (u64)(listed_all ? n_all : candidates);
       have = true;
     }
     if (step < 0) {
-      keep_n = uniform(s.rank);
-      keep_m = uniform(s.cum);
-      n = all_n = range_n;
-      m = all_m = range_m;
+      keep_m = uniform(s.cum) + mass_before(s, min_bin, range_m);
+      m = range_m;
       step = 0;
       __syncthreads();
     }
     if (!known) {  // the search's bound
       if (step == 0) {
-        if (k > 0 && (u64)k < n) {
+        if (k > 0 && (u64)k < range_n) {
           by_count = true;
           t = (u64)k - 1;
           known = true;
@@ -529,15 +598,22 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
         }
       }
       if (step == 2) {
-        if (min_p > 0.0f && keep_n < n) n = keep_n > 0 ? keep_n : 1, m = keep_n > 0 ? keep_m : (u64)ONE;
+        if (min_p > 0.0f) m = min(m, keep_m > 0 ? keep_m : (u64)ONE);
         by_count = false;
         t = bound_u(m);
         known = true;
       }
     }
+    auto entries_of = [&](int from, int to) {
+      if (counted || g.level != kNear) return count_before(s, to, range_n) - count_before(s, from, range_n);
+      if (to == BINS) return CAND + 1;
+      const float least = exp2f(42.0f - ((float)to - 0.5f) / 64.0f);  // of a weight
+      return uniform((int)fminf((float)(mass_before(s, to, range_m) - mass_before(s, from, range_m)) / least * 1.01f + 1.0f, CAND + 1.0f));
+    };
     const int bin = bin_of_total(s, by_count, t - (by_count ? g.count : g.mass));
     const u64 before_m = mass_before(s, bin, range_m);
-    const int before_n = count_before(s, bin, range_n), entries = count_before(s, bin + 1, range_n) - before_n;
+    const int before_n = count_before(s, bin, range_n);
+    const int entries = entries_of(bin, bin + 1);
     g.mass += before_m;
     g.count += (u64)before_n;
     const bool near = g.level == kNear;
@@ -566,7 +642,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
       if (near) {
         // where the searches that follow can end, from the mass that this one leaves
         u64 lo = mass_before(s, bin, range_m), hi = mass_before(s, bin + 1, range_m);
-        auto follow = [&](int w, u64 t_lo, u64 t_hi) {
+        auto follow = [&](int w, u64 t_lo, u64 t_hi) __attribute__((always_inline)) {
           iv[w][0] = bin_of_total(s, false, t_lo);
           iv[w][1] = bin_of_total(s, false, t_hi) + 1;
           lo = mass_before(s, iv[w][0], range_m);
@@ -576,40 +652,39 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
         if (step == 0 && top_p < 1.0f) follow(1, bound_p(lo), bound_p(hi));
         if (step < 2) {
           if (lo == 0) lo = 1;
-          if (min_p > 0.0f && keep_n > 0) lo = min(lo, keep_m), hi = min(hi, keep_m);
+          if (min_p > 0.0f && keep_m > 0) lo = min(lo, keep_m), hi = min(hi, keep_m);
           follow(2, bound_u(lo), bound_u(hi));
         }
         int total = entries;
+#pragma unroll
         for (int w = 1; w < 3; ++w)
-          if (iv[w][1] > iv[w][0]) total += count_before(s, iv[w][1], range_n) - count_before(s, iv[w][0], range_n);
+          if (iv[w][1] > iv[w][0]) total = min(total + entries_of(iv[w][0], iv[w][1]), CAND + 1);
         if (total > CAND || iv[1][1] >= BINS || iv[2][1] >= BINS || bin == BINS - 1)
           iv[1][0] = iv[1][1] = iv[2][0] = iv[2][1] = 0;
       }
       if (tid == 0) s.n_cand = 0;
       __syncthreads();
       if (near && bin < BINS - 1) {
-        float lo[3], hi[3];  // the intervals as logits: [lo, hi)
+        // the intervals as logits, [lo, hi]: an entry is in one that leaves it as it is
+        float lo[3], hi[3];
+#pragma unroll
         for (int w = 0; w < 3; ++w) {
-          const bool any = iv[w][1] > iv[w][0];
-          lo[w] = any ? least_in(near_bin, iv[w][1] - 1) : __builtin_inff();
-          hi[w] = any && iv[w][0] > 0 ? least_in(near_bin, iv[w][0] - 1) : __builtin_inff();
+          const int from = iv[w][0], to = iv[w][1];
+          lo[w] = to > from ? least_in(near_bin, to - 1) : __builtin_inff();
+          hi[w] = to > from && from > 0 ? below(least_in(near_bin, from - 1)) : __builtin_inff();
         }
-        each_four<BF, 4>(x0, V, [&](const float (&x)[4], int i) {
-          bool in[4], any = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            in[e] = (x[e] >= lo[0] && x[e] < hi[0]) | (x[e] >= lo[1] && x[e] < hi[1]) | (x[e] >= lo[2] && x[e] < hi[2]);
-            any |= in[e];
-          }
-          if (any)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (in[e]) keep(x[e], i + e);
+        if (iv[1][1] == iv[1][0]) lo[1] = lo[0], hi[1] = hi[0];
+        const bool three = iv[1][1] > iv[1][0] && iv[2][1] > iv[2][0];
+        if (!three && iv[2][1] > iv[2][0]) lo[1] = lo[2], hi[1] = hi[2];
+        keep_all([&](float x) __attribute__((always_inline)) {
+          bool in = (__builtin_amdgcn_fmed3f(x, lo[0], hi[0]) == x) | (__builtin_amdgcn_fmed3f(x, lo[1], hi[1]) == x);
+          if (three) in |= __builtin_amdgcn_fmed3f(x, lo[2], hi[2]) == x;
+          return in;
         });
       } else {
         const int level = g.level;
         if (level != kKeys) g.from = level, g.bin = bin, g.level = kKeys;  // inside(): this bin
-        each([&](float x, int i) {
+        each([&](float x, int i) __attribute__((always_inline)) {
           if (inside(x, i)) keep(x, i);
         });
         g.level = level;
@@ -625,7 +700,7 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
         const float x = s.cx[e];
         if (!inside(x, s.ci[e])) continue;
         const int at = atomicAdd(&s.n_list, 1);
-        if (at < LIST) s.list[at] = make_ulonglong2(order_key(x, s.ci[e]), whole(weight(x)));
+        if (at < LIST) s.list[at] = make_ulonglong2(order_key(x, s.ci[e]), weight(x));
       }
       g.level = level;
     }
@@ -644,11 +719,11 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
       }
       const u64 rank = g.count + ahead;
       const u64 lo = by_count ? rank : cum, hi = by_count ? rank + 1 : cum + w;
-      if (lo <= t && t < hi) s.rank = rank + 1, s.cum = cum + w, s.own = w, s.pos = (int)(uint32_t)key;
+      if (lo <= t && t < hi) s.cum = cum + w, s.own = w, s.pos = (int)(uint32_t)key;
     }
     __syncthreads();
     if (step == 2) break;
-    if (uniform(s.rank) < n) n = uniform(s.rank), m = uniform(s.cum);
+    m = min(m, uniform(s.cum));
     __syncthreads();
     // a divided bin's histogram is of no use for the next search
     if (!near) {
