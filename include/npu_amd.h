@@ -285,9 +285,8 @@ npu_status fused_llama_rope_append(const npu_memref *Q, const npu_memref *K, con
 /* A = softmax over the keys a token sees of Q K^T * scale, times V, per query
  * head; query head h uses key head h / (H / Hkv).  New token i of n sees the
  * prefix's keys and own keys j <= kv_len[b] - n + i; a token that sees none
- * gives 0.  What masked places of the cache hold, NaN and Inf too, does not
- * count, except that a value of a later new token of the same sequence must be
- * finite.  Q, A bf16 [T, H Dh]; prefix_table i32 [>= ceil(prefix_len / page)],
+ * gives 0.  What the cache holds in places that a token does not see, NaN and
+ * Inf too, does not count for it.  Q, A bf16 [T, H Dh]; prefix_table i32 [>= ceil(prefix_len / page)],
  * absent iff prefix_len is 0: key j of the prefix lies in page
  * prefix_table[j / page], and is read once for all sequences where each has
  * few rows.  f32 sums; the probabilities are rounded to bf16.

@@ -80,6 +80,30 @@ __device__ __forceinline__ Frag16 load_cache(const uint16_t *p) {
   return f;
 }
 
+// A later new token's values may be anything to the rows that do not see them, but in a
+// tile's product they meet a weight of 0, and 0 Inf is NaN.  So in a block that some
+// rows of a tile see more of than others, an Inf or NaN is taken out of the product
+// and added to the rows that do see it, key by key; such values are not expected,
+// and finite ones cost that block the look (four prompts of 800 to 2000 tokens: 147 ->
+// 152 us).
+// Bits 15 and 31: which of a pair is not finite.  (In whole numbers throughout: as
+// conditions, a block's would take hundreds of scalar registers.)
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
+  return ((pair & 0x7fff7fffu) + 0x00800080u) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t finite_only(uint32_t pair) { return pair & ~((not_finite(pair) >> 15) * 0xffffu); }
+// An entry that is not finite, else 0.
+__device__ __forceinline__ float not_finite_only(uint16_t v) {
+  const uint32_t x = (uint32_t)v << 16;
+  return __uint_as_float(x & (uint32_t)((int)not_finite(x) >> 31));
+}
+// A sequence's own key j in a head's pages; null: the table names no page.
+__device__ __forceinline__ const uint16_t *value_of(const ServeBatch &b, const int *table, const uint16_t *head,
+                                                    long long page_stride, int dh, int j) {
+  const int page = checked_page(table[j >> b.page_log2], b.n_pages);
+  return page < 0 ? nullptr : head + page * page_stride + (j & ((1 << b.page_log2) - 1)) * dh;
+}
+
 // One 32-key step's loads of a wave.
 template <int DH>
 struct KeyBlock {
@@ -234,7 +258,8 @@ __device__ __forceinline__ void zero_spare_rows(const PagedAttentionArgs &a, con
 // past the end is read from what pages the table names there, and masked).
 // ONCE: keys and values are loaded past the caches (48 sequences of up to 8000 keys
 // 147 -> 137 us, one of 131 000 96 -> 91; not for the short ones below, 16.8 -> 21).
-template <int DH, int NW, bool ONCE>
+// MANY: a tile's rows may be of several tokens.
+template <int DH, int NW, bool ONCE, bool MANY>
 struct TileWalk {
   static constexpr int E = DH / 16;  // MFMAs of the second product, entries of a lane's output run
   f32x4 o[E];
@@ -254,9 +279,10 @@ struct TileWalk {
 #pragma unroll
       for (int d = 0; d < DH / 32; ++d) qf[d] = load16(p + d * 32);
     }
-    int lim = 0, tile_lim = 0;
+    int lim = 0, first_lim = 0, tile_lim = 0;
     auto limits = [&]() __attribute__((always_inline)) {
       lim = visible_keys(sp, c.kv, c.n, tok);
+      first_lim = visible_keys(sp, c.kv, c.n, row0 / sp.G);
       tile_lim = visible_keys(sp, c.kv, c.n, (row0 + rows - 1) / sp.G);
     };
     const int *table = sp.b.page_table + (sp.stacked ? 0 : c.seq * sp.b.table_stride);
@@ -364,6 +390,21 @@ struct TileWalk {
           for (int i = 0; i < DH / 32; ++i) cur.v[e][i] = keep ? cur.v[e][i] : 0u;
         }
       }
+      bool left_out = false;
+      if (MANY && !x.pre && x.j + 32 > first_lim && first_lim < end) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int i = 0; i < DH / 32; ++i) any |= not_finite(cur.v[e][i]);
+        left_out = __any(any != 0);
+        if (left_out) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < DH / 32; ++i) cur.v[e][i] = finite_only(cur.v[e][i]);
+        }
+      }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         Frag16 vf;
@@ -373,6 +414,20 @@ struct TileWalk {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[e][i] *= alpha;
         MfmaBF16::mma(o[e], vf, pf);
+      }
+      if (MANY && left_out) {
+#pragma unroll 1
+        for (int k = 0; k < 32 && x.j + k < end; ++k) {
+          const uint16_t *v = value_of(sp.b, table, vh, a.vpage_stride, DH, x.j + k);
+          if (!v || x.j + k >= row_end) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // (few loads' registers at a time)
+              o[e][i] += not_finite_only(v[(q * 4 + i) * E + e]);
+            }
+        }
       }
     }
     l = sum_of_rows(l);
@@ -450,7 +505,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
   for (long long u = u0; u < u1;) {
     const int b0 = c.blk, b1 = c.nb - b0 < u1 - u ? c.nb : b0 + (int)(u1 - u);
     const int row0 = c.tile * ROWS, rows = min(ROWS, c.n * sp.G - row0);
-    TileWalk<DH, 4, true> t;
+    TileWalk<DH, 4, true, true> t;
     t.run(a, sp, c, b0, b1);
     sums.put(wave, t);
     __syncthreads();
@@ -498,7 +553,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(Paged
   UnitCursor c{group / sp.Hkv, (int)blockIdx.x % tiles, group % sp.Hkv, 0, 0, 1, group / sp.Hkv, 0, 0};
   c.kv = split_kv(sp, c.seq);
   const int row0 = c.tile * ROWS, rows = min(ROWS, sp.G - row0);
-  TileWalk<DH, NW, false> t;
+  TileWalk<DH, NW, false, false> t;
   t.run(a, sp, c, 0, -1);
   sums.put(wave, t);
   if (pre.first) {  // every NW-th part of each row a wave
@@ -573,9 +628,11 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   constexpr int E = DH / 32;             // MFMAs of the second product a k step
   __shared__ __attribute__((aligned(16))) uint16_t sk[2][TKEYS * DH], sv[2][TKEYS * DH];
   __shared__ __attribute__((aligned(16))) int s_live[2][TKEYS / 16];  // whether a buffer's sixteen keys have a page
+  __shared__ int s_left;                 // whether values have been left out of sums (and stays)
   __shared__ Share share;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
+  if (tid == 0) s_left = 0;
   zero_spare_rows<DH>(a, sp);
   long long U, u0, u1;
   UnitCursor c;
@@ -608,6 +665,8 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     const unsigned last = min((u.tile + 1) * TROWS, u.n * sp.G) - 1;
     return visible_keys(sp, u.kv, u.n, last / (unsigned)sp.G);
   };
+  // Of the keys that a tile's last row sees, as many at the end its first may not.
+  const int span = (unsigned)(TROWS - 1) / (unsigned)sp.G + 1;
   auto group_of = [&](const UnitCursor &u) __attribute__((always_inline)) {
     Group g;
     g.row0 = u.tile * TROWS;
@@ -641,7 +700,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   };
   // The pages of this wave's sixteen keys of 64 blocks from blk on, one a lane (-1: none
   // of the keys is seen, or the table names no page).  One load for many blocks: a load
-  // a block, carried to the next, was waited for behind the block's keys (158 -> XX us).
+  // a block, carried to the next, is waited for behind the block's keys.
   auto find = [&](const UnitCursor &u, int end, int blk) __attribute__((always_inline)) {
     const int b = blk + lane;
     const bool pre = b < sp.pre_blocks;
@@ -651,11 +710,13 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     return checked_page(t[j >> sp.b.page_log2], sp.b.n_pages);
   };
   u32x4 kr[NL], vr[NL];  // the next block's sixteen keys of this wave
-  int seen = 0;          // of these, the ones that a row may see
+  int seen = 0;          // of these, the ones that a row may see; + SOME: that some may not
+  constexpr int SOME = 32;
   auto fetch = [&](const UnitCursor &u, int end, int blk, int page) __attribute__((always_inline)) {
     const bool pre = blk < sp.pre_blocks;
     const int j = (pre ? blk : blk - sp.pre_blocks) * TKEYS + 16 * wave;
-    seen = page >= 0 ? (pre ? sp.b.prefix_len : end) - j : 0;
+    seen = page >= 0 ? clamp_int((pre ? sp.b.prefix_len : end) - j, 0, 16) : 0;
+    if (!pre && j + 16 > end - span) seen += SOME;
     const int in = ((u.head << sp.b.page_log2) + (j & ((1 << sp.b.page_log2) - 1))) * DH;
     const uint16_t *kp = a.k_pages + max(page, 0) * a.kpage_stride + in, *vp = a.v_pages + max(page, 0) * a.vpage_stride + in;
 #pragma unroll
@@ -665,11 +726,21 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     }
   };
   auto commit = [&](int to) __attribute__((always_inline)) {
-    if (lane == 0) s_live[to][wave] = seen > 0;
-    if (seen < 16) {  // values that no row may see must not meet p = 0
+    if (lane == 0) s_live[to][wave] = (seen & (SOME - 1)) != 0;
+    if (seen != 16) {  // values that no row may see must not meet p = 0, others that some may not
       __builtin_amdgcn_sched_barrier(0);  // (keeps the branch)
+      uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) vr[i] = masked(vr[i], i * KPL + lane / CH < seen);
+      for (int i = 0; i < NL; ++i) {
+        vr[i] = masked(vr[i], i * KPL + lane / CH < (seen & (SOME - 1)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t out = seen & SOME ? not_finite(vr[i][e]) : 0u;
+          any |= out;
+          vr[i][e] &= ~((out >> 15) * 0xffffu);
+        }
+      }
+      if (any != 0) s_left = 1;
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -864,6 +935,44 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
     --left;
     commit(buf ^ 1);
     __syncthreads();
+  }
+
+  __syncthreads();
+  if (!__builtin_amdgcn_readfirstlane(s_left)) return;
+  // What was left out of the sums, to where they are now: after the loop, which has no
+  // register to spare.
+  take_share(sp, share, U, W, u0, u1, c, w, true);
+  for (long long u = u0; u < u1;) {
+    const int first = c.blk, last = c.nb - first < u1 - u ? c.nb : first + (int)(u1 - u);  // blocks of this group
+    const Group g = group_of(c);
+    const bool starts = first == 0, ends = last == c.nb;
+    if (const int jr = wrow + r; jr < g.rows) {
+      const int head = c.head * sp.G + g.row - g.tok * sp.G;
+      const long long token = c.start + g.tok;
+      uint16_t *to = a.out + token * a.o_stride + head * DH + 4 * h;
+      PartRow<DH> *part = !starts ? parts.later + (long long)w * TROWS + jr
+                          : dense ? parts.first + token * (sp.G * sp.Hkv) + head
+                                  : parts.first + (long long)w * TROWS + jr;
+      const int *table = sp.b.page_table + c.seq * (sp.stacked ? 0 : sp.b.table_stride);
+      const uint16_t *vh = a.v_pages + ((long long)c.head << sp.b.page_log2) * DH + 4 * h;
+      // (sixteen keys together were looked at)
+      const int from = max(max(first - sp.pre_blocks, 0) * TKEYS, (g.end - span) & ~15);
+      const int end = min((last - sp.pre_blocks) * TKEYS, g.lim);
+      for (int i = 0; i < DH; i += 8) {
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = from; k < end; ++k)
+          if (const uint16_t *v = value_of(sp.b, table, vh, a.vpage_stride, DH, k))
+            for (int e = 0; e < 4; ++e) x[e] += not_finite_only(v[i + e]);
+        for (int e = 0; e < 4; ++e) {
+          if (!dense && starts && ends)
+            to[i + e] = f32_to_bf16(bf16_to_f32(to[i + e]) + x[e]);
+          else
+            part->o[i + 4 * h + e] += x[e];
+        }
+      }
+    }
+    u += last - first;
+    if (u < u1) next_group(sp, c);
   }
 }
 

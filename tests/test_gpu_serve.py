@@ -1,5 +1,7 @@
 """The serving operators on the GPU against their plain 64-bit forms
 (serve_refs.py)."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -269,6 +271,41 @@ def test_attention_ignores_what_masked_places_hold(cuda, prefix):
         x[free[0::2, 0].cuda(), :, free[0::2, 1].cuda()] = fill[0]
         x[free[1::2, 0].cuda(), :, free[1::2, 1].cuda()] = fill[1]
     _check_attend(bt, bt.rnd(4, 4 * 64))
+
+
+@pytest.mark.parametrize("news,lens,Dh,prefix", [
+    ([5, 0, 12, 1], [9, 4, 300, 64], 64, 0), ([3, 2], [9, 40], 128, 30), ([31], [2500], 128, 0),
+    ([150, 65], [150, 400], 128, 0), ([70, 40], [71, 3000], 64, 20), ([1, 200], [5, 200], 64, 0)])
+def test_attention_ignores_what_later_tokens_hold(cuda, news, lens, Dh, prefix):
+    """NaN and Inf in new tokens' keys and values: the tokens before do not see
+    them, and the others' entries are what any weight makes of them."""
+    H, Hkv, page = 4, 2, 16
+    bt = R.Batch(news, lens, Hkv, Dh, page, prefix, seed=9)
+    Q = bt.rnd(bt.T, H * Dh)
+    want, some = torch.zeros(bt.T, H, Dh, dtype=torch.float64), torch.zeros(bt.T, H, Dh, dtype=torch.bool)
+    for t, b, j in bt.tokens():
+        if t % 3 == 0 or j < 0:
+            continue
+        first, rows = t - int(bt.start[b]), slice(t, int(bt.start[b + 1]))
+        at, head, entry = (int(bt.table[b, j // page]), j % page), t % Hkv, (7 * t) % Dh
+        value = (math.nan, math.inf, -math.inf)[first % 7 % 3]
+        bt.v_pages[at[0], head, at[1], entry] = value
+        heads = slice(head * (H // Hkv), (head + 1) * (H // Hkv))
+        want[rows, heads, entry] += value
+        some[rows, heads, entry] = True
+        if rows.stop - t <= 2:  # a key too, of the last tokens
+            bt.k_pages[at[0], 1 - head, at[1], 3] = math.nan
+            heads = slice((1 - head) * (H // Hkv), (2 - head) * (H // Hkv))
+            want[rows, heads] = math.nan
+            some[rows, heads] = True
+    assert some.any()
+    got = _attend(bt, Q).cpu().double()
+    exact, mag, seen = R.attend64(bt, Q, Dh ** -0.5)
+    want, some = want.view(bt.T, -1), some.view(bt.T, -1)
+    assert torch.equal(torch.nan_to_num(got[some], nan=7.0), torch.nan_to_num(want[some], nan=7.0))
+    assert torch.isfinite(got[~some]).all()
+    bad = ((got - exact).abs() > _attend_bound(bt, Q, Dh ** -0.5, exact, mag, seen)) & ~some
+    assert not bad.any(), f"{int(bad.sum())} outside, first at {bad.nonzero()[0].tolist()}"
 
 
 def test_attention_bad_pages_are_masked(cuda):
