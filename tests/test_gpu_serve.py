@@ -540,3 +540,93 @@ def test_sample_captured(cuda):
         assert torch.equal(tokens, got[0]) and torch.equal(probs, got[1]), step
         host = x.double().cpu().numpy()
         assert tokens.tolist() == [R.sample64(host[b], float(u[b]), top_p=np.float32(0.9))[0] for b in range(4)], step
+
+
+# ---- together ------------------------------------------------------------------------
+def _model64(model, H, tokens, eps=1e-5):
+    """Logits of every position in f64, from host copies of the weights."""
+    layers, embed, g_out, w_out = model
+    f = lambda t: t.detach().cpu().double()
+    norm = lambda x, g: x * (x.square().mean(1, keepdim=True) + eps).rsqrt() * f(g)
+    x = f(embed)[tokens]
+    n, D = x.shape
+    dh = D // H
+    angle = torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, dh, 2, dtype=torch.float64) / dh)
+    hid = torch.ones(n, n, dtype=torch.bool).triu(1)
+    for p in layers:
+        xn = norm(x, p["g1"])
+        q, k, v = (xn @ f(p[w]) for w in ("wq", "wk", "wv"))
+        out = torch.empty_like(q)
+        for h in range(H):
+            c = slice(h * dh, (h + 1) * dh)
+            rot = lambda t: torch.stack([t[:, 0::2] * angle.cos() - t[:, 1::2] * angle.sin(),
+                                         t[:, 0::2] * angle.sin() + t[:, 1::2] * angle.cos()], 2).reshape(n, dh)
+            s = (rot(q[:, c]) @ rot(k[:, c]).T * dh ** -0.5).masked_fill(hid, -math.inf)
+            out[:, c] = s.softmax(1) @ v[:, c]
+        x = x + out @ f(p["wo"])
+        hn = norm(x, p["g2"])
+        g = hn @ f(p["wg"])
+        x = x + (g * torch.sigmoid(g) * (hn @ f(p["wu"]))) @ f(p["wd"])
+    return norm(x, g_out) @ f(w_out)
+
+
+@pytest.mark.parametrize("prefix", [0, 37])
+def test_serving(cuda, prefix):
+    """Prompts of several lengths, then drawn tokens, eager and replayed from a
+    graph, with a sequence leaving and another taking its slot: each step's logits
+    against the whole sequence's in f64, each drawn token against its logits.
+    The logits are off by a rounding of 2^-8 at nine places a layer (the
+    normalised rows twice, QKV, the rotated, the probabilities, A, h, the gated
+    and the layer's output) and two after: at most so many of the row's norm."""
+    from npu_amd import serving
+    H, V, L = 2, 448, 2
+    model = serving.random_model(L, 128, H, 192, V, seed=5)
+    s = serving.Server(*model, n_heads=H, slots=4, pages=40, page=16, max_pages=10)
+    g = torch.Generator().manual_seed(2)
+    draw = lambda n: torch.randint(0, V, (n,), generator=g).tolist()
+    pre = draw(prefix)
+    if prefix:
+        s.set_prefix(pre)
+    live, setting = {}, {0: {"temperature": 0.7, "top_k": 40}, 1: {"top_p": 0.9}, 2: {"min_p": 0.05}, 3: {"temperature": 0.0}}
+
+    def add(slot, n):
+        live[slot] = draw(n)
+        s.add(slot, live[slot], **setting[slot])
+
+    def check(slots):
+        logits, tokens = s.logits.cpu(), s.tokens.tolist()
+        for b in slots:
+            exact = _model64(model, H, pre + live[b])[-1]
+            assert float((logits[b].double() - exact).norm()) <= (9 * L + 2) * BF16_HALF_STEP * float(exact.norm()), b
+            kw = {k: v[b].item() for k, v in s.settings.items()}
+            assert tokens[b] == R.sample64(logits[b].double().numpy(), s.u[b].item(), **kw)[0], b
+            live[b].append(tokens[b])
+
+    def numbers():
+        s.u.copy_(torch.rand(4, generator=g))
+
+    add(0, 5), add(1, 1), add(3, 40)
+    numbers()
+    s.prefill()
+    check([0, 1, 3])
+    for _ in range(3):
+        numbers()
+        s.step()
+        check([0, 1, 3])
+    s.remove(1)
+    del live[1]
+    add(2, 70)
+    numbers()
+    s.prefill()
+    check([2])
+    graph = s.capture()
+    for _ in range(13):
+        s.make_room()
+        numbers()
+        graph.replay()
+        torch.cuda.synchronize()
+        check([0, 2, 3])
+    with pytest.raises(RuntimeError, match="is taken"):
+        s.add(0, [1])
+    with pytest.raises(ValueError, match="0 .. 447"):
+        s.add(1, [448])
