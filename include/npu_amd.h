@@ -288,8 +288,8 @@ npu_status fused_llama_rope_append(const npu_memref *Q, const npu_memref *K, con
  * gives 0.  What the cache holds in places that a token does not see, NaN and
  * Inf too, does not count for it.  Q, A bf16 [T, H Dh]; prefix_table i32 [>= ceil(prefix_len / page)],
  * absent iff prefix_len is 0: key j of the prefix lies in page
- * prefix_table[j / page], and is read once for all sequences where each has
- * few rows.  f32 sums; the probabilities are rounded to bf16.
+ * prefix_table[j / page], and is read once for all sequences where that pays
+ * (few rows each, a long prefix).  f32 sums; the probabilities are rounded to bf16.
  * workspace f32 [n], n >= npu_paged_attention_workspace: scratch that only
  * this call uses while it runs; its contents need not be kept. */
 npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_pages,

@@ -85,13 +85,22 @@ __device__ __forceinline__ Frag16 load_cache(const uint16_t *p) {
 // rows of a tile see more of than others, an Inf or NaN is taken out of the product
 // and added to the rows that do see it, key by key; such values are not expected,
 // and finite ones cost that block the look (four prompts of 800 to 2000 tokens: 147 ->
-// 152 us).
+// 154 us).
 // Bits 15 and 31: which of a pair is not finite.  (In whole numbers throughout: as
 // conditions, a block's would take hundreds of scalar registers.)
 __device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
   return ((pair & 0x7fff7fffu) + 0x00800080u) & 0x80008000u;
 }
-__device__ __forceinline__ uint32_t finite_only(uint32_t pair) { return pair & ~((not_finite(pair) >> 15) * 0xffffu); }
+// The larger magnitudes of two pairs, as bits.
+__device__ __forceinline__ uint32_t max_magnitudes(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                               __builtin_bit_cast(u16x2, b & 0x7fff7fffu)));
+}
+__device__ __forceinline__ uint32_t finite_only(uint32_t pair) {
+  const uint32_t out = not_finite(pair);
+  return pair & ~((out << 1) - (out >> 15));
+}
 // An entry that is not finite, else 0.
 __device__ __forceinline__ float not_finite_only(uint16_t v) {
   const uint32_t x = (uint32_t)v << 16;
@@ -191,7 +200,7 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     U += s.wave[v];
   }
   U = uniform(U);
-  W = split_workgroups(U, gridDim.x);
+  W = split_workgroups((U + sp.least - 1) / sp.least, gridDim.x);
   w = blockIdx.x;
   if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
   if (w >= W) return false;
@@ -392,12 +401,12 @@ struct TileWalk {
       }
       bool left_out = false;
       if (MANY && !x.pre && x.j + 32 > first_lim && first_lim < end) {
-        uint32_t any = 0;
+        uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int i = 0; i < DH / 32; ++i) any |= not_finite(cur.v[e][i]);
-        left_out = __any(any != 0);
+          for (int i = 0; i < DH / 32; ++i) top = max_magnitudes(top, cur.v[e][i]);
+        left_out = __any(not_finite(top) != 0);
         if (left_out) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -737,7 +746,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
         for (int e = 0; e < 4; ++e) {
           const uint32_t out = seen & SOME ? not_finite(vr[i][e]) : 0u;
           any |= out;
-          vr[i][e] &= ~((out >> 15) * 0xffffu);
+          vr[i][e] &= ~((out << 1) - (out >> 15));
         }
       }
       if (any != 0) s_left = 1;
@@ -1020,16 +1029,18 @@ struct RowJoin {
   }
 };
 
-// Workgroup (w, y): rows of the group whose first part workgroup w left in its slot.
+// Workgroup (y, w): rows of the group whose first part workgroup w left in its slot.  (The
+// rows run faster: groups' first parts are a constant number of slots apart, often a
+// multiple of eight, and by w they would all be one XCD's.)
 template <int DH, int SPLIT>
 __global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttentionArgs a, int G, Parts<DH> parts) {
   using J = RowJoin<DH, SPLIT>;
   __shared__ f32x4 so[SPLIT > 1 ? NT : 1];
   __shared__ float sm[SPLIT > 1 ? NT : 1], sl[SPLIT > 1 ? NT : 1];
-  const int w = blockIdx.x, ch = threadIdx.x % J::CH, sub = threadIdx.x / J::CH % J::PER;
-  const int split = threadIdx.x / (J::CH * J::PER), jr = blockIdx.y * J::PER + sub;
+  const int w = blockIdx.y, ch = threadIdx.x % J::CH, sub = threadIdx.x / J::CH % J::PER;
+  const int split = threadIdx.x / (J::CH * J::PER), jr = blockIdx.x * J::PER + sub;
   const PartInfo in = parts.info[w];
-  if ((int)blockIdx.y * J::PER >= in.rows) return;
+  if ((int)blockIdx.x * J::PER >= in.rows) return;
   J j;
   j.clear();
   if (jr < in.rows)
@@ -1043,32 +1054,38 @@ __global__ __launch_bounds__(NT) void paged_attention_join_kernel(PagedAttention
   }
 }
 
-// The same for 128-row tiles, few parts a row: a lane's four rows at once, so that
-// one round of the workgroups has all loads in flight (15.5 -> 14.0 us for the 1024
-// slots of a prompt call).
-template <int DH>
+// The same for 128-row tiles, a lane's R rows and U parts at once, so that loads are in
+// flight: four rows where groups have few parts (15.5 -> 14.0 us for the 1024 slots of
+// a prompt call), eight parts where they have many.
+template <int DH, int R, int U>
 __global__ __launch_bounds__(NT) void paged_attention_tile_join_kernel(PagedAttentionArgs a, int G, Parts<DH> parts) {
   using J = RowJoin<DH, 1>;
-  constexpr int R = 4;
-  const int w = blockIdx.x, ch = threadIdx.x % J::CH, jr0 = blockIdx.y * J::PER * R + threadIdx.x / J::CH;
+  const int w = blockIdx.y, ch = threadIdx.x % J::CH, jr0 = blockIdx.x * J::PER * R + threadIdx.x / J::CH;
   const PartInfo in = parts.info[w];
-  if ((int)blockIdx.y * J::PER * R >= in.rows) return;
+  if ((int)blockIdx.x * J::PER * R >= in.rows) return;
   J j[R];
 #pragma unroll
   for (int k = 0; k < R; ++k) j[k].clear();
-  for (int i = 0; i <= in.more; ++i) {
-    const PartRow<DH> *p = i == 0 ? parts.first + (long long)w * TROWS : parts.later + (long long)(w + i) * TROWS;
-    f32x4 o[R];
-    float m[R], l[R];
+  for (int i0 = 0; i0 <= in.more; i0 += U) {
+    f32x4 o[U][R];
+    float m[U][R], l[U][R];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const PartRow<DH> *row = p + min(jr0 + k * J::PER, in.rows - 1);
-      o[k] = *reinterpret_cast<const f32x4 *>(row->o + ch * 4);
-      m[k] = row->m;
-      l[k] = row->l;
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u, in.more);
+      const PartRow<DH> *p = i == 0 ? parts.first + (long long)w * TROWS : parts.later + (long long)(w + i) * TROWS;
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const PartRow<DH> *row = p + min(jr0 + k * J::PER, in.rows - 1);
+        o[u][k] = *reinterpret_cast<const f32x4 *>(row->o + ch * 4);
+        m[u][k] = row->m;
+        l[u][k] = row->l;
+      }
     }
 #pragma unroll
-    for (int k = 0; k < R; ++k) j[k].add(m[k], l[k], o[k]);
+    for (int u = 0; u < U; ++u)
+      if (i0 + u <= in.more)
+#pragma unroll
+        for (int k = 0; k < R; ++k) j[k].add(m[u][k], l[u][k], o[u][k]);
   }
 #pragma unroll
   for (int k = 0; k < R; ++k) {
@@ -1116,18 +1133,38 @@ struct Division {
   bool own_tiles, pre_tiles;  // 128-row tiles for the own keys' part, the prefix's
   bool whole;     // a workgroup for each group of the own keys' part
 };
-Division divide(const ServeBatch &b, int H, int Hkv) {
+bool can_stack(const ServeBatch &b, long long rows) {
+  return b.prefix_len > 0 && b.B > 1 && rows < (long long)b.B * TROWS;
+}
+// The rules' figures are us with a rule's one side and its other, G = 4, Dh = 128 unless said.
+Division divide(const ServeBatch &b, int H, int Hkv, int dh) {
   const long long G = H / Hkv, rows = b.T * G;
+  const long long own_keys = (long long)b.max_pages << b.page_log2;  // what the table can name
   Division d;
   d.W = 2 * device_cus();
-  // A prefix is shared by a product of its own where it saves reading it per
-  // sequence: more than one sequence, each with less than a tile of rows.
-  d.stacked = b.prefix_len > 0 && b.B > 1 && rows < (long long)b.B * TROWS;
-  d.own_tiles = rows >= (long long)b.B * 4 * ROWS;
-  d.pre_tiles = rows >= 4 * ROWS;
-  // Up to 1024 keys a group takes no longer than its cut parts and their join.
-  d.whole = !b.q_start && !d.own_tiles &&
-            ((long long)b.max_pages << b.page_log2) + (d.stacked ? 0 : b.prefix_len) <= 1024;
+  // A 128-row tile reads keys once for what takes 16-row tiles two reads and more, but its
+  // blocks follow each other more slowly, so there have to be enough: by 16-row
+  // tiles of all key heads.  8 sequences of 2000 to 4000 keys, 8 new tokens (128 tiles): 38
+  // us, in 16-row tiles 45; 64 new tokens of one sequence of 2000 (128): 28 to 37; 32 of
+  // them (64): 22 to 21; 4 new tokens of 8 sequences (one tile each): 35 to 30.
+  d.own_tiles = rows >= (long long)b.B * 2 * ROWS && rows * Hkv >= 96 * ROWS;
+  d.pre_tiles = rows >= 4 * ROWS;  // 16 sequences over 4096 keys of prefix: 22 us to 23; 4: 19 to 16
+  // Up to 1024 keys a group takes no longer than its cut parts and their join: 64 sequences
+  // of up to 1000 keys 39 us to 47, 8 of them 15 to 15, one 10 to 11; up to 2000, one 18 to 12.
+  const bool short_own = !b.q_start && !d.own_tiles && own_keys <= 1024;
+  const bool short_all = short_own && own_keys + b.prefix_len <= 1024;
+  // A prefix that sequences share has a product of its own, with all their rows, if each has
+  // less than a tile of rows and the keys and values that are then not read again
+  // (from the caches, mostly) are worth the launches.  In MB, if the own keys' part takes
+  // the sums in: 8 sequences, 1200 keys of prefix (34) 15 us to 17, 2 and 2400 (10)
+  // 15 to 14; if it takes a join: 16 of 1000 to 2000 keys, 2400 (147) 45 to 51, 1200
+  // (74) 43 to 41; if there are several tokens a sequence, or one launch would do:
+  // 8 of 4, 9600 (275) 41 to 51, 2000 (57) 29 to 26; 128 of one, 600 (312) 33 to 35, 48
+  // (115) 20 to 19.
+  const long long again = (long long)(b.B - 1) * b.prefix_len * Hkv * dh * 4;
+  const int least_mb = b.q_start || short_all ? 256 : short_own ? 16 : 80;
+  d.stacked = can_stack(b, rows) && again >= least_mb * 1000000LL;
+  d.whole = short_own && (d.stacked || short_all);
   return d;
 }
 
@@ -1138,15 +1175,16 @@ size_t slot_bytes(const Division &d, bool tiles) {
 
 template <int DH>
 size_t workspace_of(const ServeBatch &b, int H, int Hkv) {
-  const Division d = divide(b, H, Hkv);
-  const size_t own = slot_bytes<DH>(d, d.own_tiles);
-  if (!d.stacked) return d.W * sizeof(PartInfo) + 2 * own;
-  return 2 * (size_t)b.T * H * sizeof(PartRow<DH>) + own + slot_bytes<DH>(d, d.pre_tiles);
+  // (whatever the division makes of the arrays that the call brings)
+  const Division d = divide(b, H, Hkv, DH);
+  const size_t own = slot_bytes<DH>(d, d.own_tiles), plain = d.W * sizeof(PartInfo) + 2 * own;
+  if (!can_stack(b, (long long)b.T * (H / Hkv))) return plain;
+  return std::max(plain, 2 * (size_t)b.T * H * sizeof(PartRow<DH>) + own + slot_bytes<DH>(d, d.pre_tiles));
 }
 
 template <int DH>
 hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
-  const Division d = divide(a.b, a.H, a.Hkv);
+  const Division d = divide(a.b, a.H, a.Hkv, DH);
   const int G = a.H / a.Hkv;
   char *ws = static_cast<char *>(a.workspace);
   auto plan = [&](const char *name, int grid, int per_cu) {
@@ -1155,7 +1193,11 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
   // the own keys' part or, stacked, the prefix's
   auto attend = [&](bool tiles, bool stacked, int dense, const Parts<DH> &parts) {
     const int keys = tiles ? TKEYS : KEYS, pre_blocks = (a.b.prefix_len + keys - 1) / keys;
-    const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, tiles ? 6 : 7, d.stacked && !stacked ? 0 : pre_blocks, stacked};
+    // three blocks a workgroup at least in tiles, or writing and joining the parts of their
+    // rows takes longer: 64 tokens of one sequence of 2000 keys 28 us, with one block 37
+    // (but not for a prefix, one tile or two: 64 sequences over one of 4000 47 us, with one 44)
+    const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, tiles ? 6 : 7, d.stacked && !stacked ? 0 : pre_blocks, stacked,
+                       tiles && !stacked ? 3 : 1};
     auto kern = tiles ? paged_attention_tile_kernel<DH> : paged_attention_kernel<DH>;
     static const char *const names[2][2] = {{"llama_paged_attention", "llama_paged_attention_tiles"},
                                             {"llama_paged_attention_prefix", "llama_paged_attention_prefix_tiles"}};
@@ -1184,6 +1226,8 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
       plan("llama_paged_attention_whole", groups, wg_per_cu(kern, 64 * NW));
       hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * NW), 0, s, a, sp, tiles, d.W, pre, pre_rows);
     };
+    // eight waves where groups leave CUs idle: 16 sequences of up to 1000 keys, Dh = 64, 9.5 us
+    // to 10.9 (Dh = 128 the same either way); 128 of 8 key heads 62 to 57
     if (groups > device_cus()) launch(std::integral_constant<int, 4>{});
     else launch(std::integral_constant<int, 8>{});
   } else if (!d.stacked) {
@@ -1193,15 +1237,18 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
     parts.later = parts.first + (size_t)d.W * own_rows;
     attend(d.own_tiles, false, 0, parts);
     if (d.own_tiles) {
-      auto join = paged_attention_tile_join_kernel<DH>;
-      const int y = TROWS / (4 * RowJoin<DH, 1>::PER);
+      // parts of a group, if the workgroups share as few groups as there may be
+      const long long groups = ((long long)a.b.T * G + TROWS - 1) / TROWS * a.Hkv;
+      const bool many = d.W >= 8 * groups;
+      auto join = many ? paged_attention_tile_join_kernel<DH, 1, 8> : paged_attention_tile_join_kernel<DH, 4, 1>;
+      const int y = TROWS / ((many ? 1 : 4) * RowJoin<DH, 1>::PER);
       plan("llama_paged_attention_join", d.W * y, wg_per_cu(join, NT));
-      hipLaunchKernelGGL(join, dim3(d.W, y), dim3(NT), 0, s, a, G, parts);
+      hipLaunchKernelGGL(join, dim3(y, d.W), dim3(NT), 0, s, a, G, parts);
     } else {
       auto join = paged_attention_join_kernel<DH, NT * 4 / DH>;
       const int y = a.b.q_start ? ROWS : std::min(ROWS, G);
       plan("llama_paged_attention_join", d.W * y, wg_per_cu(join, NT));
-      hipLaunchKernelGGL(join, dim3(d.W, y), dim3(NT), 0, s, a, G, parts);
+      hipLaunchKernelGGL(join, dim3(y, d.W), dim3(NT), 0, s, a, G, parts);
     }
   } else {
     const Parts<DH> own = take(slot_bytes<DH>(d, d.own_tiles));

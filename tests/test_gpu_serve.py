@@ -225,12 +225,49 @@ def test_attention(cuda, news, lens, H, Hkv, Dh, page, prefix, kind):
     assert not spare or not A[-spare:].any()
 
 
+# A prefix long enough to have a product of its own, under few rows and many, short own
+# keys and (by the table's width) long ones, one token a sequence and several, some of
+# which see the prefix alone, and rows of no sequence.
+STACKED = [
+    ([1] * 12, [0, 1, 100, 30, 0, 3, 64, 65, 15, 16, 17, 257], 16, 8, 128, 16, 3000, {"ragged": False}),
+    ([1] * 40, [(13 * i) % 70 for i in range(40)], 4, 2, 64, 32, 1111, {"ragged": False}),
+    ([1] * 150, [i % 7 for i in range(150)], 8, 8, 64, 64, 900, {"ragged": False}),
+    ([1] * 12, [0, 1, 1100, 30, 0, 3, 64, 65, 15, 16, 17, 257], 16, 8, 128, 16, 3000, {"ragged": False}),
+    ([1] * 30, [(97 * i) % 1500 for i in range(30)], 34, 2, 64, 16, 6000, {"ragged": False}),
+    ([3] * 30, [(5 * i) % 40 for i in range(30)], 4, 4, 64, 16, 9001, {}),
+    ([5, 0, 37, 1] * 4, [5, 3, 90, 64] * 4, 16, 8, 128, 64, 4400, {}),
+    ([1, 2] * 10, [9, 20] * 10, 8, 8, 64, 16, 6950, {"extra": 4}),
+    ([20] * 8, [20, 400, 3, 77, 0, 19, 21, 1000], 16, 4, 128, 16, 18500, {"extra": 1}),
+]
+
+
+@pytest.mark.parametrize("news,lens,H,Hkv,Dh,page,prefix,kind", STACKED)
+def test_attention_over_a_long_prefix(cuda, news, lens, H, Hkv, Dh, page, prefix, kind):
+    from npu_amd import groups
+    bt = R.Batch(news, lens, Hkv, Dh, page, prefix, seed=len(news) + H, **kind)
+    # and bad pages and what no token sees, in the prefix's and the own keys'
+    bt.prefix_table[2], bt.prefix_table[-2] = bt.P, -1
+    last = prefix % page
+    if last:
+        bt.v_pages[int(bt.prefix_table[-1]), :, last:] = math.nan
+        bt.k_pages[int(bt.prefix_table[-1]), :, last:] = math.inf
+    for b, n in enumerate(lens):
+        if n % page:
+            bt.v_pages[int(bt.table[b, n // page]), :, n % page:] = math.inf
+    with groups.collect_plans() as cp:
+        A = _check_attend(bt, bt.rnd(bt.T, H * Dh))
+    assert cp.plans[0].kernel.decode().startswith("llama_paged_attention_prefix")
+    spare = bt.T - sum(news)
+    assert not spare or not A[-spare:].any()
+
+
 @pytest.mark.parametrize("news,H,Hkv,prefix,names", [
-    ([1] * 8, 8, 2, 0, ["_whole"]), ([1] * 8, 8, 2, 20, ["_prefix", "_whole"]),
-    ([1] * 16, 8, 2, 20, ["_prefix_tiles", "_whole"]), ([200], 4, 2, 20, ["_tiles", "_join"]),
-    ([1] * 8, 8, 2, 1025, ["_prefix", "_whole"]), ([1], 8, 2, 1025, ["", "_join"]), ([1, 2], 8, 2, 0, ["", "_join"]),
-    ([1, 2], 8, 2, 20, ["_prefix", "", "_join"]),
-    ([40] * 2, 4, 2, 20, ["_prefix_tiles", "_tiles", "_join"]), ([31] * 2, 4, 2, 0, ["", "_join"]),
+    ([1] * 8, 8, 2, 0, ["_whole"]), ([1] * 8, 8, 2, 20, ["_whole"]), ([1] * 7, 8, 2, 6000, ["_prefix", "_whole"]),
+    ([1] * 16, 8, 2, 3000, ["_prefix_tiles", "_whole"]), ([400], 4, 2, 20, ["_tiles", "_join"]),
+    ([1], 8, 2, 1025, ["", "_join"]), ([1, 2], 8, 2, 0, ["", "_join"]), ([1, 2], 8, 2, 20, ["", "_join"]),
+    ([1, 1, 2] * 5, 6, 2, 40000, ["_prefix", "", "_join"]),
+    ([40] * 20, 4, 2, 28000, ["_prefix_tiles", "_tiles", "_join"]), ([15] * 30, 4, 2, 0, ["", "_join"]),
+    ([16] * 30, 4, 2, 0, ["_tiles", "_join"]), ([16] * 2, 4, 2, 0, ["", "_join"]),
 ])
 def test_attention_kernels_by_rows(cuda, news, H, Hkv, prefix, names):
     """Few rows a sequence: the kernel that divides keys over waves, whole groups
