@@ -202,7 +202,8 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     U += s.wave[v];
   }
   U = uniform(U);
-  W = split_workgroups((U + sp.least - 1) / sp.least, gridDim.x);
+  const int few = sp.long_groups > 0 ? (U >= 8ll * sp.long_groups) + (U >= 16ll * sp.long_groups) : 0;
+  W = split_workgroups(U >> few, gridDim.x);
   w = blockIdx.x;
   if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
   if (w >= W) return false;
@@ -1199,11 +1200,13 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
   // the own keys' part or, stacked, the prefix's
   auto attend = [&](bool tiles, bool stacked, int dense, const Parts<DH> &parts) {
     const int keys = tiles ? TKEYS : KEYS, pre_blocks = (a.b.prefix_len + keys - 1) / keys;
-    // three blocks a workgroup at least in tiles, or writing and joining the parts of their
-    // rows takes longer: 64 tokens of one sequence of 2000 keys 28 us, with one block 37
-    // (but not for a prefix, one tile or two: 64 sequences over one of 4000 47 us, with one 44)
+    // In tiles, four blocks a workgroup where groups have sixteen, two where they have eight, or
+    // writing and joining the parts of their rows takes longer: 64 tokens of one sequence of
+    // 2000 keys 28 us, with one block each 37; but 400 tokens and nothing before them, 8 heads of
+    // 64, 15 us with one block, 21 with four.  (Not for a prefix, which is one tile or two: 64
+    // sequences over one of 4000 47 us, with one block 44.)
     const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, tiles ? 6 : 7, d.stacked && !stacked ? 0 : pre_blocks, stacked,
-                       tiles && !stacked ? 3 : 1};
+                       tiles && !stacked ? (int)((long long)a.b.T * G / TROWS + a.b.B) * a.Hkv : 0};
     auto kern = tiles ? paged_attention_tile_kernel<DH> : paged_attention_kernel<DH>;
     static const char *const names[2][2] = {{"llama_paged_attention", "llama_paged_attention_tiles"},
                                             {"llama_paged_attention_prefix", "llama_paged_attention_prefix_tiles"}};

@@ -85,7 +85,7 @@ struct AttnSplit {
   int rows, keys_log2;
   int pre_blocks;  // prefix blocks before each tile's own keys
   int stacked;     // the prefix alone: the rows of all tokens as one sequence
-  int least = 1;       // units that a workgroup takes at least
+  int long_groups = 0;  // groups, about, if workgroups are to be fewer where groups are long; 0: they are not
 };
 
 NPU_HD int split_seqs(const AttnSplit &a) { return a.stacked ? 1 : a.b.B; }
