@@ -151,14 +151,25 @@ __device__ __forceinline__ long long uniform(long long v) {
                      (unsigned)__builtin_amdgcn_readfirstlane((int)v));
 }
 
-// Inclusive sum over the lanes of a wave.
+// Inclusive sum over the lanes of a wave: within rows of 16 lanes, shifted by 1, 2, 4 and 8,
+// then a row's last lane to the row after it, and the second row's to the last two.
+template <int CTRL, int ROWS_TO>
+__device__ __forceinline__ int from_lane(int v) {  // 0 where there is none
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS_TO, 0xf, false);
+}
+template <int CTRL, int ROWS_TO>
+__device__ __forceinline__ long long from_lane(long long v) {
+  return (long long)((unsigned long long)(unsigned)from_lane<CTRL, ROWS_TO>((int)(v >> 32)) << 32 |
+                     (unsigned)from_lane<CTRL, ROWS_TO>((int)v));
+}
 template <class T>
 __device__ __forceinline__ T wave_scan(T v) {
-  const int lane = threadIdx.x & 63;
-  for (int off = 1; off < 64; off <<= 1) {
-    const T u = __shfl_up(v, off);
-    if (lane >= off) v += u;
-  }
+  v += from_lane<0x111, 0xf>(v);
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v);
+  v += from_lane<0x143, 0xc>(v);
   return v;
 }
 
@@ -227,7 +238,7 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
   c.n = span.n;
   c.start = span.start;
   c.kv = split_kv(sp, c.seq);
-  c.head = __builtin_amdgcn_readfirstlane((int)((u0 - s.base) / s.per));
+  c.head = __builtin_amdgcn_readfirstlane((int)quotient(u0 - s.base, s.per));
   c.base = s.base + c.head * s.per;
   int rest = (int)min(u0 - c.base, (long long)0x7fffffff);  // units before u0 in the tiles from c.tile on
   for (c.tile = 0;; c.tile += 64) {
@@ -777,8 +788,8 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   };
   clear();
   long long left = u1 - u0;  // blocks, the one computed included
-  int b0 = c.blk, pages0 = c.blk, pages = find(c, g.end, pages0);
   load_queries(c);
+  int b0 = c.blk, pages0 = c.blk, pages = find(c, g.end, pages0);
   fetch(c, g.end, c.blk, __builtin_amdgcn_readlane(pages, 0));
   commit(0);
   touch_queries();

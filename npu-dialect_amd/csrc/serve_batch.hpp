@@ -120,8 +120,12 @@ NPU_HD long long seq_units(const AttnSplit &a, int seq) {
   return head_units(a, split_kv(a, seq), split_span(a, seq).n) * a.Hkv;
 }
 NPU_HD int split_workgroups(long long U, int launched) { return U < launched ? (int)U : launched; }
-NPU_HD long long first_unit(long long U, int W, int w) { return U * w / W; }
-NPU_HD int unit_owner(long long U, int W, long long u) { return (int)(((u + 1) * W - 1) / U); }
+// a / b; where they fit 32 bits, as they do but for millions of units, at a fifth of the instructions
+NPU_HD long long quotient(long long a, long long b) {
+  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+NPU_HD long long first_unit(long long U, int W, int w) { return quotient(U * w, W); }
+NPU_HD int unit_owner(long long U, int W, long long u) { return (int)quotient((u + 1) * W - 1, U); }
 
 // A place in the order of the units: block blk of the nb of group (seq, tile,
 // head), whose first unit is `base`; n, start, kv: the sequence's.
