@@ -87,7 +87,7 @@ __device__ __forceinline__ Frag16 load_cache(const uint16_t *p) {
 // rows of a tile see more of than others, an Inf or NaN is taken out of the product
 // and added to the rows that do see it, key by key; such values are not expected,
 // and finite ones cost that block the look (four prompts of 800 to 2000 tokens: 147 ->
-// 154 us).
+// 154 us before the shares had pauses).
 // Bits 15 and 31: which of a pair is not finite.  (In whole numbers throughout: as
 // conditions, a block's would take hundreds of scalar registers.)
 __device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
@@ -175,7 +175,7 @@ __device__ __forceinline__ T wave_scan(T v) {
 
 // A workgroup's number w in the division, its share of the units, [u0, u1) of U,
 // and the group its first lies in; false: none (the launch has more workgroups
-// than units).  by_xcd: workgroups that the dispatcher puts on one XCD (every
+// than units, or the share is in a pause).  by_xcd: workgroups that the dispatcher puts on one XCD (every
 // eighth) take neighbouring shares, whose tiles read the same keys.
 // Every workgroup finds its own: the units of each sequence (by a lane each or,
 // where they have many tiles, by a wave each), a scan over the lanes, and in the
@@ -194,7 +194,7 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     for (int q = wave; q < seqs; q += NT / 64) {
       const int n = split_span(sp, q).n, kv = split_kv(sp, q), tiles = split_tiles(sp, n);
       long long sum = 0;
-      for (int t = lane; t < tiles; t += 64) sum += tile_blocks(sp, kv, n, t);
+      for (int t = lane; t < tiles; t += 64) sum += tile_blocks(sp, kv, n, t) + sp.pause;
       sum = wave_scan(sum);
       if (lane == 63) s.sum[q] = sum * sp.Hkv;
     }
@@ -213,7 +213,7 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     U += s.wave[v];
   }
   U = uniform(U);
-  const int few = sp.long_groups > 0 ? (U >= 8ll * sp.long_groups) + (U >= 16ll * sp.long_groups) : 0;
+  const int few = sp.long_groups > 0 ? (U >= (8ll + sp.pause) * sp.long_groups) + (U >= (16ll + sp.pause) * sp.long_groups) : 0;
   W = split_workgroups(U >> few, gridDim.x);
   w = blockIdx.x;
   if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
@@ -243,15 +243,16 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
   int rest = (int)min(u0 - c.base, (long long)0x7fffffff);  // units before u0 in the tiles from c.tile on
   for (c.tile = 0;; c.tile += 64) {
     const int tiles = split_tiles(sp, c.n);
-    const int nb = c.tile + lane < tiles ? tile_blocks(sp, c.kv, c.n, c.tile + lane) : 0;
+    const int nb = c.tile + lane < tiles ? tile_blocks(sp, c.kv, c.n, c.tile + lane) + sp.pause : 0;
     const int up_to = wave_scan(nb), all = __builtin_amdgcn_readlane(up_to, 63);
     if (rest < all) {
       const int at = __builtin_ctzll(__ballot(up_to > rest));
       c.tile += at;
       c.nb = __builtin_amdgcn_readlane(nb, at);
       const int skipped = __builtin_amdgcn_readlane(up_to, at) - c.nb;
+      c.nb -= sp.pause;
       c.base += skipped;
-      c.blk = rest - skipped;
+      c.blk = rest - skipped - sp.pause;
       break;
     }
     c.base += all;
@@ -260,7 +261,11 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
   c.blk = __builtin_amdgcn_readfirstlane(c.blk);
   c.tile = __builtin_amdgcn_readfirstlane(c.tile);
   c.base = uniform(c.base);
-  return true;
+  if (c.blk < 0) {  // in the group's pause
+    u0 -= c.blk;
+    c.blk = 0;
+  }
+  return u0 < u1;
 }
 
 // Rows of no sequence give zeros.
@@ -514,6 +519,7 @@ __device__ __forceinline__ void store_row8(uint16_t *to, const float (&acc)[8], 
 template <int DH>
 __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
                                                                 Parts<DH> parts) {
+  sp.pause = 0;  // (as it is: the compiler knows it now)
   __shared__ Share share;
   __shared__ WaveSums<DH, 4> sums;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -533,7 +539,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_kernel(PagedAttentionAr
     sums.put(wave, t);
     __syncthreads();
     const bool starts = b0 == 0, ends = b1 == c.nb;
-    const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
+    const int more = starts && !ends ? unit_owner(U, W, c.base + sp.pause + c.nb - 1) - w : 0;
     if (!dense && starts && !ends && tid == 0) parts.info[w] = PartInfo{rows, c.start, row0, c.head, more, {0, 0, 0}};
     for (int i = tid; i < rows * (DH / 8); i += NT) {
       const int jr = i / (DH / 8), jc = i % (DH / 8);
@@ -631,13 +637,18 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(Paged
 //    keys of sixteen entries, each gets four keys of its entry.
 //  - Blocks follow each other across groups: a group's last block is computed with
 //    the next one's first on its way.
-// Four prompts of 800 to 2000 tokens, 79 GFLOP: 155 us, of which 14 join parts; a block of
+// Four prompts of 800 to 2000 tokens, 79 GFLOP: 141 us, of which 12 join parts; a block of
 // 64 keys is as long as its products (0.9 us a CU at the rate of a large one) and its
 // exponentials together.  The prefix of 6001 keys under 64 sequences: 24 us.
 //  - The running maximum is only a reference: it is raised, and the sums scaled,
 //    when a row's maximum passes it by more than 2^8 (a uniform branch), so that
 //    p <= 2^8 and most blocks scale nothing.
 constexpr int TROWS = 128, TKEYS = 64;  // sixteen keys a wave fetches
+// A group's first loads, its last products and its stores take the time of blocks, and a
+// border that falls between groups leaves no parts.  Pauses of 0, 1, 2, 3 and 5 blocks: the
+// prompts above 155, 148, 144, 141 and 143 us, 64 tokens of one sequence of 2000 keys 28 and,
+// with 3, 24; but 800 tokens with nothing before them, 8 heads of 64, 19 and 26.
+constexpr int TILE_PAUSE = 3;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -648,6 +659,7 @@ __device__ __forceinline__ uint2 read_tr(const uint16_t *p) {
 template <int DH>
 __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttentionArgs a, AttnSplit sp, int dense,
                                                                      Parts<DH> parts) {
+  sp.pause = TILE_PAUSE;  // (as it is: the compiler knows it now)
   constexpr int CH = DH / 8;             // 16-byte chunks of a key
   constexpr int NL = TKEYS * CH / NT;    // loads of a wave a block, of K and of V
   constexpr int KPL = 64 / CH;           // keys that one of them covers
@@ -798,7 +810,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
   for (int buf = 0;; buf ^= 1) {
     const uint16_t *const kb = sk[buf], *const vb = sv[buf];
     const int blk = c.blk;
-    const bool same = blk + 1 < c.nb, more_blocks = left > 1;
+    const bool same = blk + 1 < c.nb, more_blocks = left > (same ? 1 : 1 + sp.pause);
     // the next block's loads: of the next group the pages are to be found first
     UnitCursor c2 = c;
     int end2 = 0;
@@ -892,7 +904,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
       }
       // MFMA i: sixteen keys k = i / E, entries 32 e + r; four keys of sixteen
       // entries a 16-lane group and read
-      constexpr int N = 4 * E, AHEAD = 4;
+      constexpr int N = 4 * E, AHEAD = 3;
       Frag16 vf[N];
       auto operand = [&](int i) __attribute__((always_inline)) {
         const uint16_t *from = vb + (va ^ (i % E) * 32) + 16 * (i / E) * DH;
@@ -913,7 +925,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
       const LanePair lp = lane_pair32(l);
       l = lp.lo + lp.hi;
       const bool starts = b0 == 0, ends = !same;
-      const int more = starts && !ends ? unit_owner(U, W, c.base + c.nb - 1) - w : 0;
+      const int more = starts && !ends ? unit_owner(U, W, c.base + sp.pause + c.nb - 1) - w : 0;
       if (!dense && starts && !ends && tid == 0)
         parts.info[w] = PartInfo{g.rows, c.start, g.row0, c.head, more, {0, 0, 0}};
       const int jr = wrow + r;
@@ -955,6 +967,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
       c = c2;
       g = group_of(c);
       b0 = 0;
+      left -= sp.pause;
     } else {
       ++c.blk;
     }
@@ -997,7 +1010,7 @@ __global__ __launch_bounds__(NT, 2) void paged_attention_tile_kernel(PagedAttent
         }
       }
     }
-    u += last - first;
+    u += last - first + sp.pause;
     if (u < u1) next_group(sp, c);
   }
 }
@@ -1161,11 +1174,13 @@ Division divide(const ServeBatch &b, int H, int Hkv, int dh) {
   d.W = 2 * device_cus();
   // A 128-row tile reads keys once for what takes 16-row tiles two reads and more, but its
   // blocks follow each other more slowly, so there have to be enough: by 16-row
-  // tiles of all key heads.  8 sequences of 2000 to 4000 keys, 8 new tokens (128 tiles): 38
-  // us, in 16-row tiles 45; 64 new tokens of one sequence of 2000 (128): 28 to 37; 32 of
-  // them (64): 22 to 21; 4 new tokens of 8 sequences (one tile each): 35 to 30.
+  // tiles of all key heads.  8 sequences of 2000 to 4000 keys, 8 new tokens (128 tiles): 33
+  // us, in 16-row tiles 46; 64 new tokens of one sequence of 2000 (128): 24 to 35; 32 of
+  // them (64): 20 to 21; 60 new tokens, twice, of 12 heads and 77 keys before (90): 14 to 13;
+  // 4 new tokens of 8 sequences (one tile each): 30 to 30.
   d.own_tiles = rows >= (long long)b.B * 2 * ROWS && rows * Hkv >= 96 * ROWS;
-  d.pre_tiles = rows >= 4 * ROWS;  // 16 sequences over 4096 keys of prefix: 22 us to 23; 4: 19 to 16
+  // 64 sequences over 4096 keys of prefix: 32 us to 44; 32: 29 to 29; 16: 25 to 23; 4: 20 to 16
+  d.pre_tiles = rows >= 8 * ROWS;
   // Up to 1024 keys a group takes no longer than its cut parts and their join: 64 sequences
   // of up to 1000 keys 39 us to 47, 8 of them 15 to 15, one 10 to 11; up to 2000, one 18 to 12.
   const bool short_own = !b.q_start && !d.own_tiles && own_keys <= 1024;
@@ -1176,7 +1191,7 @@ Division divide(const ServeBatch &b, int H, int Hkv, int dh) {
   // the sums in: 8 sequences, 1200 keys of prefix (34) 15 us to 17, 2 and 2400 (10)
   // 15 to 14; if it takes a join: 16 of 1000 to 2000 keys, 2400 (147) 45 to 51, 1200
   // (74) 43 to 41; if there are several tokens a sequence, or one launch would do:
-  // 8 of 4, 9600 (275) 41 to 51, 2000 (57) 29 to 26; 128 of one, 600 (312) 33 to 35, 48
+  // 8 of 4, 9600 (275) 40 to 49, 2000 (57) 31 to 23; 128 of one, 600 (312) 33 to 35, 48
   // (115) 20 to 19.
   const long long again = (long long)(b.B - 1) * b.prefix_len * Hkv * dh * 4;
   const int least_mb = b.q_start || short_all ? 256 : short_own ? 16 : 80;
@@ -1212,12 +1227,12 @@ hipError_t launch_dh(const PagedAttentionArgs &a, hipStream_t s) {
   auto attend = [&](bool tiles, bool stacked, int dense, const Parts<DH> &parts) {
     const int keys = tiles ? TKEYS : KEYS, pre_blocks = (a.b.prefix_len + keys - 1) / keys;
     // In tiles, four blocks a workgroup where groups have sixteen, two where they have eight, or
-    // writing and joining the parts of their rows takes longer: 64 tokens of one sequence of
-    // 2000 keys 28 us, with one block each 37; but 400 tokens and nothing before them, 8 heads of
+    // writing and joining the parts of their rows takes longer (without pauses 64 tokens of one
+    // sequence of 2000 keys 28 us, with one block each 37); but 400 tokens and nothing before them, 8 heads of
     // 64, 15 us with one block, 21 with four.  (Not for a prefix, which is one tile or two: 64
     // sequences over one of 4000 47 us, with one block 44.)
     const AttnSplit sp{a.b, G, a.Hkv, tiles ? TROWS : ROWS, tiles ? 6 : 7, d.stacked && !stacked ? 0 : pre_blocks, stacked,
-                       tiles && !stacked ? (int)((long long)a.b.T * G / TROWS + a.b.B) * a.Hkv : 0};
+                       tiles ? TILE_PAUSE : 0, tiles && !stacked ? (int)((long long)a.b.T * G / TROWS + a.b.B) * a.Hkv : 0};
     auto kern = tiles ? paged_attention_tile_kernel<DH> : paged_attention_kernel<DH>;
     static const char *const names[2][2] = {{"llama_paged_attention", "llama_paged_attention_tiles"},
                                             {"llama_paged_attention_prefix", "llama_paged_attention_prefix_tiles"}};

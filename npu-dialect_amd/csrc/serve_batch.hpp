@@ -76,8 +76,9 @@ NPU_HD Place place_of_token(const ServeBatch &b, int t) {
 // least, so that rows without keys are written too.  Units are numbered by
 // sequence, key head, tile, block (tiles that stand together read the same keys); workgroup w of W takes the units
 // [U w / W, U (w + 1) / W): equal shares whatever the lengths, a group cut at
-// most at the workgroups' borders.  W is at most U (split_workgroups), so that
-// every one of them has work and a cut group's parts are those of consecutive
+// most at the workgroups' borders.  Before a group's blocks come `pause` units in
+// which nothing is done: what a group costs beside its blocks.  W is at most U (split_workgroups), so that
+// every one of them has units and a cut group's parts are those of consecutive
 // workgroups.
 struct AttnSplit {
   ServeBatch b;
@@ -85,6 +86,7 @@ struct AttnSplit {
   int rows, keys_log2;
   int pre_blocks;  // prefix blocks before each tile's own keys
   int stacked;     // the prefix alone: the rows of all tokens as one sequence
+  int pause = 0;
   int long_groups = 0;  // groups, about, if workgroups are to be fewer where groups are long; 0: they are not
 };
 
@@ -113,7 +115,7 @@ NPU_HD int tile_blocks(const AttnSplit &a, int kv, int n, int tile) {
 NPU_HD long long head_units(const AttnSplit &a, int kv, int n) {
   const int tiles = split_tiles(a, n);
   long long sum = 0;
-  for (int t = 0; t < tiles; ++t) sum += tile_blocks(a, kv, n, t);
+  for (int t = 0; t < tiles; ++t) sum += tile_blocks(a, kv, n, t) + a.pause;
   return sum;
 }
 NPU_HD long long seq_units(const AttnSplit &a, int seq) {
@@ -128,7 +130,8 @@ NPU_HD long long first_unit(long long U, int W, int w) { return quotient(U * w, 
 NPU_HD int unit_owner(long long U, int W, long long u) { return (int)quotient((u + 1) * W - 1, U); }
 
 // A place in the order of the units: block blk of the nb of group (seq, tile,
-// head), whose first unit is `base`; n, start, kv: the sequence's.
+// head), whose first unit is `base`; n, start, kv: the sequence's.  blk < 0: in the
+// group's pause.
 struct UnitCursor {
   int seq, tile, head, blk, nb, n, start, kv;
   long long base;
@@ -151,17 +154,17 @@ NPU_HD UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long lo
     c.base += per * c.head;
     for (;; ++c.tile) {
       c.nb = tile_blocks(a, c.kv, c.n, c.tile);
-      if (u < c.base + c.nb) break;
-      c.base += c.nb;
+      if (u < c.base + c.nb + a.pause) break;
+      c.base += c.nb + a.pause;
     }
-    c.blk = (int)(u - c.base);
+    c.blk = (int)(u - c.base) - a.pause;
     return c;
   }
   return c;  // u is past the last unit
 }
 // The next group (the caller knows that there is one).
 NPU_HD void next_group(const AttnSplit &a, UnitCursor &c) {
-  c.base += c.nb;
+  c.base += c.nb + a.pause;
   c.blk = 0;
   if (++c.tile >= split_tiles(a, c.n)) {
     c.tile = 0;

@@ -66,4 +66,45 @@ long long serve_segments(const HostBatch *h, int G, int Hkv, int rows, int keys,
   return n;
 }
 
+// The same, as the tile kernel walks them, with a pause of that many units before each group:
+// a share may begin in one, hold nothing else, or end in one.
+long long serve_segments_paused(const HostBatch *h, int G, int Hkv, int rows, int keys, int pre_blocks, int pause,
+                                int launched, int *out, long long most) {
+  AttnSplit a{batch(h), G, Hkv, rows, __builtin_ctz(keys), pre_blocks, 0};
+  a.pause = pause;
+  long long U = 0, n = 0;
+  for (int s = 0; s < split_seqs(a); ++s) U += seq_units(a, s);
+  const int W = split_workgroups(U, launched);
+  for (int w = 0; w < W; ++w) {
+    long long u = first_unit(U, W, w);
+    const long long end = first_unit(U, W, w + 1);
+    UnitCursor c = seek_unit(a, 0, 0, u);
+    if (c.base > u || u >= c.base + c.nb + pause) return -1;
+    if (c.blk < 0) {
+      u -= c.blk;
+      c.blk = 0;
+      if (u >= end) continue;
+    }
+    long long left = end - u;
+    for (int b0 = c.blk, blk = b0;; ++blk) {
+      if (c.base + pause + blk < u || c.base + pause + blk >= end) return -3;
+      const bool same = blk + 1 < c.nb, more = left > (same ? 1 : 1 + pause);
+      if (!same || !more) {
+        if (unit_owner(U, W, c.base + pause + b0) != w || unit_owner(U, W, c.base + pause + blk) != w) return -1;
+        if (n >= most) return -2;
+        const int seg[8] = {w, c.seq, c.tile, c.head, b0, blk + 1, c.nb, c.start};
+        for (int i = 0; i < 8; ++i) out[8 * n + i] = seg[i];
+        ++n;
+        if (!more) break;
+        next_group(a, c);
+        left -= pause;
+        b0 = 0;
+        blk = -1;
+      }
+      --left;
+    }
+  }
+  return n;
+}
+
 }  // extern "C"

@@ -263,7 +263,7 @@ def test_attention_over_a_long_prefix(cuda, news, lens, H, Hkv, Dh, page, prefix
 
 @pytest.mark.parametrize("news,H,Hkv,prefix,names", [
     ([1] * 8, 8, 2, 0, ["_whole"]), ([1] * 8, 8, 2, 20, ["_whole"]), ([1] * 7, 8, 2, 6000, ["_prefix", "_whole"]),
-    ([1] * 16, 8, 2, 3000, ["_prefix_tiles", "_whole"]), ([400], 4, 2, 20, ["_tiles", "_join"]),
+    ([1] * 32, 8, 2, 3000, ["_prefix_tiles", "_whole"]), ([400], 4, 2, 20, ["_tiles", "_join"]),
     ([1], 8, 2, 1025, ["", "_join"]), ([1, 2], 8, 2, 0, ["", "_join"]), ([1, 2], 8, 2, 20, ["", "_join"]),
     ([1, 1, 2] * 5, 6, 2, 40000, ["_prefix", "", "_join"]),
     ([40] * 20, 4, 2, 28000, ["_prefix_tiles", "_tiles", "_join"]), ([15] * 30, 4, 2, 0, ["", "_join"]),

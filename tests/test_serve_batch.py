@@ -119,6 +119,33 @@ def test_every_block_of_every_tile_is_one_workgroups(host, news, lens, G, Hkv, r
         assert (mine[1:, 4] == 0).all() and (mine[:-1, 5] == mine[:-1, 6]).all()
 
 
+@pytest.mark.parametrize("news,lens,G,Hkv,rows,keys,pre,W", SPLITS + [
+    ([200, 3], [200, 900], 4, 2, 128, 64, 1, 50), ([1] * 50, [1] * 50, 1, 2, 128, 64, 0, 130)])
+@pytest.mark.parametrize("pause", [1, 3])
+def test_every_block_is_one_workgroups_with_pauses_between_groups(host, news, lens, G, Hkv, rows, keys, pre, W, pause):
+    cap = -(-max(max(lens), 1) // 16)
+    b = _batch(np.zeros((len(news), cap)), lens, np.concatenate([[0], np.cumsum(news)]), sum(news), 4, 1)
+    most = 1 << 16
+    out = np.zeros((most, 8), np.int32)
+    host.serve_segments_paused.restype = C.c_longlong
+    n = host.serve_segments_paused(C.byref(b), G, Hkv, rows, keys, pre, pause, W, C.c_void_p(out.ctypes.data),
+                                   C.c_longlong(most))
+    assert n >= 0, n
+    segs, seen, last = out[:n], {}, {}
+    want = {(s, t, h): nb for _, s, t, h, _, _, nb, _ in _segments(host, b, G, Hkv, rows, keys, pre, 0, W).tolist()}
+    for w, s, tile, h, b0, b1, nb, st in segs.tolist():
+        assert nb == want[(s, tile, h)] and b0 == seen.get((s, tile, h), 0) < b1 and st == sum(news[:s])
+        assert b0 == 0 or last[(s, tile, h)] == w - 1  # parts of consecutive workgroups
+        seen[(s, tile, h)], last[(s, tile, h)] = b1, w
+    assert seen == want
+    # shares equal in blocks and pauses, but for what is cut at their ends
+    cost = np.zeros(W)
+    for w, s, tile, h, b0, b1, nb, st in segs.tolist():
+        cost[w] += b1 - b0 + (pause if b0 == 0 else 0)
+    units = sum(nb + pause for nb in want.values())
+    assert cost.max() <= -(-units // min(W, units)) + pause
+
+
 def test_the_stacked_prefix_is_one_sequence(host):
     b = _batch(np.zeros((5, 1)), [3] * 5, None, 5, 4, 1)
     segs = _segments(host, b, 4, 2, 16, 128, 9, 1, 6)
