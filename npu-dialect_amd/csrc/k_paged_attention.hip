@@ -27,7 +27,7 @@
 // sequences of up to 8000 keys, 8 key heads of 128, 776 MB: 138 us; one of 131 000, 537 MB:
 // 96 us; 5.6 TB/s both, more than a copy's rate.
 //
-// The probabilities are rounded to bf16 for the second product (2^-9 of each
+// The probabilities are rounded to bf16 for the second product (2^-8 of each
 // term, as the prompt's attention does); sums, maxima and outputs are f32.
 #include <hip/hip_runtime.h>
 
