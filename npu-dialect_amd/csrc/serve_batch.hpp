@@ -74,12 +74,12 @@ NPU_HD Place place_of_token(const ServeBatch &b, int t) {
 // `pre_blocks` blocks and its own up to what its last token sees, are cut into
 // blocks of 2^keys_log2; a (tile, key head)'s blocks are a group of units, one at
 // least, so that rows without keys are written too.  Units are numbered by
-// sequence, key head, tile, block (tiles that stand together read the same keys); workgroup w of W takes the units
-// [U w / W, U (w + 1) / W): equal shares whatever the lengths, a group cut at
-// most at the workgroups' borders.  Before a group's blocks come `pause` units in
-// which nothing is done: what a group costs beside its blocks.  W is at most U (split_workgroups), so that
-// every one of them has units and a cut group's parts are those of consecutive
-// workgroups.
+// sequence, key head, tile, block (tiles that stand together read the same
+// keys); workgroup w of W takes the units [U w / W, U (w + 1) / W): equal shares
+// whatever the lengths, a group cut at most at the workgroups' borders.  Before a
+// group's blocks come `pause` units in which nothing is done: what a group costs
+// beside its blocks.  W is at most U (split_workgroups), so that every one of them
+// has units and a cut group's parts are those of consecutive workgroups.
 struct AttnSplit {
   ServeBatch b;
   int G, Hkv;
