@@ -13,6 +13,8 @@ device, so step() can be captured (capture()) and replayed while pages are
 added to the table between replays.  ``python -m npu_amd.serving`` runs a small
 random model.
 """
+import weakref
+
 import torch
 
 from . import groups
@@ -98,6 +100,7 @@ class Server:
         self.no_residual = torch.zeros_like(self.logits)
         self.sample_ws = groups.sample_workspace(self.logits)
         self.one = self._buffers(slots)
+        self.graphs = weakref.WeakSet()  # captured steps: they hold one's addresses and prefix_len
 
     def _tokens(self, tokens):
         tokens = [int(t) for t in tokens]
@@ -137,9 +140,11 @@ class Server:
 
     def set_prefix(self, tokens):
         """The keys and values of tokens that every sequence begins with, computed
-        once; before any sequence is added."""
+        once; before any sequence is added and any step captured."""
         if self.prefix_len or any(self.lens) or self.waiting:
             raise RuntimeError("a prefix comes before all sequences")
+        if self.graphs:
+            raise RuntimeError("a prefix comes before capture(): a captured step goes on without it")
         tokens = self._tokens(tokens)
         dev, n = self.embed.device, len(tokens)
         if n > self.pages.max_pages * self.pages.page:
@@ -227,6 +232,8 @@ class Server:
             self._step()
         self.kv_len.copy_(state[0])
         self.tokens.copy_(state[1])
+        graph.server = self  # what it reads and writes lives as long
+        self.graphs.add(graph)
         return graph
 
 

@@ -667,3 +667,29 @@ def test_serving(cuda, prefix):
         s.add(0, [1])
     with pytest.raises(ValueError, match="0 .. 447"):
         s.add(1, [448])
+
+
+def test_a_prefix_is_refused_while_a_captured_step_lives(cuda):
+    """...and the step goes on as captured; without it the prefix is taken."""
+    from npu_amd import serving
+    s = serving.Server(*serving.random_model(1, 128, 2, 192, 64, seed=6), n_heads=2, slots=2, pages=8, page=16, max_pages=3)
+    s.add(0, [1, 2, 3], temperature=0.0)
+    first = s.prefill().tolist()[0]
+    graph = s.capture()
+    s.make_room()
+    graph.replay()
+    torch.cuda.synchronize()
+    second = s.tokens.tolist()[0]
+    s.remove(0)
+    with pytest.raises(RuntimeError, match="captured"):
+        s.set_prefix([5] * 20)
+    s.add(0, [1, 2, 3], temperature=0.0)
+    assert s.prefill().tolist()[0] == first
+    s.make_room()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert s.tokens.tolist()[0] == second
+    s.remove(0)
+    del graph
+    s.set_prefix([5] * 20)
+    assert s.prefix_len == 20

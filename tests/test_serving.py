@@ -18,3 +18,41 @@ def test_pages_grow_by_need_and_are_given_back():
     p.release(0)
     assert len(p.free) == 3 and p.owned[0] == []
     assert [at for at, _ in p.grow(1, 48)] == [2]
+
+
+@pytest.fixture
+def server(monkeypatch):
+    """A Server on the host, whose groups do nothing, and torch.cuda's graphs as stand-ins."""
+    import contextlib
+
+    import torch
+
+    from npu_amd import serving
+
+    class Stream:
+        def wait_stream(self, other):
+            pass
+
+    class Graph:
+        pass
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", Graph)
+    monkeypatch.setattr(torch.cuda, "graph", lambda g: contextlib.nullcontext())
+    monkeypatch.setattr(serving, "decoder_layer", lambda p, bufs, *a: bufs["out"])
+    monkeypatch.setattr(serving.Server, "_draw", lambda self, x: self.tokens)
+    return serving.Server(*serving.random_model(1, 64, 1, 64, 32, device="cpu"), n_heads=1, slots=2, pages=8, page=16,
+                          max_pages=3)
+
+
+def test_no_prefix_while_a_captured_step_lives(server):
+    """A captured step holds the addresses of the step's buffers and the prefix's length."""
+    graph, one = server.capture(), server.one
+    with pytest.raises(RuntimeError, match="captured"):
+        server.set_prefix([1, 2, 3])
+    assert server.one is one and server.prefix_len == 0 and len(server.pages.free) == 8
+    del graph
+    server.set_prefix([1, 2, 3])
+    assert server.prefix_len == 3 and server.one is not one
