@@ -51,20 +51,34 @@ class Pages:
         self.free = list(range(pages - 1, -1, -1))
         self.owned = [[] for _ in range(slots)]
 
-    def take(self, n):
+    def _check(self, n):
         if n > len(self.free):
             raise RuntimeError(f"the cache has {len(self.free)} free pages, {n} are needed")
+
+    def take(self, n):
+        self._check(n)
         return [self.free.pop() for _ in range(n)]
 
     def grow(self, slot, keys):
         """New pages of a slot for its first ``keys`` keys: [(place, page)]."""
-        need = -(-keys // self.page)
-        if need > self.max_pages:
-            raise RuntimeError(f"{keys} keys need {need} pages, the table holds {self.max_pages}")
-        own = self.owned[slot]
-        at = len(own)
-        own.extend(self.take(max(0, need - at)))
-        return list(enumerate(own))[at:]
+        return [(at, page) for _, at, page in self.grow_all({slot: keys})]
+
+    def grow_all(self, keys):
+        """The same for several slots, {slot: keys}: [(slot, place, page)], or
+        an error and no page for any of them."""
+        new = {}
+        for slot, n in keys.items():
+            need = -(-n // self.page)
+            if need > self.max_pages:
+                raise RuntimeError(f"{n} keys need {need} pages, the table holds {self.max_pages}")
+            new[slot] = max(0, need - len(self.owned[slot]))
+        self._check(sum(new.values()))
+        placed = []
+        for slot, n in new.items():
+            at = len(self.owned[slot])
+            self.owned[slot].extend(self.take(n))
+            placed += [(slot, at + i, page) for i, page in enumerate(self.owned[slot][at:])]
+        return placed
 
     def release(self, slot):
         self.free.extend(reversed(self.owned[slot]))
@@ -134,8 +148,8 @@ class Server:
         return groups.fused_sample_tokens(self.logits, self.u, self.tokens, self.sample_ws, probs=self.probs,
                                           **self.settings)
 
-    def _place(self, slot, keys):
-        for at, page in self.pages.grow(slot, keys):
+    def _place(self, keys):
+        for slot, at, page in self.pages.grow_all(keys):
             self.page_table[slot, at] = page
 
     def set_prefix(self, tokens):
@@ -163,7 +177,7 @@ class Server:
         if self.lens[slot] or slot in self.waiting:
             raise RuntimeError(f"slot {slot} is taken")
         tokens = self._tokens(tokens)
-        self._place(slot, len(tokens))
+        self._place({slot: len(tokens)})
         self.waiting[slot] = tokens
         for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
             self.settings[name][slot] = value
@@ -206,13 +220,12 @@ class Server:
         return self._step()
 
     def make_room(self):
-        """Pages for the next token of every sequence; the host's part of a step."""
+        """Pages for the next token of every sequence; the host's part of a step.
+        Where a table or the cache is full it raises and changes nothing."""
         if self.waiting:
             raise RuntimeError("sequences wait for prefill()")
-        for s, n in enumerate(self.lens):
-            if n:
-                self._place(s, n + 1)
-                self.lens[s] = n + 1
+        self._place({s: n + 1 for s, n in enumerate(self.lens) if n})
+        self.lens = [n + 1 if n else 0 for n in self.lens]
 
     def _step(self):
         self.kv_len.add_((self.kv_len > 0).int())

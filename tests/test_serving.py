@@ -56,3 +56,28 @@ def test_no_prefix_while_a_captured_step_lives(server):
     del graph
     server.set_prefix([1, 2, 3])
     assert server.prefix_len == 3 and server.one is not one
+
+
+def test_room_is_made_for_all_sequences_or_none(server):
+    """A full table, then no free page: nothing has changed, and the next attempt is the same."""
+    state = lambda: (list(server.lens), list(server.pages.free), [list(p) for p in server.pages.owned],
+                     server.page_table.tolist())
+    server.add(0, [1] * 16), server.add(1, [1] * 48)
+    server.prefill()
+    before = state()
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="the table holds 3"):
+            server.make_room()
+        assert state() == before
+    server.remove(1)
+    server.add(1, [1] * 32)
+    server.prefill()
+    server.pages.free, rest = server.pages.free[:1], server.pages.free[1:]
+    before = state()
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="1 free pages, 2 are needed"):
+            server.make_room()
+        assert state() == before
+    server.pages.free += rest
+    server.make_room()
+    assert server.lens == [17, 33] and server.page_table[0, 1] >= 0 and server.page_table[1, 2] >= 0
