@@ -248,6 +248,7 @@ npu_status fused_llama_rmsnorm_swiglu(const npu_memref *h, const npu_memref *g2,
  * The layer's groups above take a whole prompt; the entry points below keep
  * its keys and values from step to step, attend to them, and choose tokens.
  * Beyond the conventions at the top:
+ *  - An operand that may be absent is so by a null descriptor or data pointer.
  *  - Row operands (Q, K, V, Qo, A) may have any row stride that keeps rows
  *    16-byte aligned (slices of one [T, (H + 2 Hkv) Dh] buffer), and Qo may be
  *    Q.  1-D operands and tables need contiguous rows, 4-byte aligned.
@@ -287,7 +288,7 @@ npu_status fused_llama_rope_append(const npu_memref *Q, const npu_memref *K, con
  * prefix's keys and own keys j <= kv_len[b] - n + i; a token that sees none
  * gives 0.  What the cache holds in places that a token does not see, NaN and
  * Inf too, does not count for it.  Q, A bf16 [T, H Dh]; prefix_table i32 [>= ceil(prefix_len / page)],
- * absent iff prefix_len is 0: key j of the prefix lies in page
+ * absent or empty iff prefix_len is 0: key j of the prefix lies in page
  * prefix_table[j / page], and is read once for all sequences where that pays
  * (few rows each, a long prefix).  f32 sums; the probabilities are rounded to bf16.
  * workspace f32 [n], n >= npu_paged_attention_workspace: scratch that only

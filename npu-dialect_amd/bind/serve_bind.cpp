@@ -42,7 +42,9 @@ bool describe(PyObject *o, const char *name, bool optional, npu_memref *m) {
     return false;
   }
   m->rank = (int32_t)t.dim();
-  m->allocated = m->aligned = t.data_ptr();
+  // (an empty tensor has no address, and none would mean an operand that is not present: the
+  // entry point refuses its size)
+  m->allocated = m->aligned = t.numel() > 0 ? t.data_ptr() : m;
   for (int d = 0; d < m->rank; ++d) {
     m->sizes[d] = t.size(d);
     m->strides[d] = t.stride(d);

@@ -268,7 +268,7 @@ npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_
     if (prefix_table->sizes[0] < need)
       return fail(NPU_ERR_INVALID_ARG, "prefix_table: %lld pages, the prefix needs %lld",
                   (long long)prefix_table->sizes[0], need);
-  } else if (!absent(prefix_table)) {
+  } else if (!absent(prefix_table) && prefix_table->sizes[0] != 0) {  // (no pages are a prefix's of no keys)
     return fail(NPU_ERR_INVALID_ARG, "prefix_table: given, prefix_len is 0");
   }
   if (!(scale > 0.0f) || scale > 3e38f) return fail(NPU_ERR_INVALID_ARG, "scale must be positive and finite");

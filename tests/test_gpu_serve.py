@@ -693,3 +693,30 @@ def test_a_prefix_is_refused_while_a_captured_step_lives(cuda):
     del graph
     s.set_prefix([5] * 20)
     assert s.prefix_len == 20
+
+
+def test_empty_tensors_are_refused_not_taken_as_absent(cuda):
+    from npu_amd import groups
+    from npu_amd.groups import NpuError
+    x, u = torch.zeros((2, 8), device="cuda"), torch.zeros(2, device="cuda")
+    tokens, ws = torch.full((2,), -7, dtype=torch.int32, device="cuda"), groups.sample_workspace(x)
+    empty = lambda d: torch.empty(0, dtype=d, device="cuda")
+    for name in ("temperature", "top_k", "top_p", "min_p", "probs"):
+        kw = {name: empty(torch.int32 if name == "top_k" else torch.float32)}
+        with pytest.raises(NpuError, match=rf"{name}: size\[0\] = 0 must be positive"):
+            groups.fused_sample_tokens(x, u, tokens, ws, **kw)
+    with pytest.raises(NpuError, match=r"u: size\[0\] = 0"):
+        groups.fused_sample_tokens(x, empty(torch.float32), tokens, ws)
+    bt = R.Batch([1, 1], [3, 20], 2, 64, 16, 0, ragged=False, seed=4)
+    Q = bt.rnd(2, 4 * 64)
+    A = torch.zeros_like(Q)
+    ws = groups.paged_attention_workspace(Q, bt.k_pages, bt.page_table, 0)
+    attend = lambda **kw: groups.fused_llama_paged_attention(Q, bt.k_pages, bt.v_pages, bt.page_table, bt.kv_len, A,
+                                                             0.125, ws, **kw)
+    for name, kw in (("q_start", {}), ("prefix_table", {"prefix_len": 3})):
+        with pytest.raises(NpuError, match=rf"{name}: size\[0\] = 0"):
+            attend(**{name: empty(torch.int32)}, **kw)
+    torch.cuda.synchronize()
+    assert (tokens == -7).all() and not A.any()
+    want = attend().clone()
+    assert torch.equal(attend(prefix_table=empty(torch.int32)), want)  # a prefix of no keys has no pages
