@@ -194,8 +194,8 @@ class Server:
                 "prefix_table": self.prefix_table, "prefix_len": self.prefix_len}
 
     def prefill(self):
-        """The added sequences' tokens; draws each one's next (the other slots'
-        rows of tokens and logits keep no meaning until the next step)."""
+        """The added sequences' tokens; draws each one's next (the other slots keep
+        their tokens; their rows of probs and logits mean nothing until the next step)."""
         dev, new = self.embed.device, [self.waiting.get(s, []) for s in range(self.slots)]
         start = torch.tensor([0] + [len(t) for t in new], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
         tokens = torch.tensor([t for ts in new for t in ts], dtype=torch.int64, device=dev)
@@ -232,8 +232,9 @@ class Server:
         return self._draw(self._run(self.one, self.tokens, self._batch(None)))
 
     def capture(self):
-        """step() as a graph: make_room() before each replay()."""
-        state = (self.kv_len.clone(), self.tokens.clone())
+        """step() as a graph: make_room() before each replay().  The last step's
+        tokens, probs and logits stay."""
+        state = [(t, t.clone()) for t in (self.kv_len, self.tokens, self.probs, self.logits)]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):  # once, uncaptured: the first call of a kernel asks for its occupancy
@@ -243,8 +244,8 @@ class Server:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._step()
-        self.kv_len.copy_(state[0])
-        self.tokens.copy_(state[1])
+        for t, was in state:
+            t.copy_(was)
         graph.server = self  # what it reads and writes lives as long
         self.graphs.add(graph)
         return graph

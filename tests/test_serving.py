@@ -81,3 +81,21 @@ def test_room_is_made_for_all_sequences_or_none(server):
     server.pages.free += rest
     server.make_room()
     assert server.lens == [17, 33] and server.page_table[0, 1] >= 0 and server.page_table[1, 2] >= 0
+
+
+def test_capture_leaves_what_the_last_step_gave(server, monkeypatch):
+    """Tokens, their probabilities and the logits, for whoever reads them after capture()."""
+    import torch
+
+    def draw(self, x):
+        self.logits += 1
+        self.probs += 1
+        return self.tokens.add_(1)
+
+    monkeypatch.setattr(type(server), "_draw", draw)
+    server.add(0, [1, 2, 3])
+    server.prefill()
+    shown = lambda: [t.clone() for t in (server.kv_len, server.tokens, server.probs, server.logits)]
+    before = shown()
+    server.capture()
+    assert all(map(torch.equal, shown(), before))
