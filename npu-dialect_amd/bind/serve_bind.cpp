@@ -4,6 +4,7 @@
 // A serving step calls these entry points once per layer and token with nine to
 // eleven tensors each, and a small batch's kernels run for 3 to 5 us: packing the
 // descriptors in Python took 12 us of a call, here they take less than one.
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -56,8 +57,30 @@ struct Operand {
   const char *name;
   bool optional;
 };
+// The tensors' one device has to be the current one, which the kernels run on: another's memory
+// may not be theirs to reach.  (ops[0] is never optional.)
+template <int N>
+bool on_current_device(PyObject *const *args, const Operand (&ops)[N]) {
+  if (!THPVariable_Check(args[0]) || !THPVariable_Unpack(args[0]).is_cuda()) return true;  // describe() says so
+  const c10::Device first = THPVariable_Unpack(args[0]).device();
+  for (int i = 1; i < N; ++i) {
+    if (!THPVariable_Check(args[i])) continue;
+    const at::Tensor &t = THPVariable_Unpack(args[i]);
+    if (t.is_cuda() && t.device() != first) {
+      PyErr_Format(PyExc_ValueError, "%s: on %s, %s on %s", ops[i].name, t.device().str().c_str(), ops[0].name, first.str().c_str());
+      return false;
+    }
+  }
+  const int current = c10::hip::current_device();
+  if (first.index() != current) {
+    PyErr_Format(PyExc_ValueError, "%s: on %s, the current device is cuda:%d", ops[0].name, first.str().c_str(), current);
+    return false;
+  }
+  return true;
+}
 template <int N>
 bool describe_all(PyObject *const *args, const Operand (&ops)[N], npu_memref (&m)[N]) {
+  if (!on_current_device(args, ops)) return false;
   for (int i = 0; i < N; ++i)
     if (!describe(args[i], ops[i].name, ops[i].optional, &m[i])) return false;
   return true;

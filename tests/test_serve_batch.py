@@ -277,3 +277,30 @@ def test_wrappers_refuse_host_tensors():
         groups.fused_llama_rope_append(t(1, 64), t(1, 64), t(1, 64), t(16, 32, d=torch.float32),
                                        t(16, 32, d=torch.float32), t(1, 1, 16, 64), t(1, 1, 16, 64), i(1, 1), i(1),
                                        t(1, 64))
+
+
+def _fake(number):
+    """sample_tokens' operands as tensors without memory on a device of any number."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        e = lambda *s, d=torch.float32: torch.empty(s, dtype=d, device="cuda:0")
+        args = {"logits": e(2, 64), "u": e(2), "tokens": e(2, d=torch.int32), "workspace": e(4)}
+    for t in args.values():
+        t.fake_device = torch.device("cuda", number)
+    return args
+
+
+def test_wrappers_refuse_tensors_of_several_devices():
+    from npu_amd import groups
+    for name in ("u", "tokens", "workspace"):
+        args = dict(_fake(0), **{name: _fake(1)[name]})
+        with pytest.raises(ValueError, match=f"{name}: on cuda:1, logits on cuda:0"):
+            groups.fused_sample_tokens(**args)
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_tensors_of_another_than_the_current_device(cuda):
+    from npu_amd import groups
+    with pytest.raises(ValueError, match="logits: on cuda:1, the current device is cuda:0"):
+        groups.fused_sample_tokens(**_fake(1))
