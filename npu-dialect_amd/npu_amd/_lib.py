@@ -187,7 +187,8 @@ def serve():
     try:
         from . import _serve
     except ImportError as e:
-        raise RuntimeError(f"npu_amd._serve not built: build it with `make -C {SRC_DIR}`") from e
+        raise RuntimeError(f"npu_amd._serve not built: build it with `make -C {SRC_DIR}`, whose PYTHON "
+                           "has to have this torch") from e
     return _serve
 
 

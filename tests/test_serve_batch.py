@@ -304,3 +304,14 @@ def test_wrappers_refuse_tensors_of_another_than_the_current_device(cuda):
     from npu_amd import groups
     with pytest.raises(ValueError, match="logits: on cuda:1, the current device is cuda:0"):
         groups.fused_sample_tokens(**_fake(1))
+
+
+# ---- the build -----------------------------------------------------------------------
+@pytest.mark.parametrize("python,built", [("python3", True), ("false", False)])
+def test_the_python_binding_is_built_where_there_is_a_torch_to_bind_to(python, built):
+    """The library itself needs hipcc and g++ alone."""
+    import subprocess
+    said = subprocess.run(["make", "-n", "-B", "-C", _lib.SRC_DIR, f"PYTHON={python}"], check=True, capture_output=True,
+                          text=True).stdout
+    assert "libnpu_amd.so" in said and "libnpu_host.so" in said and "npu_calibrate" in said
+    assert ("serve_bind.cpp" in said) == built
