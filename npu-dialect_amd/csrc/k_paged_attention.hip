@@ -173,35 +173,54 @@ __device__ __forceinline__ T wave_scan(T v) {
   return v;
 }
 
+__device__ __forceinline__ long long lane_value(long long v, int lane) {
+  return (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+                     (unsigned)__builtin_amdgcn_readlane((int)v, lane));
+}
+
+// serve_batch.hpp's wave.
+struct Wave64 {
+  using Ints = int;
+  int lane;
+  template <class F>
+  __device__ __forceinline__ int each(F f) const {
+    return f(lane);
+  }
+  template <class F>
+  __device__ __forceinline__ long long sum(F f) const {
+    return lane_value(wave_scan((long long)f(lane)), 63);
+  }
+  __device__ __forceinline__ int scan(int v) const { return wave_scan(v); }
+  __device__ __forceinline__ int at(int v, int l) const { return __builtin_amdgcn_readlane(v, l); }
+  __device__ __forceinline__ int above(int v, int x) const { return __builtin_ctzll(__ballot(v > x)); }
+  __device__ __forceinline__ int same(int v) const { return __builtin_amdgcn_readfirstlane(v); }
+  __device__ __forceinline__ long long same(long long v) const { return uniform(v); }
+};
+
 // A workgroup's number w in the division, its share of the units, [u0, u1) of U,
 // and the group its first lies in; false: none (the launch has more workgroups
-// than units, or the share is in a pause).  by_xcd: workgroups that the dispatcher puts on one XCD (every
-// eighth) take neighbouring shares, whose tiles read the same keys.
-// Every workgroup finds its own: the units of each sequence (by a lane each or,
-// where they have many tiles, by a wave each), a scan over the lanes, and in the
-// sequence that holds u0 a scan over its tiles.
+// than units, or the share is in a pause).  Every workgroup finds its own: the
+// units of each sequence, a scan over the lanes, and in the sequence that holds u0 a
+// scan over its tiles.
 struct Share {
   long long sum[NT], wave[NT / 64];
-  long long base, per;  // of the sequence: its first unit, the units of a key head
-  int seq;
+  SeqUnits seq;  // the one that holds u0
 };
 __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long long &U, int &W, long long &u0,
                                            long long &u1, UnitCursor &c, int &w, bool by_xcd) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int seqs = split_seqs(sp), per = (seqs + NT - 1) / NT;
+  const int seqs = split_seqs(sp), per = seqs_per_lane(sp, NT);
+  const Wave64 lanes{lane};
   long long mine = 0;
-  if (seqs <= NT && (unsigned)sp.b.T * sp.G / (unsigned)sp.rows >= 16u * seqs) {
+  if (sum_by_waves(sp, NT)) {
     for (int q = wave; q < seqs; q += NT / 64) {
-      const int n = split_span(sp, q).n, kv = split_kv(sp, q), tiles = split_tiles(sp, n);
-      long long sum = 0;
-      for (int t = lane; t < tiles; t += 64) sum += tile_blocks(sp, kv, n, t) + sp.pause;
-      sum = wave_scan(sum);
-      if (lane == 63) s.sum[q] = sum * sp.Hkv;
+      const long long units = head_units_by(lanes, sp, split_kv(sp, q), split_span(sp, q).n) * sp.Hkv;
+      if (lane == 63) s.sum[q] = units;
     }
     __syncthreads();
     if (tid < seqs) mine = s.sum[tid];
   } else {
-    for (int q = tid * per; q < min(seqs, (tid + 1) * per); ++q) mine += seq_units(sp, q);
+    mine = lane_units(sp, tid, per);
   }
   const long long in_wave = wave_scan(mine);
   if (lane == 63) s.wave[wave] = in_wave;
@@ -213,58 +232,20 @@ __device__ __forceinline__ bool take_share(const AttnSplit &sp, Share &s, long l
     U += s.wave[v];
   }
   U = uniform(U);
-  const int few = sp.long_groups > 0 ? (U >= (8ll + sp.pause) * sp.long_groups) + (U >= (16ll + sp.pause) * sp.long_groups) : 0;
-  W = split_workgroups(U >> few, gridDim.x);
-  w = blockIdx.x;
-  if (by_xcd && W == (int)gridDim.x && W % 8 == 0) w = (w & 7) * (W >> 3) + (w >> 3);
-  if (w >= W) return false;
-  u0 = first_unit(U, W, w);
-  u1 = first_unit(U, W, w + 1);
-  if (u0 >= before && u0 < before + mine) {  // one lane's sequences hold u0
-    int q = tid * per;
-    long long units = mine;
-    for (; per > 1; ++q) {
-      units = seq_units(sp, q);
-      if (u0 < before + units) break;
-      before += units;
-    }
-    s.seq = q;
-    s.base = before;
-    s.per = units / sp.Hkv;
-  }
+  ShareRange r;
+  const bool some = share_of(sp, U, gridDim.x, blockIdx.x, by_xcd, r);
+  W = r.W;
+  w = r.w;
+  if (!some) return false;
+  u0 = r.u0;
+  u1 = r.u1;
+  // one lane's sequences hold u0
+  if (u0 >= before && u0 < before + mine) s.seq = seq_in_lane(sp, tid, per, before, mine, u0);
   __syncthreads();
-  c.seq = __builtin_amdgcn_readfirstlane(s.seq);
-  const SeqSpan span = split_span(sp, c.seq);
-  c.n = span.n;
-  c.start = span.start;
-  c.kv = split_kv(sp, c.seq);
-  c.head = __builtin_amdgcn_readfirstlane((int)quotient(u0 - s.base, s.per));
-  c.base = s.base + c.head * s.per;
-  int rest = (int)min(u0 - c.base, (long long)0x7fffffff);  // units before u0 in the tiles from c.tile on
-  for (c.tile = 0;; c.tile += 64) {
-    const int tiles = split_tiles(sp, c.n);
-    const int nb = c.tile + lane < tiles ? tile_blocks(sp, c.kv, c.n, c.tile + lane) + sp.pause : 0;
-    const int up_to = wave_scan(nb), all = __builtin_amdgcn_readlane(up_to, 63);
-    if (rest < all) {
-      const int at = __builtin_ctzll(__ballot(up_to > rest));
-      c.tile += at;
-      c.nb = __builtin_amdgcn_readlane(nb, at);
-      const int skipped = __builtin_amdgcn_readlane(up_to, at) - c.nb;
-      c.nb -= sp.pause;
-      c.base += skipped;
-      c.blk = rest - skipped - sp.pause;
-      break;
-    }
-    c.base += all;
-    rest -= all;
-  }
-  c.blk = __builtin_amdgcn_readfirstlane(c.blk);
-  c.tile = __builtin_amdgcn_readfirstlane(c.tile);
-  c.base = uniform(c.base);
-  if (c.blk < 0) {  // in the group's pause
-    u0 -= c.blk;
-    c.blk = 0;
-  }
+  SeqUnits seq = s.seq;
+  seq.seq = __builtin_amdgcn_readfirstlane(seq.seq);
+  c = seek_in_seq(lanes, sp, seq, u0);
+  skip_pause(c, u0);
   return u0 < u1;
 }
 

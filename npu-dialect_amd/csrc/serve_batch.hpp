@@ -1,8 +1,8 @@
 // serve_batch.hpp -- where a serving batch's tokens, keys and work lie: the
-// lookups in kv_len, q_start and the page tables, and the division of an
-// attention over workgroups.  Plain functions of the arrays, compiled for the
-// device by the kernels and for the host by a test: every index that a kernel
-// forms from a caller's array is formed here.
+// lookups in kv_len and q_start, the check of a page number, and the division of an
+// attention over workgroups, with the search by which each finds its share.  Plain
+// functions of the arrays, compiled for the device by the kernels and for the host by
+// tests.
 #pragma once
 
 #ifdef __HIPCC__
@@ -136,32 +136,6 @@ struct UnitCursor {
   int seq, tile, head, blk, nb, n, start, kv;
   long long base;
 };
-// The group of unit u, from sequence seq on, whose first unit is `base`.
-NPU_HD UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long long u) {
-  UnitCursor c{seq, 0, 0, 0, 1, 0, 0, 0, base};
-  const int seqs = split_seqs(a);
-  for (; c.seq < seqs; ++c.seq) {
-    const SeqSpan sp = split_span(a, c.seq);
-    c.n = sp.n;
-    c.start = sp.start;
-    c.kv = split_kv(a, c.seq);
-    const long long per = head_units(a, c.kv, c.n);
-    if (u >= c.base + per * a.Hkv) {
-      c.base += per * a.Hkv;
-      continue;
-    }
-    c.head = (int)((u - c.base) / per);
-    c.base += per * c.head;
-    for (;; ++c.tile) {
-      c.nb = tile_blocks(a, c.kv, c.n, c.tile);
-      if (u < c.base + c.nb + a.pause) break;
-      c.base += c.nb + a.pause;
-    }
-    c.blk = (int)(u - c.base) - a.pause;
-    return c;
-  }
-  return c;  // u is past the last unit
-}
 // The next group (the caller knows that there is one).
 NPU_HD void next_group(const AttnSplit &a, UnitCursor &c) {
   c.base += c.nb + a.pause;
@@ -181,5 +155,148 @@ NPU_HD void next_group(const AttnSplit &a, UnitCursor &c) {
   }
   c.nb = tile_blocks(a, c.kv, c.n, c.tile);
 }
+
+// ---- a workgroup's share of the units, found by its lanes together -----------------
+// `wave` stands for 64 lanes: each(f) is f(lane) of all of them (as Ints), sum(f) the
+// total of f(lane), scan() the inclusive sums over the lanes, at() one lane's value,
+// above() the first lane whose value exceeds another, same() a value that all lanes have.
+// The kernels' wave is the hardware's, HostWave 64 numbers.
+
+// Units of one key head of a sequence of n new tokens, its tiles over the lanes.
+template <class Wave>
+NPU_HD long long head_units_by(const Wave &wave, const AttnSplit &a, int kv, int n) {
+  const int tiles = split_tiles(a, n);
+  return wave.sum([&](int lane) {
+    long long sum = 0;
+    for (int t = lane; t < tiles; t += 64) sum += tile_blocks(a, kv, n, t) + a.pause;
+    return sum;
+  });
+}
+// Whether the sequences' units are summed by a wave each, for as many as there are lanes at
+// most; else by a lane each, or by a lane for `per` of them.
+NPU_HD bool sum_by_waves(const AttnSplit &a, int lanes) {
+  const int seqs = split_seqs(a);
+  return seqs <= lanes && (unsigned)a.b.T * a.G / (unsigned)a.rows >= 16u * seqs;
+}
+NPU_HD int seqs_per_lane(const AttnSplit &a, int lanes) { return (split_seqs(a) + lanes - 1) / lanes; }
+NPU_HD long long lane_units(const AttnSplit &a, int tid, int per) {
+  const int seqs = split_seqs(a), end = seqs - tid * per < per ? seqs : (tid + 1) * per;
+  long long sum = 0;
+  for (int q = tid * per; q < end; ++q) sum += seq_units(a, q);
+  return sum;
+}
+// Workgroup `block` of those launched is number w of the W that have units, and takes [u0, u1)
+// of all U; false: it has none.  by_xcd: workgroups that the dispatcher puts on one XCD (every
+// eighth) take neighbouring shares.
+struct ShareRange {
+  int W, w;
+  long long u0, u1;
+};
+NPU_HD bool share_of(const AttnSplit &a, long long U, int launched, int block, bool by_xcd, ShareRange &s) {
+  const long long groups = a.long_groups;
+  const int few = groups > 0 ? (U >= (8 + a.pause) * groups) + (U >= (16 + a.pause) * groups) : 0;
+  s.W = split_workgroups(U >> few, launched);
+  s.w = by_xcd && s.W == launched && s.W % 8 == 0 ? (block & 7) * (s.W >> 3) + (block >> 3) : block;
+  if (s.w >= s.W) return false;
+  s.u0 = first_unit(U, s.W, s.w);
+  s.u1 = first_unit(U, s.W, s.w + 1);
+  return true;
+}
+// A sequence, its first unit and the units of one of its key heads.
+struct SeqUnits {
+  int seq;
+  long long base, per_head;
+};
+// Of lane tid's sequences, which have `units` from unit `base` on, the one that holds unit u.
+NPU_HD SeqUnits seq_in_lane(const AttnSplit &a, int tid, int per, long long base, long long units, long long u) {
+  int q = tid * per;
+  for (; per > 1; ++q) {
+    units = seq_units(a, q);
+    if (u < base + units) break;
+    base += units;
+  }
+  return SeqUnits{q, base, units / a.Hkv};
+}
+// The group of unit u in its sequence: a scan over the sequence's tiles.
+template <class Wave>
+NPU_HD UnitCursor seek_in_seq(const Wave &wave, const AttnSplit &a, const SeqUnits &s, long long u) {
+  const SeqSpan sp = split_span(a, s.seq);
+  UnitCursor c{s.seq, 0, 0, 0, 1, sp.n, sp.start, split_kv(a, s.seq), s.base};
+  c.head = wave.same((int)quotient(u - s.base, s.per_head));
+  c.base += c.head * s.per_head;
+  const long long in_head = u - c.base;
+  int rest = (int)(in_head < 0x7fffffff ? in_head : 0x7fffffff);  // units before u in the tiles from c.tile on
+  for (;; c.tile += 64) {
+    const int tiles = split_tiles(a, c.n);
+    const typename Wave::Ints nb = wave.each(
+        [&](int lane) { return c.tile + lane < tiles ? tile_blocks(a, c.kv, c.n, c.tile + lane) + a.pause : 0; });
+    const typename Wave::Ints up_to = wave.scan(nb);
+    const int all = wave.at(up_to, 63);
+    if (rest < all) {
+      const int at = wave.above(up_to, rest), here = wave.at(nb, at), skipped = wave.at(up_to, at) - here;
+      c.tile += at;
+      c.nb = here - a.pause;
+      c.base += skipped;
+      c.blk = rest - skipped - a.pause;
+      break;
+    }
+    c.base += all;
+    rest -= all;
+  }
+  c.blk = wave.same(c.blk);
+  c.tile = wave.same(c.tile);
+  c.base = wave.same(c.base);
+  return c;
+}
+// Past the group's pause, from where u0 counts on.
+NPU_HD void skip_pause(UnitCursor &c, long long &u0) {
+  if (c.blk < 0) {
+    u0 -= c.blk;
+    c.blk = 0;
+  }
+}
+
+#ifndef __HIPCC__
+struct HostWave {
+  struct Ints {
+    int v[64];
+  };
+  template <class F>
+  Ints each(F f) const {
+    Ints r;
+    for (int l = 0; l < 64; ++l) r.v[l] = f(l);
+    return r;
+  }
+  template <class F>
+  long long sum(F f) const {
+    long long s = 0;
+    for (int l = 0; l < 64; ++l) s += f(l);
+    return s;
+  }
+  Ints scan(Ints x) const {
+    for (int l = 1; l < 64; ++l) x.v[l] += x.v[l - 1];
+    return x;
+  }
+  int at(const Ints &x, int l) const { return x.v[l]; }
+  int above(const Ints &x, int y) const {
+    int l = 0;
+    while (x.v[l] <= y) ++l;
+    return l;
+  }
+  template <class T>
+  T same(T v) const {
+    return v;
+  }
+};
+// The group of unit u, from sequence seq on, whose first unit is `base`.
+inline UnitCursor seek_unit(const AttnSplit &a, int seq, long long base, long long u) {
+  for (; seq < split_seqs(a); ++seq) {
+    const long long units = seq_units(a, seq);
+    if (u < base + units) return seek_in_seq(HostWave(), a, SeqUnits{seq, base, units / a.Hkv}, u);
+    base += units;
+  }
+  return UnitCursor{seq, 0, 0, 0, 1, 0, 0, 0, base};  // u is past the last unit
+}
+#endif
 
 }  // namespace npu
