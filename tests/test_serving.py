@@ -93,6 +93,7 @@ def test_capture_leaves_what_the_last_step_gave(server, monkeypatch):
         return self.tokens.add_(1)
 
     monkeypatch.setattr(type(server), "_draw", draw)
+    server.logits.zero_()
     server.add(0, [1, 2, 3])
     server.prefill()
     shown = lambda: [t.clone() for t in (server.kv_len, server.tokens, server.probs, server.logits)]
