@@ -1148,23 +1148,39 @@ bool can_stack(const ServeBatch &b, long long rows) {
   return b.prefix_len > 0 && b.B > 1 && rows < (long long)b.B * TROWS;
 }
 // The rules' figures are us with a rule's one side and its other, G = 4, Dh = 128 unless said.
+// Whether one token a sequence sees no more keys of a sequence's own than a workgroup takes.
+bool short_table(const ServeBatch &b) { return !b.q_start && (long long)b.max_pages << b.page_log2 <= 1024; }
+// 128-row tiles for the own keys' part.  Such a tile reads keys once for what takes 16-row
+// tiles two reads and more, but its blocks follow each other more slowly, so there have to be
+// enough: by 16-row tiles of all key heads.  8 sequences of 2000 to 4000 keys, 8 new tokens (128
+// tiles): 33 us, in 16-row tiles 46; 64 new tokens of one sequence of 2000 (128): 24 to 35; 32 of
+// them (64): 20 to 21; 60 new tokens, twice, of 12 heads and 77 keys before (90): 14 to 13;
+// 4 new tokens of 8 sequences (one tile each): 30 to 30.
+// Between one 16-row tile a sequence and two there have to be more of them: 5 new tokens of 64
+// sequences of 500 to 2000 keys (640) 86 to 137, of 16 (160) 30 to 43, one token and 20 query heads
+// of 64 (320) 46 to 74; 15 new tokens of 30, G = 2, 500 keys (112) 21 to 18; but whole groups
+// are faster: one token, 24 query heads, 64 sequences of 100 to 1000 keys 31 to 28.
+// T and B do not say how the tokens are spread, and one long sequence in 16-row tiles costs
+// several times the call: 127 sequences of one token and one of 800 264 to 549, 255 and 256
+// tokens after 16000 keys 325 to 899.  So with seven 128-row tiles' rows beyond a token each
+// they are taken, at a cost where the rows are spread evenly: 2 tokens of 256 sequences 244 to
+// 237, 4 of 128 139 to 133; with fewer rows it would be larger (4 of 64 91 to 77).
+bool tiles_for_own(const ServeBatch &b, long long G, int Hkv, bool short_own_keys) {
+  const long long rows = b.T * G, tiles16 = rows * Hkv / ROWS;
+  if (rows >= (long long)b.B * 2 * ROWS) return tiles16 >= 96;
+  return tiles16 >= 128 && !short_own_keys && (rows > (long long)b.B * ROWS || ((long long)b.T - b.B) * G >= 7 * TROWS);
+}
 Division divide(const ServeBatch &b, int H, int Hkv, int dh) {
   const long long G = H / Hkv, rows = b.T * G;
   const long long own_keys = (long long)b.max_pages << b.page_log2;  // what the table can name
   Division d;
   d.W = 2 * device_cus();
-  // A 128-row tile reads keys once for what takes 16-row tiles two reads and more, but its
-  // blocks follow each other more slowly, so there have to be enough: by 16-row
-  // tiles of all key heads.  8 sequences of 2000 to 4000 keys, 8 new tokens (128 tiles): 33
-  // us, in 16-row tiles 46; 64 new tokens of one sequence of 2000 (128): 24 to 35; 32 of
-  // them (64): 20 to 21; 60 new tokens, twice, of 12 heads and 77 keys before (90): 14 to 13;
-  // 4 new tokens of 8 sequences (one tile each): 30 to 30.
-  d.own_tiles = rows >= (long long)b.B * 2 * ROWS && rows * Hkv >= 96 * ROWS;
+  d.own_tiles = tiles_for_own(b, G, Hkv, short_table(b));
   // 64 sequences over 4096 keys of prefix: 32 us to 44; 32: 29 to 29; 16: 25 to 23; 4: 20 to 16
   d.pre_tiles = rows >= 8 * ROWS;
   // Up to 1024 keys a group takes no longer than its cut parts and their join: 64 sequences
   // of up to 1000 keys 39 us to 47, 8 of them 15 to 15, one 10 to 11; up to 2000, one 18 to 12.
-  const bool short_own = !b.q_start && !d.own_tiles && own_keys <= 1024;
+  const bool short_own = short_table(b) && !d.own_tiles;
   const bool short_all = short_own && own_keys + b.prefix_len <= 1024;
   // A prefix that sequences share has a product of its own, with all their rows, if each has
   // less than a tile of rows and the keys and values that are then not read again
@@ -1188,9 +1204,10 @@ size_t slot_bytes(const Division &d, bool tiles) {
 
 template <int DH>
 size_t workspace_of(const ServeBatch &b, int H, int Hkv) {
-  // (whatever the division makes of the arrays that the call brings)
+  // (whatever the division makes of the arrays that the call brings: the larger tiles, if any
+  // table has them)
   const Division d = divide(b, H, Hkv, DH);
-  const size_t own = slot_bytes<DH>(d, d.own_tiles), plain = d.W * sizeof(PartInfo) + 2 * own;
+  const size_t own = slot_bytes<DH>(d, tiles_for_own(b, H / Hkv, Hkv, false)), plain = d.W * sizeof(PartInfo) + 2 * own;
   if (!can_stack(b, (long long)b.T * (H / Hkv))) return plain;
   return std::max(plain, 2 * (size_t)b.T * H * sizeof(PartRow<DH>) + own + slot_bytes<DH>(d, d.pre_tiles));
 }

@@ -720,3 +720,25 @@ def test_empty_tensors_are_refused_not_taken_as_absent(cuda):
     assert (tokens == -7).all() and not A.any()
     want = attend().clone()
     assert torch.equal(attend(prefix_table=empty(torch.int32)), want)  # a prefix of no keys has no pages
+
+
+@pytest.mark.parametrize("news,lens,G,Hkv,Dh,kind,names", [
+    # a prompt in one of many slots, and pieces of prompts among sequences of one token
+    ([0] * 30 + [700] + [0] * 9, [0] * 30 + [700] + [50] * 9, 1, 4, 64, {}, ["_tiles", "_join"]),
+    ([0] * 290 + [5000], [0] * 290 + [5020], 1, 1, 64, {}, ["_tiles", "_join"]),
+    ([1] * 60 + [300] + [1] * 20, [30 * (i % 9) for i in range(60)] + [900] + [40] * 20, 4, 2, 128, {}, ["_tiles", "_join"]),
+    ([1] * 100 + [240], [7 * i for i in range(100)] + [1000], 4, 2, 64, {}, ["_tiles", "_join"]),
+    ([1] * 100 + [220], [7 * i for i in range(100)] + [1000], 4, 2, 64, {}, ["", "_join"]),
+    # as many rows each: one 16-row tile, two
+    ([4] * 64, [11 * i for i in range(64)], 4, 2, 64, {}, ["", "_join"]),
+    ([5] * 64, [11 * i for i in range(64)], 4, 2, 64, {}, ["_tiles", "_join"]),
+    ([1] * 60, [13 * i for i in range(60)], 20, 2, 64, {"ragged": False, "max_pages": 70}, ["_tiles", "_join"]),
+    ([1] * 60, [13 * i for i in range(60)], 20, 2, 64, {"ragged": False, "max_pages": 64}, ["_whole"]),
+])
+def test_attention_of_uneven_batches(cuda, news, lens, G, Hkv, Dh, kind, names):
+    """Tokens spread over the sequences in any way: no long one in small tiles."""
+    from npu_amd import groups
+    bt = R.Batch(news, lens, Hkv, Dh, 16, 0, seed=len(news) + G, **kind)
+    with groups.collect_plans() as cp:
+        _check_attend(bt, bt.rnd(bt.T, G * Hkv * Dh))
+    assert [p.kernel.decode() for p in cp.plans] == ["llama_paged_attention" + n for n in names]
