@@ -258,7 +258,9 @@ npu_status fused_llama_rmsnorm_swiglu(const npu_memref *h, const npu_memref *g2,
  *  - The batch: B sequences (the rows of page_table i32 [B, max_pages]).
  *    Sequence b has the new tokens q_start[b] .. q_start[b+1]-1 of the T rows
  *    (q_start i32 [B+1], not decreasing; absent: T = B, token b is b's), and
- *    kv_len[b] own keys, the new tokens' included, 0 allowed.  Own key j lies
+ *    kv_len[b] own keys, the new tokens' included, 0 allowed.  (The host sees T
+ *    and B alone: sequences without new tokens are better left out of a batch
+ *    where it chooses between kernels by tokens a sequence.)  Own key j lies
  *    in page page_table[b][j / page] at slot j % page.  All sequences share
  *    prefix_len keys before their own (0: none).  New token i of n is own key
  *    j = kv_len[b] - n + i, at position prefix_len + j.

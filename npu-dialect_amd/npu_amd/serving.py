@@ -189,8 +189,10 @@ class Server:
         self.kv_len[slot] = 0
         self.page_table[slot] = -1
 
-    def _batch(self, q_start):
-        return {"page_table": self.page_table, "kv_len": self.kv_len, "q_start": q_start,
+    def _batch(self, q_start=None, slots=None):
+        """Of all slots, a token each, or of those that have new tokens."""
+        of = lambda t: t if slots is None else t[slots]
+        return {"page_table": of(self.page_table), "kv_len": of(self.kv_len), "q_start": q_start,
                 "prefix_table": self.prefix_table, "prefix_len": self.prefix_len}
 
     def prefill(self):
@@ -205,7 +207,10 @@ class Server:
         for s, t in self.waiting.items():
             self.lens[s] = len(t)
             self.kv_len[s] = len(t)
-        x = self._run(self._buffers(len(tokens)), tokens, self._batch(start))
+        # (a slot without new tokens would count as a sequence where tiles are chosen)
+        slots = torch.tensor(sorted(self.waiting), device=dev)
+        batch = self._batch(torch.cat([start[:1], start[slots + 1]]), slots)
+        x = self._run(self._buffers(len(tokens), batch["page_table"]), tokens, batch)
         last = (start[1:].long() - 1).clamp(min=0)
         self._draw(x[last])
         fresh = (start[1:] > start[:-1])
@@ -229,7 +234,7 @@ class Server:
 
     def _step(self):
         self.kv_len.add_((self.kv_len > 0).int())
-        return self._draw(self._run(self.one, self.tokens, self._batch(None)))
+        return self._draw(self._run(self.one, self.tokens, self._batch()))
 
     def capture(self):
         """step() as a graph: make_room() before each replay().  The last step's

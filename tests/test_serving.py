@@ -100,3 +100,22 @@ def test_capture_leaves_what_the_last_step_gave(server, monkeypatch):
     before = shown()
     server.capture()
     assert all(map(torch.equal, shown(), before))
+
+
+def test_prefill_takes_the_waiting_sequences_alone(server, monkeypatch):
+    """A batch of the slots that have new tokens: the others would count as sequences where
+    the attention chooses its tiles."""
+    from npu_amd import serving
+    ran = []
+    monkeypatch.setattr(serving, "decoder_layer", lambda p, bufs, cache, batch, *a: ran.append((bufs, batch)) or bufs["out"])
+    server.add(1, list(range(20)))
+    server.prefill()
+    (bufs, batch), = ran
+    assert batch["q_start"].tolist() == [0, 20] and batch["kv_len"].tolist() == [20]
+    assert batch["page_table"].tolist() == [server.page_table[1].tolist()] and bufs["Q"].shape[0] == 20
+    server.remove(1)
+    server.add(1, [4] * 3), server.add(0, [5, 6])
+    server.prefill()
+    _, batch = ran[1]
+    assert batch["q_start"].tolist() == [0, 2, 5] and batch["kv_len"].tolist() == [2, 3]
+    assert batch["page_table"].tolist() == server.page_table.tolist()
