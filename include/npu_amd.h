@@ -322,7 +322,8 @@ int64_t npu_paged_attention_workspace(int64_t T, int64_t B, int32_t n_heads, int
  *   logits f32 or bf16 [B, V], V <= 2^20, rows at any stride; u, temperature,
  *   top_p, min_p f32 [B], top_k i32 [B] (each but u may be absent: off,
  *   temperature 1); tokens i32 [B]; probs f32 [B], may be absent; workspace
- *   f32 [n], n >= npu_sample_workspace.
+ *   f32 [n], n >= npu_sample_workspace: scratch of one call at a time (a few
+ *   bytes, which the kernel there is leaves alone).
  * Weights are f64 rounded to 2^-42, their sums exact: the same input gives the
  * same token every time. */
 npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u,

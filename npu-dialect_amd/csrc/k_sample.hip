@@ -742,8 +742,6 @@ __global__ __launch_bounds__(ST, 1) void sample_tokens_kernel(SampleArgs a) {
 
 }  // namespace
 
-size_t sample_workspace(int, int) { return 16; }
-
 hipError_t launch_sample_tokens(const SampleArgs &a, hipStream_t s) {
   auto kern = a.bf16 ? sample_tokens_kernel<true> : sample_tokens_kernel<false>;
   {

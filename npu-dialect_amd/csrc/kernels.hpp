@@ -128,9 +128,7 @@ struct SampleArgs {
   const int *top_k;                              // may be null
   int *tokens;
   float *probs;  // may be null
-  void *workspace;
 };
-size_t sample_workspace(int B, int V);  // bytes
 hipError_t launch_sample_tokens(const SampleArgs &a, hipStream_t s);
 
 }  // namespace npu

@@ -283,9 +283,10 @@ npu_status fused_llama_paged_attention(const npu_memref *Q, const npu_memref *k_
                   [&] { return npu::launch_llama_paged_attention(a, static_cast<hipStream_t>(stream)); });
 }
 
+// (a row's state is in LDS: the workspace is checked, for kernels that share a row, and not used)
 int64_t npu_sample_workspace(int64_t B, int64_t V) {
   if (B <= 0 || B > kMaxInt || V <= 0 || V > 1 << 20) return -1;
-  return (int64_t)((npu::sample_workspace((int)B, (int)V) + sizeof(float) - 1) / sizeof(float));
+  return 4;
 }
 
 npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u, const npu_memref *temperature,
@@ -297,6 +298,7 @@ npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u, co
   if (!logits) return fail(NPU_ERR_INVALID_ARG, "logits: null descriptor");
   a.bf16 = logits->dtype == NPU_BF16;
   const void *pl, *p[7] = {};
+  void *ws;
   NPU_TRY(check_rows(logits, "logits", a.bf16 ? NPU_BF16 : NPU_F32, a.bf16 ? 2 : 4, &pl, &a.row_stride));
   const long long B = logits->sizes[0], V = logits->sizes[1];
   if (V > 1 << 20) return fail(NPU_ERR_UNSUPPORTED, "logits: %lld columns, at most 2^20", V);
@@ -307,7 +309,7 @@ npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u, co
   if (!absent(min_p)) NPU_TRY(check_vec(min_p, "min_p", NPU_F32, B, &p[4]));
   NPU_TRY(check_vec(tokens, "tokens", NPU_I32, B, &p[5]));
   if (!absent(probs)) NPU_TRY(check_vec(probs, "probs", NPU_F32, B, &p[6]));
-  NPU_TRY(check_workspace(workspace, npu_sample_workspace(B, V), &a.workspace));
+  NPU_TRY(check_workspace(workspace, npu_sample_workspace(B, V), &ws));
   a.logits = pl;
   a.B = (int)B;
   a.V = (int)V;

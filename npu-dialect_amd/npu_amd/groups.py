@@ -251,7 +251,8 @@ def fused_llama_paged_attention(Q, k_pages, v_pages, page_table, kv_len, A, scal
 
 def sample_workspace(logits):
     """A workspace for fused_sample_tokens calls on logits of this shape; one
-    for each call that may run at the same time."""
+    for each call that may run at the same time (a few bytes, which the kernel
+    there is leaves alone)."""
     import torch
     n = _lib.lib().npu_sample_workspace(*logits.shape)
     if n < 0:
