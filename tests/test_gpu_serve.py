@@ -742,3 +742,75 @@ def test_attention_of_uneven_batches(cuda, news, lens, G, Hkv, Dh, kind, names):
     with groups.collect_plans() as cp:
         _check_attend(bt, bt.rnd(bt.T, G * Hkv * Dh))
     assert [p.kernel.decode() for p in cp.plans] == ["llama_paged_attention" + n for n in names]
+
+
+def test_two_threads_on_two_streams(cuda):
+    """Each of the serving calls on two streams at the same time, with workspaces of their own:
+    the bits of the same calls alone, and each thread's own errors and plans."""
+    import threading
+
+    from npu_amd import _lib, groups
+    batches = [R.Batch([1] * 40, [97 * i % 1500 for i in range(40)], 2, 128, 16, 0, ragged=False, max_pages=96, seed=11),
+               R.Batch([200, 0, 90], [260, 5, 400], 2, 128, 16, 40, seed=12)]
+    logits = [_logits(20, 40000, 13), _logits(9, 50001, 14, dtype=torch.bfloat16)]
+
+    def prepare(i):
+        bt, x = batches[i], logits[i]
+        cos, sin = (t.cuda() for t in R.rope_tables(bt.prefix + bt.max_pages * bt.page, 64))
+        Q = bt.rnd(bt.T, 8 * 128)
+        K, V, B = bt.rnd(bt.T, 256), bt.rnd(bt.T, 256), x.shape[0]
+        Qo, A = torch.zeros_like(Q), torch.zeros_like(Q)
+        tokens = torch.zeros(B, dtype=torch.int32, device="cuda")
+        ws, sws = groups.paged_attention_workspace(Q, bt.k_pages, bt.page_table, bt.prefix), groups.sample_workspace(x)
+        u, p = torch.linspace(0, 0.99, B, device="cuda"), torch.full((B,), 0.9, device="cuda")
+
+        def run(stream):
+            groups.fused_llama_rope_append(Q, K, V, cos, sin, bt.k_pages, bt.v_pages, bt.page_table, bt.kv_len, Qo,
+                                           q_start=bt.q_start, prefix_len=bt.prefix, stream=stream)
+            groups.fused_llama_paged_attention(Qo, bt.k_pages, bt.v_pages, bt.page_table, bt.kv_len, A, 0.09, ws,
+                                               q_start=bt.q_start, prefix_table=bt.prefix_table, prefix_len=bt.prefix,
+                                               stream=stream)
+            groups.fused_sample_tokens(x, u, tokens, sws, top_p=p, stream=stream)
+
+        return run, (Qo, A, bt.k_pages, bt.v_pages, tokens)
+
+    prepared = [prepare(i) for i in range(2)]
+    alone = []
+    for run, outs in prepared:
+        run(None)
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in outs])
+        for t in (outs[0], outs[1], outs[4]):
+            t.zero_()
+    torch.cuda.synchronize()
+    errors, plans, together = [], [set(), set()], threading.Barrier(2)
+
+    def worker(i):
+        try:
+            stream = torch.cuda.Stream()
+            together.wait()
+            for n in range(6):
+                prepared[i][0](stream)
+                plans[i].add(tuple(bytes(p.kernel) for p in _lib.last_launch_plans()))
+                if i == 0:
+                    try:
+                        groups.fused_sample_tokens(logits[0], logits[0][0], prepared[0][1][4], logits[0][0])
+                    except groups.NpuError as e:
+                        assert "u: size 40000" in str(e), e
+            if i == 1:
+                assert _lib.lib().npu_last_error() == b""
+            stream.synchronize()
+        except Exception as e:  # raised below, in the test's own thread
+            errors.append(repr(e))
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    assert not any(t.is_alive() for t in threads) and not errors, errors
+    torch.cuda.synchronize()
+    assert plans == [{(b"sample_tokens",)}] * 2
+    for (_, outs), want in zip(prepared, alone):
+        for got, w in zip(outs, want):
+            assert torch.equal(got, w)
