@@ -618,7 +618,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_whole_kernel(Paged
 //    keys of sixteen entries, each gets four keys of its entry.
 //  - Blocks follow each other across groups: a group's last block is computed with
 //    the next one's first on its way.
-// Four prompts of 800 to 2000 tokens, 79 GFLOP: 141 us, of which 12 join parts; a block of
+// Four prompts of 800 to 2000 tokens, 79 GFLOP: 146 us, of which 12 join parts; a block of
 // 64 keys is as long as its products (0.9 us a CU at the rate of a large one) and its
 // exponentials together.  The prefix of 6001 keys under 64 sequences: 24 us.
 //  - The running maximum is only a reference: it is raised, and the sums scaled,

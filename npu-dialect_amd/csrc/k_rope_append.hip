@@ -6,7 +6,7 @@
 //
 // Bound by its bytes: every row is read once and written once (four prompts of 2500 to
 // 4100 tokens, 32 + 2 8 heads of 128, 328 MB: 65 us, 5.0 TB/s; a step of 48 tokens:
-// 4.9 us, a call of nothing).  A lane takes
+// 5.1 us, a call of nothing).  A lane takes
 // sixteen entries of one head as two 16-byte runs that hold eight whole pairs
 // (consecutive runs for interleaved pairs, one run of each half otherwise), so
 // every access is 16 bytes wide and no pair crosses lanes.  A workgroup takes

@@ -17,7 +17,7 @@
 //
 // A workgroup takes a row.  What bounds it: each pass over a long row is at the rate
 // of the memory behind the L2 (256 rows of 128000 f32, 131 MB: 18 us), and in the
-// histogram's pass the f64 arithmetic and the LDS atomics (46 us of those rows' 125), so
+// histogram's pass the f64 arithmetic and the LDS atomics (46 us of those rows' 126), so
 // passes and work in them are saved:
 //  - the maximum, always;
 //  - with top-k, the entries that can be among the k: at least k of the lanes' own
@@ -26,7 +26,7 @@
 //  - else the histogram, with every entry's weight, and then the entries of the
 //    bins that the searches end in, in one pass for all of them: the bin that one
 //    search ends in bounds the mass that the next one starts from.
-// A row alone (one of 32000: 19 us, of which 5 are a call of nothing) is a chain of
+// A row alone (one of 32000: 19 us in the kernel) is a chain of
 // such steps, each with a barrier and an LDS or memory latency.
 // A bin of more than LIST entries (equal logits, say) is divided further by the
 // order's own key, the logit's bits and then the index, eleven bits at a time.
@@ -89,7 +89,7 @@ __device__ __forceinline__ double exp2_small(double y) {
 // The weights of a row: 2^42 2^y, y = (x - top) rate, as a whole power, a table of
 // 64ths and the Taylor polynomial of what is left, |r| <= 1/128, to degree 4 (the next
 // term is 4e-14, a third of the last bit of a weight's whole number).  A polynomial of
-// degree 9 in place of the table took 133 us for 256 rows of 128000 f32 to this one's 125.
+// degree 9 in place of the table took 133 us for 256 rows of 128000 f32 to this one's 126.
 constexpr int TABLE = 64;
 struct Weights {
   const double *table;  // 2^42 2^(j / 64), in LDS

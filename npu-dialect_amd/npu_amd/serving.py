@@ -28,7 +28,8 @@ def decoder_layer(p, bufs, cache, batch, n_heads, eps=1e-5, stream=None):
     k_pages, v_pages = cache
     at = (batch["page_table"], batch["kv_len"])
     dh = k_pages.shape[3]
-    # the rotation by position is the append's: here cos 1, sin 0
+    # the rotation by position is the append's: here cos 1, sin 0 (Q and K are rounded to
+    # bf16 by both, once more than where the QKV group rotates)
     groups.fused_llama_qkv_rope(bufs["x"], p["g1"], p["wq"], p["wk"], p["wv"], bufs["ones"], bufs["zeros"],
                                 bufs["Q"], bufs["K"], bufs["V"], eps, stream)
     groups.fused_llama_rope_append(bufs["Q"], bufs["K"], bufs["V"], p["cos_t"], p["sin_t"], k_pages, v_pages, *at,
