@@ -47,13 +47,13 @@ def listed():
         # A weight [K, N] to four bits, when a model is loaded.
         {"name": "quantize_weight", "op": "quantize", "R": 14336, "K": 4096, "kind": "weight"},
         # ---- product: one token in the tests' layer.
-        {"name": "product_token", "op": "product", "M": 1, "N": 1408, "K": 512, "a": "e4m3", "out": "bf16"},
+        {"name": "product_token", "op": "product", "M": 1, "N": 1408, "K": 512, "a": "e4m3"},
         # A decoding step: the weight's bytes.
-        {"name": "product_step_t48", "op": "product", "M": 48, "N": 14336, "K": 4096, "a": "e4m3", "out": "bf16"},
+        {"name": "product_step_t48", "op": "product", "M": 48, "N": 14336, "K": 4096, "a": "e4m3"},
         # Prompts of an odd number of tokens, activations in eight bits.
-        {"name": "product_prompt", "op": "product", "M": 4099, "N": 4096, "K": 14336, "a": "e4m3", "out": "bf16"},
+        {"name": "product_prompt", "op": "product", "M": 4099, "N": 4096, "K": 14336, "a": "e4m3"},
         # A large batch of prompts, both operands in four bits.
-        {"name": "product_large", "op": "product", "M": 8192, "N": 8192, "K": 8192, "a": "e2m1", "out": "bf16"},
+        {"name": "product_large", "op": "product", "M": 8192, "N": 8192, "K": 8192, "a": "e2m1"},
         # ---- log probabilities: a step's answers with their alternatives, an odd
         # vocabulary.
         {"name": "logprobs_step_b48", "op": "logprobs", "T": 48, "V": 50257, "dtype": "bf16", "top": 20},
@@ -74,7 +74,7 @@ def _draw(rng, op):
                 "kind": rng.choice(["gated", "plain", "f32", "weight"])}
     if op == "product":
         return {"op": op, "M": _log_int(rng, 1, 8192), "N": _log_int(rng, 16, 16384), "K": 32 * _log_int(rng, 2, 512),
-                "a": rng.choice(["e4m3", "e2m1"]), "out": rng.choice(["bf16", "bf16", "f32"])}
+                "a": rng.choice(["e4m3", "e2m1"])}
     return {"op": op, "T": _log_int(rng, 1, 2000), "V": _log_int(rng, 1000, 160000),
             "dtype": rng.choice(["f32", "bf16"]), "top": rng.choice([0, 1, 5, 20])}
 
@@ -162,7 +162,7 @@ def prepare(case, seed):
         st["q"], st["scale"] = new(U8, r, k // 2) if four else new(E4M3, r, k), new(E8M0, r, k // 32)
         st["values"] = new(BF16, r, k) if four else None
     elif case["op"] == "product":
-        st["out"] = new(BF16 if case["out"] == "bf16" else F32, case["M"], case["N"])
+        st["out"] = new(BF16, case["M"], case["N"])
     else:
         t, k = case["T"], case["top"]
         st["logprobs"], st["entropy"], st["ranks"] = new(F32, t), new(F32, t), new(I32, t)
@@ -312,7 +312,7 @@ def work(case):
     if case["op"] == "product":
         m, n, k = case["M"], case["N"], case["K"]
         a = m * k if case["a"] == "e4m3" else m * k // 2
-        return {"bytes": a + n * k // 2 + (m + n) * k // 32 + m * n * (2 if case["out"] == "bf16" else 4),
+        return {"bytes": a + n * k // 2 + (m + n) * k // 32 + 2 * m * n,
                 "flops": 2 * m * n * k}
     n = case["T"] * case["V"]
     return {"bytes": n * (2 if case["dtype"] == "bf16" else 4) + (16 + 8 * case["top"]) * case["T"], "flops": 6 * n}
