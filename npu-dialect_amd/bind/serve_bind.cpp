@@ -36,6 +36,10 @@ bool describe(PyObject *o, const char *name, bool optional, npu_memref *m) {
     case at::kBFloat16: m->dtype = NPU_BF16; break;
     case at::kChar: m->dtype = NPU_I8; break;
     case at::kInt: m->dtype = NPU_I32; break;
+    case at::kByte:
+    case at::kFloat8_e8m0fnu:
+    case at::kFloat4_e2m1fn_x2: m->dtype = NPU_U8; break;
+    case at::kFloat8_e4m3fn: m->dtype = NPU_E4M3; break;
     default: PyErr_Format(PyExc_TypeError, "%s: unsupported tensor dtype %s", name, c10::toString(t.scalar_type())); return false;
   }
   if (t.dim() > NPU_MAX_RANK) {
@@ -165,10 +169,58 @@ PyObject *sample_tokens(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+PyObject *token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  static const Operand ops[8] = {{"logits", false}, {"tokens", false}, {"logprobs", false}, {"entropy", true},
+                                 {"ranks", true}, {"top_tokens", true}, {"top_logprobs", true}, {"workspace", false}};
+  return guarded([&]() -> PyObject * {
+    npu_memref m[8];
+    npu_stream s;
+    if (!counted(n, 9) || !describe_all(a, ops, m) || !stream_of(a[8], &s)) return nullptr;
+    return PyLong_FromLong(fused_token_logprobs(&m[0], &m[1], &m[2], &m[3], &m[4], &m[5], &m[6], &m[7], s));
+  });
+}
+
+PyObject *mx_quantize(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  static const Operand ops[5] = {{"x", false}, {"gate", true}, {"q", false}, {"scale", false}, {"values", true}};
+  return guarded([&]() -> PyObject * {
+    npu_memref m[5];
+    npu_stream s;
+    if (!counted(n, 6) || !describe_all(a, ops, m) || !stream_of(a[5], &s)) return nullptr;
+    return PyLong_FromLong(fused_mx_quantize(&m[0], &m[1], &m[2], &m[3], &m[4], s));
+  });
+}
+
+PyObject *add_rmsnorm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  static const Operand ops[6] = {{"x", false}, {"delta", true}, {"g", false}, {"h", true}, {"q", false}, {"scale", true}};
+  return guarded([&]() -> PyObject * {
+    npu_memref m[6];
+    npu_stream s;
+    if (!counted(n, 8) || !describe_all(a, ops, m)) return nullptr;
+    const double eps = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred() || !stream_of(a[7], &s)) return nullptr;
+    return PyLong_FromLong(fused_llama_add_rmsnorm(&m[0], &m[1], &m[2], &m[3], &m[4], &m[5], (float)eps, s));
+  });
+}
+
+PyObject *mx_matmul(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  static const Operand ops[6] = {{"a", false}, {"a_scale", false}, {"w", false}, {"w_scale", false}, {"out", false},
+                                 {"workspace", false}};
+  return guarded([&]() -> PyObject * {
+    npu_memref m[6];
+    npu_stream s;
+    if (!counted(n, 7) || !describe_all(a, ops, m) || !stream_of(a[6], &s)) return nullptr;
+    return PyLong_FromLong(fused_mx_matmul(&m[0], &m[1], &m[2], &m[3], &m[4], &m[5], s));
+  });
+}
+
 PyMethodDef methods[] = {
     {"rope_append", (PyCFunction)(void (*)(void))rope_append, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
     {"sample_tokens", (PyCFunction)(void (*)(void))sample_tokens, METH_FASTCALL, nullptr},
+    {"token_logprobs", (PyCFunction)(void (*)(void))token_logprobs, METH_FASTCALL, nullptr},
+    {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
+    {"add_rmsnorm", (PyCFunction)(void (*)(void))add_rmsnorm, METH_FASTCALL, nullptr},
+    {"mx_matmul", (PyCFunction)(void (*)(void))mx_matmul, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serve", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

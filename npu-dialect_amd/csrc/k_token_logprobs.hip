@@ -1,0 +1,423 @@
+// k_token_logprobs.hip -- of each row of logits: the log probability and rank of a given
+// token, the entropy, and the k best entries.
+//
+//   m = max x, S = sum 2^d, W = sum 2^d d, d = (x - m) log2 e;
+//   log p(x) = (x - m) - ln S, entropy = ln S - ln 2 W / S.
+//
+// A row is read once.  It is cut into parts, each of which a workgroup of four waves holds
+// in registers (NCH runs of 16 bytes a lane), so that the maximum is known before the
+// sums begin and an entry costs one exponential; a second kernel joins the parts where a row
+// has several.  The exponent d is one fma, x log2 e - c, c = m log2 e rounded; what c's rounding
+// left, the same for all entries, is taken off the sums' logarithm at the end.
+//
+// The k best: at least k of a wave's 64 lanes have a maximum that is no less than the
+// k-th largest of these, so that the part's k best are among the entries that reach the
+// largest of the waves' such bounds: of the order of k entries, which go to a list
+// in LDS and are ranked by comparing each with all.  A list that overflows (a row of equal
+// logits, say) is searched for the k best one after the other instead.
+//
+// Reading the row bounds it where rows are many, the chain of one part's steps and the
+// join where they are few.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "kernels.hpp"
+#include "npu_device.hpp"
+#include "plans.hpp"
+
+namespace npu {
+
+namespace {
+
+constexpr int LT = 256;      // lanes of a workgroup
+constexpr int LIST = 1024;   // entries that are ranked at once
+constexpr int MAX_K = 32;
+constexpr int MAX_PARTS = LT;  // of a row: 129 at most with 8 runs a lane (2^20 f32)
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+
+typedef unsigned long long u64;
+
+// An entry's place in the order as a number, smaller first: by logit, descending, then index.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 is 0
+  return b & 0x80000000u ? b : ~b & 0x7fffffffu;
+}
+__device__ __forceinline__ float from_order(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o : ~o & 0x7fffffffu); }
+constexpr u64 NO_KEY = ~0ull;
+
+// The next float below one that is not -Inf.
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return x == 0.0f ? __uint_as_float(0x80000001u) : __uint_as_float(x > 0.0f ? b - 1 : b + 1);
+}
+
+// A part's result, and behind it the k keys.
+struct Part {
+  float m, S, W;  // m -Inf: no entry above -Inf (S, W 0)
+  int before;     // entries before the token
+};
+__device__ __forceinline__ u64 *keys_of(Part *p) { return reinterpret_cast<u64 *>(p + 1); }
+__host__ __device__ constexpr size_t part_bytes(int k) { return sizeof(Part) + 8 * (size_t)k; }
+
+// What the joined sums give; lane `t` of the caller writes alternative t.
+__device__ __forceinline__ void finish(const TokenLogprobsArgs &a, long long row, const Part &p, const u64 *keys, int t) {
+  const float inf = __builtin_inff(), lnS = p.S > 0.0f ? logf(p.S) : 0.0f;
+  // ((x - m) is exact or far from 0)
+  auto logp = [&](float x) { return !(x > -inf) ? -inf : x == p.m ? -lnS : (x - p.m) - lnS; };
+  if (t == 0) {
+    const int token = a.tokens[row];
+    const bool given = token >= 0 && token < a.V;
+    float lp = 0.0f;
+    if (given) {
+      const long long at = row * a.row_stride + token;
+      lp = logp(a.bf16 ? bf16_to_f32(static_cast<const uint16_t *>(a.logits)[at]) : static_cast<const float *>(a.logits)[at]);
+    }
+    a.logprobs[row] = lp;
+    if (a.ranks) a.ranks[row] = given ? p.before : -1;
+    if (a.entropy) a.entropy[row] = p.S > 0.0f ? lnS - LN2 * (p.W / p.S) : 0.0f;
+  }
+  if (t < a.k) {
+    const u64 key = keys[t];
+    const float x = from_order((uint32_t)(key >> 32));
+    const bool in = key != NO_KEY && (p.m < inf || x == inf);
+    a.top_tokens[row * a.toks_stride + t] = in ? (int)(uint32_t)key : -1;
+    a.top_logprobs[row * a.tops_stride + t] = in ? logp(x) : -inf;
+  }
+}
+
+// The k smallest of n keys in LDS, in order, to `out`; called by all lanes of a workgroup.
+__device__ __forceinline__ void rank_keys(const u64 *list, int n, int k, u64 *out) {
+  for (int e = threadIdx.x; e < n; e += blockDim.x) {
+    const u64 key = list[e];
+    int ahead = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) ahead += list[j] < key;
+    if (ahead < k) out[ahead] = key;
+  }
+}
+
+template <bool BF, int NCH>
+__global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a, int parts) {
+  constexpr int PER = BF ? 8 : 4, ES = BF ? 2 : 4, NW = LT / 64;
+  __shared__ u64 list[LIST];
+  __shared__ u64 best[MAX_K];
+  __shared__ float wave_a[NW], wave_b[NW];
+  __shared__ int wave_c[NW];
+  __shared__ uint32_t wave_o[NW];
+  __shared__ u64 wave_k[NW];
+  __shared__ int n_list;
+  const float inf = __builtin_inff();
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long long row = blockIdx.x / (unsigned)parts;
+  const int part = blockIdx.x % (unsigned)parts;
+  const char *p = static_cast<const char *>(a.logits) + row * a.row_stride * ES;
+  // runs of 16 bytes at aligned places; what lies before the first whole one, and after the
+  // last, at most PER - 1 entries each, goes to lanes of the part whose range has it
+  const int skew = (int)((uintptr_t)p & 15) / ES;
+  const u32x4 *body = reinterpret_cast<const u32x4 *>(p - skew * ES);
+  const int whole0 = skew ? 1 : 0, whole1 = (a.V + skew) / PER;
+  const int c0 = part * NCH * LT + tid;
+  u32x4 v[NCH];
+  constexpr uint32_t NONE = BF ? 0xff80ff80u : 0xff800000u;  // -Inf
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = c0 + i * LT;
+    v[i] = u32x4{NONE, NONE, NONE, NONE};
+    if (c >= whole0 && c < whole1) v[i] = body[c];
+  }
+  auto entry = [&](int j) __attribute__((always_inline)) {
+    return BF ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[j]) : reinterpret_cast<const float *>(p)[j];
+  };
+  int edge_j = -1;
+  if (part == 0 && tid < PER && tid < min(whole0 * PER - skew, a.V)) edge_j = tid;
+  const int tail = max(whole1, whole0);
+  if (part == tail / (NCH * LT) && tid >= PER && tid < 2 * PER) {
+    const int j = tail * PER - skew + tid - PER;
+    if (j < a.V) edge_j = j;
+  }
+  float edge = -inf;
+  if (edge_j >= 0) edge = entry(edge_j);
+  const int token = a.tokens[row];
+  const bool given = token >= 0 && token < a.V;
+  float xt = -inf;
+  if (given) xt = entry(token);
+  if (!(xt > -inf)) xt = -inf;
+  if (tid == 0) n_list = 0;
+  auto get = [&](u32x4 u, int e) __attribute__((always_inline)) {
+    return BF ? __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16) : __uint_as_float(u[e]);
+  };
+  // (the entries are taken out of the runs again each time: all of them would not fit)
+  auto packed = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(v[i]));
+  };
+  // every entry of the part again, from memory: f(x, j)
+  auto again = [&](auto f) __attribute__((always_inline)) {
+    const int from = max(0, part * NCH * LT * PER - skew), to = min(a.V, (part + 1) * NCH * LT * PER - skew);
+#pragma unroll 1
+    for (int j = from + tid; j < to; j += LT) f(entry(j), j);
+  };
+  // the lane's maximum, the part's
+  float mine = fmaxf(edge, -inf), run_max[NCH];  // (no NaN)
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    run_max[i] = -inf;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) run_max[i] = fmaxf(fmaxf(run_max[i], get(v[i], e)), get(v[i], e + 1));
+    mine = fmaxf(mine, run_max[i]);
+  }
+  packed();
+  {
+    float m = mine;
+    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    if (lane == 0) wave_a[wave] = m;
+    if (a.k > 0) {
+      // the k-th largest of the wave's lanes' maxima, bit by bit (as numbers that rise with x)
+      const uint32_t up = ~order_bits(mine);
+      uint32_t bound = 0;
+#pragma unroll 1
+      for (int b = 31; b >= (BF ? 16 : 0); --b) {
+        const uint32_t at = bound | 1u << b;
+        if (__popcll(__ballot(up >= at)) >= a.k) bound = at;
+      }
+      if (lane == 0) wave_o[wave] = bound;
+    }
+  }
+  __syncthreads();
+  float m = wave_a[0];
+  uint32_t bound = a.k > 0 ? wave_o[0] : 0;
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    m = fmaxf(m, wave_a[w]);
+    if (a.k > 0) bound = max(bound, wave_o[w]);
+  }
+  // sums, the rank, the list
+  const float least = fmaxf(from_order(~bound), -3.402823466e38f);  // (-Inf is no candidate)
+  // (next to f32's ends the fma's terms overflow: those rows are summed from x - m below)
+  const bool far = !(fabsf(m) < 1e37f);
+  const float c = far ? 0.0f : m * LOG2E, rest = far ? 0.0f : fmaf(m, LOG2E, -c);
+  const float at_before = xt > -inf ? below(xt) : -inf;
+  float S = 0.0f, W = 0.0f;
+  int before = 0;
+  auto add = [&](float x, float over) __attribute__((always_inline)) {
+    const float d = fmaxf(fmaf(x, LOG2E, -c), -1000.0f), w = __builtin_amdgcn_exp2f(d);
+    S += w;
+    W = fmaf(w, d, W);
+    before += x > over;
+  };
+  auto keep = [&](float x, int j) __attribute__((always_inline)) {
+    if (x >= least) {
+      const int at = atomicAdd(&n_list, 1);
+      if (at < LIST) list[at] = (u64)order_bits(x) << 32 | (uint32_t)j;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int j0 = (c0 + i * LT) * PER - skew;
+    const float over = j0 + PER <= token ? at_before : xt;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) add(get(v[i], e), over);
+  }
+  if (edge_j >= 0) add(edge, edge_j < token ? at_before : xt);
+  packed();
+  if (a.k > 0 && mine >= least) {
+    uint32_t runs = 0;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) runs |= (uint32_t)(run_max[i] >= least) << i;
+    while (runs) {
+      const int at = __builtin_ctz(runs);
+      runs &= runs - 1;
+      u32x4 u = v[0];
+#pragma unroll
+      for (int i = 1; i < NCH; ++i)
+        if (at == i) u = v[i];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) keep(get(u, e), (c0 + at * LT) * PER - skew + e);
+    }
+    if (edge_j >= 0) keep(edge, edge_j);
+  }
+  if (!given) {
+    before = 0;
+  } else if (!(xt > -inf)) {
+    // behind all above -Inf, and those like it with a lower index
+    before = 0;
+    again([&](float x, int j) { before += j < token || x > -inf; });
+  } else if (tid < PER) {
+    // the run that holds the token: its equals before it, unless they were edges
+    const int run = (token + skew) / PER, j = run * PER - skew + tid;
+    if (run >= whole0 && run < whole1 && run / (NCH * LT) == part && j < token) before += entry(j) == xt;
+  }
+  if (far) {
+    S = W = 0.0f;
+    if (m > -inf)
+      again([&](float x, int) {
+        const float d = x == m ? 0.0f : fmaxf((x - m) * LOG2E, -1000.0f), w = __builtin_amdgcn_exp2f(d);
+        S += w;
+        W = fmaf(w, d, W);
+      });
+  }
+  S = wave_sum(S);
+  W = wave_sum(W);
+  for (int off = 32; off; off >>= 1) before += __shfl_xor(before, off);
+  __syncthreads();  // (wave_a was read above)
+  if (lane == 0) wave_a[wave] = S, wave_b[wave] = W, wave_c[wave] = before;
+  __syncthreads();
+  const int n = n_list;
+  if (a.k > 0) {
+    if (tid < a.k) best[tid] = NO_KEY;
+    __syncthreads();
+    if (n <= LIST) {
+      rank_keys(list, n, a.k, best);
+    } else {
+      u64 last = 0;  // (no candidate's key: NaN's place in the order)
+#pragma unroll 1
+      for (int r = 0; r < a.k; ++r) {
+        u64 next = NO_KEY;
+        again([&](float x, int j) {
+          const u64 key = (u64)order_bits(x) << 32 | (uint32_t)j;
+          if (x >= least && key > last) next = min(next, key);
+        });
+        for (int off = 32; off; off >>= 1) next = min(next, (u64)__shfl_xor(next, off));
+        if (lane == 0) wave_k[wave] = next;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) next = min(next, wave_k[w]);
+        if (tid == 0) best[r] = next;
+        last = next;
+        __syncthreads();
+      }
+    }
+    __syncthreads();
+  }
+  Part out{m, 0.0f, 0.0f, 0};
+#pragma unroll
+  for (int w = 0; w < NW; ++w) out.S += wave_a[w], out.W += wave_b[w], out.before += wave_c[w];
+  // S and W of exact exponents: each is off by `rest`
+  if (out.S > 0.0f) {
+    out.W = out.W - rest * out.S;
+    const float f = __builtin_amdgcn_exp2f(-rest);
+    out.S *= f;
+    out.W *= f;
+  }
+  if (parts == 1) {
+    finish(a, row, out, best, tid);
+    return;
+  }
+  Part *to = reinterpret_cast<Part *>(static_cast<char *>(a.workspace) + (row * parts + part) * part_bytes(a.k));
+  if (tid == 0) *to = out;
+  if (tid < a.k) keys_of(to)[tid] = best[tid];
+}
+
+// A row's parts.  The k best are in the k lists whose first keys come first, and no later than
+// the last of those first keys.
+__global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsArgs a, int parts) {
+  __shared__ u64 heads[MAX_PARTS], list[MAX_K * MAX_K], best[MAX_K];
+  __shared__ u64 bound;
+  __shared__ int n_list;
+  const float inf = __builtin_inff();
+  const int tid = threadIdx.x;
+  const long long row = blockIdx.x;
+  const size_t step = part_bytes(a.k);
+  char *from = static_cast<char *>(a.workspace) + row * parts * step;
+  auto part = [&](int i) { return reinterpret_cast<Part *>(from + i * step); };
+  if (tid < parts && a.k > 0) heads[tid] = keys_of(part(tid))[0];
+  if (tid < a.k) best[tid] = NO_KEY;
+  if (tid == 0) n_list = 0, bound = NO_KEY;
+  // every lane sums all parts, in order
+  Part out{-inf, 0.0f, 0.0f, 0};
+  for (int i = 0; i < parts; ++i) out.m = fmaxf(out.m, part(i)->m);
+  for (int i = 0; i < parts; ++i) {
+    const Part p = *part(i);
+    out.before += p.before;
+    if (!(p.S > 0.0f)) continue;
+    const float d = p.m == out.m ? 0.0f : fmaxf((p.m - out.m) * LOG2E, -1000.0f), f = __builtin_amdgcn_exp2f(d);
+    out.S = fmaf(f, p.S, out.S);
+    out.W = fmaf(f, fmaf(d, p.S, p.W), out.W);
+  }
+  __syncthreads();
+  if (a.k > 0) {
+    if (tid < parts && parts >= a.k && heads[tid] != NO_KEY) {
+      int ahead = 0;
+      for (int j = 0; j < parts; ++j) ahead += heads[j] < heads[tid];
+      if (ahead == a.k - 1) bound = heads[tid];
+    }
+    __syncthreads();
+    const u64 last = bound;
+    for (int e = tid; e < parts * a.k; e += LT) {
+      const int i = e / a.k;
+      if (heads[i] > last || heads[i] == NO_KEY) continue;
+      const u64 key = keys_of(part(i))[e - i * a.k];
+      if (key > last || key == NO_KEY) continue;
+      list[atomicAdd(&n_list, 1)] = key;  // (at most k lists of k: with fewer real heads than k, all of them)
+    }
+    __syncthreads();
+    rank_keys(list, n_list, a.k, best);
+    __syncthreads();
+  }
+  finish(a, row, out, best, tid);
+}
+
+// Runs of 16 bytes a lane holds: the most (8: half of the registers that eight workgroups
+// on a CU leave) that still give every CU four workgroups, as far as a join takes the parts.
+struct Cut {
+  int nch, parts;
+};
+Cut cut_rows(int T, int V, bool bf16) {
+  const int per = bf16 ? 8 : 4;
+  const long long chunks = (V + per - 1) / per + 1;  // (a row that begins and ends inside a run)
+  auto parts = [&](int nch) { return (chunks + nch * LT - 1) / (nch * LT); };
+  int nch = 8;
+  while (nch > 1 && (long long)T * parts(nch) < 4LL * device_cus() && parts(nch / 2) <= MAX_PARTS) nch /= 2;
+  return Cut{nch, (int)parts(nch)};
+}
+
+}  // namespace
+
+size_t token_logprobs_workspace(int T, int V, int k) {
+  size_t most = 16;
+  for (bool bf16 : {false, true}) {
+    const Cut c = cut_rows(T, V, bf16);
+    if (c.parts > 1) most = std::max(most, (size_t)T * c.parts * part_bytes(k));
+  }
+  return most;
+}
+
+hipError_t launch_token_logprobs(const TokenLogprobsArgs &a, hipStream_t s) {
+  const Cut cut = cut_rows(a.T, a.V, a.bf16);
+  const long long grid = (long long)a.T * cut.parts;
+  auto kern = a.bf16 ? (cut.nch == 8 ? token_logprobs_kernel<true, 8> : cut.nch == 4 ? token_logprobs_kernel<true, 4>
+                        : cut.nch == 2 ? token_logprobs_kernel<true, 2> : token_logprobs_kernel<true, 1>)
+                     : (cut.nch == 8 ? token_logprobs_kernel<false, 8> : cut.nch == 4 ? token_logprobs_kernel<false, 4>
+                        : cut.nch == 2 ? token_logprobs_kernel<false, 2> : token_logprobs_kernel<false, 1>);
+  const double es = a.bf16 ? 2.0 : 4.0;
+  {
+    npu_launch_plan p = make_plan("token_logprobs", (int)grid, wg_per_cu(kern, LT), (int)grid, 16);
+    const double n = std::min((double)a.V, (double)cut.nch * LT * (a.bf16 ? 8 : 4));
+    p.load_phases = 2;
+    p.tile_valu = n / 64 * 12.0;
+    p.tile_lds_bytes = 8.0 * a.k * a.k;
+    p.tile_load_bytes = n * es;
+    p.tile_store_bytes = (double)part_bytes(a.k);
+    p.hbm_bytes = (double)a.T * a.V * es;
+    plans_add(p);
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(LT), 0, s, a, cut.parts);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || cut.parts == 1) return e;
+  {
+    npu_launch_plan p = make_plan("token_logprobs_join", a.T, wg_per_cu(token_logprobs_join_kernel, LT), a.T, 16);
+    p.load_phases = 3;
+    p.tile_valu = cut.parts * 20.0 * (LT / 64) + std::ceil(cut.parts / 64.0) * cut.parts * 4.0 + 4.0 * a.k * a.k;
+    p.tile_lds_bytes = 8.0 * cut.parts * cut.parts;
+    p.tile_load_bytes = (double)cut.parts * part_bytes(a.k);
+    p.tile_store_bytes = 12.0 + 8.0 * a.k;
+    p.hbm_bytes = 0.0;
+    plans_add(p);
+  }
+  hipLaunchKernelGGL(token_logprobs_join_kernel, dim3(a.T), dim3(LT), 0, s, a, cut.parts);
+  return hipGetLastError();
+}
+
+}  // namespace npu

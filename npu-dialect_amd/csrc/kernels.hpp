@@ -130,5 +130,51 @@ struct SampleArgs {
   float *probs;  // may be null
 };
 hipError_t launch_sample_tokens(const SampleArgs &a, hipStream_t s);
+struct TokenLogprobsArgs {
+  const void *logits;  // f32, or bf16 bits
+  bool bf16;
+  long long row_stride;  // elements
+  int T, V, k;
+  const int *tokens;
+  float *logprobs, *entropy, *top_logprobs;  // all but logprobs may be null
+  int *ranks, *top_tokens;                   // may be null
+  long long toks_stride, tops_stride;        // of top_tokens and top_logprobs
+  void *workspace;
+};
+size_t token_logprobs_workspace(int T, int V, int k);  // bytes
+hipError_t launch_token_logprobs(const TokenLogprobsArgs &a, hipStream_t s);
+
+// Microscaled blocks (mx_device.hpp); strides in elements of the operand (e2m1: bytes).
+struct MxQuantizeArgs {
+  const void *x;         // bf16 bits, or f32
+  const uint16_t *gate;  // may be null
+  uint8_t *q, *scale;
+  uint16_t *values;  // may be null
+  bool f32, e4m3, columns;  // columns: entry (r, k) of x lies at k x_stride + r
+  long long x_stride, gate_stride, q_stride, scale_stride, values_stride;
+  int R, K;
+};
+hipError_t launch_mx_quantize(const MxQuantizeArgs &a, hipStream_t s);
+struct AddRmsnormArgs {
+  const uint16_t *x, *delta;  // delta may be null
+  const float *g;
+  uint16_t *h;  // may be null
+  uint8_t *q, *scale;
+  int kind;  // mx_device.hpp
+  long long x_stride, delta_stride, h_stride, q_stride, scale_stride;
+  int T, D;
+  float eps;
+};
+hipError_t launch_add_rmsnorm(const AddRmsnormArgs &a, hipStream_t s);
+struct MxMatmulArgs {
+  const uint8_t *a, *a_scale, *w, *w_scale;
+  uint16_t *out;
+  bool e4m3;  // a; else e2m1
+  long long a_stride, as_stride, w_stride, ws_stride, out_stride;
+  int M, N, K;
+  void *workspace;
+};
+size_t mx_matmul_workspace(int M, int N, int K);  // bytes
+hipError_t launch_mx_matmul(const MxMatmulArgs &a, hipStream_t s);
 
 }  // namespace npu

@@ -1,113 +1,12 @@
-// serve_abi.hip -- the extern "C" boundary of the serving entry points: their
-// operands may be strided rows and caches past 2^31 elements, which the group
-// entry points' descriptor check refuses.
+// serve_abi.hip -- the extern "C" boundary of the serving entry points.
 #include <hip/hip_runtime.h>
-
-#include <cstdarg>
-#include <cstdio>
 
 #include "../../include/npu_amd.h"
 #include "kernels.hpp"
 #include "plans.hpp"
+#include "serve_check.hpp"
 
 namespace {
-
-npu_status fail(npu_status code, const char *fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  npu::set_last_error(buf);
-  return code;
-}
-
-#define NPU_TRY(expr)                 \
-  do {                                \
-    npu_status _s = (expr);           \
-    if (_s != NPU_OK) return _s;      \
-  } while (0)
-
-// A launcher's result; what it throws (the plan list's allocation) ends here.
-template <class F>
-npu_status launched(const char *what, F launch) {
-  try {
-    const hipError_t e = launch();
-    if (e != hipSuccess) return fail(NPU_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    npu::set_last_error("");
-    return NPU_OK;
-  } catch (...) {
-    return fail(NPU_ERR_OOM, "%s: out of host memory", what);
-  }
-}
-
-constexpr long long kMaxInt = (1LL << 31) - 1;
-
-bool absent(const npu_memref *m) { return !m || !m->aligned; }
-
-int elem_size(int32_t dt) { return dt == NPU_BF16 ? 2 : dt == NPU_I8 ? 1 : 4; }
-
-// Rank, element type, positive sizes below 2^31 and the data pointer's
-// alignment; *ptr: the first element.
-npu_status check_base(const npu_memref *m, const char *name, int32_t rank, int32_t dtype, int align,
-                      const void **ptr) {
-  if (!m) return fail(NPU_ERR_INVALID_ARG, "%s: null descriptor", name);
-  if (m->rank != rank) return fail(NPU_ERR_INVALID_ARG, "%s: rank %d, expected %d", name, m->rank, rank);
-  if (m->dtype != dtype)
-    return fail(NPU_ERR_INVALID_ARG, "%s: element type %d, expected %d", name, m->dtype, dtype);
-  if (!m->aligned) return fail(NPU_ERR_INVALID_ARG, "%s: null data pointer", name);
-  if (m->offset < 0) return fail(NPU_ERR_INVALID_ARG, "%s: negative offset", name);
-  for (int d = 0; d < rank; ++d)
-    if (m->sizes[d] <= 0 || m->sizes[d] > kMaxInt)
-      return fail(NPU_ERR_INVALID_ARG, "%s: size[%d] = %lld must be positive and below 2^31", name, d,
-                  (long long)m->sizes[d]);
-  const char *base = static_cast<const char *>(m->aligned) + m->offset * elem_size(dtype);
-  if (reinterpret_cast<uintptr_t>(base) % align != 0)
-    return fail(NPU_ERR_UNSUPPORTED, "%s: data pointer is not %d-byte aligned", name, align);
-  *ptr = base;
-  return NPU_OK;
-}
-
-// [rows, cols] with contiguous rows at a stride that keeps them aligned.
-npu_status check_rows(const npu_memref *m, const char *name, int32_t dtype, int align, const void **ptr,
-                      long long *stride) {
-  NPU_TRY(check_base(m, name, 2, dtype, align, ptr));
-  if (m->sizes[1] > 1 && m->strides[1] != 1)
-    return fail(NPU_ERR_UNSUPPORTED, "%s: stride[1] = %lld, rows must be contiguous", name, (long long)m->strides[1]);
-  *stride = m->sizes[0] > 1 ? m->strides[0] : m->sizes[1];
-  if (*stride < m->sizes[1])
-    return fail(NPU_ERR_UNSUPPORTED, "%s: stride[0] = %lld, rows of %lld overlap", name, *stride,
-                (long long)m->sizes[1]);
-  if (m->sizes[0] > 1 && *stride * elem_size(dtype) % align != 0)
-    return fail(NPU_ERR_UNSUPPORTED, "%s: rows at a stride of %lld are not %d-byte aligned", name, *stride, align);
-  return NPU_OK;
-}
-
-npu_status check_vec(const npu_memref *m, const char *name, int32_t dtype, long long n, const void **ptr) {
-  NPU_TRY(check_base(m, name, 1, dtype, 4, ptr));
-  if (m->sizes[0] > 1 && m->strides[0] != 1)
-    return fail(NPU_ERR_UNSUPPORTED, "%s: stride %lld, must be contiguous", name, (long long)m->strides[0]);
-  if (n >= 0 && m->sizes[0] != n)
-    return fail(NPU_ERR_INVALID_ARG, "%s: size %lld, expected %lld", name, (long long)m->sizes[0], n);
-  return NPU_OK;
-}
-
-npu_status expect_cols(const npu_memref *m, const char *name, long long rows, long long cols) {
-  if (m->sizes[0] != rows || m->sizes[1] != cols)
-    return fail(NPU_ERR_INVALID_ARG, "%s: [%lld,%lld], expected [%lld,%lld]", name, (long long)m->sizes[0],
-                (long long)m->sizes[1], rows, cols);
-  return NPU_OK;
-}
-
-npu_status check_workspace(const npu_memref *m, long long need, void **ptr) {
-  const void *p;
-  NPU_TRY(check_base(m, "workspace", 1, NPU_F32, 16, &p));
-  if (m->sizes[0] > 1 && m->strides[0] != 1) return fail(NPU_ERR_UNSUPPORTED, "workspace: must be contiguous");
-  if (m->sizes[0] < need)
-    return fail(NPU_ERR_INVALID_ARG, "workspace: %lld elements, %lld needed", (long long)m->sizes[0], need);
-  *ptr = const_cast<void *>(p);
-  return NPU_OK;
-}
 
 // One half of the cache: bf16 [P, Hkv, page, Dh], each page contiguous.
 npu_status check_pages(const npu_memref *m, const char *name, const void **ptr, long long *stride) {
@@ -322,6 +221,53 @@ npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u, co
   a.probs = const_cast<float *>(static_cast<const float *>(p[6]));
   return launched("fused_sample_tokens launch",
                   [&] { return npu::launch_sample_tokens(a, static_cast<hipStream_t>(stream)); });
+}
+
+int64_t npu_token_logprobs_workspace(int64_t T, int64_t V, int32_t k) {
+  if (T <= 0 || T > 1 << 23 || V <= 0 || V > 1 << 20 || k < 0 || k > 32) return -1;
+  return (int64_t)(npu::token_logprobs_workspace((int)T, (int)V, k) / sizeof(float));
+}
+
+npu_status fused_token_logprobs(const npu_memref *logits, const npu_memref *tokens, const npu_memref *logprobs,
+                                const npu_memref *entropy, const npu_memref *ranks, const npu_memref *top_tokens,
+                                const npu_memref *top_logprobs, const npu_memref *workspace, npu_stream stream) {
+  npu::plans_reset();
+  npu::TokenLogprobsArgs a{};
+  if (!logits) return fail(NPU_ERR_INVALID_ARG, "logits: null descriptor");
+  a.bf16 = logits->dtype == NPU_BF16;
+  const void *pl, *p[6] = {};
+  NPU_TRY(check_rows(logits, "logits", a.bf16 ? NPU_BF16 : NPU_F32, a.bf16 ? 2 : 4, &pl, &a.row_stride));
+  const long long T = logits->sizes[0], V = logits->sizes[1];
+  if (V > 1 << 20) return fail(NPU_ERR_UNSUPPORTED, "logits: %lld columns, at most 2^20", V);
+  if (T > 1 << 23) return fail(NPU_ERR_UNSUPPORTED, "logits: %lld rows, at most 2^23", T);
+  NPU_TRY(check_vec(tokens, "tokens", NPU_I32, T, &p[0]));
+  NPU_TRY(check_vec(logprobs, "logprobs", NPU_F32, T, &p[1]));
+  if (!absent(entropy)) NPU_TRY(check_vec(entropy, "entropy", NPU_F32, T, &p[2]));
+  if (!absent(ranks)) NPU_TRY(check_vec(ranks, "ranks", NPU_I32, T, &p[3]));
+  if (absent(top_tokens) != absent(top_logprobs))
+    return fail(NPU_ERR_INVALID_ARG, "top_tokens and top_logprobs: one without the other");
+  long long k = 0;
+  if (!absent(top_tokens)) {
+    NPU_TRY(check_rows(top_tokens, "top_tokens", NPU_I32, 4, &p[4], &a.toks_stride));
+    k = top_tokens->sizes[1];
+    if (k > 32) return fail(NPU_ERR_UNSUPPORTED, "top_tokens: %lld columns, at most 32", k);
+    NPU_TRY(expect_cols(top_tokens, "top_tokens", T, k));
+    NPU_TRY(check_rows(top_logprobs, "top_logprobs", NPU_F32, 4, &p[5], &a.tops_stride));
+    NPU_TRY(expect_cols(top_logprobs, "top_logprobs", T, k));
+  }
+  NPU_TRY(check_workspace(workspace, npu_token_logprobs_workspace(T, V, (int32_t)k), &a.workspace));
+  a.logits = pl;
+  a.T = (int)T;
+  a.V = (int)V;
+  a.k = (int)k;
+  a.tokens = static_cast<const int *>(p[0]);
+  a.logprobs = const_cast<float *>(static_cast<const float *>(p[1]));
+  a.entropy = const_cast<float *>(static_cast<const float *>(p[2]));
+  a.ranks = const_cast<int *>(static_cast<const int *>(p[3]));
+  a.top_tokens = const_cast<int *>(static_cast<const int *>(p[4]));
+  a.top_logprobs = const_cast<float *>(static_cast<const float *>(p[5]));
+  return launched("fused_token_logprobs launch",
+                  [&] { return npu::launch_token_logprobs(a, static_cast<hipStream_t>(stream)); });
 }
 
 }  // extern "C"

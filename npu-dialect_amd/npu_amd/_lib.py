@@ -149,6 +149,12 @@ SIGNATURES = {
     "npu_paged_attention_workspace": (_I64, [_I64, _I64, _I32, _I32, _I32, _I32]),
     "fused_sample_tokens": (_I32, [_MR] * 9 + [_P]),
     "npu_sample_workspace": (_I64, [_I64, _I64]),
+    "fused_token_logprobs": (_I32, [_MR] * 8 + [_P]),
+    "npu_token_logprobs_workspace": (_I64, [_I64, _I64, _I32]),
+    "fused_mx_quantize": (_I32, [_MR] * 5 + [_P]),
+    "fused_llama_add_rmsnorm": (_I32, [_MR] * 6 + [C.c_float, _P]),
+    "fused_mx_matmul": (_I32, [_MR] * 6 + [_P]),
+    "npu_mx_matmul_workspace": (_I64, [_I64, _I64, _I64]),
     "npu_group_launch": (_I32, [C.c_char_p, C.POINTER(NpuGroupAttrs), _ARG, _I32, _ARG, _I32,
                                 _P]),
     "npu_last_launch_plans": (_I32, [C.POINTER(NpuLaunchPlan), _I32]),

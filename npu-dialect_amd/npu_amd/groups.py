@@ -271,6 +271,64 @@ def fused_sample_tokens(logits, u, tokens, workspace, temperature=None, top_k=No
     return tokens
 
 
+def token_logprobs_workspace(logits, k=0):
+    """A workspace for fused_token_logprobs calls on logits of this shape with k
+    alternatives; one for each call that may run at the same time."""
+    import torch
+    n = _lib.lib().npu_token_logprobs_workspace(*logits.shape, int(k))
+    if n < 0:
+        raise ValueError(f"no log probabilities with {k} alternatives from logits of shape {tuple(logits.shape)}")
+    return torch.empty(n, dtype=torch.float32, device=logits.device)
+
+
+def fused_token_logprobs(logits, tokens, logprobs, workspace, entropy=None, ranks=None, top_tokens=None,
+                         top_logprobs=None, stream=None):
+    """logprobs[t] = log softmax(logits[t])[tokens[t]]; entropy[t] of that softmax,
+    ranks[t]: the entries before the token's (by logit, then index), top_tokens and
+    top_logprobs [T, k], k <= 32: the first k.  A token outside the row asks for
+    nothing: log probability 0, rank -1.  logits f32 or bf16."""
+    st = _lib.serve().token_logprobs(logits, tokens, logprobs, entropy, ranks, top_tokens, top_logprobs, workspace,
+                                     _raw(stream))
+    _check(st, "fused_token_logprobs")
+    return logprobs
+
+
+def fused_mx_quantize(x, q, scale, gate=None, values=None, stream=None):
+    """x (bf16, f32 [R, K]; with gate: x silu(gate)) in blocks of 32 along K that share a
+    power of two: q float8_e4m3fn [R, K], or e2m1 as uint8 or float4_e2m1fn_x2 [R, K / 2],
+    scale uint8 or float8_e8m0fnu [R, K / 32]; values (bf16) what they stand for.
+    A weight w [K, N] is given as w.t()."""
+    st = _lib.serve().mx_quantize(x, gate, q, scale, values, _raw(stream))
+    _check(st, "fused_mx_quantize")
+    return q, scale
+
+
+def fused_llama_add_rmsnorm(x, g, q, scale=None, delta=None, h=None, eps=1e-5, stream=None):
+    """h = x + delta (bf16); q = h / sqrt(mean(h^2) + eps) * g in blocks as
+    fused_mx_quantize's, with scale, or in bf16 without."""
+    st = _lib.serve().add_rmsnorm(x, delta, g, h, q, scale, eps, _raw(stream))
+    _check(st, "fused_llama_add_rmsnorm")
+    return q
+
+
+def mx_matmul_workspace(a, w):
+    """A workspace for fused_mx_matmul calls of these shapes; one for each call that may run
+    at the same time."""
+    import torch
+    n = _lib.lib().npu_mx_matmul_workspace(a.shape[0], w.shape[0], 2 * w.shape[1])
+    if n < 0:
+        raise ValueError(f"no product of blocks {tuple(a.shape)} with {tuple(w.shape)}")
+    return torch.empty(n, dtype=torch.float32, device=a.device)
+
+
+def fused_mx_matmul(a, a_scale, w, w_scale, out, workspace, stream=None):
+    """out = a @ w.T (bf16) of blocks as fused_mx_quantize gives them: a e4m3 or
+    e2m1 [M, K], w e2m1 [N, K]."""
+    st = _lib.serve().mx_matmul(a, a_scale, w, w_scale, out, workspace, _raw(stream))
+    _check(st, "fused_mx_matmul")
+    return out
+
+
 class Empty:
     """A tensor.empty argument of an outlined group: a shape and element type,
     and optionally the tensor that holds it (None: no data; the group never

@@ -6,7 +6,7 @@ import struct
 
 from ._lib import NpuMemref
 
-F32, BF16, I8, I32 = 0, 1, 2, 3
+F32, BF16, I8, I32, U8, E4M3 = 0, 1, 2, 3, 4, 5
 
 _DTYPE_CODES = None
 
@@ -16,7 +16,8 @@ def _codes():
     if _DTYPE_CODES is None:
         import torch
         _DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8,
-                        torch.int32: I32}
+                        torch.int32: I32, torch.uint8: U8, torch.float8_e8m0fnu: U8,
+                        torch.float4_e2m1fn_x2: U8, torch.float8_e4m3fn: E4M3}
     return _DTYPE_CODES
 
 
