@@ -392,8 +392,8 @@ npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
                                    const npu_memref *g, const npu_memref *h, const npu_memref *q,
                                    const npu_memref *scale, float eps, npu_stream stream);
 /* out[m][n] = sum over k of a[m][k] w[n][k].
- *   a e4m3 or e2m1 [M, K] with a_scale; w e2m1 [N, K] with w_scale; out bf16
- *   [M, N], rows at any stride; workspace f32 [n], n >= npu_mx_matmul_workspace:
+ *   a e4m3 or e2m1 [M, K] with a_scale; w e2m1 [N, K] with w_scale, rows at strides
+ *   below 2^23 bytes; out bf16 [M, N], rows at any stride; workspace f32 [n], n >= npu_mx_matmul_workspace:
  *   scratch that only this call uses while it runs.
  * Products and sums on the scaled matrix instructions: f32 sums in a fixed order, whose
  * terms of 128 k with e4m3 the instruction aligns to the largest (error up

@@ -1,6 +1,8 @@
 // mx_abi.hip -- the extern "C" boundary of the entry points in microscaled floats.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/npu_amd.h"
 #include "kernels.hpp"
 #include "mx_device.hpp"
@@ -8,7 +10,7 @@
 
 namespace {
 
-constexpr long long kMaxK = 1 << 20, kMaxEntries = 1LL << 34;
+constexpr long long kMaxK = 1 << 20, kMaxEntries = 1LL << 34, kMaxStride = 1 << 23;
 
 npu_status check_rows_k(const char *name, long long rows, long long K) {
   if (K % 32 != 0 || K > kMaxK)
@@ -147,6 +149,9 @@ npu_status fused_mx_matmul(const npu_memref *a, const npu_memref *a_scale, const
   if (w && w->dtype == NPU_E4M3) return fail(NPU_ERR_UNSUPPORTED, "w: e4m3, expected e2m1");
   const long long N = w ? w->sizes[0] : 0;
   NPU_TRY(check_blocks(w, w_scale, "w", "w_scale", N, K, &w_e4m3, &pw, &pws, &m.w_stride, &m.ws_stride));
+  // (the kernels' offsets within a tile have 32 bits)
+  const long long stride = std::max(std::max(m.a_stride, m.as_stride), std::max(m.w_stride, m.ws_stride));
+  if (stride >= kMaxStride) return fail(NPU_ERR_UNSUPPORTED, "a, w: rows at a stride of %lld bytes, at most 2^23", stride);
   NPU_TRY(check_rows(out, "out", NPU_BF16, 2, &po, &m.out_stride));
   NPU_TRY(expect_cols(out, "out", M, N));
   if (M >= kMaxEntries / N) return fail(NPU_ERR_UNSUPPORTED, "out: 2^34 entries or more");

@@ -285,7 +285,9 @@ def _product(a, sa, w, sw, out=None, stream=None):
 
 def _exact(a, sa, w, sw, kind):
     A, W = torch.from_numpy(R.values(a, sa, kind)), torch.from_numpy(R.values(w, sw, "e2m1"))
-    return A @ W.t(), A.abs() @ W.abs().t()
+    if A.numel() * W.shape[0] > 2 ** 31:
+        A, W = A.cuda(), W.cuda()
+    return (A @ W.t().contiguous()).cpu(), (A.abs() @ W.abs().t().contiguous()).cpu()
 
 
 def _check_product(a, sa, w, sw, kind, **kw):
@@ -315,6 +317,34 @@ def test_product(cuda, M, N, K, kind):
     w, sw = _blocks(N, K, "e2m1", K, small=True)
     exact, _ = _exact(a, sa, w, sw, kind)
     assert torch.equal(_product(a, sa, w, sw).cpu(), exact.float().to(BF16))
+    _check_product(*_blocks(M, K, kind, M + 1), *_blocks(N, K, "e2m1", N + 2), kind)
+
+
+FEW, JOIN, TILES = ["mx_matmul_few"], ["mx_join"], ["mx_scales", "mx_matmul_tile"]
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("M,N,K,kernels", [
+    (64, 1030, 14336, FEW + JOIN),           # K in parts, an odd width of them
+    (16, 171, 10656, FEW + JOIN),
+    (300, 130, 14016, FEW + JOIN),           # parts whose last is shorter
+    (1000, 1000, 4096, FEW),
+    (2048, 1100, 1600, TILES),               # tiles of 128
+    (1400, 39, 7392, TILES + JOIN),          # in parts
+    (1281, 1500, 1056, TILES),
+    (4101, 2050, 1024, TILES),
+    (4101, 4096, 4096, TILES + FEW),         # tiles of 256, and the rows past whole ones
+    (4096, 4030, 4000, TILES),
+])
+def test_product_kernels(cuda, M, N, K, kernels, kind):
+    from npu_amd import groups
+    a, sa = _blocks(M, K, kind, M + N, small=True)
+    w, sw = _blocks(N, K, "e2m1", K, small=True)
+    exact, _ = _exact(a, sa, w, sw, kind)
+    with groups.collect_plans() as cp:
+        got = _product(a, sa, w, sw)
+    assert torch.equal(got.cpu(), exact.float().to(BF16))
+    assert [p.kernel.decode() for p in cp.plans] == kernels
     _check_product(*_blocks(M, K, kind, M + 1), *_blocks(N, K, "e2m1", N + 2), kind)
 
 
