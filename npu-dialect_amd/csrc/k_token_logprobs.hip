@@ -10,14 +10,15 @@
 // has several.  The exponent d is one fma, x log2 e - c, c = m log2 e rounded; what c's rounding
 // left, the same for all entries, is taken off the sums' logarithm at the end.
 //
-// The k best: at least k of a wave's 64 lanes have a maximum that is no less than the
-// k-th largest of these, so that the part's k best are among the entries that reach the
-// largest of the waves' such bounds: of the order of k entries, which go to a list
-// in LDS and are ranked by comparing each with all.  A list that overflows (a row of equal
+// The k best: at least k of the lanes have a maximum that is no less than the k-th largest
+// of these, so that the part's k best are among the entries that reach it: little more
+// than k, which go to a list in LDS and are ranked by comparing each with all.  One
+// wave looks for that bound while the others sum.  A list that overflows (a row of equal
 // logits, say) is searched for the k best one after the other instead.
 //
-// Reading the row bounds it where rows are many, the chain of one part's steps and the
-// join where they are few.
+// Reading the rows bounds it where they are many (2000 rows of 128000 bf16, 512 MB: 118 us in the
+// kernel without alternatives 103, 5.0 TB/s, and 5 in the join), the chain of a part's steps and the
+// join where they are few (48 rows of 50257: 7 and 4.5).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   __shared__ u64 best[MAX_K];
   __shared__ float wave_a[NW], wave_b[NW];
   __shared__ int wave_c[NW];
-  __shared__ uint32_t wave_o[NW];
+  __shared__ uint32_t ups[LT], bound;
   __shared__ u64 wave_k[NW];
   __shared__ int n_list;
   const float inf = __builtin_inff();
@@ -173,28 +174,33 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
     float m = mine;
     for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     if (lane == 0) wave_a[wave] = m;
-    if (a.k > 0) {
-      // the k-th largest of the wave's lanes' maxima, bit by bit (as numbers that rise with x)
-      const uint32_t up = ~order_bits(mine);
-      uint32_t bound = 0;
-#pragma unroll 1
-      for (int b = 31; b >= (BF ? 16 : 0); --b) {
-        const uint32_t at = bound | 1u << b;
-        if (__popcll(__ballot(up >= at)) >= a.k) bound = at;
-      }
-      if (lane == 0) wave_o[wave] = bound;
-    }
+    if (a.k > 0) ups[tid] = ~order_bits(mine);  // (a number that rises with it)
   }
   __syncthreads();
   float m = wave_a[0];
-  uint32_t bound = a.k > 0 ? wave_o[0] : 0;
 #pragma unroll
-  for (int w = 1; w < NW; ++w) {
-    m = fmaxf(m, wave_a[w]);
-    if (a.k > 0) bound = max(bound, wave_o[w]);
+  for (int w = 1; w < NW; ++w) m = fmaxf(m, wave_a[w]);
+  if (a.k > 0 && wave == 0) {
+    // the k-th largest of the lanes' maxima, two bits at a time down to the 16th (what is left of f32 makes
+    // the bound a little lower)
+    uint32_t up[NW], found = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) up[w] = ups[64 * w + lane];
+    auto reach = [&](uint32_t at) __attribute__((always_inline)) {
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) n += __popcll(__ballot(up[w] >= at));
+      return n;
+    };
+#pragma unroll 1
+    for (int b = 30; b >= 16; b -= 2) {
+      const uint32_t at1 = found | 1u << b, at2 = found | 2u << b, at3 = found | 3u << b;
+      const int n1 = reach(at1), n2 = reach(at2), n3 = reach(at3);
+      found = n3 >= a.k ? at3 : n2 >= a.k ? at2 : n1 >= a.k ? at1 : found;
+    }
+    if (lane == 0) bound = found;
   }
   // sums, the rank, the list
-  const float least = fmaxf(from_order(~bound), -3.402823466e38f);  // (-Inf is no candidate)
   // (next to f32's ends the fma's terms overflow: those rows are summed from x - m below)
   const bool far = !(fabsf(m) < 1e37f);
   const float c = far ? 0.0f : m * LOG2E, rest = far ? 0.0f : fmaf(m, LOG2E, -c);
@@ -207,11 +213,8 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
     W = fmaf(w, d, W);
     before += x > over;
   };
-  auto keep = [&](float x, int j) __attribute__((always_inline)) {
-    if (x >= least) {
-      const int at = atomicAdd(&n_list, 1);
-      if (at < LIST) list[at] = (u64)order_bits(x) << 32 | (uint32_t)j;
-    }
+  auto keep = [&](int at, float x, int j) __attribute__((always_inline)) {
+    if (at < LIST) list[at] = (u64)order_bits(x) << 32 | (uint32_t)j;
   };
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -222,6 +225,11 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   }
   if (edge_j >= 0) add(edge, edge_j < token ? at_before : xt);
   packed();
+  float least = __builtin_inff();
+  if (a.k > 0) {
+    __syncthreads();
+    least = fmaxf(from_order(~bound), -3.402823466e38f);  // (-Inf is no candidate)
+  }
   if (a.k > 0 && mine >= least) {
     uint32_t runs = 0;
 #pragma unroll
@@ -233,10 +241,15 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
 #pragma unroll
       for (int i = 1; i < NCH; ++i)
         if (at == i) u = v[i];
+      int n = 0;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) keep(get(u, e), (c0 + at * LT) * PER - skew + e);
+      for (int e = 0; e < PER; ++e) n += get(u, e) >= least;
+      int to = atomicAdd(&n_list, n);  // (one for a run: its answer is a wait)
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (get(u, e) >= least) keep(to++, get(u, e), (c0 + at * LT) * PER - skew + e);
     }
-    if (edge_j >= 0) keep(edge, edge_j);
+    if (edge >= least) keep(atomicAdd(&n_list, 1), edge, edge_j);
   }
   if (!given) {
     before = 0;
@@ -310,47 +323,63 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   if (tid < a.k) keys_of(to)[tid] = best[tid];
 }
 
-// A row's parts.  The k best are in the k lists whose first keys come first, and no later than
-// the last of those first keys.
+// A row's parts, one a lane; their sums in a fixed order (a wave's lanes, then the waves).  The k
+// best come no later than the k-th of the lists' first keys (of so many of each that there are k):
+// most of the keys need not be ranked.
 __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsArgs a, int parts) {
+  constexpr int NW = LT / 64;
   __shared__ u64 heads[MAX_PARTS], list[MAX_K * MAX_K], best[MAX_K];
+  __shared__ float wave_m[NW], wave_s[NW], wave_w[NW];
+  __shared__ int wave_b[NW];
   __shared__ u64 bound;
   __shared__ int n_list;
   const float inf = __builtin_inff();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long long row = blockIdx.x;
   const size_t step = part_bytes(a.k);
   char *from = static_cast<char *>(a.workspace) + row * parts * step;
   auto part = [&](int i) { return reinterpret_cast<Part *>(from + i * step); };
-  if (tid < parts && a.k > 0) heads[tid] = keys_of(part(tid))[0];
+  Part p{-inf, 0.0f, 0.0f, 0};
+  if (tid < parts) p = *part(tid);
+  const int depth = parts >= a.k ? 1 : (a.k + parts - 1) / parts, n_heads = a.k > 0 ? parts * depth : 0;  // (below 2 MAX_K, or parts)
+  const u64 head = tid < n_heads ? keys_of(part(tid / depth))[tid % depth] : NO_KEY;
+  heads[tid] = head;
   if (tid < a.k) best[tid] = NO_KEY;
   if (tid == 0) n_list = 0, bound = NO_KEY;
-  // every lane sums all parts, in order
-  Part out{-inf, 0.0f, 0.0f, 0};
-  for (int i = 0; i < parts; ++i) out.m = fmaxf(out.m, part(i)->m);
-  for (int i = 0; i < parts; ++i) {
-    const Part p = *part(i);
-    out.before += p.before;
-    if (!(p.S > 0.0f)) continue;
+  float m = p.m;
+  int before = p.before;
+  for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off)), before += __shfl_xor(before, off);
+  if (lane == 0) wave_m[wave] = m, wave_b[wave] = before;
+  __syncthreads();
+  Part out{wave_m[0], 0.0f, 0.0f, 0};
+#pragma unroll
+  for (int w = 1; w < NW; ++w) out.m = fmaxf(out.m, wave_m[w]);
+  float S = 0.0f, W = 0.0f;
+  if (p.S > 0.0f) {
     const float d = p.m == out.m ? 0.0f : fmaxf((p.m - out.m) * LOG2E, -1000.0f), f = __builtin_amdgcn_exp2f(d);
-    out.S = fmaf(f, p.S, out.S);
-    out.W = fmaf(f, fmaf(d, p.S, p.W), out.W);
+    S = f * p.S;
+    W = f * fmaf(d, p.S, p.W);
+  }
+  S = wave_sum(S);
+  W = wave_sum(W);
+  if (lane == 0) wave_s[wave] = S, wave_w[wave] = W;
+  if (head != NO_KEY) {
+    int ahead = 0;
+#pragma unroll 4
+    for (int j = 0; j < n_heads; ++j) ahead += heads[j] < head;
+    if (ahead == a.k - 1) bound = head;
   }
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) out.S += wave_s[w], out.W += wave_w[w], out.before += wave_b[w];
   if (a.k > 0) {
-    if (tid < parts && parts >= a.k && heads[tid] != NO_KEY) {
-      int ahead = 0;
-      for (int j = 0; j < parts; ++j) ahead += heads[j] < heads[tid];
-      if (ahead == a.k - 1) bound = heads[tid];
-    }
-    __syncthreads();
     const u64 last = bound;
     for (int e = tid; e < parts * a.k; e += LT) {
       const int i = e / a.k;
-      if (heads[i] > last || heads[i] == NO_KEY) continue;
+      if (heads[i * depth] > last || heads[i * depth] == NO_KEY) continue;
       const u64 key = keys_of(part(i))[e - i * a.k];
       if (key > last || key == NO_KEY) continue;
-      list[atomicAdd(&n_list, 1)] = key;  // (at most k lists of k: with fewer real heads than k, all of them)
+      list[atomicAdd(&n_list, 1)] = key;  // (of at most k lists: with fewer real heads than k, all there are)
     }
     __syncthreads();
     rank_keys(list, n_list, a.k, best);
@@ -359,8 +388,10 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
   finish(a, row, out, best, tid);
 }
 
-// Runs of 16 bytes a lane holds: the most (8: half of the registers that eight workgroups
-// on a CU leave) that still give every CU four workgroups, as far as a join takes the parts.
+// Runs of 16 bytes a lane holds: the most (8: more would halve the workgroups on a CU), or fewer
+// where that leaves CUs without two workgroups, as far as a join takes the parts.  us with 8, 4, 2
+// and 1 runs: 48 rows of 50257 bf16 and 20 alternatives 14.2, 14.0, 13.1, 13.9; one of 128000 13.0,
+// 12.2, 12.1, 12.7; 256 and 5 27, 29, 37, 55; 2000 124, 154, 215, 368.
 struct Cut {
   int nch, parts;
 };
@@ -369,7 +400,7 @@ Cut cut_rows(int T, int V, bool bf16) {
   const long long chunks = (V + per - 1) / per + 1;  // (a row that begins and ends inside a run)
   auto parts = [&](int nch) { return (chunks + nch * LT - 1) / (nch * LT); };
   int nch = 8;
-  while (nch > 1 && (long long)T * parts(nch) < 4LL * device_cus() && parts(nch / 2) <= MAX_PARTS) nch /= 2;
+  while (nch > 2 && (long long)T * parts(nch) < 2LL * device_cus() && parts(nch / 2) <= MAX_PARTS) nch /= 2;
   return Cut{nch, (int)parts(nch)};
 }
 
@@ -388,9 +419,9 @@ hipError_t launch_token_logprobs(const TokenLogprobsArgs &a, hipStream_t s) {
   const Cut cut = cut_rows(a.T, a.V, a.bf16);
   const long long grid = (long long)a.T * cut.parts;
   auto kern = a.bf16 ? (cut.nch == 8 ? token_logprobs_kernel<true, 8> : cut.nch == 4 ? token_logprobs_kernel<true, 4>
-                        : cut.nch == 2 ? token_logprobs_kernel<true, 2> : token_logprobs_kernel<true, 1>)
+                        : token_logprobs_kernel<true, 2>)
                      : (cut.nch == 8 ? token_logprobs_kernel<false, 8> : cut.nch == 4 ? token_logprobs_kernel<false, 4>
-                        : cut.nch == 2 ? token_logprobs_kernel<false, 2> : token_logprobs_kernel<false, 1>);
+                        : token_logprobs_kernel<false, 2>);
   const double es = a.bf16 ? 2.0 : 4.0;
   {
     npu_launch_plan p = make_plan("token_logprobs", (int)grid, wg_per_cu(kern, LT), (int)grid, 16);
@@ -409,7 +440,7 @@ hipError_t launch_token_logprobs(const TokenLogprobsArgs &a, hipStream_t s) {
   {
     npu_launch_plan p = make_plan("token_logprobs_join", a.T, wg_per_cu(token_logprobs_join_kernel, LT), a.T, 16);
     p.load_phases = 3;
-    p.tile_valu = cut.parts * 20.0 * (LT / 64) + std::ceil(cut.parts / 64.0) * cut.parts * 4.0 + 4.0 * a.k * a.k;
+    p.tile_valu = 100.0 * (LT / 64) + std::ceil(cut.parts / 64.0) * cut.parts * 4.0 + 4.0 * a.k * a.k;
     p.tile_lds_bytes = 8.0 * cut.parts * cut.parts;
     p.tile_load_bytes = (double)cut.parts * part_bytes(a.k);
     p.tile_store_bytes = 12.0 + 8.0 * a.k;
