@@ -347,7 +347,8 @@ int64_t npu_sample_workspace(int64_t B, int64_t V);
  * each the same.  An alternative of p = 0 for that reason, or past the row's end, is
  * token -1 with -Inf.  A row of -Inf alone has log p = -Inf everywhere and entropy 0.
  * A token outside [0, V) asks for nothing: log probability 0, rank -1.
- *   logits f32 or bf16 [T, V], T <= 2^23, V <= 2^20, rows at any stride; tokens i32 [T];
+ *   logits f32 or bf16 [T, V], T <= 2^23, V <= 2^20, fewer than 2^34 entries, rows at any
+ *   stride; tokens i32 [T];
  *   logprobs f32 [T]; entropy f32 [T], ranks i32 [T], may be absent;
  *   top_tokens i32 and top_logprobs f32 [T, k], k <= 32, rows at any stride,
  *   both or neither; workspace f32 [n], n >= npu_token_logprobs_workspace:
@@ -385,7 +386,7 @@ npu_status fused_mx_quantize(const npu_memref *x, const npu_memref *gate, const 
                              const npu_memref *scale, const npu_memref *values,
                              npu_stream stream);
 /* h = bf16(x + delta); q = h / sqrt(mean(h^2) + eps) * g, in f32, to blocks or to bf16.
- *   x, delta, h bf16 [T, D], D <= 32768 a multiple of 32; g f32 [D]; q e4m3 or
+ *   x, delta, h bf16 [T, D], T <= 2^23, D <= 32768 a multiple of 32; g f32 [D]; q e4m3 or
  *   e2m1 with scale, or bf16 [T, D] without; delta may be absent (h = x), and h
  *   may be absent, or x, or delta. */
 npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
@@ -393,7 +394,8 @@ npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
                                    const npu_memref *scale, float eps, npu_stream stream);
 /* out[m][n] = sum over k of a[m][k] w[n][k].
  *   a e4m3 or e2m1 [M, K] with a_scale; w e2m1 [N, K] with w_scale, rows at strides
- *   below 2^23 bytes; out bf16 [M, N], rows at any stride; workspace f32 [n], n >= npu_mx_matmul_workspace:
+ *   below 2^23 bytes; out bf16 [M, N], M and N up to 2^23, fewer than 2^32 entries, rows at any
+ *   stride; workspace f32 [n], n >= npu_mx_matmul_workspace:
  *   scratch that only this call uses while it runs.
  * Products and sums on the scaled matrix instructions: f32 sums in a fixed order, whose
  * terms of 128 k with e4m3 the instruction aligns to the largest (error up

@@ -10,7 +10,8 @@
 
 namespace {
 
-constexpr long long kMaxK = 1 << 20, kMaxEntries = 1LL << 34, kMaxStride = 1 << 23;
+// (a launch's lanes are counted in 32 bits: kMaxRows and kMaxOut keep every grid below that)
+constexpr long long kMaxK = 1 << 20, kMaxEntries = 1LL << 34, kMaxStride = 1 << 23, kMaxRows = 1 << 23, kMaxOut = 1LL << 32;
 
 npu_status check_rows_k(const char *name, long long rows, long long K) {
   if (K % 32 != 0 || K > kMaxK)
@@ -95,6 +96,7 @@ npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
   const long long T = x->sizes[0], D = x->sizes[1];
   if (D % 32 != 0 || D > 32768)
     return fail(NPU_ERR_UNSUPPORTED, "x: rows of %lld, expected a multiple of 32 up to 32768", D);
+  if (T > kMaxRows) return fail(NPU_ERR_UNSUPPORTED, "x: %lld rows, at most 2^23", T);
   NPU_TRY(check_rows_k("x", T, D));
   if (!absent(delta)) {
     NPU_TRY(check_rows(delta, "delta", NPU_BF16, 16, &pd, &a.delta_stride));
@@ -132,8 +134,8 @@ npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
 }
 
 int64_t npu_mx_matmul_workspace(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || M > kMaxInt || N > kMaxInt || K % 32 != 0 || K > kMaxK || M * K >= kMaxEntries ||
-      N * K >= kMaxEntries || M >= kMaxEntries / N)
+  if (M <= 0 || N <= 0 || K <= 0 || M > kMaxRows || N > kMaxRows || K % 32 != 0 || K > kMaxK || M * K >= kMaxEntries ||
+      N * K >= kMaxEntries || M * N >= kMaxOut)
     return -1;
   return (int64_t)(npu::mx_matmul_workspace((int)M, (int)N, (int)K) / sizeof(float));
 }
@@ -154,7 +156,8 @@ npu_status fused_mx_matmul(const npu_memref *a, const npu_memref *a_scale, const
   if (stride >= kMaxStride) return fail(NPU_ERR_UNSUPPORTED, "a, w: rows at a stride of %lld bytes, at most 2^23", stride);
   NPU_TRY(check_rows(out, "out", NPU_BF16, 2, &po, &m.out_stride));
   NPU_TRY(expect_cols(out, "out", M, N));
-  if (M >= kMaxEntries / N) return fail(NPU_ERR_UNSUPPORTED, "out: 2^34 entries or more");
+  if (M > kMaxRows || N > kMaxRows) return fail(NPU_ERR_UNSUPPORTED, "out: [%lld,%lld], at most 2^23 each", M, N);
+  if (M * N >= kMaxOut) return fail(NPU_ERR_UNSUPPORTED, "out: 2^32 entries or more");
   NPU_TRY(check_workspace(workspace, npu_mx_matmul_workspace(M, N, K), &m.workspace));
   m.a = u8(pa);
   m.a_scale = u8(pas);

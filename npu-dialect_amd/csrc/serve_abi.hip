@@ -224,7 +224,7 @@ npu_status fused_sample_tokens(const npu_memref *logits, const npu_memref *u, co
 }
 
 int64_t npu_token_logprobs_workspace(int64_t T, int64_t V, int32_t k) {
-  if (T <= 0 || T > 1 << 23 || V <= 0 || V > 1 << 20 || k < 0 || k > 32) return -1;
+  if (T <= 0 || T > 1 << 23 || V <= 0 || V > 1 << 20 || T * V >= 1LL << 34 || k < 0 || k > 32) return -1;
   return (int64_t)(npu::token_logprobs_workspace((int)T, (int)V, k) / sizeof(float));
 }
 
@@ -240,6 +240,7 @@ npu_status fused_token_logprobs(const npu_memref *logits, const npu_memref *toke
   const long long T = logits->sizes[0], V = logits->sizes[1];
   if (V > 1 << 20) return fail(NPU_ERR_UNSUPPORTED, "logits: %lld columns, at most 2^20", V);
   if (T > 1 << 23) return fail(NPU_ERR_UNSUPPORTED, "logits: %lld rows, at most 2^23", T);
+  if (T * V >= 1LL << 34) return fail(NPU_ERR_UNSUPPORTED, "logits: 2^34 entries or more");
   NPU_TRY(check_vec(tokens, "tokens", NPU_I32, T, &p[0]));
   NPU_TRY(check_vec(logprobs, "logprobs", NPU_F32, T, &p[1]));
   if (!absent(entropy)) NPU_TRY(check_vec(entropy, "entropy", NPU_F32, T, &p[2]));

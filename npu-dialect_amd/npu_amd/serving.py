@@ -6,13 +6,19 @@ serving operators between them.
     s.add(slot, prompt)                          # a new sequence's tokens
     s.prefill()                                  # -> their first drawn tokens
     s.step()                                     # a token for every sequence
+    s.score(tokens)                              # the log probabilities of given tokens
 
 A step launches, per layer, QKV, rotate and append, attention over the pages and the
 three groups after it, then the head and the draw; nothing in it waits for the
 device, so step() can be captured (capture()) and replayed while pages are
-added to the table between replays.  ``python -m npu_amd.serving`` runs a small
-random model.
+added to the table between replays.  With ``alternatives`` a step also leaves its
+tokens' log probabilities and the best other tokens.
+
+``Server(*quantize_model(layers, embed, g_out, w_out), ...)`` holds the weights in four
+bits (e2m1 in blocks of 32) and takes activations in eight to the products.
+``python -m npu_amd.serving [--mx]`` runs a small random model.
 """
+import sys
 import weakref
 
 import torch
@@ -42,6 +48,46 @@ def decoder_layer(p, bufs, cache, batch, n_heads, eps=1e-5, stream=None):
     groups.fused_llama_rmsnorm_swiglu(bufs["h"], p["g2"], p["wg"], p["wu"], bufs["act"], eps, stream)
     groups.fused_llama_matmul_residual(bufs["act"], p["wd"], bufs["h"], bufs["out"], stream)
     return bufs["out"]
+
+
+def mx_weight(w):
+    """A weight [K, N] as (e2m1 [N, K / 2], scales [N, K / 32]), for fused_mx_matmul."""
+    k, n = w.shape
+    q = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+    return groups.fused_mx_quantize(w.t(), q, torch.empty((n, k // 32), dtype=torch.uint8, device=w.device))
+
+
+def quantize_model(layers, embed, g_out, w_out):
+    """The model with its weights in four bits: QKV's and the gate's and the other's side by
+    side; gains and the embedding as they are."""
+    side = lambda p, *names: mx_weight(torch.cat([p[n] for n in names], 1))
+    return [{"g1": p["g1"], "g2": p["g2"], "wqkv": side(p, "wq", "wk", "wv"), "wo": side(p, "wo"),
+             "wgu": side(p, "wg", "wu"), "wd": side(p, "wd")} for p in layers], embed, g_out, mx_weight(w_out)
+
+
+def mx_decoder_layer(p, bufs, cache, batch, n_heads, eps=1e-5, stream=None, delta=None):
+    """One decoder layer with weights of quantize_model: bufs["x"] becomes x + delta (what the
+    layer before left, None: nothing) plus attention, and the rest of this layer's output, to be added
+    to it, is returned.  ``bufs``: x, qkv, A, o, gu, d, q and s (e4m3 [T, D] and its scales),
+    qf and sf ([T, F]), ws, mx_ws; the others as decoder_layer's."""
+    k_pages, v_pages = cache
+    at = (batch["page_table"], batch["kv_len"])
+    x, qkv, gu, q, s, ws = (bufs[n] for n in ("x", "qkv", "gu", "q", "s", "mx_ws"))
+    D, F, dh = x.shape[1], gu.shape[1] // 2, k_pages.shape[3]
+    Q, K, V = qkv[:, :D], qkv[:, D:2 * D], qkv[:, 2 * D:]
+    groups.fused_llama_add_rmsnorm(x, p["g1"], q, s, delta=delta, h=x, eps=eps, stream=stream)
+    groups.fused_mx_matmul(q, s, *p["wqkv"], qkv, ws, stream)
+    groups.fused_llama_rope_append(Q, K, V, p["cos_t"], p["sin_t"], k_pages, v_pages, *at, Q, q_start=batch["q_start"],
+                                   prefix_len=batch["prefix_len"], stream=stream)
+    groups.fused_llama_paged_attention(Q, k_pages, v_pages, *at, bufs["A"], dh ** -0.5, bufs["ws"],
+                                       q_start=batch["q_start"], prefix_table=batch["prefix_table"],
+                                       prefix_len=batch["prefix_len"], stream=stream)
+    groups.fused_mx_quantize(bufs["A"], q, s, stream=stream)
+    groups.fused_mx_matmul(q, s, *p["wo"], bufs["o"], ws, stream)
+    groups.fused_llama_add_rmsnorm(x, p["g2"], q, s, delta=bufs["o"], h=x, eps=eps, stream=stream)
+    groups.fused_mx_matmul(q, s, *p["wgu"], gu, ws, stream)
+    groups.fused_mx_quantize(gu[:, F:], bufs["qf"], bufs["sf"], gate=gu[:, :F], stream=stream)
+    return groups.fused_mx_matmul(bufs["qf"], bufs["sf"], *p["wd"], bufs["d"], ws, stream)
 
 
 class Pages:
@@ -88,14 +134,19 @@ class Pages:
 
 class Server:
     """``layers``: decoder_layer's parameters without the position tables, bf16 [K, N]
-    weights and f32 gains; embed bf16 [vocabulary, D]; w_out bf16 [D, vocabulary]."""
+    weights and f32 gains; embed bf16 [vocabulary, D]; w_out bf16 [D, vocabulary]; or what
+    quantize_model makes of them.  ``alternatives``: None, or how many other tokens (0: none) a
+    step leaves beside its tokens' log probabilities: logprobs, entropy, ranks [slots],
+    top_tokens, top_logprobs [slots, alternatives], of the whole softmax of its logits."""
 
     def __init__(self, layers, embed, g_out, w_out, n_heads, slots, pages, page=64, max_pages=64, eps=1e-5,
-                 theta=10000.0):
+                 theta=10000.0, alternatives=None):
         dev, (self.V, self.D) = embed.device, embed.shape
+        self.mx = "wqkv" in layers[0]
         self.embed, self.g_out, self.w_out, self.H, self.eps = embed, g_out, w_out, n_heads, eps
         dh = self.D // n_heads
-        self.slots, self.pages, self.F = slots, Pages(pages, page, slots, max_pages), layers[0]["wg"].shape[1]
+        self.slots, self.pages = slots, Pages(pages, page, slots, max_pages)
+        self.F = layers[0]["wgu"][0].shape[0] // 2 if self.mx else layers[0]["wg"].shape[1]
         # positions count the prefix, which is itself a sequence of the table's width at most
         angle = torch.arange(2 * max_pages * page, device=dev, dtype=torch.float64)[:, None] * \
             theta ** (-torch.arange(0, dh, 2, device=dev, dtype=torch.float64) / dh)
@@ -112,8 +163,16 @@ class Server:
                          "top_p": torch.ones(slots, device=dev), "min_p": torch.zeros(slots, device=dev)}
         self.lens, self.waiting = [0] * slots, {}
         self.logits = torch.empty((slots, self.V), dtype=torch.bfloat16, device=dev)
-        self.no_residual = torch.zeros_like(self.logits)
         self.sample_ws = groups.sample_workspace(self.logits)
+        self.head = self._head_buffers(slots)
+        self.answers = {}
+        if alternatives is not None:
+            f, k = (lambda *shape: torch.zeros(shape, device=dev)), alternatives
+            self.answers = {"logprobs": f(slots), "entropy": f(slots), "ranks": ints(slots) - 1,
+                            "top_tokens": ints(slots, k) - 1 if k else None, "top_logprobs": f(slots, k) if k else None}
+            self.answers_ws = groups.token_logprobs_workspace(self.logits, k)
+            for name, t in self.answers.items():
+                setattr(self, name, t)
         self.one = self._buffers(slots)
         self.graphs = weakref.WeakSet()  # captured steps: they hold one's addresses and prefix_len
 
@@ -126,28 +185,62 @@ class Server:
     def _buffers(self, T, page_table=None):
         dev = self.embed.device
         e = lambda n: torch.empty((T, n), dtype=torch.bfloat16, device=dev)
-        b = {n: e(self.D) for n in ("x", "Q", "K", "V", "A", "h", "out")}
-        b["act"] = e(self.F)
-        b["ones"] = torch.ones((T, self.D // self.H // 2), device=dev)
-        b["zeros"] = torch.zeros_like(b["ones"])
-        b["ws"] = groups.paged_attention_workspace(b["Q"], self.cache[0][0],
+        if self.mx:
+            b = {n: e(self.D) for n in ("x", "A", "o", "d")}
+            b["qkv"], b["gu"] = e(3 * self.D), e(2 * self.F)
+            b["q"], b["s"] = self._blocks(T, self.D)
+            b["qf"], b["sf"] = self._blocks(T, self.F)
+            p = self.layers[0]
+            b["mx_ws"] = max((groups.mx_matmul_workspace(b[a], p[w][0]) for a, w in
+                              (("q", "wqkv"), ("q", "wo"), ("q", "wgu"), ("qf", "wd"))), key=torch.numel)
+        else:
+            b = {n: e(self.D) for n in ("x", "Q", "K", "V", "A", "h", "out")}
+            b["act"] = e(self.F)
+            b["ones"] = torch.ones((T, self.D // self.H // 2), device=dev)
+            b["zeros"] = torch.zeros_like(b["ones"])
+        b["ws"] = groups.paged_attention_workspace(b["A"], self.cache[0][0],
                                                    self.page_table if page_table is None else page_table,
                                                    self.prefix_len)
         return b
 
+    def _blocks(self, T, K):
+        dev = self.embed.device
+        return (torch.empty((T, K), dtype=torch.float8_e4m3fn, device=dev),
+                torch.empty((T, K // 32), dtype=torch.uint8, device=dev))
+
+    def _head_buffers(self, T):
+        """What the head keeps for T rows."""
+        if not self.mx:
+            return {"no_residual": torch.zeros((T, self.V), dtype=torch.bfloat16, device=self.embed.device)}
+        q, s = self._blocks(T, self.D)
+        return {"q": q, "s": s, "ws": groups.mx_matmul_workspace(q, self.w_out[0])}
+
     def _run(self, bufs, tokens, batch):
         # (a row without a token is drawn as -1)
         torch.index_select(self.embed, 0, tokens.clamp(min=0), out=bufs["x"])
+        if self.mx:
+            delta = None
+            for p, cache in zip(self.layers, self.cache):
+                delta = mx_decoder_layer(p, bufs, cache, batch, self.H, self.eps, delta=delta)
+            return bufs["x"].add_(delta)
         for p, cache in zip(self.layers, self.cache):
             bufs["x"].copy_(decoder_layer(p, bufs, cache, batch, self.H, self.eps))
         return bufs["x"]
 
-    def _draw(self, x):
+    def _head(self, x, head, logits):
+        if self.mx:
+            groups.fused_llama_add_rmsnorm(x, self.g_out, head["q"], head["s"], eps=self.eps)
+            return groups.fused_mx_matmul(head["q"], head["s"], *self.w_out, logits, head["ws"])
         x = x.float()
         x = (x * (x.square().mean(1, keepdim=True) + self.eps).rsqrt() * self.g_out).to(torch.bfloat16)
-        groups.fused_llama_matmul_residual(x, self.w_out, self.no_residual, self.logits)
-        return groups.fused_sample_tokens(self.logits, self.u, self.tokens, self.sample_ws, probs=self.probs,
-                                          **self.settings)
+        return groups.fused_llama_matmul_residual(x, self.w_out, head["no_residual"], logits)
+
+    def _draw(self, x):
+        self._head(x, self.head, self.logits)
+        groups.fused_sample_tokens(self.logits, self.u, self.tokens, self.sample_ws, probs=self.probs, **self.settings)
+        if self.answers:
+            groups.fused_token_logprobs(self.logits, self.tokens, workspace=self.answers_ws, **self.answers)
+        return self.tokens
 
     def _place(self, keys):
         for slot, at, page in self.pages.grow_all(keys):
@@ -172,6 +265,34 @@ class Server:
                    "prefix_len": 0})
         self.prefix_table, self.prefix_len = table[0, :len(own)].contiguous(), n
         self.one = self._buffers(self.slots)
+
+    def score(self, tokens, rows=128):
+        """Of a sequence of tokens (after the prefix), without a slot: the log probability of
+        each after the first, given those before it, and the entropy there, both
+        [len - 1].  ``rows``: of logits at a time."""
+        tokens = self._tokens(tokens)
+        dev, n = self.embed.device, len(tokens)
+        if n > self.pages.max_pages * self.pages.page:
+            raise ValueError(f"{n} tokens, the table holds {self.pages.max_pages * self.pages.page}")
+        own = self.pages.take(-(-n // self.pages.page))
+        try:
+            table = torch.tensor([own + [-1] * (self.pages.max_pages - len(own))], dtype=torch.int32, device=dev)
+            lens, ids = torch.tensor([n], dtype=torch.int32, device=dev), torch.tensor(tokens, device=dev)
+            x = self._run(self._buffers(n, table), ids, {
+                "page_table": table, "kv_len": lens, "q_start": torch.cat([lens * 0, lens]),
+                "prefix_table": self.prefix_table, "prefix_len": self.prefix_len})
+            logprobs, entropy = torch.zeros(n - 1, device=dev), torch.zeros(n - 1, device=dev)
+            following = ids[1:].to(torch.int32)
+            for r0 in range(0, n - 1, rows):
+                r1 = min(n - 1, r0 + rows)
+                logits = torch.empty((r1 - r0, self.V), dtype=torch.bfloat16, device=dev)
+                self._head(x[r0:r1], self._head_buffers(r1 - r0), logits)
+                groups.fused_token_logprobs(logits, following[r0:r1], logprobs[r0:r1],
+                                            groups.token_logprobs_workspace(logits), entropy=entropy[r0:r1])
+        finally:
+            # (later work that is given these pages comes behind on the stream)
+            self.pages.free.extend(reversed(own))
+        return logprobs, entropy
 
     def add(self, slot, tokens, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """A sequence of these tokens (after the prefix) in a free slot."""
@@ -198,7 +319,7 @@ class Server:
 
     def prefill(self):
         """The added sequences' tokens; draws each one's next (the other slots keep
-        their tokens; their rows of probs and logits mean nothing until the next step)."""
+        their tokens; their rows of probs, logits and alternatives mean nothing until the next step)."""
         dev, new = self.embed.device, [self.waiting.get(s, []) for s in range(self.slots)]
         start = torch.tensor([0] + [len(t) for t in new], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
         tokens = torch.tensor([t for ts in new for t in ts], dtype=torch.int64, device=dev)
@@ -239,8 +360,9 @@ class Server:
 
     def capture(self):
         """step() as a graph: make_room() before each replay().  The last step's
-        tokens, probs and logits stay."""
-        state = [(t, t.clone()) for t in (self.kv_len, self.tokens, self.probs, self.logits)]
+        tokens, probs, logits and alternatives stay."""
+        state = [(t, t.clone()) for t in (self.kv_len, self.tokens, self.probs, self.logits, *self.answers.values())
+                 if t is not None]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):  # once, uncaptured: the first call of a kernel asks for its occupancy
@@ -271,7 +393,9 @@ def random_model(n_layers, D, H, F, V, seed=0, device="cuda"):
 def main():
     g = torch.Generator().manual_seed(1)
     draw = lambda n: torch.randint(0, 4096, (n,), generator=g).tolist()
-    s = Server(*random_model(4, 512, 8, 1408, 4096), n_heads=8, slots=8, pages=128)
+    model = random_model(4, 512, 8, 1408, 4096)
+    s = Server(*(quantize_model(*model) if "--mx" in sys.argv[1:] else model), n_heads=8, slots=8, pages=128,
+               alternatives=3)
     s.set_prefix(draw(100))
     for slot, n in enumerate((5, 40, 1, 130, 77)):
         s.add(slot, draw(n), temperature=0.8, top_k=50, top_p=0.95)
@@ -284,7 +408,10 @@ def main():
         graph.replay()
         out.append(s.tokens.tolist())
     for slot in range(5):
-        print(f"sequence {slot}: {[row[slot] for row in out]}")
+        print(f"sequence {slot}: {[row[slot] for row in out]}; the last at log p {s.logprobs[slot]:.2f}, "
+              f"best {s.top_tokens[slot].tolist()}")
+    logprobs, entropy = s.score([row[3] for row in out])
+    print(f"sequence 3's tokens alone: log p {logprobs.mean():.2f}, entropy {entropy.mean():.2f} each")
 
 
 if __name__ == "__main__":

@@ -506,3 +506,340 @@ def test_logprobs_strides_streams_and_repeats(cuda):
         _, _, _, tops, lps = zip(*[R.logprobs64(_np64(wide)[t], t, 5) for t in range(7)])
         assert ids[:, 3:8].tolist() == list(map(list, tops)) and np.allclose(big[:, 1:6].cpu(), lps, atol=1e-4)
         assert (big[:, 0] == 4).all() and (big[:, 6:] == 4).all() and (ids[:, :3] == 4).all() and (ids[:, 8:] == 4).all()
+
+
+def test_tokens_and_their_log_probabilities_agree(cuda):
+    """The rank of a drawn token is its place among the alternatives, and greedy draws have rank 0."""
+    from npu_amd import groups
+    x = _logits(64, 5003, 9, BF16)
+    new = lambda *s, dtype=F32: torch.full(s, 55, dtype=dtype, device="cuda")
+    tok, probs, lp, rk = new(64, dtype=torch.int32), new(64), new(64), new(64, dtype=torch.int32)
+    tt, tl, ws = new(64, 32, dtype=torch.int32), new(64, 32), groups.token_logprobs_workspace(x, 32)
+    temperature, top_k = torch.ones(64, device="cuda"), torch.full((64,), 32, dtype=torch.int32, device="cuda")
+    temperature[:8] = 0
+    u = torch.rand(64, generator=torch.Generator().manual_seed(4)).cuda()
+    groups.fused_sample_tokens(x, u, tok, groups.sample_workspace(x), temperature=temperature, top_k=top_k, probs=probs)
+    groups.fused_token_logprobs(x, tok, lp, ws, ranks=rk, top_tokens=tt, top_logprobs=tl)
+    r = rk.long()[:, None]
+    assert (rk[:8] == 0).all() and (rk < 32).all()
+    assert torch.equal(tt.gather(1, r)[:, 0], tok) and torch.equal(tl.gather(1, r)[:, 0], lp)
+    # the drawn token's share of the 32: both within a few f32 roundings of sums and exponentials
+    share = (lp - tl.logsumexp(1)).exp()
+    assert ((share - probs).abs()[8:] <= 1e-5 * probs[8:]).all()
+
+
+# ---- captured, on two streams, together ------------------------------------------------
+def test_captured(cuda):
+    """Each call captured: replays, with eager work and changed inputs between, give the eager call's
+    bits; two graphs in turn with a workspace each."""
+    from npu_amd import groups
+    x, g = _rnd(300, 512, seed=1).to(BF16).cuda(), torch.ones(512, device="cuda")
+    w, sw = _blocks(700, 512, "e2m1", 2)
+    w2, sw2 = _blocks(300, 9984, "e2m1", 3)
+    a2, sa2 = _blocks(40, 9984, "e4m3", 4)  # (K in parts)
+    a3, sa3 = _blocks(2000, 512, "e4m3", 5)  # (tiles)
+    q, s = _mx(300, 512, "e4m3")
+    delta, h = _rnd(300, 512, seed=6).to(BF16).cuda(), torch.empty_like(x)
+    new = lambda *sh, dtype=BF16: torch.zeros(sh, dtype=dtype, device="cuda")
+    out, out2, out3, v = new(300, 700), new(40, 300), new(2000, 700), new(300, 512)
+    q4, s4 = _mx(300, 512, "e2m1")
+    tok = torch.arange(300, dtype=torch.int32, device="cuda")
+    lp, tt, tl = new(300, dtype=F32), new(300, 4, dtype=torch.int32), new(300, 4, dtype=F32)
+    logits = _rnd(300, 9001, seed=7).cuda()
+    ws = [[groups.mx_matmul_workspace(q, w), groups.mx_matmul_workspace(a2, w2), groups.mx_matmul_workspace(a3, w),
+           groups.token_logprobs_workspace(logits, 4)] for _ in range(3)]
+
+    def calls(ws):
+        stream = torch.cuda.current_stream()
+        groups.fused_llama_add_rmsnorm(x, g, q, s, delta=delta, h=h, stream=stream)
+        groups.fused_mx_matmul(q, s, w, sw, out, ws[0], stream)
+        groups.fused_mx_quantize(h, q4, s4, values=v, stream=stream)
+        groups.fused_mx_matmul(a2, sa2, w2, sw2, out2, ws[1], stream)
+        groups.fused_mx_matmul(a3, sa3, w, sw, out3, ws[2], stream)
+        groups.fused_token_logprobs(logits, tok, lp, ws[3], top_tokens=tt, top_logprobs=tl, stream=stream)
+
+    outs = (h, q.view(U8), s, out, q4, s4, v, out2, out3, lp, tt, tl)
+    calls(ws[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for i in (0, 1):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            calls(ws[i])
+    for step in range(5):
+        x.copy_(_rnd(300, 512, seed=10 + step) * (step + 1))
+        logits.copy_(_rnd(300, 9001, seed=20 + step) * step)
+        sw2.copy_(sw2.roll(1, 0))
+        a3.view(U8).copy_(a3.view(U8).roll(1, 0))
+        graphs[step % 2].replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in outs]
+        for t in outs:
+            t.zero_()
+        calls(ws[2])
+        torch.cuda.synchronize()
+        for i, (t, r) in enumerate(zip(outs, replayed)):
+            assert torch.equal(t, r), (step, i)
+
+
+def test_two_threads_on_two_streams(cuda):
+    """Each call on two streams at the same time: the bits of the same calls alone."""
+    import threading
+
+    from npu_amd import groups
+
+    def prepare(i):
+        M, N, K = ((2100, 1500, 2080), (40, 900, 9984))[i]
+        (a, sa), (w, sw) = _blocks(M, K, "e4m3", i), _blocks(N, K, "e2m1", i + 5)
+        x, g = _rnd(500, 2048, seed=i).to(BF16).cuda(), torch.ones(2048, device="cuda")
+        q, s = _mx(500, 2048, "e4m3")
+        q4, s4 = _mx(2048, 512, "e2m1")
+        wide = _rnd(512, 2048, seed=i + 2).to(BF16).cuda()
+        logits = _logits((30, 9)[i], 70001, i, (F32, BF16)[i])
+        T = logits.shape[0]
+        tok, lp = torch.arange(T, dtype=torch.int32, device="cuda"), torch.zeros(T, device="cuda")
+        tt, tl = torch.zeros((T, 7), dtype=torch.int32, device="cuda"), torch.zeros((T, 7), device="cuda")
+        out, ws, lws = torch.zeros((M, N), dtype=BF16, device="cuda"), groups.mx_matmul_workspace(a, w), groups.token_logprobs_workspace(logits, 7)
+
+        def run(stream):
+            groups.fused_llama_add_rmsnorm(x, g, q, s, stream=stream)
+            groups.fused_mx_matmul(a, sa, w, sw, out, ws, stream)
+            groups.fused_mx_quantize(wide.t(), q4, s4, stream=stream)
+            groups.fused_token_logprobs(logits, tok, lp, lws, top_tokens=tt, top_logprobs=tl, stream=stream)
+
+        return run, (q.view(U8), s, out, q4, s4, lp, tt, tl)
+
+    prepared, alone = [prepare(i) for i in range(2)], []
+    for run, outs in prepared:
+        run(None)
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in outs])
+        for t in outs:
+            t.zero_()
+    torch.cuda.synchronize()
+    errors, together = [], threading.Barrier(2)
+
+    def worker(i):
+        try:
+            stream = torch.cuda.Stream()
+            together.wait()
+            for _ in range(8):
+                prepared[i][0](stream)
+            stream.synchronize()
+        except Exception as e:  # raised below, in the test's own thread
+            errors.append(repr(e))
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    assert not any(t.is_alive() for t in threads) and not errors, errors
+    torch.cuda.synchronize()
+    for (_, outs), want in zip(prepared, alone):
+        for i, (got, w) in enumerate(zip(outs, want)):
+            assert torch.equal(got, w), i
+
+
+def test_python_refusals(cuda):
+    """Host tensors, other types and empty tensors are refused before any launch."""
+    from npu_amd import groups
+    from npu_amd.groups import NpuError
+    x = torch.ones((4, 64), dtype=BF16, device="cuda")
+    q, s = _mx(4, 64, "e4m3")
+    with pytest.raises(ValueError, match="x: expected a tensor on the GPU"):
+        groups.fused_mx_quantize(x.cpu(), q, s)
+    with pytest.raises(TypeError, match="scale: unsupported tensor dtype"):
+        groups.fused_mx_quantize(x, q, s.double())
+    with pytest.raises(TypeError, match="q: expected a tensor"):
+        groups.fused_mx_quantize(x, None, s)
+    with pytest.raises(NpuError, match=r"gate: size\[0\] = 0|gate: rank"):
+        groups.fused_mx_quantize(x, q, s, gate=torch.empty((0, 64), dtype=BF16, device="cuda"))
+    with pytest.raises(NpuError, match="q: element type"):
+        groups.fused_mx_quantize(x, q.view(torch.int8), s)
+    with pytest.raises(ValueError, match="no product of blocks"):
+        groups.mx_matmul_workspace(q, torch.zeros((5, 17), dtype=U8, device="cuda"))
+    with pytest.raises(ValueError, match="33 alternatives"):
+        groups.token_logprobs_workspace(x, 33)
+    # other torch types of the same bytes are taken
+    q4, s4 = _mx(4, 64, "e2m1")
+    groups.fused_mx_quantize(x, q4.view(torch.float4_e2m1fn_x2), s4.view(torch.float8_e8m0fnu))
+    assert (R.values(q4, s4, "e2m1") == 1).all()
+
+
+def test_rows_past_32_bits(cuda):
+    """Operands and outputs whose last rows lie past 2^31 elements, or 2^32 bytes."""
+    from npu_amd import groups
+    K, far = 64, (1 << 32) // 64 + 9
+    big = torch.zeros((far, K), dtype=BF16, device="cuda")  # 8.6 GB
+    big[-1] = _rnd(K, seed=1).to(BF16)
+    q = torch.zeros((far, K // 2), dtype=U8, device="cuda")
+    s = torch.full((far, 2), 9, dtype=U8, device="cuda")
+    groups.fused_mx_quantize(big, q, s)
+    c, sc = R.quantize(_np64(big[-1:]), "e2m1")
+    assert np.array_equal(R.codes(q[-1:], "e2m1"), c) and np.array_equal(s[-1:].cpu().numpy(), sc) and not s[:-1].any()
+    del big, q, s
+    T, D = 1 << 23, 288  # 4.8 GB
+    x = torch.zeros((T, D), dtype=BF16, device="cuda")
+    x[-1] = _rnd(D, seed=1).to(BF16)
+    h, (q, s) = torch.empty_like(x), _mx(T, D, "e2m1")
+    groups.fused_llama_add_rmsnorm(x, torch.ones(D, device="cuda"), q, s, delta=x, h=h)
+    assert torch.equal(h[-1], x[-1] * 2) and q[-1].any() and not q[:-1].any() and not h[:-1].any()
+    del x, h, q, s
+    # a, then out past 2^32 bytes; tiles and few rows
+    for M, N, K in ((1 << 22, 40, 1056), (1 << 21, 1100, 160), (1 << 22, 600, 96)):
+        a = torch.zeros((M, K), dtype=U8, device="cuda")
+        a[-1] = 0x38  # 1.0
+        a = a.view(torch.float8_e4m3fn)
+        w, sw = _blocks(N, K, "e2m1", 2, small=True)
+        out = torch.full((M, N), 5.0, dtype=BF16, device="cuda")
+        one = torch.full((M, K // 32), 127, dtype=U8, device="cuda")
+        groups.fused_mx_matmul(a, one, w, sw, out, groups.mx_matmul_workspace(a, w))
+        want = torch.from_numpy(R.values(w, sw, "e2m1").sum(1)).float().to(BF16)
+        assert torch.equal(out[-1].cpu(), want) and not out[:-1].any(), (M, N, K)
+        del a, out, one
+    V = 1 << 20
+    x = torch.zeros((2200, V), dtype=BF16, device="cuda")
+    x[-1, 12345] = 8.0
+    lp, tt, tl = torch.zeros(2200, device="cuda"), torch.zeros((2200, 1), dtype=torch.int32, device="cuda"), torch.zeros((2200, 1), device="cuda")
+    tok = torch.full((2200,), 12345, dtype=torch.int32, device="cuda")
+    groups.fused_token_logprobs(x, tok, lp, groups.token_logprobs_workspace(x, 1), top_tokens=tt, top_logprobs=tl)
+    exact = 8.0 - math.log(V - 1 + math.exp(8.0))
+    assert abs(float(lp[-1]) - exact) < 1e-5 and tt[-1] == 12345 and (tt[:-1] == 0).all()
+    assert (lp[:-1] + math.log(V)).abs().max() < 1e-5
+
+
+# ---- a decoder in microscaled floats ---------------------------------------------------
+def _unpacked(model):
+    """The model's weights as the values that quantize_model's blocks stand for, bf16 [K, N] (which
+    holds them: two bits and a power of two)."""
+    layers, embed, g_out, w_out = model
+    back = lambda qs: torch.from_numpy(R.values(*qs, "e2m1").T).to(BF16)
+    out = []
+    for p in layers:
+        (wq, wk, wv), (wg, wu) = back(p["wqkv"]).chunk(3, 1), back(p["wgu"]).chunk(2, 1)
+        out.append({"g1": p["g1"], "g2": p["g2"], "wq": wq, "wk": wk, "wv": wv, "wo": back(p["wo"]), "wg": wg, "wu": wu,
+                    "wd": back(p["wd"])})
+    return out, embed, g_out, back(w_out)
+
+
+def test_decoder_layer_stage_by_stage(cuda):
+    """mx_decoder_layer against its operators one by one, each checked against 64 bits on what the one
+    before gave it."""
+    import serve_refs as S
+    from npu_amd import groups, serving
+    D, H, F, T = 128, 2, 192, 37
+    layers, _, _, _ = serving.quantize_model(*serving.random_model(1, D, H, F, 64, seed=3))
+    bt = S.Batch([30, 7], [30, 19], H, 64, 16, 0, seed=3)
+    cos, sin = (t.cuda() for t in S.rope_tables(bt.max_pages * 16, 32))
+    p = dict(layers[0], cos_t=cos, sin_t=sin)
+    x, delta = _rnd(T, D, seed=1).to(BF16).cuda(), _rnd(T, D, seed=2).to(BF16).cuda()
+    batch = {"page_table": bt.page_table, "kv_len": bt.kv_len, "q_start": bt.q_start, "prefix_table": None, "prefix_len": 0}
+    e = lambda n: torch.full((T, n), 5.0, dtype=BF16, device="cuda")
+    pages = (bt.k_pages.clone(), bt.v_pages.clone())
+    ws = groups.paged_attention_workspace(x, pages[0], bt.page_table, 0)
+
+    q, s = _check_norm(x, p["g1"], "e4m3", delta=delta)
+    h = (x.float() + delta.float()).to(BF16)
+    _check_product(q, s, *p["wqkv"], "e4m3")
+    qkv = _product(q, s, *p["wqkv"])
+    Q, K, V = qkv[:, :D], qkv[:, D:2 * D], qkv[:, 2 * D:]
+    groups.fused_llama_rope_append(Q, K, V, cos, sin, *pages, bt.page_table, bt.kv_len, Q, q_start=bt.q_start)
+    A = groups.fused_llama_paged_attention(Q, *pages, bt.page_table, bt.kv_len, e(D), 64 ** -0.5, ws, q_start=bt.q_start)
+    qa, sa = _check_quantize(A, "e4m3")
+    _check_product(qa, sa, *p["wo"], "e4m3")
+    o = _product(qa, sa, *p["wo"])
+    q2, s2 = _check_norm(h, p["g2"], "e4m3", delta=o)
+    _check_product(q2, s2, *p["wgu"], "e4m3")
+    gu = _product(q2, s2, *p["wgu"])
+    qf, sf = _mx(T, F, "e4m3")
+    groups.fused_mx_quantize(gu[:, F:], qf, sf, gate=gu[:, :F])
+    R.check_near(qf, sf, _np64(gu[:, F:]) * R.silu64(_np64(gu[:, :F])), SILU_EPS, "e4m3")
+    _check_product(qf, sf, *p["wd"], "e4m3")
+    d = _product(qf, sf, *p["wd"])
+
+    bufs = {"x": x.clone(), "qkv": e(3 * D), "gu": e(2 * F), "A": e(D), "o": e(D), "d": e(D), "ws": ws}
+    (bufs["q"], bufs["s"]), (bufs["qf"], bufs["sf"]) = _mx(T, D, "e4m3"), _mx(T, F, "e4m3")
+    bufs["mx_ws"] = groups.mx_matmul_workspace(bufs["q"], p["wgu"][0])
+    cache = (bt.k_pages, bt.v_pages)
+    got = serving.mx_decoder_layer(p, bufs, cache, batch, H, delta=delta)
+    torch.cuda.synchronize()
+    assert torch.equal(got, d) and torch.equal(bufs["x"], (h.float() + o.float()).to(BF16))
+    assert torch.equal(cache[0], pages[0]) and torch.equal(cache[1], pages[1])
+
+
+@pytest.mark.parametrize("prefix", [0, 37])
+@pytest.mark.parametrize("mx", [True, False])
+def test_serving_with_alternatives_and_scores(cuda, mx, prefix):
+    """Prompts, then drawn tokens, eager and replayed: logits against the whole sequence's in f64 with
+    the values of the weights; tokens, log probabilities and alternatives against those logits; and the scores of
+    given tokens against the f64 model's.
+    The logits are off by a rounding of 2^-8 at nine places a layer and two after, and in
+    microscaled floats by one of 2^-4 at four a layer and one after: at most so many of the row's
+    norm."""
+    import serve_refs as S
+    from npu_amd import serving
+    from test_gpu_serve import _model64
+    H, V, L = 2, 448, 1
+    model = serving.random_model(L, 128, H, 192, V, seed=5)
+    if mx:
+        model = serving.quantize_model(*model)
+    exact_model = _unpacked(model) if mx else model
+    exact_model = tuple([{k: v.cpu() for k, v in p.items()} for p in m] if isinstance(m, list) else m.cpu() for m in exact_model)
+    bound = (9 * L + 2) * BF16_HALF_STEP + ((4 * L + 1) * 2.0 ** -4 if mx else 0.0)
+    s = serving.Server(*model, n_heads=H, slots=3, pages=30, page=16, max_pages=8, alternatives=5)
+    g = torch.Generator().manual_seed(2)
+    draw = lambda n: torch.randint(0, V, (n,), generator=g).tolist()
+    pre = draw(prefix)
+    if prefix:
+        s.set_prefix(pre)
+    live = {0: draw(5), 2: draw(40)}
+    s.add(0, live[0], temperature=0.7, top_k=40)
+    s.add(2, live[2], temperature=0.0)
+
+    def check(slots):
+        logits, tokens = s.logits.cpu(), s.tokens.tolist()
+        for b in slots:
+            exact = _model64(exact_model, H, pre + live[b])[-1]
+            assert float((logits[b].double() - exact).norm()) <= bound * float(exact.norm()), b
+            kw = {k: v[b].item() for k, v in s.settings.items()}
+            row = logits[b].double().numpy()
+            assert tokens[b] == S.sample64(row, s.u[b].item(), **kw)[0], b
+            lp, entropy, rank, top, tops = R.logprobs64(row, tokens[b], 5)
+            # (448 entries: a lane's one, the sums' steps, exponents up to 2^5: below 2^-17)
+            assert abs(s.logprobs[b].item() - lp) <= 2.0 ** -17 * (1 + abs(lp)) and abs(s.entropy[b].item() - entropy) <= 2.0 ** -14
+            assert s.ranks[b].item() == rank and s.top_tokens[b].tolist() == top
+            assert all(abs(x - y) <= 2.0 ** -17 * (1 + abs(y)) for x, y in zip(s.top_logprobs[b].tolist(), tops))
+            live[b].append(tokens[b])
+
+    s.u.copy_(torch.rand(3, generator=g))
+    s.prefill()
+    check([0, 2])
+    s.u.copy_(torch.rand(3, generator=g))
+    s.step()
+    check([0, 2])
+    graph = s.capture()
+    for _ in range(4):
+        s.make_room()
+        s.u.copy_(torch.rand(3, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        check([0, 2])
+    free = list(s.pages.free)
+    logprobs, entropy = s.score(live[2], rows=17)
+    exact = _model64(exact_model, H, pre + live[2])[prefix:-1]
+    lp = exact.log_softmax(1)
+    want = lp.gather(1, torch.tensor(live[2][1:])[:, None])[:, 0]
+    # a log probability moves by at most twice the largest change of a logit
+    off = 2 * bound * exact.norm(dim=1) + 2.0 ** -8 * exact.abs().amax(1)
+    assert ((logprobs.cpu().double() - want).abs() <= off).all()
+    assert (entropy.cpu() >= 0).all() and (entropy.cpu() <= math.log(V) + 1e-5).all()
+    assert sorted(free) == sorted(s.pages.free)
+    s.make_room()
+    s.u.copy_(torch.rand(3, generator=g))
+    graph.replay()
+    torch.cuda.synchronize()
+    check([0, 2])  # (a score leaves the sequences as they are)
+    with pytest.raises(ValueError, match="the table holds 128"):
+        s.score([1] * 129)
+    assert s.score([7])[0].numel() == 0

@@ -34,11 +34,11 @@ def refused(name, args, more, status, text):
 def test_workspaces():
     lib = npu_amd.lib()
     assert lib.npu_mx_matmul_workspace(1, 1, 32) > 0 and lib.npu_mx_matmul_workspace(5000, 4096, 14336) > 0
-    for bad in ((0, 1, 32), (1, 0, 32), (1, 1, 0), (1, 1, 33), (-1, 1, 32), (1, 1, (1 << 20) + 32), (1 << 31, 1, 32),
-                (1 << 20, 1 << 15, 32), (1 << 15, 1, 1 << 20)):
+    for bad in ((0, 1, 32), (1, 0, 32), (1, 1, 0), (1, 1, 33), (-1, 1, 32), (1, 1, (1 << 20) + 32), ((1 << 23) + 1, 1, 32),
+                (1, (1 << 23) + 1, 32), (1 << 17, 1 << 15, 32), (1 << 15, 1, 1 << 20)):
         assert lib.npu_mx_matmul_workspace(*bad) == -1, bad
     assert lib.npu_token_logprobs_workspace(1, 1, 0) > 0 and lib.npu_token_logprobs_workspace(8, 1 << 20, 32) > 0
-    for bad in ((0, 1, 0), (1, 0, 0), (1, (1 << 20) + 1, 0), (1, 5, 33), (1, 5, -1), ((1 << 23) + 1, 5, 0)):
+    for bad in ((0, 1, 0), (1, 0, 0), (1, (1 << 20) + 1, 0), (1, 5, 33), (1, 5, -1), ((1 << 23) + 1, 5, 0), (1 << 15, 1 << 19, 0)):
         assert lib.npu_token_logprobs_workspace(*bad) == -1, bad
 
 
@@ -85,6 +85,7 @@ NORM = {"x": mr([4, 64], BF16), "delta": mr([4, 64], BF16), "g": mr([64]), "h": 
     ({"x": mr([4, 64])}, 1e-5, 1, "x: element type"),
     ({"x": mr([4, 40], BF16)}, 1e-5, 2, "multiple of 32 up to 32768"),
     ({"x": mr([4, 32800], BF16)}, 1e-5, 2, "multiple of 32 up to 32768"),
+    ({"x": mr([(1 << 23) + 1, 64], BF16)}, 1e-5, 2, "at most 2^23"),
     ({"delta": mr([4, 32], BF16)}, 1e-5, 1, "delta: [4,32]"),
     ({"g": mr([32])}, 1e-5, 1, "g: size 32, expected 64"),
     ({"g": mr([64], BF16)}, 1e-5, 1, "g: element type"),
@@ -123,6 +124,12 @@ PRODUCT = {"a": mr([4, 64], E4M3), "a_scale": mr([4, 2], U8), "w": mr([8, 32], U
     ({"out": mr([4, 8])}, 1, "out: element type"),
     ({"out": mr([8, 4], BF16)}, 1, "out: [8,4]"),
     ({"out": mr([4, 8], BF16, [1, 4])}, 2, "rows must be contiguous"),
+    ({"a": mr([4, 64], E4M3, [1 << 23, 1])}, 2, "at most 2^23"),
+    ({"w_scale": mr([8, 2], U8, [1 << 23, 1])}, 2, "at most 2^23"),
+    ({"a": mr([(1 << 23) + 1, 64], E4M3), "a_scale": mr([(1 << 23) + 1, 2], U8), "out": mr([(1 << 23) + 1, 8], BF16)}, 2,
+     "at most 2^23 each"),
+    ({"a": mr([1 << 20, 64], E4M3), "a_scale": mr([1 << 20, 2], U8), "w": mr([4096, 32], U8), "w_scale": mr([4096, 2], U8),
+      "out": mr([1 << 20, 4096], BF16)}, 2, "2^32 entries"),
     ({"workspace": None}, 1, "workspace: null descriptor"),
     ({"workspace": mr([1])}, 1, "needed"),
     ({"workspace": mr([1 << 20], I32)}, 1, "workspace: element type"),
@@ -140,6 +147,7 @@ LOGPROBS = {"logits": mr([4, 100], BF16), "tokens": mr([4], I32), "logprobs": mr
     ({"logits": mr([4, 100], I32)}, 1, "logits: element type"),
     ({"logits": mr([4, (1 << 20) + 1])}, 2, "at most 2^20"),
     ({"logits": mr([(1 << 23) + 1, 4])}, 2, "at most 2^23"),
+    ({"logits": mr([1 << 15, 1 << 19], BF16)}, 2, "2^34 entries"),
     ({"logits": mr([4, 100], BF16, [100, 2])}, 2, "rows must be contiguous"),
     ({"tokens": mr([4])}, 1, "tokens: element type"),
     ({"tokens": mr([3], I32)}, 1, "tokens: size 3"),
