@@ -4,7 +4,15 @@
 // One instruction, v_mfma_scale_f32_16x16x128_f8f6f4, takes a step of 128 k with both operands'
 // scales: of an e2m1 operand lane l holds row l % 16's block l / 16 (16 bytes), of an e4m3
 // one the row's 16-byte runs l / 16 and 4 + l / 16, and of a scale operand that block's
-// byte.  w goes first, so that a lane gets four neighbouring n of one m.
+// byte.  w goes first, so that a lane gets four neighbouring n of one m.  e2m1 by e2m1 is summed
+// as f32 sums are; with an e4m3 operand the instruction lines the terms of a step up to the largest
+// and drops what lies some 2^-12 of the magnitudes below it.
+//
+// Few rows are bound by w's bytes and by what a CU's L1 passes on: 48 rows of e4m3 by 14336 x 4096
+// 14.4 us (1 row 7.2, 4.3 TB/s of w), one by 4096 x 4096 4.1, half of it launch.  Many rows are
+// bound by the matrix units and the clock that their power leaves: 8192^3 e2m1 276 us, 4.0 PFLOP/s,
+// without any loads of its operands 228; 4099 rows of e4m3 by 4096 x 14336 179 us, 2.7 PFLOP/s (half of
+// what the same instructions reach on operands that do not change).
 //
 #include <hip/hip_runtime.h>
 
@@ -238,7 +246,8 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
 // of 512 k, lane group g and row a word with the scales of the row's blocks 4j + g, j = 0 .. 3, a
 // byte each (0 past the row's end), rows filled up to whole tiles.  A wave's load of them is
 // four runs of 64 bytes; from the rows themselves it was sixteen requests of 16 bytes, as
-// many in all as the elements took, and the L2's rate of requests was the bound.
+// many in all as the elements took, and the L2's rate of requests was the bound.  Small tiles, of
+// which a call has few, take them from the rows all the same (DIRECT): the first kernel's 4 us are more.
 constexpr int TILE = 256;  // rows are filled up to a multiple of this
 
 __global__ __launch_bounds__(256) void mx_scales_kernel(MxMatmulArgs a, uint32_t *a_out, uint32_t *w_out, int a_rows, int w_rows, int chunks) {
@@ -301,7 +310,9 @@ struct TileOrder {
   }
 };
 
-template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF>
+// Loads of a stage go out spread between the products of an earlier one: all at once they held up
+// the wave (8192^3 e2m1 308 us, so 275; with stages of 64-byte rows and scales from the rows 422).
+template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
 __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArgs a, TileOrder order, const uint32_t *a_scales,
                                                                      const uint32_t *w_scales, int a_rows, int w_rows, int part_chunks,
                                                                      float *parts) {
@@ -347,17 +358,41 @@ __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArg
     __builtin_amdgcn_global_load_lds((global_u8 *)((of_a ? a_tile : w_tile) + (src[i] + (uint32_t)at)),
                                      (lds_u8 *)(lds + buf * STAGE + (wave + i * NW) * 1024), 16, 0, 0);
   };
-  const uint32_t *as_at = a_scales + (4LL * c0 + g) * a_rows + m0 + wm * TM * 16 + r;
-  const uint32_t *ws_at = w_scales + (4LL * c0 + g) * w_rows + n0 + wn * TN * 16 + r;
   uint32_t as_next[TM], ws_next[TN];
+  // the next chunk's scales: the first kernel's words, or (DIRECT) the rows' own bytes
+  const uint32_t *as_at = nullptr, *ws_at = nullptr;
+  uint32_t as_row[TM], ws_row[TN];
+  const uint8_t *as_tile = a.a_scale + m0 * a.as_stride, *ws_tile = a.w_scale + n0 * a.ws_stride;
+  const int blocks = a.K / 32;
+  int next_block = 16 * c0 + 4 * g;
+  if constexpr (DIRECT) {
+#pragma unroll
+    for (int t = 0; t < TM; ++t) as_row[t] = (uint32_t)min((wm * TM + t) * 16 + r, last_m) * (uint32_t)a.as_stride;
+#pragma unroll
+    for (int t = 0; t < TN; ++t) ws_row[t] = (uint32_t)min((wn * TN + t) * 16 + r, last_n) * (uint32_t)a.ws_stride;
+  } else {
+    as_at = a_scales + (4LL * c0 + g) * a_rows + m0 + wm * TM * 16 + r;
+    ws_at = w_scales + (4LL * c0 + g) * w_rows + n0 + wn * TN * 16 + r;
+  }
   auto load_scales = [&]() __attribute__((always_inline)) {
+    if constexpr (DIRECT) {
+      const ScaleWord word(next_block, blocks);
 #pragma unroll
-    for (int t = 0; t < TM; ++t) as_next[t] = as_at[t * 16];
+      for (int t = 0; t < TM; ++t) as_next[t] = word.of(as_tile + as_row[t]);
 #pragma unroll
-    for (int t = 0; t < TN; ++t) ws_next[t] = ws_at[t * 16];
-    as_at += 4LL * a_rows;
-    ws_at += 4LL * w_rows;
+      for (int t = 0; t < TN; ++t) ws_next[t] = word.of(ws_tile + ws_row[t]);
+      next_block += 16;
+    } else {
+#pragma unroll
+      for (int t = 0; t < TM; ++t) as_next[t] = as_at[t * 16];
+#pragma unroll
+      for (int t = 0; t < TN; ++t) ws_next[t] = ws_at[t * 16];
+      as_at += 4LL * a_rows;
+      ws_at += 4LL * w_rows;
+    }
   };
+  const uint32_t pick = 0x0c0c0400u + 0x0101u * (uint32_t)g;
+  auto taken = [&](uint32_t v) __attribute__((always_inline)) { return DIRECT ? scales_by_step(v, pick) : (int)v; };
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -411,9 +446,9 @@ __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArg
 #pragma unroll 1
   for (int c = 0, s = 0; c < chunks; ++c) {
 #pragma unroll
-    for (int t = 0; t < TM; ++t) as[t] = (int)as_next[t];
+    for (int t = 0; t < TM; ++t) as[t] = taken(as_next[t]);
 #pragma unroll
-    for (int t = 0; t < TN; ++t) ws[t] = (int)ws_next[t];
+    for (int t = 0; t < TN; ++t) ws[t] = taken(ws_next[t]);
     if (c + 1 < chunks) load_scales();
     stage(s++, std::integral_constant<int, 0>{});
     if constexpr (E4M3) {
@@ -486,14 +521,15 @@ hipError_t matmul_few(const MxMatmulArgs &a, int parts, hipStream_t s) {
   return join(a, parts, parts_at(a, parts, 0), s);
 }
 
-template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF>
+template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
 hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
   constexpr int STAGE = BM * 128 + BN * (E4M3 ? 64 : 128), LDS = NBUF * STAGE;
   static_assert(LDS <= 160 * 1024 && TILE % BM == 0 && TILE % BN == 0, "a CU's LDS; whole tiles of scales");
   const ScaleWords w = scale_words(a.M, a.N, a.K);
   const int part_chunks = (w.chunks + want_parts - 1) / want_parts, parts = (w.chunks + part_chunks - 1) / part_chunks;  // (none empty)
+  float *sums = parts_at(a, parts, DIRECT ? 0 : w.bytes);
   uint32_t *a_words = static_cast<uint32_t *>(a.workspace), *w_words = a_words + 4 * (size_t)w.chunks * w.a_rows;
-  {
+  if (!DIRECT) {
     const dim3 grid((unsigned)((w.a_rows + w.w_rows) / 256), (unsigned)((w.chunks + 7) / 8));
     npu_launch_plan p = make_plan("mx_scales", (int)(grid.x * grid.y), wg_per_cu(mx_scales_kernel, 256), (int)(grid.x * grid.y), 8);
     p.tile_valu = 4 * 8 * 30.0;
@@ -504,7 +540,7 @@ hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  auto kern = mx_matmul_tile_kernel<E4M3, BM, BN, WM, WN, NBUF>;
+  auto kern = mx_matmul_tile_kernel<E4M3, BM, BN, WM, WN, NBUF, DIRECT>;
   const int tiles_m = (int)((a.M + (long long)BM - 1) / BM), tiles_n = (int)((a.N + (long long)BN - 1) / BN);
   static const hipError_t lds_ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (lds_ok != hipSuccess) return lds_ok;
@@ -519,19 +555,20 @@ hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
   p.hbm_bytes = (double)a.K * (a.M * (E4M3 ? 1.03 : 0.53) + a.N * 0.53) + 2.0 * a.M * a.N;
   plans_add(p);
   hipLaunchKernelGGL(kern, dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(WM * WN * 64), LDS, s, a, TileOrder{tiles_m, tiles_n}, a_words,
-                     w_words, w.a_rows, w.w_rows, part_chunks, parts_at(a, parts, w.bytes));
-  return join(a, parts, parts_at(a, parts, w.bytes), s);
+                     w_words, w.a_rows, w.w_rows, part_chunks, sums);
+  return join(a, parts, sums, s);
 }
 
 // ---- which kernel ------------------------------------------------------------------------
-// A call is a few-rows kernel, or tiles of 128 or 256, with K in one part or in up to eight, by the
-// least of the times that these estimate, in us, from measurements of 448 shapes (M 1 .. 4096, N 512 ..
-// 14336, K 512 .. 14336, both types).  The choice takes 2.5 % more than each shape's fastest on
-// average: 48 rows by 4096 x 14336 in 64-column groups and four parts 17 us, in one 43, in tiles 23;
-// 1 row by the same in 16-column groups 11, in tiles 82; 1024 rows in tiles of 128 28, of 256 53;
-// 4096 rows 69 and 59.
+// A call is a few-rows kernel, or tiles of 64, 128 or 256, with K in one part or in up to eight, by
+// the least of the times that these estimate, in us, from measurements of 700 shapes (M 1 .. 4096,
+// N 512 .. 14336, K 512 .. 14336, both types).  The choice takes 2 % more than each shape's fastest
+// of these on average.  In us, e4m3: 1 row by 4096 x 14336 in 16-column groups 10.4, in 32-column ones
+// of two parts 9.9; 48 rows by the same 20.6, 16.9, in tiles of 64 and eight parts 15.7, in tiles of 128
+// 27; 512 rows by 4096 x 4096 in tiles of 64 18.4, of 128 24.4; 1000 rows 35.7 and 27.8;
+// 4096 rows in tiles of 128 67, of 256 62, by 4096 x 14336 218 and 177.
 struct Choice {
-  int tile;        // 128 or 256; 0: few rows
+  int tile;        // 64, 128 or 256; 0: few rows
   int mt, nt;      // groups of 16 mt x 16 nt (few rows)
   int parts;
   double us;
@@ -553,7 +590,12 @@ double tile_us(bool e4m3, int tile, int M, int N, int K, int parts, int cus) {
   const int chunks = ceil_div(K, 512), per = ceil_div(chunks, parts), real = ceil_div(chunks, per);
   const double steps = std::min(ceil_div(K, 128), 4 * per), tiles = (double)ceil_div(M, tile) * ceil_div(N, tile) * real;
   double us;
-  if (tile == 256) {
+  if (tile == 64) {  // (a CU takes three workgroups of e4m3's, two of e2m1's)
+    const double each[2][3] = {{0.303, 0.373, 0.373}, {0.345, 0.473, 0.657}};
+    const int most = e4m3 ? 3 : 2;
+    const double rounds = std::floor(tiles / ((double)most * cus)), left = tiles / cus - most * rounds;
+    us = 2.9 + rounds * (each[e4m3][2] * steps + (e4m3 ? 1.1 : 1.7)) + (left > 0 ? each[e4m3][(int)std::ceil(left) - 1] * steps : 0.0);
+  } else if (tile == 256) {
     const double alone = e4m3 ? 1.24 : 0.78, full = e4m3 ? 1.42 : 0.93, rounds = std::floor(tiles / cus), left = tiles / cus - rounds;
     us = 9.5 + rounds * (full * steps + 4.0) + (left > 0 ? (alone + (full - alone) * left) * steps + 2.0 : 0.0);
   } else {
@@ -568,7 +610,7 @@ Choice choose(bool e4m3, int M, int N, int K, int cus) {
   const int steps = ceil_div(K, 128);
   for (int parts = 1; parts <= 8; parts *= 2) {
     if (K >= 128 && parts <= ceil_div(K, 512))
-      for (int tile : {128, 256}) {
+      for (int tile : {64, 128, 256}) {
         if (tile == 256 && parts > 1) continue;  // (where K has to be divided, smaller tiles are the faster)
         const double us = tile_us(e4m3, tile, M, N, K, parts, cus);
         if (us < best.us) best = Choice{tile, 0, 0, parts, us};
@@ -602,7 +644,7 @@ Calls choose_calls(bool e4m3, int M, int N, int K, int cus) {
 }
 
 size_t call_bytes(const Choice &c, int M, int N, int K) {
-  return (c.tile ? scale_words(M, N, K).bytes : 0) + (c.parts > 1 ? c.parts * part_bytes(M, N) : 0);
+  return (c.tile > 64 ? scale_words(M, N, K).bytes : 0) + (c.parts > 1 ? c.parts * part_bytes(M, N) : 0);
 }
 
 // (what 256 registers hold without spilling)
@@ -617,8 +659,9 @@ hipError_t few_call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
 template <bool E4M3>
 hipError_t call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
   // (stages of e4m3 are shorter: three of them, and eight waves of 64 x 128, are the faster)
-  if (c.tile == 256) return E4M3 ? matmul_tiles<E4M3, 256, 256, 4, 2, E4M3 ? 3 : 2>(a, c.parts, s) : matmul_tiles<E4M3, 256, 256, 2, 4, 2>(a, c.parts, s);
-  if (c.tile == 128) return matmul_tiles<E4M3, 128, 128, 2, 2, E4M3 ? 3 : 2>(a, c.parts, s);
+  if (c.tile == 256) return E4M3 ? matmul_tiles<E4M3, 256, 256, 4, 2, E4M3 ? 3 : 2, false>(a, c.parts, s) : matmul_tiles<E4M3, 256, 256, 2, 4, 2, false>(a, c.parts, s);
+  if (c.tile == 128) return matmul_tiles<E4M3, 128, 128, 2, 2, E4M3 ? 3 : 2, false>(a, c.parts, s);
+  if (c.tile == 64) return matmul_tiles<E4M3, 64, 64, 2, 2, 4, true>(a, c.parts, s);
   if (c.mt == 1) return few_call<E4M3, 1>(a, c, s);
   if (c.mt == 2) return few_call<E4M3, 2>(a, c, s);
   if (c.mt == 3) return few_call<E4M3, 3>(a, c, s);

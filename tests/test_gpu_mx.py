@@ -320,18 +320,22 @@ def test_product(cuda, M, N, K, kind):
     _check_product(*_blocks(M, K, kind, M + 1), *_blocks(N, K, "e2m1", N + 2), kind)
 
 
-FEW, JOIN, TILES = ["mx_matmul_few"], ["mx_join"], ["mx_scales", "mx_matmul_tile"]
+FEW, JOIN, SMALL, TILES = ["mx_matmul_few"], ["mx_join"], ["mx_matmul_tile"], ["mx_scales", "mx_matmul_tile"]
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("M,N,K,kernels", [
-    (64, 1030, 14336, FEW + JOIN),           # K in parts, an odd width of them
+    (33, 1030, 14336, FEW + JOIN),           # K in parts, an odd width of them
     (16, 171, 10656, FEW + JOIN),
     (300, 130, 14016, FEW + JOIN),           # parts whose last is shorter
-    (1000, 1000, 4096, FEW),
-    (2048, 1100, 1600, TILES),               # tiles of 128
-    (1400, 39, 7392, TILES + JOIN),          # in parts
-    (1281, 1500, 1056, TILES),
+    (500, 700, 2080, FEW),
+    (100, 7000, 544, SMALL),                 # tiles of 64, a last step of a quarter
+    (600, 1000, 2080, SMALL),
+    (1281, 1500, 1056, SMALL),
+    (1025, 700, 7392, SMALL),
+    (1400, 39, 7392, SMALL + JOIN),          # in parts
+    (200, 4100, 14336, TILES + JOIN),        # of 128
+    (2048, 2100, 1600, TILES),
     (4101, 2050, 1024, TILES),
     (4101, 4096, 4096, TILES + FEW),         # tiles of 256, and the rows past whole ones
     (4096, 4030, 4000, TILES),
@@ -349,7 +353,7 @@ def test_product_kernels(cuda, M, N, K, kernels, kind):
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
-@pytest.mark.parametrize("M,N,K", [(3, 40, 96), (70, 130, 544), (300, 520, 1184), (20, 24, 160)])
+@pytest.mark.parametrize("M,N,K", [(3, 40, 96), (70, 130, 544), (300, 520, 1184), (20, 24, 160), (1030, 600, 1184), (2100, 2050, 544)])
 def test_product_strides_streams_and_repeats(cuda, M, N, K, kind):
     """Operands and the output inside wider buffers (output rows at any address), a side stream;
     the same call gives the same bits, and nothing beside the output changes."""
@@ -370,7 +374,7 @@ def test_product_strides_streams_and_repeats(cuda, M, N, K, kind):
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
-@pytest.mark.parametrize("M,N,K", [(5, 40, 544), (300, 300, 1184)])
+@pytest.mark.parametrize("M,N,K", [(5, 40, 544), (300, 300, 1184), (1030, 600, 1184)])
 def test_product_of_nan_blocks(cuda, M, N, K, kind):
     """A NaN scale makes its row of a, or column of w, NaN, and no other; scales of the least and
     largest sizes; zero blocks."""
