@@ -61,6 +61,8 @@ int64_t dtype_size(int32_t dt) {
     case NPU_BF16: return 2;
     case NPU_I8: return 1;
     case NPU_I32: return 4;
+    case NPU_U8: return 1;
+    case NPU_E4M3: return 1;
     default: return 0;
   }
 }
@@ -71,6 +73,8 @@ const char *dtype_name(int32_t dt) {
     case NPU_BF16: return "bf16";
     case NPU_I8: return "i8";
     case NPU_I32: return "i32";
+    case NPU_U8: return "u8";
+    case NPU_E4M3: return "e4m3";
     default: return "?";
   }
 }

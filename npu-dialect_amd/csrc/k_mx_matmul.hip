@@ -500,12 +500,18 @@ hipError_t join(const MxMatmulArgs &a, int parts, const float *sums, hipStream_t
   return hipGetLastError();
 }
 
+// The dynamic LDS limit of a kernel, raised once per device.
+bool lds_allowed(const void *kern, int lds) {
+  return cached_per_kernel(kern, [&](int) {
+    return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess ? 1 : 0;
+  });
+}
+
 template <bool E4M3, int MT, int NT>
 hipError_t matmul_few(const MxMatmulArgs &a, int parts, hipStream_t s) {
   constexpr int LDS = SW * MT * NT * 1024;
   auto kern = mx_matmul_few_kernel<E4M3, MT, NT>;
-  static const hipError_t lds_ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (lds_ok != hipSuccess) return lds_ok;
+  if (!lds_allowed(reinterpret_cast<const void *>(kern), LDS)) return hipErrorInvalidValue;
   const int steps = (a.K + 127) / 128, per_wave = 2 * ((steps + 2 * parts * SW - 1) / (2 * parts * SW));  // (whole lines)
   const long long groups_m = (a.M + 16LL * MT - 1) / (16 * MT), grid = (a.N + 16LL * NT - 1) / (16 * NT) * groups_m;
   npu_launch_plan p = make_plan("mx_matmul_few", (int)(grid * parts), wg_per_cu(kern, SW * 64, LDS), (int)(grid * parts), 8);
@@ -542,8 +548,7 @@ hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
   }
   auto kern = mx_matmul_tile_kernel<E4M3, BM, BN, WM, WN, NBUF, DIRECT>;
   const int tiles_m = (int)((a.M + (long long)BM - 1) / BM), tiles_n = (int)((a.N + (long long)BN - 1) / BN);
-  static const hipError_t lds_ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (lds_ok != hipSuccess) return lds_ok;
+  if (!lds_allowed(reinterpret_cast<const void *>(kern), LDS)) return hipErrorInvalidValue;
   npu_launch_plan p = make_plan("mx_matmul_tile", tiles_m * tiles_n * parts, wg_per_cu(kern, WM * WN * 64, LDS), tiles_m * tiles_n * parts, 8);
   const double steps = (a.K + 127) / 128 / (double)parts;
   p.unit_waves = WM * WN;

@@ -270,6 +270,8 @@ class Server:
         """Of a sequence of tokens (after the prefix), without a slot: the log probability of
         each after the first, given those before it, and the entropy there, both
         [len - 1].  ``rows``: of logits at a time."""
+        if rows < 1:
+            raise ValueError(f"{rows} rows at a time")
         tokens = self._tokens(tokens)
         dev, n = self.embed.device, len(tokens)
         if n > self.pages.max_pages * self.pages.page:

@@ -846,4 +846,6 @@ def test_serving_with_alternatives_and_scores(cuda, mx, prefix):
     check([0, 2])  # (a score leaves the sequences as they are)
     with pytest.raises(ValueError, match="the table holds 128"):
         s.score([1] * 129)
+    with pytest.raises(ValueError, match="0 rows"):
+        s.score([1, 2], rows=0)
     assert s.score([7])[0].numel() == 0
