@@ -62,21 +62,38 @@ struct Part {
 __device__ __forceinline__ u64 *keys_of(Part *p) { return reinterpret_cast<u64 *>(p + 1); }
 __host__ __device__ constexpr size_t part_bytes(int k) { return sizeof(Part) + 8 * (size_t)k; }
 
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp_mov<0xb1>(v));   // lane ^ 1
+  v = fmaxf(v, dpp_mov<0x4e>(v));   // lane ^ 2
+  v = fmaxf(v, dpp_mov<0x141>(v));  // the other half of eight
+  v = fmaxf(v, dpp_mov<0x140>(v));  // of sixteen
+  auto of = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
+  return fmaxf(fmaxf(of(0), of(16)), fmaxf(of(32), of(48)));
+}
+
+// The token's logit (-Inf: NaN, or none), read where the kernels begin.
+struct Given {
+  bool given;
+  int token;
+  float x;
+  __device__ __forceinline__ Given(const TokenLogprobsArgs &a, long long row) {
+    token = a.tokens[row];
+    given = token >= 0 && token < a.V;
+    x = -__builtin_inff();
+    const long long at = row * a.row_stride + token;
+    if (given) x = a.bf16 ? bf16_to_f32(static_cast<const uint16_t *>(a.logits)[at]) : static_cast<const float *>(a.logits)[at];
+    if (!(x > -__builtin_inff())) x = -__builtin_inff();
+  }
+};
+
 // What the joined sums give; lane `t` of the caller writes alternative t.
-__device__ __forceinline__ void finish(const TokenLogprobsArgs &a, long long row, const Part &p, const u64 *keys, int t) {
+__device__ __forceinline__ void finish(const TokenLogprobsArgs &a, long long row, const Given &tok, const Part &p, const u64 *keys, int t) {
   const float inf = __builtin_inff(), lnS = p.S > 0.0f ? logf(p.S) : 0.0f;
   // ((x - m) is exact or far from 0)
   auto logp = [&](float x) { return !(x > -inf) ? -inf : x == p.m ? -lnS : (x - p.m) - lnS; };
   if (t == 0) {
-    const int token = a.tokens[row];
-    const bool given = token >= 0 && token < a.V;
-    float lp = 0.0f;
-    if (given) {
-      const long long at = row * a.row_stride + token;
-      lp = logp(a.bf16 ? bf16_to_f32(static_cast<const uint16_t *>(a.logits)[at]) : static_cast<const float *>(a.logits)[at]);
-    }
-    a.logprobs[row] = lp;
-    if (a.ranks) a.ranks[row] = given ? p.before : -1;
+    a.logprobs[row] = tok.given ? logp(tok.x) : 0.0f;
+    if (a.ranks) a.ranks[row] = tok.given ? p.before : -1;
     if (a.entropy) a.entropy[row] = p.S > 0.0f ? lnS - LN2 * (p.W / p.S) : 0.0f;
   }
   if (t < a.k) {
@@ -140,11 +157,9 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   }
   float edge = -inf;
   if (edge_j >= 0) edge = entry(edge_j);
-  const int token = a.tokens[row];
-  const bool given = token >= 0 && token < a.V;
-  float xt = -inf;
-  if (given) xt = entry(token);
-  if (!(xt > -inf)) xt = -inf;
+  const Given tok(a, row);
+  const int token = tok.token;
+  const float xt = tok.x;
   if (tid == 0) n_list = 0;
   auto get = [&](u32x4 u, int e) __attribute__((always_inline)) {
     return BF ? __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16) : __uint_as_float(u[e]);
@@ -171,8 +186,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   }
   packed();
   {
-    float m = mine;
-    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    const float m = wave_max(mine);
     if (lane == 0) wave_a[wave] = m;
     if (a.k > 0) ups[tid] = ~order_bits(mine);  // (a number that rises with it)
   }
@@ -251,7 +265,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
     }
     if (edge >= least) keep(atomicAdd(&n_list, 1), edge, edge_j);
   }
-  if (!given) {
+  if (!tok.given) {
     before = 0;
   } else if (!(xt > -inf)) {
     // behind all above -Inf, and those like it with a lower index
@@ -273,7 +287,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   }
   S = wave_sum(S);
   W = wave_sum(W);
-  for (int off = 32; off; off >>= 1) before += __shfl_xor(before, off);
+  before = (int)wave_sum((float)before);  // (a row has at most 2^20)
   __syncthreads();  // (wave_a was read above)
   if (lane == 0) wave_a[wave] = S, wave_b[wave] = W, wave_c[wave] = before;
   __syncthreads();
@@ -315,7 +329,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
     out.W *= f;
   }
   if (parts == 1) {
-    finish(a, row, out, best, tid);
+    finish(a, row, tok, out, best, tid);
     return;
   }
   Part *to = reinterpret_cast<Part *>(static_cast<char *>(a.workspace) + (row * parts + part) * part_bytes(a.k));
@@ -336,6 +350,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
   const float inf = __builtin_inff();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long long row = blockIdx.x;
+  const Given tok(a, row);
   const size_t step = part_bytes(a.k);
   char *from = static_cast<char *>(a.workspace) + row * parts * step;
   auto part = [&](int i) { return reinterpret_cast<Part *>(from + i * step); };
@@ -343,12 +358,14 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
   if (tid < parts) p = *part(tid);
   const int depth = parts >= a.k ? 1 : (a.k + parts - 1) / parts, n_heads = a.k > 0 ? parts * depth : 0;  // (below 2 MAX_K, or parts)
   const u64 head = tid < n_heads ? keys_of(part(tid / depth))[tid % depth] : NO_KEY;
+  // (the first of the keys below, asked for now)
+  const int n_keys = parts * a.k, at0 = tid < n_keys ? tid / a.k : 0;
+  const u64 key0 = tid < n_keys ? keys_of(part(at0))[tid - at0 * a.k] : NO_KEY;
   heads[tid] = head;
   if (tid < a.k) best[tid] = NO_KEY;
   if (tid == 0) n_list = 0, bound = NO_KEY;
-  float m = p.m;
-  int before = p.before;
-  for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off)), before += __shfl_xor(before, off);
+  const float m = wave_max(p.m);
+  const int before = (int)wave_sum((float)p.before);
   if (lane == 0) wave_m[wave] = m, wave_b[wave] = before;
   __syncthreads();
   Part out{wave_m[0], 0.0f, 0.0f, 0};
@@ -374,10 +391,10 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
   for (int w = 0; w < NW; ++w) out.S += wave_s[w], out.W += wave_w[w], out.before += wave_b[w];
   if (a.k > 0) {
     const u64 last = bound;
-    for (int e = tid; e < parts * a.k; e += LT) {
+    for (int e = tid; e < n_keys; e += LT) {
       const int i = e / a.k;
       if (heads[i * depth] > last || heads[i * depth] == NO_KEY) continue;
-      const u64 key = keys_of(part(i))[e - i * a.k];
+      const u64 key = e < LT ? key0 : keys_of(part(i))[e - i * a.k];
       if (key > last || key == NO_KEY) continue;
       list[atomicAdd(&n_list, 1)] = key;  // (of at most k lists: with fewer real heads than k, all there are)
     }
@@ -385,7 +402,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
     rank_keys(list, n_list, a.k, best);
     __syncthreads();
   }
-  finish(a, row, out, best, tid);
+  finish(a, row, tok, out, best, tid);
 }
 
 // Runs of 16 bytes a lane holds: the most (8: more would halve the workgroups on a CU), or fewer
