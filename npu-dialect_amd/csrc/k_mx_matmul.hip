@@ -94,11 +94,13 @@ struct ScaleWord {
     shift = over < 4 ? 8 * over : 0;
     keep = over < 4 ? ~0u : 0u;
   }
-  __device__ __forceinline__ uint32_t of(const uint8_t *row) const {
+  __device__ __forceinline__ uint32_t load(const uint8_t *row) const {
     uint32_t v;
     __builtin_memcpy(&v, row + at, 4);
-    return (v & keep) >> shift;
+    return v;
   }
+  __device__ __forceinline__ uint32_t of(uint32_t v) const { return (v & keep) >> shift; }
+  __device__ __forceinline__ uint32_t of(const uint8_t *row) const { return of(load(row)); }
 };
 __device__ __forceinline__ uint32_t scale_bytes(const uint8_t *row, int b, int blocks) {  // rows of less than four
   uint32_t v = 0;
@@ -247,7 +249,8 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
 // byte each (0 past the row's end), rows filled up to whole tiles.  A wave's load of them is
 // four runs of 64 bytes; from the rows themselves it was sixteen requests of 16 bytes, as
 // many in all as the elements took, and the L2's rate of requests was the bound.  Small tiles, of
-// which a call has few, take them from the rows all the same (DIRECT): the first kernel's 4 us are more.
+// which a call has few, make their own words in LDS, for OWN chunks at a time: the first kernel's 4 us
+// are more.
 constexpr int TILE = 256;  // rows are filled up to a multiple of this
 
 __global__ __launch_bounds__(256) void mx_scales_kernel(MxMatmulArgs a, uint32_t *a_out, uint32_t *w_out, int a_rows, int w_rows, int chunks) {
@@ -312,7 +315,9 @@ struct TileOrder {
 
 // Loads of a stage go out spread between the products of an earlier one: all at once they held up
 // the wave (8192^3 e2m1 308 us, so 275; with stages of 64-byte rows and scales from the rows 422).
-template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
+// The scales' words too come to LDS by such loads, a chunk ahead: taken through registers they
+// had the compiler wait for every load under way, once a chunk.
+template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, int OWN>
 __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArgs a, TileOrder order, const uint32_t *a_scales,
                                                                      const uint32_t *w_scales, int a_rows, int w_rows, int part_chunks,
                                                                      float *parts) {
@@ -320,7 +325,9 @@ __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArg
   constexpr int AROW = 128, WROW = E4M3 ? 64 : 128, ABYTES = BM * AROW, STAGE = ABYTES + BN * WROW;
   constexpr int PA = ABYTES / 1024, PIECES = STAGE / 1024 / NW;
   constexpr int EACH = (PIECES + TM - 1) / TM;  // loads of a row of tiles
+  constexpr int ROWS = BM + BN, PITCH = OWN ? ROWS + 4 : ROWS;  // of the scales' words, a line for each lane group of a chunk
   static_assert(STAGE % (1024 * NW) == 0 && PA % NW == 0, "whole loads for every wave");
+  static_assert(OWN || ROWS * 16 == NW * 1024, "a load of a chunk's words for every wave");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int wm = wave % WM, wn = wave / WM;
@@ -358,62 +365,76 @@ __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArg
     __builtin_amdgcn_global_load_lds((global_u8 *)((of_a ? a_tile : w_tile) + (src[i] + (uint32_t)at)),
                                      (lds_u8 *)(lds + buf * STAGE + (wave + i * NW) * 1024), 16, 0, 0);
   };
-  uint32_t as_next[TM], ws_next[TN];
-  // the next chunk's scales: the first kernel's words, or (DIRECT) the rows' own bytes
-  const uint32_t *as_at = nullptr, *ws_at = nullptr;
-  uint32_t as_row[TM], ws_row[TN];
-  const uint8_t *as_tile = a.a_scale + m0 * a.as_stride, *ws_tile = a.w_scale + n0 * a.ws_stride;
-  const int blocks = a.K / 32;
-  int next_block = 16 * c0 + 4 * g;
-  if constexpr (DIRECT) {
+  uint32_t *words = reinterpret_cast<uint32_t *>(lds + NBUF * STAGE);  // of OWN chunks, or of two
+  // chunk c's words from the first kernel's: four rows of a lane group a lane
+  const int line = (wave * 256 + lane * 4) / ROWS, line_at = (wave * 256 + lane * 4) % ROWS;
+  const uint32_t *words_at = line_at < BM ? a_scales + (4LL * c0 + line) * a_rows + m0 + line_at
+                                          : w_scales + (4LL * c0 + line) * w_rows + n0 + (line_at - BM);
+  const long long words_step = 4LL * (line_at < BM ? a_rows : w_rows);
+  auto load_words = [&](int c) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((global_u8 *)words_at, (lds_u8 *)(words + (c & 1) * 4 * ROWS + wave * 256), 16, 0, 0);
+    words_at += words_step;
+  };
+  // or those of chunks c .. c + OWN - 1 from the rows: step j's four of a chunk a lane, to the word of lane group j
+  auto make_words = [&](int c) __attribute__((always_inline)) {
+    constexpr int A_ROW = OWN ? OWN * 4 : 4, EACH_LANE = ROWS * A_ROW / (NW * 64), AT_ONCE = NW * 64 / A_ROW;  // rows
+    const int q = threadIdx.x % A_ROW, j = q & 3;
+    const ScaleWord word(16 * (c0 + c) + 4 * q, a.K / 32);
+    uint32_t x[EACH_LANE];
 #pragma unroll
-    for (int t = 0; t < TM; ++t) as_row[t] = (uint32_t)min((wm * TM + t) * 16 + r, last_m) * (uint32_t)a.as_stride;
+    for (int i = 0; i < EACH_LANE; ++i) {
+      const int row = threadIdx.x / A_ROW + i * AT_ONCE;
+      x[i] = word.load(row < BM ? a.a_scale + (m0 + min(row, last_m)) * a.as_stride : a.w_scale + (n0 + min(row - BM, last_n)) * a.ws_stride);
+    }
+    const uint32_t pick = 0x0c0c0400u + 0x0101u * (uint32_t)j;  // byte j of each of two
 #pragma unroll
-    for (int t = 0; t < TN; ++t) ws_row[t] = (uint32_t)min((wn * TN + t) * 16 + r, last_n) * (uint32_t)a.ws_stride;
-  } else {
-    as_at = a_scales + (4LL * c0 + g) * a_rows + m0 + wm * TM * 16 + r;
-    ws_at = w_scales + (4LL * c0 + g) * w_rows + n0 + wn * TN * 16 + r;
-  }
-  auto load_scales = [&]() __attribute__((always_inline)) {
-    if constexpr (DIRECT) {
-      const ScaleWord word(next_block, blocks);
-#pragma unroll
-      for (int t = 0; t < TM; ++t) as_next[t] = word.of(as_tile + as_row[t]);
-#pragma unroll
-      for (int t = 0; t < TN; ++t) ws_next[t] = word.of(ws_tile + ws_row[t]);
-      next_block += 16;
-    } else {
-#pragma unroll
-      for (int t = 0; t < TM; ++t) as_next[t] = as_at[t * 16];
-#pragma unroll
-      for (int t = 0; t < TN; ++t) ws_next[t] = ws_at[t * 16];
-      as_at += 4LL * a_rows;
-      ws_at += 4LL * w_rows;
+    for (int i = 0; i < EACH_LANE; ++i) {
+      const int v = (int)word.of(x[i]);
+      auto of = [&](auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xf, 0xf, false); };  // a lane of the quad
+      const uint32_t x0 = of(std::integral_constant<int, 0x00>{}), x1 = of(std::integral_constant<int, 0x55>{});
+      const uint32_t x2 = of(std::integral_constant<int, 0xaa>{}), x3 = of(std::integral_constant<int, 0xff>{});
+      words[q * PITCH + threadIdx.x / A_ROW + i * AT_ONCE] =
+          __builtin_amdgcn_perm(__builtin_amdgcn_perm(x3, x2, pick), __builtin_amdgcn_perm(x1, x0, pick), 0x05040100u);
     }
   };
-  const uint32_t pick = 0x0c0c0400u + 0x0101u * (uint32_t)g;
-  auto taken = [&](uint32_t v) __attribute__((always_inline)) { return DIRECT ? scales_by_step(v, pick) : (int)v; };
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  load_scales();
+  // (the waits count loads: their order stays)
+  if constexpr (!OWN) load_words(0);
 #pragma unroll
-  for (int s = 0; s < NBUF - 1; ++s) static_for<PIECES>([&](auto i) __attribute__((always_inline)) { load(min(s, stages - 1), s, i); });
+  for (int s = 0; s < NBUF - 1; ++s) {
+    asm volatile("" ::: "memory");
+    static_for<PIECES>([&](auto i) __attribute__((always_inline)) { load(min(s, stages - 1), s, i); });
+  }
   // this lane's runs in a stage: k 0 .. 127 of e4m3 are its runs g and 4 + g, a step of e2m1 run g
   const int a_at = (wm * TM * 16 + r) * AROW + 16 * (g ^ swap128(r)), a_more = a_at ^ 64;
   const int w_at = ABYTES + (wn * TN * 16 + r) * WROW + 16 * (g ^ (E4M3 ? swap64(r) : swap128(r))), w_more = w_at ^ 64;
+  const uint32_t *as_at = words + g * PITCH + wm * TM * 16 + r, *ws_at = words + g * PITCH + BM + wn * TN * 16 + r;
   int as[TM], ws[TN];
   int buf = 0;
+  if constexpr (OWN) make_words(0);
   // A stage's products, a row of tiles at a time: the next row's operand is read ahead, and
   // the loads of a later stage go out one by one between them (all at once they hold up the wave).
-  auto stage = [&](int s, auto j) __attribute__((always_inline)) {
-    constexpr int STEP = decltype(j)::value, ROWS = SPS * TM;
-    wait_loads<(NBUF - 2) * PIECES>();
+  // MORE: the chunk has another behind it, whose words its first stage asks for.
+  auto stage = [&](int c, int s, auto j, auto more) __attribute__((always_inline)) {
+    constexpr int STEP = decltype(j)::value, TILE_ROWS = SPS * TM, AT = STEP / SPS;
+    constexpr bool WORDS = !OWN && decltype(more)::value;
+    // (the words are older than the loads of the stage that asked for them)
+    wait_loads<(NBUF - 2) * PIECES + (WORDS && AT >= 1 && AT <= NBUF - 2)>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    if constexpr (STEP == 0) {
+      const int slot = 4 * PITCH * (OWN ? c % (OWN ? OWN : 1) : c & 1);
+#pragma unroll
+      for (int t = 0; t < TM; ++t) as[t] = (int)as_at[slot + t * 16];
+#pragma unroll
+      for (int t = 0; t < TN; ++t) ws[t] = (int)ws_at[slot + t * 16];
+      if constexpr (WORDS) load_words(c + 1);
+    }
     const int ahead = min(s + NBUF - 1, stages - 1), free = buf == 0 ? NBUF - 1 : buf - 1;
     const uint8_t *base = lds + buf * STAGE;
     buf = buf == NBUF - 1 ? 0 : buf + 1;
@@ -431,9 +452,9 @@ __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArg
     };
     read_w(std::integral_constant<int, 0>{});
     read_a(std::integral_constant<int, 0>{});
-    static_for<ROWS>([&](auto row) __attribute__((always_inline)) {
+    static_for<TILE_ROWS>([&](auto row) __attribute__((always_inline)) {
       constexpr int R = decltype(row)::value, H = R / TM;
-      if constexpr (R + 1 < ROWS) read_a(std::integral_constant<int, R + 1>{});
+      if constexpr (R + 1 < TILE_ROWS) read_a(std::integral_constant<int, R + 1>{});
       if constexpr (SPS == 2 && R == TM - 2) read_w(std::integral_constant<int, 1>{});
       constexpr int P0 = std::min(PIECES, R * EACH), P1 = std::min(PIECES, (R + 1) * EACH);
       static_for<P1 - P0>([&](auto i) __attribute__((always_inline)) { load(ahead, free, std::integral_constant<int, P0 + decltype(i)::value>{}); });
@@ -443,20 +464,35 @@ __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArg
       __builtin_amdgcn_sched_barrier(0);
     });
   };
+  int s = 0;
 #pragma unroll 1
-  for (int c = 0, s = 0; c < chunks; ++c) {
-#pragma unroll
-    for (int t = 0; t < TM; ++t) as[t] = taken(as_next[t]);
-#pragma unroll
-    for (int t = 0; t < TN; ++t) ws[t] = taken(ws_next[t]);
-    if (c + 1 < chunks) load_scales();
-    stage(s++, std::integral_constant<int, 0>{});
+  for (int c = 0; c + 1 < chunks; ++c) {
+    constexpr std::true_type MORE{};
+    if constexpr (OWN) {
+      if (c > 0 && c % OWN == 0) make_words(c);
+    }
+    stage(c, s++, std::integral_constant<int, 0>{}, MORE);
     if constexpr (E4M3) {
-      if (s < stages) stage(s++, std::integral_constant<int, 1>{});
-      if (s < stages) stage(s++, std::integral_constant<int, 2>{});
-      if (s < stages) stage(s++, std::integral_constant<int, 3>{});
+      stage(c, s++, std::integral_constant<int, 1>{}, MORE);
+      stage(c, s++, std::integral_constant<int, 2>{}, MORE);
+      stage(c, s++, std::integral_constant<int, 3>{}, MORE);
     } else {
-      if (s < stages) stage(s++, std::integral_constant<int, 2>{});
+      stage(c, s++, std::integral_constant<int, 2>{}, MORE);
+    }
+  }
+  {
+    constexpr std::false_type MORE{};
+    const int c = chunks - 1;
+    if constexpr (OWN) {
+      if (c > 0 && c % OWN == 0) make_words(c);
+    }
+    stage(c, s++, std::integral_constant<int, 0>{}, MORE);
+    if constexpr (E4M3) {
+      if (s < stages) stage(c, s++, std::integral_constant<int, 1>{}, MORE);
+      if (s < stages) stage(c, s++, std::integral_constant<int, 2>{}, MORE);
+      if (s < stages) stage(c, s++, std::integral_constant<int, 3>{}, MORE);
+    } else {
+      if (s < stages) stage(c, s++, std::integral_constant<int, 2>{}, MORE);
     }
   }
   wait_loads<0>();  // (the loads of stages past the last one)
@@ -527,15 +563,15 @@ hipError_t matmul_few(const MxMatmulArgs &a, int parts, hipStream_t s) {
   return join(a, parts, parts_at(a, parts, 0), s);
 }
 
-template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
+template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, int OWN>
 hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
-  constexpr int STAGE = BM * 128 + BN * (E4M3 ? 64 : 128), LDS = NBUF * STAGE;
+  constexpr int STAGE = BM * 128 + BN * (E4M3 ? 64 : 128), LDS = NBUF * STAGE + (OWN ? OWN * 16 * (BM + BN + 4) : 32 * (BM + BN));
   static_assert(LDS <= 160 * 1024 && TILE % BM == 0 && TILE % BN == 0, "a CU's LDS; whole tiles of scales");
   const ScaleWords w = scale_words(a.M, a.N, a.K);
   const int part_chunks = (w.chunks + want_parts - 1) / want_parts, parts = (w.chunks + part_chunks - 1) / part_chunks;  // (none empty)
-  float *sums = parts_at(a, parts, DIRECT ? 0 : w.bytes);
+  float *sums = parts_at(a, parts, OWN ? 0 : w.bytes);
   uint32_t *a_words = static_cast<uint32_t *>(a.workspace), *w_words = a_words + 4 * (size_t)w.chunks * w.a_rows;
-  if (!DIRECT) {
+  if (!OWN) {
     const dim3 grid((unsigned)((w.a_rows + w.w_rows) / 256), (unsigned)((w.chunks + 7) / 8));
     npu_launch_plan p = make_plan("mx_scales", (int)(grid.x * grid.y), wg_per_cu(mx_scales_kernel, 256), (int)(grid.x * grid.y), 8);
     p.tile_valu = 4 * 8 * 30.0;
@@ -546,7 +582,7 @@ hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  auto kern = mx_matmul_tile_kernel<E4M3, BM, BN, WM, WN, NBUF, DIRECT>;
+  auto kern = mx_matmul_tile_kernel<E4M3, BM, BN, WM, WN, NBUF, OWN>;
   const int tiles_m = (int)((a.M + (long long)BM - 1) / BM), tiles_n = (int)((a.N + (long long)BN - 1) / BN);
   if (!lds_allowed(reinterpret_cast<const void *>(kern), LDS)) return hipErrorInvalidValue;
   npu_launch_plan p = make_plan("mx_matmul_tile", tiles_m * tiles_n * parts, wg_per_cu(kern, WM * WN * 64, LDS), tiles_m * tiles_n * parts, 8);
@@ -664,9 +700,9 @@ hipError_t few_call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
 template <bool E4M3>
 hipError_t call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
   // (stages of e4m3 are shorter: three of them, and eight waves of 64 x 128, are the faster)
-  if (c.tile == 256) return E4M3 ? matmul_tiles<E4M3, 256, 256, 4, 2, E4M3 ? 3 : 2, false>(a, c.parts, s) : matmul_tiles<E4M3, 256, 256, 2, 4, 2, false>(a, c.parts, s);
-  if (c.tile == 128) return matmul_tiles<E4M3, 128, 128, 2, 2, E4M3 ? 3 : 2, false>(a, c.parts, s);
-  if (c.tile == 64) return matmul_tiles<E4M3, 64, 64, 2, 2, 4, true>(a, c.parts, s);
+  if (c.tile == 256) return E4M3 ? matmul_tiles<E4M3, 256, 256, 4, 2, E4M3 ? 3 : 2, 0>(a, c.parts, s) : matmul_tiles<E4M3, 256, 256, 2, 4, 2, 0>(a, c.parts, s);
+  if (c.tile == 128) return matmul_tiles<E4M3, 128, 128, 2, 2, E4M3 ? 3 : 2, 0>(a, c.parts, s);
+  if (c.tile == 64) return matmul_tiles<E4M3, 64, 64, 2, 2, 3, 8>(a, c.parts, s);
   if (c.mt == 1) return few_call<E4M3, 1>(a, c, s);
   if (c.mt == 2) return few_call<E4M3, 2>(a, c, s);
   if (c.mt == 3) return few_call<E4M3, 3>(a, c, s);
