@@ -9,11 +9,10 @@
 // and drops what lies some 2^-12 of the magnitudes below it.
 //
 // Few rows are bound by w's bytes and by what a CU's L1 passes on: 48 rows of e4m3 by 14336 x 4096
-// 14.4 us (1 row 7.2, 4.3 TB/s of w), one by 4096 x 4096 4.1, half of it launch.  Many rows are
-// bound by the matrix units and the clock that their power leaves: 8192^3 e2m1 276 us, 4.0 PFLOP/s,
-// without any loads of its operands 228; 4099 rows of e4m3 by 4096 x 14336 179 us, 2.7 PFLOP/s (half of
+// 10.7 us (1 row 7.2, 4.3 TB/s of w), one by 4096 x 4096 4.1, half of it launch.  Many rows are
+// bound by the matrix units and the clock that their power leaves: 8192^3 e2m1 267 us, 4.1 PFLOP/s,
+// without any loads of its operands 228; 4099 rows of e4m3 by 4096 x 14336 177 us, 2.7 PFLOP/s (half of
 // what the same instructions reach on operands that do not change).
-//
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -314,9 +313,10 @@ struct TileOrder {
 };
 
 // Loads of a stage go out spread between the products of an earlier one: all at once they held up
-// the wave (8192^3 e2m1 308 us, so 275; with stages of 64-byte rows and scales from the rows 422).
+// the wave (8192^3 e2m1 308 us, so 276; with stages of 64-byte rows and scales from the rows 422).
 // The scales' words too come to LDS by such loads, a chunk ahead: taken through registers they
-// had the compiler wait for every load under way, once a chunk.
+// had the compiler wait for every load under way, once a chunk (276 us; 267 so; 512 rows of e4m3 by
+// 4096 x 4096 in tiles of 64 18.4, of 64 x 128 13.8 so).
 template <bool E4M3, int BM, int BN, int WM, int WN, int NBUF, int OWN>
 __global__ __launch_bounds__(WM *WN * 64) void mx_matmul_tile_kernel(MxMatmulArgs a, TileOrder order, const uint32_t *a_scales,
                                                                      const uint32_t *w_scales, int a_rows, int w_rows, int part_chunks,
@@ -601,49 +601,54 @@ hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
 }
 
 // ---- which kernel ------------------------------------------------------------------------
-// A call is a few-rows kernel, or tiles of 64, 128 or 256, with K in one part or in up to eight, by
-// the least of the times that these estimate, in us, from measurements of 700 shapes (M 1 .. 4096,
-// N 512 .. 14336, K 512 .. 14336, both types).  The choice takes 2 % more than each shape's fastest
-// of these on average.  In us, e4m3: 1 row by 4096 x 14336 in 16-column groups 10.4, in 32-column ones
-// of two parts 9.9; 48 rows by the same 20.6, 16.9, in tiles of 64 and eight parts 15.7, in tiles of 128
-// 27; 512 rows by 4096 x 4096 in tiles of 64 18.4, of 128 24.4; 1000 rows 35.7 and 27.8;
-// 4096 rows in tiles of 128 67, of 256 62, by 4096 x 14336 218 and 177.
+// A call is a few-rows kernel in groups of up to 48 rows by 16 or 32 columns, or tiles of 32 x 64, 64 x 128,
+// 128 x 128 or 256 x 256, with K in one part or in up to eight, by the least of the times that these
+// estimate, in us, from measurements of 480 shapes (M 1 .. 4096, N 512 .. 14336, K 512 .. 14336, both types).
+// The choice takes 4 % more than each shape's fastest of these on average, and these 1.3 % more than
+// the fastest of 22 tried.  In us, e4m3, parts after the slash:
+//   rows      by                  16 cols  32 cols  32 x 64  64 x 128  128 x 128  256 x 256
+//      1   4096 x 14336 (N x K)    9.9/1    10.1/4   10.6/4    12.6/8    14.9/8
+//     48  14336 x 4096            21.2/1    14.5/1   10.8/1    13.3/2    15.1/2
+//    512   4096 x 4096            54.9/1    39.8/1   19.4/1    13.8/1    18.9/1     49.6
+//   1000   4096 x 4096             113/1    79.3/1   33.7/1    21.9/1    21.0/1     50.9
+//   4096   4096 x 14336                                448/1     271/1     239/1      173
 struct Choice {
-  int tile;        // 64, 128 or 256; 0: few rows
+  int tile;        // rows of a tile; 0: few rows
   int mt, nt;      // groups of 16 mt x 16 nt (few rows)
   int parts;
   double us;
 };
 constexpr int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-double join_us(int M, int N, int parts) { return parts > 1 ? 3.2 + parts * 8.0 * M * N / 2.9e6 : 0.0; }
-
 // A group's time is its wave's steps, whose operands eight waves bring through one L1.
 double few_us(bool e4m3, int M, int N, int K, int mt, int nt, int parts, int cus) {
   const int per_wave = 2 * ceil_div(ceil_div(K, 128), 2 * SW * parts);
   const double rounds = std::ceil((double)ceil_div(M, 16 * mt) * ceil_div(N, 16 * nt) * parts / cus);
-  const double group = per_wave * (0.244 * nt + 0.159 * mt * (e4m3 ? 2 : 1)) + 0.046 * mt * nt;
-  return 2.15 + group * (1.0 + 0.98 * (rounds - 1.0)) + join_us(M, N, parts);
+  const double group = per_wave * (e4m3 ? 0.20 * nt + 0.33 * mt : 0.23 * nt + 0.21 * mt);
+  return 2.1 + group * (1.0 + (e4m3 ? 0.92 : 0.81) * (rounds - 1.0)) + (parts > 1 ? 2.6 + 4.8e-6 * parts * M * N : 0.0);
 }
 
-// A step takes a CU longer where more of its workgroups, or more CUs, share what it reads.
-double tile_us(bool e4m3, int tile, int M, int N, int K, int parts, int cus) {
+// Rounds of as many workgroups as fit the CUs, then what is left, a step of which takes as long as
+// that many workgroups on a CU have it take.
+struct TileCost {
+  int m, n, fit;
+  double call, round, step[3];
+};
+const TileCost kTiles[2][4] = {{{32, 64, 2, 3.7, 1.5, {0.107, 0.163}},
+                                {64, 128, 1, 4.0, 2.0, {0.212}},
+                                {128, 128, 2, 4.3, 5.3, {0.403, 0.609}},
+                                {256, 256, 1, 15.1, 9.8, {0.843}}},
+                               {{32, 64, 3, 3.8, 2.0, {0.148, 0.244, 0.331}},
+                                {64, 128, 2, 4.3, 3.5, {0.294, 0.505}},
+                                {128, 128, 1, 5.4, 3.2, {0.488}},
+                                {256, 256, 1, 15.3, 8.8, {1.374}}}};
+double tile_us(bool e4m3, const TileCost &t, int M, int N, int K, int parts, int cus) {
   const int chunks = ceil_div(K, 512), per = ceil_div(chunks, parts), real = ceil_div(chunks, per);
-  const double steps = std::min(ceil_div(K, 128), 4 * per), tiles = (double)ceil_div(M, tile) * ceil_div(N, tile) * real;
-  double us;
-  if (tile == 64) {  // (a CU takes three workgroups of e4m3's, two of e2m1's)
-    const double each[2][3] = {{0.303, 0.373, 0.373}, {0.345, 0.473, 0.657}};
-    const int most = e4m3 ? 3 : 2;
-    const double rounds = std::floor(tiles / ((double)most * cus)), left = tiles / cus - most * rounds;
-    us = 2.9 + rounds * (each[e4m3][2] * steps + (e4m3 ? 1.1 : 1.7)) + (left > 0 ? each[e4m3][(int)std::ceil(left) - 1] * steps : 0.0);
-  } else if (tile == 256) {
-    const double alone = e4m3 ? 1.24 : 0.78, full = e4m3 ? 1.42 : 0.93, rounds = std::floor(tiles / cus), left = tiles / cus - rounds;
-    us = 9.5 + rounds * (full * steps + 4.0) + (left > 0 ? (alone + (full - alone) * left) * steps + 2.0 : 0.0);
-  } else {
-    const double one = e4m3 ? 0.54 : 0.48, two = e4m3 ? 0.85 : 0.64, rounds = std::floor(tiles / (2.0 * cus)), left = tiles / cus - 2.0 * rounds;
-    us = 6.5 + rounds * (two * steps + 2.0) + (left > 1.0 ? two : left > 0 ? one : 0.0) * steps;
-  }
-  return us + join_us(M, N, real);
+  const double steps = std::min(ceil_div(K, 128), 4 * per), tiles = (double)ceil_div(M, t.m) * ceil_div(N, t.n) * real / cus;
+  const double rounds = std::floor(tiles / t.fit), left = tiles - rounds * t.fit, full = t.step[t.fit - 1];
+  // (one to a CU: the fewer CUs run, the faster)
+  const double last = left <= 0 ? 0.0 : t.fit > 1 ? t.step[(int)std::ceil(left) - 1] : full * (0.73 + 0.27 * left);
+  return t.call + rounds * (full * steps + t.round) + last * steps + (real > 1 ? 2.6 + 1.2e-6 * real * M * N : 0.0);
 }
 
 Choice choose(bool e4m3, int M, int N, int K, int cus) {
@@ -651,20 +656,20 @@ Choice choose(bool e4m3, int M, int N, int K, int cus) {
   const int steps = ceil_div(K, 128);
   for (int parts = 1; parts <= 8; parts *= 2) {
     if (K >= 128 && parts <= ceil_div(K, 512))
-      for (int tile : {64, 128, 256}) {
-        if (tile == 256 && parts > 1) continue;  // (where K has to be divided, smaller tiles are the faster)
-        const double us = tile_us(e4m3, tile, M, N, K, parts, cus);
-        if (us < best.us) best = Choice{tile, 0, 0, parts, us};
+      for (const TileCost &t : kTiles[e4m3]) {
+        if (t.m == 256 && parts > 1) continue;  // (where K has to be divided, smaller tiles are the faster)
+        const double us = tile_us(e4m3, t, M, N, K, parts, cus);
+        if (us < best.us) best = Choice{t.m, 0, 0, parts, us};
       }
     // (a thousand rows are tiles' whatever N and K)
     if (M > 1024 && K >= 128) continue;
     if (parts > 1 && steps < SW * parts) continue;
-    for (int mt = M > 48 ? 3 : ceil_div(M, 16); mt <= (M > 48 ? 4 : ceil_div(M, 16)); ++mt)
-      for (int nt : {1, 2, mt == 4 ? 2 : mt == 3 ? 3 : 4}) {
-        if (nt > 1 && N < 16 * nt) break;
-        const double us = few_us(e4m3, M, N, K, mt, nt, parts, cus);
-        if (us < best.us) best = Choice{0, mt, nt, parts, us};
-      }
+    const int mt = std::min(3, ceil_div(M, 16));
+    for (int nt : {1, 2}) {
+      if (nt > 1 && N < 16 * nt) break;
+      const double us = few_us(e4m3, M, N, K, mt, nt, parts, cus);
+      if (us < best.us) best = Choice{0, mt, nt, parts, us};
+    }
   }
   return best;
 }
@@ -685,28 +690,19 @@ Calls choose_calls(bool e4m3, int M, int N, int K, int cus) {
 }
 
 size_t call_bytes(const Choice &c, int M, int N, int K) {
-  return (c.tile > 64 ? scale_words(M, N, K).bytes : 0) + (c.parts > 1 ? c.parts * part_bytes(M, N) : 0);
+  return (c.tile == 256 ? scale_words(M, N, K).bytes : 0) + (c.parts > 1 ? c.parts * part_bytes(M, N) : 0);
 }
 
-// (what 256 registers hold without spilling)
-template <int MT>
-constexpr int WIDEST = MT == 4 ? 2 : MT == 3 ? 3 : 4;
-template <bool E4M3, int MT>
-hipError_t few_call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
-  if (c.nt == 1) return matmul_few<E4M3, MT, 1>(a, c.parts, s);
-  if (c.nt == 2) return matmul_few<E4M3, MT, 2>(a, c.parts, s);
-  return matmul_few<E4M3, MT, WIDEST<MT>>(a, c.parts, s);
-}
 template <bool E4M3>
 hipError_t call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
-  // (stages of e4m3 are shorter: three of them, and eight waves of 64 x 128, are the faster)
+  // (stages of e4m3 are shorter: eight waves of 64 x 128 are the faster there)
   if (c.tile == 256) return E4M3 ? matmul_tiles<E4M3, 256, 256, 4, 2, E4M3 ? 3 : 2, 0>(a, c.parts, s) : matmul_tiles<E4M3, 256, 256, 2, 4, 2, 0>(a, c.parts, s);
-  if (c.tile == 128) return matmul_tiles<E4M3, 128, 128, 2, 2, E4M3 ? 3 : 2, 0>(a, c.parts, s);
-  if (c.tile == 64) return matmul_tiles<E4M3, 64, 64, 2, 2, 3, 8>(a, c.parts, s);
-  if (c.mt == 1) return few_call<E4M3, 1>(a, c, s);
-  if (c.mt == 2) return few_call<E4M3, 2>(a, c, s);
-  if (c.mt == 3) return few_call<E4M3, 3>(a, c, s);
-  return few_call<E4M3, 4>(a, c, s);
+  if (c.tile == 128) return matmul_tiles<E4M3, 128, 128, 4, 2, E4M3 ? 3 : 2, E4M3 ? 4 : 2>(a, c.parts, s);
+  if (c.tile == 64) return matmul_tiles<E4M3, 64, 128, 2, 4, 3, E4M3 ? 8 : 4>(a, c.parts, s);
+  if (c.tile == 32) return matmul_tiles<E4M3, 32, 64, 1, 4, 4, 8>(a, c.parts, s);
+  if (c.mt == 1) return c.nt == 1 ? matmul_few<E4M3, 1, 1>(a, c.parts, s) : matmul_few<E4M3, 1, 2>(a, c.parts, s);
+  if (c.mt == 2) return c.nt == 1 ? matmul_few<E4M3, 2, 1>(a, c.parts, s) : matmul_few<E4M3, 2, 2>(a, c.parts, s);
+  return c.nt == 1 ? matmul_few<E4M3, 3, 1>(a, c.parts, s) : matmul_few<E4M3, 3, 2>(a, c.parts, s);
 }
 
 }  // namespace

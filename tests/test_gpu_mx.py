@@ -320,27 +320,30 @@ def test_product(cuda, M, N, K, kind):
     _check_product(*_blocks(M, K, kind, M + 1), *_blocks(N, K, "e2m1", N + 2), kind)
 
 
-FEW, JOIN, SMALL, TILES = ["mx_matmul_few"], ["mx_join"], ["mx_matmul_tile"], ["mx_scales", "mx_matmul_tile"]
+FEW, JOIN, TILES, WORDS = ["mx_matmul_few"], ["mx_join"], ["mx_matmul_tile"], ["mx_scales"]
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
-@pytest.mark.parametrize("M,N,K,kernels", [
-    (33, 1030, 14336, FEW + JOIN),           # K in parts, an odd width of them
-    (16, 171, 10656, FEW + JOIN),
-    (300, 130, 14016, FEW + JOIN),           # parts whose last is shorter
-    (500, 700, 2080, FEW),
-    (100, 7000, 544, SMALL),                 # tiles of 64, a last step of a quarter
-    (600, 1000, 2080, SMALL),
-    (1281, 1500, 1056, SMALL),
-    (1025, 700, 7392, SMALL),
-    (1400, 39, 7392, SMALL + JOIN),          # in parts
-    (200, 4100, 14336, TILES + JOIN),        # of 128
-    (2048, 2100, 1600, TILES),
-    (4101, 2050, 1024, TILES),
-    (4101, 4096, 4096, TILES + FEW),         # tiles of 256, and the rows past whole ones
-    (4096, 4030, 4000, TILES),
+@pytest.mark.parametrize("M,N,K,kernels,tile", [
+    (33, 1030, 14336, TILES + JOIN, (32, 64)),       # K in parts, an odd width of them
+    (16, 171, 10656, FEW + JOIN, None),
+    (51, 265, 8352, FEW + JOIN, None),
+    (300, 130, 14016, TILES + JOIN, (32, 64)),       # parts whose last is shorter
+    (45, 200, 992, FEW, None),
+    (500, 700, 2080, TILES, (32, 64)),
+    (100, 7000, 544, TILES, (32, 64)),               # a last step of a quarter
+    (1281, 1500, 1056, TILES, (64, 128)),
+    (1587, 65, 7200, TILES + JOIN, (64, 128)),
+    (130, 5000, 14336, TILES + JOIN, (64, 128)),
+    (1025, 700, 7392, TILES, (32, 64)),
+    (1400, 39, 7392, TILES + JOIN, (32, 64)),
+    (1500, 4100, 2080, TILES, (128, 128)),
+    (8505, 68, 12736, TILES + JOIN, (128, 128)),
+    (8358, 201, 1696, TILES, (128, 128)),
+    (4101, 4096, 4096, WORDS + TILES + FEW, (256, 256)),  # and the rows past whole ones
+    (4096, 4030, 4000, WORDS + TILES, (256, 256)),
 ])
-def test_product_kernels(cuda, M, N, K, kernels, kind):
+def test_product_kernels(cuda, M, N, K, kernels, tile, kind):
     from npu_amd import groups
     a, sa = _blocks(M, K, kind, M + N, small=True)
     w, sw = _blocks(N, K, "e2m1", K, small=True)
@@ -349,6 +352,10 @@ def test_product_kernels(cuda, M, N, K, kernels, kind):
         got = _product(a, sa, w, sw)
     assert torch.equal(got.cpu(), exact.float().to(BF16))
     assert [p.kernel.decode() for p in cp.plans] == kernels
+    if tile:
+        m = M // 256 * 256 if FEW[0] in kernels else M
+        tiles = -(-m // tile[0]) * -(-N // tile[1])
+        assert {p.kernel.decode(): p.grid for p in cp.plans}["mx_matmul_tile"] in [tiles * parts for parts in range(1, 9)]
     _check_product(*_blocks(M, K, kind, M + 1), *_blocks(N, K, "e2m1", N + 2), kind)
 
 
