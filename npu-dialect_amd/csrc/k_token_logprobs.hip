@@ -10,8 +10,8 @@
 // has several.  The exponent d is one fma, x log2 e - c, c = m log2 e rounded; what c's rounding
 // left, the same for all entries, is taken off the sums' logarithm at the end.
 //
-// The k best: at least k of the lanes have a maximum that is no less than the k-th largest
-// of these, so that the part's k best are among the entries that reach it: little more
+// The k best: at least k of 64 groups of lanes have a maximum that is no less than the k-th largest
+// of theirs, so that the part's k best are among the entries that reach it: little more
 // than k, which go to a list in LDS and are ranked by comparing each with all.  One
 // wave looks for that bound while the others sum.  A list that overflows (a row of equal
 // logits, say) is searched for the k best one after the other instead.
@@ -195,17 +195,12 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
 #pragma unroll
   for (int w = 1; w < NW; ++w) m = fmaxf(m, wave_a[w]);
   if (a.k > 0 && wave == 0) {
-    // the k-th largest of the lanes' maxima, two bits at a time down to the 16th (what is left of f32 makes
-    // the bound a little lower)
-    uint32_t up[NW], found = 0;
+    // the k-th largest of the maxima of NW lanes each, two bits at a time down to the 16th (what is left
+    // of f32 makes the bound a little lower)
+    uint32_t up = 0, found = 0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) up[w] = ups[64 * w + lane];
-    auto reach = [&](uint32_t at) __attribute__((always_inline)) {
-      int n = 0;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) n += __popcll(__ballot(up[w] >= at));
-      return n;
-    };
+    for (int w = 0; w < NW; ++w) up = max(up, ups[64 * w + lane]);
+    auto reach = [&](uint32_t at) __attribute__((always_inline)) { return __popcll(__ballot(up >= at)); };
 #pragma unroll 1
     for (int b = 30; b >= 16; b -= 2) {
       const uint32_t at1 = found | 1u << b, at2 = found | 2u << b, at3 = found | 3u << b;
@@ -237,7 +232,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
 #pragma unroll
     for (int e = 0; e < PER; ++e) add(get(v[i], e), over);
   }
-  if (edge_j >= 0) add(edge, edge_j < token ? at_before : xt);
+  add(edge, edge_j < token ? at_before : xt);  // (-Inf: none)
   packed();
   float least = __builtin_inff();
   if (a.k > 0) {
