@@ -16,9 +16,10 @@
 // wave looks for that bound while the others sum.  A list that overflows (a row of equal
 // logits, say) is searched for the k best one after the other instead.
 //
-// Reading the rows bounds it where they are many (2000 rows of 128000 bf16, 512 MB: 118 us in the
-// kernel without alternatives 103, 5.0 TB/s, and 5 in the join), the chain of a part's steps and the
-// join where they are few (48 rows of 50257: 7 and 4.5).
+// Where rows are many, their bytes and the vector instructions bound it alike: 2000 rows of 128000 bf16,
+// 512 MB, 116 us with five alternatives, 4.4 TB/s, of which 6 are the join (some 900 instructions a
+// wave for its 4096 entries, and 64 exponentials).  Where they are few, the chain of a part's steps and the join:
+// 48 rows of 50257 7.4 and 4.5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -216,23 +217,41 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   const float at_before = xt > -inf ? below(xt) : -inf;
   float S = 0.0f, W = 0.0f;
   int before = 0;
-  auto add = [&](float x, float over) __attribute__((always_inline)) {
+  auto add = [&](float x) __attribute__((always_inline)) {
     const float d = fmaxf(fmaf(x, LOG2E, -c), -1000.0f), w = __builtin_amdgcn_exp2f(d);
     S += w;
     W = fmaf(w, d, W);
-    before += x > over;
   };
   auto keep = [&](int at, float x, int j) __attribute__((always_inline)) {
     if (at < LIST) list[at] = (u64)order_bits(x) << 32 | (uint32_t)j;
   };
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int j0 = (c0 + i * LT) * PER - skew;
-    const float over = j0 + PER <= token ? at_before : xt;
+    // (runs of a wave without an entry before the token are most of them, where a model gave the token)
+    if (__any(run_max[i] >= xt)) {
+      const float over = (c0 + i * LT) * PER - skew + PER <= token ? at_before : xt;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) add(get(v[i], e), over);
+      for (int e = 0; e < PER; ++e) before += get(v[i], e) > over;
+    }
+    asm volatile("" : "+v"(v[i]));
+#pragma unroll
+    for (int e = 0; e < PER; e += 4) {
+      // (four at a time: a result of the exponential is not there for the next instruction)
+      float x[4], d[4], w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = get(v[i], e + q);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) d[q] = fmaxf(fmaf(x[q], LOG2E, -c), -1000.0f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = __builtin_amdgcn_exp2f(d[q]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) W = fmaf(w[q], d[q], W);
+      S += (w[0] + w[1]) + (w[2] + w[3]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
-  add(edge, edge_j < token ? at_before : xt);  // (-Inf: none)
+  add(edge);  // (-Inf: none)
+  before += edge > (edge_j < token ? at_before : xt);
   packed();
   float least = __builtin_inff();
   if (a.k > 0) {
