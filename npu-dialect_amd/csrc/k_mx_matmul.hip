@@ -693,6 +693,26 @@ size_t call_bytes(const Choice &c, int M, int N, int K) {
   return (c.tile == 256 ? scale_words(M, N, K).bytes : 0) + (c.parts > 1 ? c.parts * part_bytes(M, N) : 0);
 }
 
+// Of a shape's calls by type, and what the larger needs of the workspace.  A thread keeps its latest 64 shapes':
+// a call asks three times, and each time takes 0.2 to 0.7 us.
+struct Decided {
+  int M, N, K, cus;
+  Calls calls[2];
+  size_t bytes;
+};
+const Decided &decided(int M, int N, int K) {
+  static thread_local Decided kept[64];
+  const int cus = device_cus();
+  Decided &d = kept[((uint32_t)M * 2654435761u ^ (uint32_t)N * 2246822519u ^ (uint32_t)K * 3266489917u) >> 26];
+  if (d.M == M && d.N == N && d.K == K && d.cus == cus) return d;
+  d = Decided{M, N, K, cus, {choose_calls(false, M, N, K, cus), choose_calls(true, M, N, K, cus)}, 16};
+  for (const Calls &c : d.calls) {
+    d.bytes = std::max(d.bytes, call_bytes(c.first, c.m, N, K));
+    if (c.m < M) d.bytes = std::max(d.bytes, call_bytes(c.rest, M - c.m, N, K));
+  }
+  return d;
+}
+
 template <bool E4M3>
 hipError_t call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
   // (stages of e4m3 are shorter: eight waves of 64 x 128 are the faster there)
@@ -707,18 +727,10 @@ hipError_t call(const MxMatmulArgs &a, const Choice &c, hipStream_t s) {
 
 }  // namespace
 
-size_t mx_matmul_workspace(int M, int N, int K) {
-  size_t most = 16;
-  for (bool e4m3 : {false, true}) {
-    const Calls c = choose_calls(e4m3, M, N, K, device_cus());
-    most = std::max(most, call_bytes(c.first, c.m, N, K));
-    if (c.m < M) most = std::max(most, call_bytes(c.rest, M - c.m, N, K));
-  }
-  return most;
-}
+size_t mx_matmul_workspace(int M, int N, int K) { return decided(M, N, K).bytes; }
 
 hipError_t launch_mx_matmul(const MxMatmulArgs &a, hipStream_t s) {
-  const Calls c = choose_calls(a.e4m3, a.M, a.N, a.K, device_cus());
+  const Calls c = decided(a.M, a.N, a.K).calls[a.e4m3];
   MxMatmulArgs b = a;
   b.M = c.m;
   const hipError_t e = a.e4m3 ? call<true>(b, c.first, s) : call<false>(b, c.first, s);

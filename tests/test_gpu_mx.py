@@ -306,7 +306,8 @@ def _check_product(a, sa, w, sw, kind, **kw):
 PRODUCTS = [(1, 1, 32), (1, 16, 32), (1, 17, 64), (3, 5, 96), (16, 16, 128), (17, 33, 160), (15, 100, 1024), (33, 64, 1056),
             (64, 48, 512), (65, 130, 1408), (1, 1408, 512), (48, 300, 4096), (100, 257, 256), (128, 128, 128), (129, 255, 288),
             (256, 256, 512), (257, 511, 1184), (300, 1408, 768), (500, 700, 2080), (513, 96, 640), (40, 1000, 14336),
-            (200, 300, 9984), (1000, 1000, 32), (777, 1, 96), (1, 5000, 224)]
+            (200, 300, 9984), (1000, 1000, 32), (777, 1, 96), (1, 5000, 224), (719, 40, 128), (6650, 1840, 192),
+            (8600, 140, 128)]
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
@@ -381,7 +382,7 @@ def test_product_strides_streams_and_repeats(cuda, M, N, K, kind):
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
-@pytest.mark.parametrize("M,N,K", [(5, 40, 544), (300, 300, 1184), (1030, 600, 1184)])
+@pytest.mark.parametrize("M,N,K", [(5, 40, 544), (300, 300, 1184), (1030, 600, 1184), (1600, 70, 7200), (2100, 2050, 544)])
 def test_product_of_nan_blocks(cuda, M, N, K, kind):
     """A NaN scale makes its row of a, or column of w, NaN, and no other; scales of the least and
     largest sizes; zero blocks."""
