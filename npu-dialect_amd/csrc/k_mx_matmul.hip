@@ -136,7 +136,7 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
   }
   // A load takes 64 bytes of each of 16 rows, half a line.  All the same half costs the L1 as much as
   // whole lines, so of each two such loads odd rows' halves come in the other order (48 rows by
-  // 14336 x 4096: 14.2 us in one order, 11.8 so; sixteen rows are a whole number of lines apart).
+  // 14336 x 4096: a sixth less time; sixteen rows are a whole number of lines apart).
   const bool w_odd = (r ^ (int)(((uintptr_t)w + (uint32_t)r * (uint32_t)a.w_stride) >> 6)) & 1;
   const bool x_odd = (r ^ (int)(((uintptr_t)x + (uint32_t)r * (uint32_t)a.a_stride) >> 6)) & 1;
   auto load_line = [&](const uint8_t *rows, uint32_t row, int at, int end, bool odd, u32x4 &first, u32x4 &second) __attribute__((always_inline)) {

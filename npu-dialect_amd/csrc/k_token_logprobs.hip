@@ -19,7 +19,7 @@
 // Where rows are many, their bytes and the vector instructions bound it alike: 2000 rows of 128000 bf16,
 // 512 MB, 116 us with five alternatives, 4.4 TB/s, of which 6 are the join (some 900 instructions a
 // wave for its 4096 entries, and 64 exponentials).  Where they are few, the chain of a part's steps and the join:
-// 48 rows of 50257 7.4 and 4.5.
+// 48 rows of 50257 with 20 alternatives 7.3 and 4.3, without 4.6 and 2.3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -34,7 +34,7 @@ namespace npu {
 namespace {
 
 constexpr int LT = 256;      // lanes of a workgroup
-constexpr int LIST = 1024;   // entries that are ranked at once
+constexpr int LIST = 1024;   // entries that are ranked at once (a multiple of 16)
 constexpr int MAX_K = 32;
 constexpr int MAX_PARTS = LT;  // of a row: 129 at most with 8 runs a lane (2^20 f32)
 constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
@@ -106,13 +106,30 @@ __device__ __forceinline__ void finish(const TokenLogprobsArgs &a, long long row
   }
 }
 
-// The k smallest of n keys in LDS, in order, to `out`; called by all lanes of a workgroup.
-__device__ __forceinline__ void rank_keys(const u64 *list, int n, int k, u64 *out) {
+// How many of n keys in LDS are smaller; NO_KEY lies behind them up to a multiple of 16 (read one by
+// one, what a multiple leaves took most of the time).
+__device__ __forceinline__ int keys_below(const u64 *list, int n, u64 key) {
+  int ahead = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; j += 16) {
+    ulonglong2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const ulonglong2 *>(list + j + 2 * i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ahead += (int)(v[i].x < key) + (int)(v[i].y < key);
+  }
+  return ahead;
+}
+// The k smallest of n keys in LDS, in order, to `out`; called by all lanes of a workgroup.  (list's first
+// LT entries were NO_KEY before)
+__device__ __forceinline__ void rank_keys(u64 *list, int n, int k, u64 *out) {
+  if (n > LT) {
+    if (threadIdx.x < (-n & 15)) list[n + threadIdx.x] = NO_KEY;
+    __syncthreads();
+  }
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
     const u64 key = list[e];
-    int ahead = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) ahead += list[j] < key;
+    const int ahead = keys_below(list, n, key);
     if (ahead < k) out[ahead] = key;
   }
 }
@@ -120,7 +137,7 @@ __device__ __forceinline__ void rank_keys(const u64 *list, int n, int k, u64 *ou
 template <bool BF, int NCH>
 __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a, int parts) {
   constexpr int PER = BF ? 8 : 4, ES = BF ? 2 : 4, NW = LT / 64;
-  __shared__ u64 list[LIST];
+  __shared__ __attribute__((aligned(16))) u64 list[LIST];
   __shared__ u64 best[MAX_K];
   __shared__ float wave_a[NW], wave_b[NW];
   __shared__ int wave_c[NW];
@@ -162,6 +179,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   const int token = tok.token;
   const float xt = tok.x;
   if (tid == 0) n_list = 0;
+  if (a.k > 0) list[tid] = NO_KEY;
   auto get = [&](u32x4 u, int e) __attribute__((always_inline)) {
     return BF ? __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16) : __uint_as_float(u[e]);
   };
@@ -356,7 +374,8 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
 // most of the keys need not be ranked.
 __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsArgs a, int parts) {
   constexpr int NW = LT / 64;
-  __shared__ u64 heads[MAX_PARTS], list[MAX_K * MAX_K], best[MAX_K];
+  __shared__ __attribute__((aligned(16))) u64 heads[MAX_PARTS], list[MAX_K * MAX_K];
+  __shared__ u64 best[MAX_K];
   __shared__ float wave_m[NW], wave_s[NW], wave_w[NW];
   __shared__ int wave_b[NW];
   __shared__ u64 bound;
@@ -376,6 +395,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
   const int n_keys = parts * a.k, at0 = tid < n_keys ? tid / a.k : 0;
   const u64 key0 = tid < n_keys ? keys_of(part(at0))[tid - at0 * a.k] : NO_KEY;
   heads[tid] = head;
+  list[tid] = NO_KEY;
   if (tid < a.k) best[tid] = NO_KEY;
   if (tid == 0) n_list = 0, bound = NO_KEY;
   const float m = wave_max(p.m);
@@ -394,12 +414,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_join_kernel(TokenLogprobsAr
   S = wave_sum(S);
   W = wave_sum(W);
   if (lane == 0) wave_s[wave] = S, wave_w[wave] = W;
-  if (head != NO_KEY) {
-    int ahead = 0;
-#pragma unroll 4
-    for (int j = 0; j < n_heads; ++j) ahead += heads[j] < head;
-    if (ahead == a.k - 1) bound = head;
-  }
+  if (head != NO_KEY && keys_below(heads, n_heads, head) == a.k - 1) bound = head;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NW; ++w) out.S += wave_s[w], out.W += wave_w[w], out.before += wave_b[w];

@@ -500,6 +500,17 @@ def test_logprobs_of_hard_rows(cuda, dtype):
             _check_logprobs(x, tokens, k)
 
 
+@pytest.mark.parametrize("n", [15, 16, 17, 255, 256, 257, 300, 1000, 1024, 1025, 1500])
+def test_logprobs_of_many_equal_best(cuda, n):
+    """n entries of a part share the largest logit: as many candidates, past what is listed at once."""
+    x = torch.full((2, 4000), -1.0)
+    x[0, 7:7 + n] = 3.0
+    x[1, torch.randperm(4000, generator=torch.Generator().manual_seed(n))[:n]] = 3.0
+    for dtype in (F32, BF16):
+        for k in (1, 15, 32):
+            _check_logprobs(x.to(dtype).cuda(), [7 + n // 2, 3999], k)
+
+
 def test_logprobs_strides_streams_and_repeats(cuda):
     """Rows at odd addresses, strided alternatives, outputs left out; the same call gives the same
     bits."""
