@@ -2,11 +2,12 @@
 // weight's columns; and the residual's addition and norm with such an output.
 //
 //   quantise: x, or x g / (1 + exp(-g)), in blocks of 32 (mx_device.hpp);
-//   norm: h = bf16(x + delta), y = h / sqrt(mean(h^2) + eps) g, in blocks or bf16.
+//   norm: h = bf16(x + delta), y = h / sqrt(mean(h^2) + eps) g, in blocks or bf16; the sum and
+//   the root in 64 bits (whose range squares of bf16 do not leave), the entries in 32.
 //
 // Everything is read once and written once.  A lane takes eight entries (16 bytes of
 // bf16) and a quad a block, whose largest magnitude two DPP moves give.  The bytes bound
-// them all where rows are many: 4099 rows of 14336 gated bf16 to e4m3 58.8 us, 5.0 TB/s.
+// them all where rows are many: 4099 rows of 14336 gated bf16 to e4m3 59.9 us, 4.9 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -45,10 +46,27 @@ __device__ __forceinline__ float silu(float g) {
   return g < -87.0f ? 0.0f : g * __builtin_amdgcn_rcpf(1.0f + d);
 }
 
-// Eight entries of a block from a lane, the block's other three lanes beside it.
-template <int KIND>
-__device__ __forceinline__ void store_block(const float (&y)[8], uint8_t *q, uint8_t *scale, uint16_t *values) {
-  const uint32_t byte = scale_byte<KIND>(quad_max(magnitude(y)));
+// The same in 64 bits: exp(-g) = 2^n e^r, n = -g log2 e to the nearest, |r| < 0.347, by its Taylor
+// series to r^13 (what is left is below 2^-56).
+__device__ __forceinline__ double silu64(float gate) {
+  if (gate < -87.0f) return 0.0;
+  if (gate > 87.0f) return gate;
+  const double g = gate, n = rint(-g * 1.4426950408889634), r = fma(-n, 0.6931471805599453, -g) - n * 2.3190468138462996e-17;
+  double e = 1.0;
+#pragma unroll
+  for (int k = 13; k >= 1; --k) e = fma(e * (1.0 / k), r, 1.0);
+  return g / (1.0 + ldexp(e, (int)n));
+}
+
+// Eight entries of a block from a lane, the block's other three lanes beside it.  upper(): the
+// largest upper half of theirs in 64 bits (nullptr: they are exact).
+template <int KIND, class Upper>
+__device__ __forceinline__ void store_block(const float (&y)[8], Upper upper, uint8_t *q, uint8_t *scale, uint16_t *values) {
+  uint32_t mag = quad_max(magnitude(y));
+  if constexpr (!std::is_null_pointer_v<Upper>) {
+    if (next_to_power(mag)) mag = from_upper(quad_max(upper()));
+  }
+  const uint32_t byte = scale_byte<KIND>(mag);
   const float inv = inverse_scale(byte);
   const bool bad = byte == 255;
   float v[8];
@@ -86,8 +104,23 @@ __global__ __launch_bounds__(QT) void mx_quantize_kernel(MxQuantizeArgs a, Div31
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= silu(g[e]);
     }
-    store_block<KIND>(y, a.q + r * a.q_stride + (KIND == kToE4m3 ? k : k >> 1), a.scale + r * a.scale_stride + (k >> 5),
-                      a.values ? a.values + r * a.values_stride + k : nullptr);
+    auto store = [&](auto upper) __attribute__((always_inline)) {
+      store_block<KIND>(y, upper, a.q + r * a.q_stride + (KIND == kToE4m3 ? k : k >> 1), a.scale + r * a.scale_stride + (k >> 5),
+                        a.values ? a.values + r * a.values_stride + k : nullptr);
+    };
+    if constexpr (GATE) {
+      store([&]() __attribute__((always_inline)) {
+        uint32_t m = 0;
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const float x = bf16_to_f32(static_cast<const uint16_t *>(a.x)[r * a.x_stride + k + e]);
+          m = max(m, upper_magnitude(x * silu64(bf16_to_f32(a.gate[r * a.gate_stride + k + e]))));
+        }
+        return m;
+      });
+    } else {
+      store(nullptr);
+    }
   }
 }
 
@@ -199,17 +232,33 @@ __global__ __launch_bounds__(CT) void mx_quantize_columns_kernel(MxQuantizeArgs 
   }
 }
 
+__device__ __forceinline__ double wave_sum64(double v) {
+  auto moved = [&](auto ctrl) __attribute__((always_inline)) {
+    constexpr int C = decltype(ctrl)::value;
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), C, 0xf, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), C, 0xf, 0xf, false));
+  };
+  v += moved(std::integral_constant<int, 0xb1>{});   // lane ^ 1
+  v += moved(std::integral_constant<int, 0x4e>{});   // lane ^ 2
+  v += moved(std::integral_constant<int, 0x141>{});  // the other half of eight
+  v += moved(std::integral_constant<int, 0x140>{});  // of sixteen
+  auto of = [&](int l) __attribute__((always_inline)) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+  };
+  return ((of(0) + of(16)) + of(32)) + of(48);
+}
+
 // One row by LPR lanes, CH runs of eight entries a lane, so that the row stays in registers between
 // its sum and its scaling: 8191 rows of 4096 with h in and out and e4m3 46.9 us, 5.0 TB/s.
 template <int KIND, int LPR, int CH>
 __global__ __launch_bounds__(LPR < QT ? QT : LPR) void add_rmsnorm_kernel(AddRmsnormArgs a) {
   constexpr int WG = LPR < QT ? QT : LPR, ROWS = WG / LPR;
-  __shared__ float part[LPR > 64 ? LPR / 64 : 1];
+  __shared__ double part[LPR > 64 ? LPR / 64 : 1];
   const int t = threadIdx.x % LPR;
   const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / LPR;
   if (ROWS > 1 && row >= a.T) return;  // (whole waves, and no barrier below)
   float y[CH][8];
-  float sum = 0.0f;
+  double sum = 0.0;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int k = (c * LPR + t) * 8;
@@ -230,28 +279,42 @@ __global__ __launch_bounds__(LPR < QT ? QT : LPR) void add_rmsnorm_kernel(AddRms
     }
     if (a.h) *reinterpret_cast<u32x4 *>(a.h + row * a.h_stride + k) = u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(y[c][e], y[c][e], sum);
+    for (int e = 0; e < 8; ++e) sum = fma((double)y[c][e], (double)y[c][e], sum);
   }
-  sum = wave_sum(sum);
+  sum = wave_sum64(sum);
   if constexpr (LPR > 64) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
     __syncthreads();
-    sum = 0.0f;
+    sum = 0.0;
 #pragma unroll
     for (int w = 0; w < LPR / 64; ++w) sum += part[w];
   }
-  const float r = 1.0f / sqrtf(sum / (float)a.D + a.eps);
+  // 1 / sqrt, the instruction's 24 bits and two of Newton's steps (0 and Inf as they are)
+  const double mean = fma(sum, a.inv_D, (double)a.eps);
+  double root = __builtin_amdgcn_rsq(mean);
+  if (mean > 0.0 && mean < __builtin_inf()) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) root = root * fma(-0.5 * mean * root, root, 1.5);
+  }
+  const float r = (float)root;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int k = (c * LPR + t) * 8;
     if (k >= a.D) continue;
     const f32x4 g0 = *reinterpret_cast<const f32x4 *>(a.g + k), g1 = *reinterpret_cast<const f32x4 *>(a.g + k + 4);
+    float z[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[c][e] = y[c][e] * r * (e < 4 ? g0[e] : g1[e - 4]);
+    for (int e = 0; e < 8; ++e) z[e] = y[c][e] * r * (e < 4 ? g0[e] : g1[e - 4]);
     if constexpr (KIND == kToBf16) {
-      *reinterpret_cast<u32x4 *>(a.q + 2 * (row * a.q_stride + k)) = pack_bf16x8(y[c]);
+      *reinterpret_cast<u32x4 *>(a.q + 2 * (row * a.q_stride + k)) = pack_bf16x8(z);
     } else {
-      store_block<KIND>(y[c], a.q + row * a.q_stride + (KIND == kToE4m3 ? k : k >> 1),
+      auto upper = [&]() __attribute__((always_inline)) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, upper_magnitude(y[c][e] * root * (double)(e < 4 ? g0[e] : g1[e - 4])));
+        return m;
+      };
+      store_block<KIND>(z, upper, a.q + row * a.q_stride + (KIND == kToE4m3 ? k : k >> 1),
                         a.scale + row * a.scale_stride + (k >> 5), nullptr);
     }
   }

@@ -164,6 +164,7 @@ struct AddRmsnormArgs {
   long long x_stride, delta_stride, h_stride, q_stride, scale_stride;
   int T, D;
   float eps;
+  double inv_D;  // 1 / D
 };
 hipError_t launch_add_rmsnorm(const AddRmsnormArgs &a, hipStream_t s);
 struct MxMatmulArgs {

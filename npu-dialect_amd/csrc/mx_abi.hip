@@ -129,6 +129,7 @@ npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
   a.T = (int)T;
   a.D = (int)D;
   a.eps = eps;
+  a.inv_D = 1.0 / (double)D;
   return launched("fused_llama_add_rmsnorm launch",
                   [&] { return npu::launch_add_rmsnorm(a, static_cast<hipStream_t>(stream)); });
 }

@@ -20,6 +20,18 @@ __device__ __forceinline__ uint32_t magnitude(const float (&y)[N]) {
   return m;
 }
 
+// The scale takes a whole step where the largest magnitude passes a power of two.  Whether it does,
+// f32's roundings (together below 2^-20) decide next to one: there the entries count as they are
+// in 64 bits, by the upper halves of those (cut off, not rounded).
+__device__ __forceinline__ bool next_to_power(uint32_t mag) {
+  return ((mag + 8) & 0x7fffffu) < 16 && mag >= 0x00800000u && mag < 0x7f7ffff0u;
+}
+__device__ __forceinline__ uint32_t upper_magnitude(double y) { return (uint32_t)__double2hiint(y) & 0x7fffffffu; }
+// A magnitude of that exponent.
+__device__ __forceinline__ uint32_t from_upper(uint32_t upper) {
+  return (uint32_t)min(max((int)(upper >> 20) - (1023 - 127), 0), 254) << 23;
+}
+
 // The scale of a block whose largest magnitude has these bits: its exponent (that of
 // subnormals counts as the least) less the largest element's, 8 (448 = 1.75 2^8) or 2
 // (6 = 1.5 2^2), at least 2^-127.

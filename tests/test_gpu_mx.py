@@ -131,6 +131,31 @@ def test_quantize_gated(cuda, R_, K, kind):
     R.check_near(q, s, _np64(x) * R.silu64(_np64(gate)), SILU_EPS, kind)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+def test_quantize_gated_next_to_powers_of_two(cuda, kind):
+    """Products that lie within f32's roundings of a power of two, where the scale takes a step: it is
+    that of the formula in 64 bits."""
+    from npu_amd import groups
+    gate = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF16)
+    g64 = _np64(gate)
+    silu = R.silu64(np.where(np.isfinite(g64) & (np.abs(g64) > 1e-20) & (g64 > -60) & (g64 < 1e30), g64, 0.0))
+    pairs = []
+    for m in range(128):
+        x = 1.0 + m / 128
+        frac = np.frexp(np.abs(x * silu))[0]  # [1/2, 1): next to either end is next to a power of two
+        near = (silu != 0) & ((frac - 0.5 < 2.0 ** -21) | (1.0 - frac < 2.0 ** -21)) & (frac != 0.5)
+        pairs += [(x, i) for i in np.nonzero(near)[0]]
+    assert len(pairs) >= 8
+    xs = torch.zeros((len(pairs), 32))
+    gs = torch.zeros((len(pairs), 32), dtype=BF16)
+    for row, (x, i) in enumerate(pairs):
+        xs[row, row % 32], gs[row, row % 32] = x, gate[i]
+    q, s = _mx(len(pairs), 32, kind)
+    groups.fused_mx_quantize(xs.to(BF16).cuda(), q, s, gate=gs.cuda())
+    c, sc = R.quantize(xs.double().numpy() * np.where(xs.numpy() != 0, R.silu64(_np64(gs)), 0.0), kind)
+    assert np.array_equal(s.cpu().numpy(), sc)
+
+
 def test_quantize_gates_far_out(cuda):
     """Gates of any size: large ones pass, very negative ones close, NaN and +Inf make their
     block NaN."""
@@ -176,10 +201,9 @@ def test_quantize_strides_and_streams(cuda, kind):
 
 
 # ---- norm ------------------------------------------------------------------------------
-# The mean's f32 sum: 32 terms of a lane in turn, six steps over lanes, up to 16 waves, the
-# squares' own rounding and the division, (32 + 6 + 16 + 2) 2^-24 of it and half of that of its
-# root; root, reciprocal and two products 2^-24 (and 2^-23 for each of the first two)
-NORM_EPS = (56 / 2 + 6) * 2.0 ** -24
+# The mean and its root's reciprocal are in 64 bits; the latter's rounding to f32 and two products,
+# 2^-24 each, and what these roundings make of each other
+NORM_EPS = 3.01 * 2.0 ** -24
 
 
 def _check_norm(x, g, kind, delta=None, h="new", eps=1e-5, stream=None):
@@ -237,6 +261,35 @@ def test_norm_in_place_strided_and_zero(cuda):
     q, s = _check_norm(torch.zeros((2, 160), dtype=BF16, device="cuda"), g, "e4m3")
     assert not s.any() and not q.view(U8).any()
     _check_norm(torch.full((1, 160), 2.0 ** -60, dtype=BF16, device="cuda"), g, "bf16", eps=0.0)
+
+
+@pytest.mark.parametrize("T,D", [(64, 96), (40, 2080), (30, 4096), (6, 16416)])
+def test_norm_next_to_powers_of_two(cuda, T, D):
+    """Gains that put each block's largest entry within 2^-24 of a power of two: the scale is that of the
+    formula in 64 bits, its roundings (2^-51 or so) far below the distances there are."""
+    from npu_amd import groups
+    for row in range(0, T, max(1, T // 6)):
+        x = _rnd(1, D, seed=row).to(BF16)
+        hd = _np64(x)
+        y = hd / np.sqrt((hd * hd).mean(1, keepdims=True) + 1e-5)
+        b = np.abs(y).reshape(-1, 32)
+        g = np.full(b.shape, 2.0 ** -6)
+        top = b.argmax(1)
+        at = np.arange(len(b)), top
+        g[at] = 2.0 ** (np.arange(len(b)) % 5) / b[at]
+        g = torch.from_numpy(g.reshape(-1)).float()
+        y = (y * g.double().numpy()).reshape(1, D)
+        for kind in ("e4m3", "e2m1"):
+            q, s = _mx(1, D, kind)
+            groups.fused_llama_add_rmsnorm(x.cuda(), g.cuda(), q, s, eps=1e-5)
+            assert np.array_equal(s.cpu().numpy(), R.quantize(y, kind)[1])
+
+
+def test_norm_of_huge_and_tiny_rows(cuda):
+    """Squares outside f32's range: the mean is in 64 bits."""
+    g = torch.ones(512, device="cuda")
+    for size in (2.0 ** 120, 2.0 ** 70, 2.0 ** -70, 2.0 ** -120):
+        _check_norm((_rnd(3, 512, seed=4) * size).to(BF16).cuda(), g, "e4m3", eps=0.0)
 
 
 def test_norm_not_finite(cuda):
