@@ -376,7 +376,7 @@ int64_t npu_token_logprobs_workspace(int64_t T, int64_t V, int32_t k);
  * The conventions of the serving entry points hold: operands that may be
  * absent, rows at any stride that keeps them 16-byte aligned (scales: any
  * stride).  Every operand holds fewer than 2^34 entries. */
-/* x (with gate: x silu(gate), silu(z) = z / (1 + exp(-z)), in f32) to blocks.  Here and below a
+/* x (with gate: x silu(gate), silu(z) = z / (1 + exp(-z)), in f32) to blocks.  A
  * block's scale is that of the formula in 64 bits, also where f32's roundings would pass a power of two.
  *   x bf16 or f32 [R, K]; gate bf16 [R, K] where x is bf16, may be absent;
  *   q e4m3 or e2m1, scale; values bf16 [R, K], may be absent: what q and scale
@@ -386,8 +386,8 @@ int64_t npu_token_logprobs_workspace(int64_t T, int64_t V, int32_t k);
 npu_status fused_mx_quantize(const npu_memref *x, const npu_memref *gate, const npu_memref *q,
                              const npu_memref *scale, const npu_memref *values,
                              npu_stream stream);
-/* h = bf16(x + delta); q = h / sqrt(mean(h^2) + eps) * g, the mean and its root in 64 bits, the rest
- * in f32, to blocks or to bf16.
+/* h = bf16(x + delta); q = h / sqrt(mean(h^2) + eps) * g to blocks or to bf16, rounded once: known to
+ * some 2^-45 before.
  *   x, delta, h bf16 [T, D], T <= 2^23, D <= 32768 a multiple of 32; g f32 [D]; q e4m3 or
  *   e2m1 with scale, or bf16 [T, D] without; delta may be absent (h = x), and h
  *   may be absent, or x, or delta. */
