@@ -256,9 +256,9 @@ __device__ __forceinline__ float scaled(float h, float r, float rest, float g) {
   const float p = h * r, p_rest = fmaf(h, rest, fmaf(h, r, -p)), pg = p * g, pg_rest = fmaf(p_rest, g, fmaf(p, g, -pg));
   const float z = pg + pg_rest, z_rest = pg_rest - (z - pg);
   const uint32_t bits = __float_as_uint(z);
-  const uint32_t step = (uint32_t)((int)(bits ^ __float_as_uint(z_rest)) >> 31) | 1u;  // away from 0, or towards it
-  const uint32_t odd = z_rest != 0.0f && !(bits & 1u) ? bits + step : bits;
-  return fabsf(pg_rest) < fabsf(pg) ? __uint_as_float(odd) : pg;  // (0, Inf, NaN)
+  const uint32_t odd = (bits + (uint32_t)((int)(bits ^ __float_as_uint(z_rest)) >> 31)) | 1u;  // (cut off, and what was cut)
+  const uint32_t out = z_rest != 0.0f ? odd : bits;
+  return fabsf(pg_rest) < fabsf(pg) ? __uint_as_float(out) : pg;  // (0, Inf, NaN)
 }
 
 // One row by LPR lanes, CH runs of eight entries a lane, so that the row stays in registers between
