@@ -922,3 +922,21 @@ def test_serving_with_alternatives_and_scores(cuda, mx, prefix):
     with pytest.raises(ValueError, match="0 rows"):
         s.score([1, 2], rows=0)
     assert s.score([7])[0].numel() == 0
+
+
+def test_server_without_alternatives_and_refusals(cuda):
+    """alternatives=0: log probabilities alone; too many and weights that are no whole blocks are refused."""
+    from npu_amd import serving
+    model = serving.random_model(1, 128, 2, 192, 320, seed=3)
+    s = serving.Server(*serving.quantize_model(*model), n_heads=2, slots=2, pages=8, page=16, max_pages=4, alternatives=0)
+    s.add(1, [3, 4, 5], temperature=0.0)
+    s.u.fill_(0.5)
+    s.prefill()
+    s.step()
+    lp, entropy, rank, _, _ = R.logprobs64(s.logits[1].cpu().double().numpy(), s.tokens[1].item(), 1)
+    assert s.top_tokens is None and s.ranks[1].item() == rank == 0
+    assert abs(s.logprobs[1].item() - lp) <= 2.0 ** -17 * (1 + abs(lp)) and abs(s.entropy[1].item() - entropy) <= 2.0 ** -14
+    with pytest.raises(ValueError, match="33 alternatives"):
+        serving.Server(*model, n_heads=2, slots=2, pages=8, page=16, max_pages=4, alternatives=33)
+    with pytest.raises(Exception, match="multiple of 32"):
+        serving.mx_weight(torch.zeros((48, 64), dtype=BF16, device="cuda"))
