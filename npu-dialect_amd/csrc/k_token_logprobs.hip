@@ -8,7 +8,9 @@
 // in registers (NCH runs of 16 bytes a lane), so that the maximum is known before the
 // sums begin and an entry costs one exponential; a second kernel joins the parts where a row
 // has several.  The exponent d is one fma, x log2 e - c, c = m log2 e rounded; what c's rounding
-// left, the same for all entries, is taken off the sums' logarithm at the end.
+// left, the same for all entries, is taken off the sums' logarithm at the end.  It grows with m
+// (2^-4 at 1e6, past the exponential's range from 2e9 on): from 1e6 on, which only masked rows and
+// parts reach, d is (x - m) log2 e (2000 rows of 128000 all but masked at -1e30: 116 us, others 103).
 //
 // The k best: at least k of 64 groups of lanes have a maximum that is no less than the k-th largest
 // of theirs, so that the part's k best are among the entries that reach it: little more
@@ -229,8 +231,7 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
     if (lane == 0) bound = found;
   }
   // sums, the rank, the list
-  // (next to f32's ends the fma's terms overflow: those rows are summed from x - m below)
-  const bool far = !(fabsf(m) < 1e37f);
+  const bool far = !(fabsf(m) < 1e6f);  // summed from x - m below
   const float c = far ? 0.0f : m * LOG2E, rest = far ? 0.0f : fmaf(m, LOG2E, -c);
   const float at_before = xt > -inf ? below(xt) : -inf;
   float S = 0.0f, W = 0.0f;
@@ -310,12 +311,23 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   }
   if (far) {
     S = W = 0.0f;
-    if (m > -inf)
-      again([&](float x, int) {
-        const float d = x == m ? 0.0f : fmaxf((x - m) * LOG2E, -1000.0f), w = __builtin_amdgcn_exp2f(d);
-        S += w;
-        W = fmaf(w, d, W);
-      });
+    auto add_far = [&](float x) __attribute__((always_inline)) {
+      const float d = x == m ? 0.0f : fmaxf((x - m) * LOG2E, -1000.0f), w = __builtin_amdgcn_exp2f(d);
+      S += w;
+      W = fmaf(w, d, W);
+    };
+    if (m > -inf) {  // (a run at a time: all at once cost every other row 2 %)
+#pragma unroll 1
+      for (int at = 0; at < NCH; ++at) {
+        u32x4 u = v[0];
+#pragma unroll
+        for (int i = 1; i < NCH; ++i)
+          if (at == i) u = v[i];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) add_far(get(u, e));
+      }
+      add_far(edge);
+    }
   }
   S = wave_sum(S);
   W = wave_sum(W);
