@@ -20,6 +20,7 @@
 #include <cstring>
 
 #include "kernels.hpp"
+#include "mx_columns.hpp"
 #include "mx_device.hpp"
 #include "plans.hpp"
 
@@ -120,14 +121,18 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
   extern __shared__ f32x4 sums[];  // [SW][MT NT][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int bn = blockIdx.x / groups_m, bm = blockIdx.x - bn * groups_m;
-  // (the last group of n begins earlier where N is no multiple: it has whole tiles, and computes some again)
-  const long long n0 = min((long long)bn * (16 * NT), max(0LL, (long long)a.N - 16 * NT)), m0 = (long long)bm * (16 * MT);
+  const FewColumns columns(bn, NT, a.N);
+  const long long n0 = columns.n0, m0 = (long long)bm * (16 * MT);
   const int blocks = a.K / 32, s0 = (blockIdx.y * SW + wave) * per_wave, s1 = min(steps, s0 + per_wave);
   // Rows past the last: its own again, not stored.  (offsets fit 32 bits: strides are below 2^23)
   const uint8_t *w = a.w + n0 * a.w_stride, *ws = a.w_scale + n0 * a.ws_stride, *x = a.a + m0 * a.a_stride, *xs = a.a_scale + m0 * a.as_stride;
-  const int w_row = (int)min((long long)r, a.N - 1 - n0);  // (below r for N < 16 alone, of which NT is 1)
-  const uint32_t w_at = (uint32_t)w_row * (uint32_t)a.w_stride, ws_at = (uint32_t)w_row * (uint32_t)a.ws_stride;
-  uint32_t x_at[MT], xs_at[MT];
+  uint32_t w_at[NT], ws_at[NT], x_at[MT], xs_at[MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = columns.row(t, r);
+    w_at[t] = (uint32_t)row * (uint32_t)a.w_stride;
+    ws_at[t] = (uint32_t)row * (uint32_t)a.ws_stride;
+  }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int row = (int)min((long long)(16 * t + r), a.M - 1 - m0);
@@ -164,12 +169,12 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
     if (blocks >= 4) {
       const ScaleWord word(b, blocks);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) was[t] = word.of(ws + t * 16 * a.ws_stride + ws_at);
+      for (int t = 0; t < NT; ++t) was[t] = word.of(ws + ws_at[t]);
 #pragma unroll
       for (int t = 0; t < MT; ++t) xas[t] = word.of(xs + xs_at[t]);
     } else {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) was[t] = scale_bytes(ws + t * 16 * a.ws_stride + ws_at, b, blocks);
+      for (int t = 0; t < NT; ++t) was[t] = scale_bytes(ws + ws_at[t], b, blocks);
 #pragma unroll
       for (int t = 0; t < MT; ++t) xas[t] = scale_bytes(xs + xs_at[t], b, blocks);
     }
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
     auto load_w = [&](auto j) __attribute__((always_inline)) {
       constexpr int J = decltype(j)::value;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) load_line(w + t * 16 * a.w_stride, w_at, 64 * (s + J), a.K / 2, w_odd, wv[J][t], wv[J + 1][t]);
+      for (int t = 0; t < NT; ++t) load_line(w, w_at[t], 64 * (s + J), a.K / 2, w_odd, wv[J][t], wv[J + 1][t]);
     };
     auto load_a = [&](auto j) __attribute__((always_inline)) {
       constexpr int J = decltype(j)::value, AT = E4M3 ? 2 * (J & 1) : J;
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(SW * 64, NT *MT >= 3 ? 2 : 4) void mx_matmul_few_ke
     f32x4 v = sums[it * 64 + lane];
 #pragma unroll
     for (int q = 1; q < SW; ++q) v += sums[(q * (MT * NT) + it) * 64 + lane];
-    put(a, parts, m0 + 16 * (it / NT) + r, n0 + 16 * (it % NT) + 4 * g, v);
+    put(a, parts, m0 + 16 * (it / NT) + r, columns.first(it % NT, g), v);
   }
 }
 
