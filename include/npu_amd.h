@@ -376,8 +376,9 @@ int64_t npu_token_logprobs_workspace(int64_t T, int64_t V, int32_t k);
  * The conventions of the serving entry points hold: operands that may be
  * absent, rows at any stride that keeps them 16-byte aligned (scales: any
  * stride).  Every operand holds fewer than 2^34 entries. */
-/* x (with gate: x silu(gate), silu(z) = z / (1 + exp(-z)), in f32) to blocks.  A
- * block's scale is that of the formula in 64 bits, also where f32's roundings would pass a power of two.
+/* x (with gate: x silu(gate), silu(z) = z / (1 + exp(-z)), 0 for a gate of -Inf; in f32, past whose
+ * largest number an entry is Inf) to blocks.  A block's scale is that of the formula in 64 bits, also
+ * where f32's roundings would pass a power of two, or a gate closes so far that silu leaves f32's range.
  *   x bf16 or f32 [R, K]; gate bf16 [R, K] where x is bf16, may be absent;
  *   q e4m3 or e2m1, scale; values bf16 [R, K], may be absent: what q and scale
  *   stand for.

@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_mx import BF16, F32, _check_logprobs
+import mx_refs as R
+from test_gpu_mx import BF16, F32, SILU_EPS, _check_logprobs, _mx, _np64, _rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,51 @@ def test_logprobs_of_rows_about_a_far_value(cuda, m):
 
 def _spread(rows, cols, seed):
     return torch.randn((rows, cols), generator=torch.Generator().manual_seed(seed)) * 2
+
+
+# ---- gates that close --------------------------------------------------------------------
+def _check_gated(x, gate, kind):
+    """Scales those of the formula in 64 bits; elements within half a step, silu's error and f32's least
+    step (2^-150, which the least scale makes 2^-23)."""
+    from npu_amd import groups
+    q, s = _mx(*x.shape, kind)
+    groups.fused_mx_quantize(x.cuda(), q, s, gate=gate.cuda())
+    g = _np64(gate)
+    y = _np64(x) * np.where(np.isneginf(g), 0.0, R.silu64(np.where(np.isneginf(g), 0.0, g)))
+    mag = np.abs(y.reshape(len(y), -1, 32)).max(2)
+    sc = R.scale_of(mag, kind)
+    assert np.array_equal(s.cpu().numpy(), sc), np.argwhere(s.cpu().numpy() != sc)[:5].tolist()
+    most = R.TABLE[kind][7 if kind == "e2m1" else 126]
+    t = np.clip(y * np.repeat(np.ldexp(1.0, 127 - sc), 32, 1), -most, most)
+    err = np.abs(np.array(R.TABLE[kind])[R.codes(q, kind)] - t)
+    assert (err <= R.half_step(t * (1 + SILU_EPS), kind) + SILU_EPS * np.abs(t) + 2.0 ** -23).all()
+    return q, s
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 20, 2.0 ** 100, 1.9 * 2.0 ** 126])
+def test_quantize_gates_that_close(cuda, size, kind):
+    """Each gate from -80 to -280, alone in a block of zeros and beside others like it, by x of any size."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(BF16)
+    gates = bits[(bits <= -80) & (bits >= -280)]
+    n = len(gates)
+    assert n > 200
+    gate = torch.zeros((n, 64), dtype=BF16)
+    rows = torch.arange(n)
+    gate[rows, rows % 32] = gates
+    gate[:, 32:] = gates[(rows[:, None] + torch.arange(32)) % n]
+    x = torch.zeros((n, 64))
+    x[:, :32] = size
+    x[:, 32:] = size * (1 + torch.rand((n, 32), generator=torch.Generator().manual_seed(3)) * 0.05)
+    _check_gated(x.to(BF16), gate, kind)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+def test_quantize_gates_of_all_sizes_together(cuda, kind):
+    """Rows whose lanes take either form, x of sizes over all exponents; -Inf and the type's lowest value close."""
+    x = _rnd(301, 416, seed=7) * 2.0 ** torch.randint(-60, 124, (301, 416), generator=torch.Generator().manual_seed(8))
+    gate = (_rnd(301, 416, seed=9) * 60).clamp(max=8)
+    gate[::3] = _rnd(101, 416, seed=10)
+    gate[5, ::2], gate[6], gate[7, 40:60] = -math.inf, -math.inf, float(torch.finfo(BF16).min)
+    q, s = _check_gated(x.to(BF16), gate.to(BF16), kind)
+    assert not s[6].any() and (R.values(q, s, kind)[6] == 0).all()
