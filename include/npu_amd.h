@@ -388,7 +388,7 @@ npu_status fused_mx_quantize(const npu_memref *x, const npu_memref *gate, const 
                              const npu_memref *scale, const npu_memref *values,
                              npu_stream stream);
 /* h = bf16(x + delta); q = h / sqrt(mean(h^2) + eps) * g to blocks or to bf16, rounded once: known to
- * some 2^-45 before.
+ * some 2^-50 before, rows of subnormals among them; past f32's largest number it is Inf.
  *   x, delta, h bf16 [T, D], T <= 2^23, D <= 32768 a multiple of 32; g f32 [D]; q e4m3 or
  *   e2m1 with scale, or bf16 [T, D] without; delta may be absent (h = x), and h
  *   may be absent, or x, or delta. */

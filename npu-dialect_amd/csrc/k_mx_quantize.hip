@@ -2,8 +2,8 @@
 // weight's columns; and the residual's addition and norm with such an output.
 //
 //   quantise: x, or x g / (1 + exp(-g)), in blocks of 32 (mx_device.hpp);
-//   norm: h = bf16(x + delta), y = h / sqrt(mean(h^2) + eps) g, in blocks or bf16; the sum and
-//   the root in 64 bits (whose range squares of bf16 do not leave), the entries in pairs of 32.
+//   norm: h = bf16(x + delta), y = h / sqrt(mean(h^2) + eps) g, in blocks or bf16; the sum,
+//   the root and the entries in 64 bits (whose range squares of bf16 and their roots do not leave).
 //
 // Everything is read once and written once.  A lane takes eight entries (16 bytes of
 // bf16) and a quad a block, whose largest magnitude two DPP moves give.  The bytes bound
@@ -258,22 +258,21 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return ((of(0) + of(16)) + of(32)) + of(48);
 }
 
-// h (r + rest) g, rounded to odd: where it is no f32, that neighbour whose last bit is set, so that a
-// further rounding to fewer bits gives what it would give of the exact value.  What the two
-// products leave of it is known to some 2^-45 of it.
-__device__ __forceinline__ float scaled(float h, float r, float rest, float g) {
-#pragma clang fp contract(off)
-  const float p = h * r, p_rest = fmaf(h, rest, fmaf(h, r, -p)), pg = p * g, pg_rest = fmaf(p_rest, g, fmaf(p, g, -pg));
-  const float z = pg + pg_rest, z_rest = pg_rest - (z - pg);
-  const uint32_t bits = __float_as_uint(z);
-  const uint32_t odd = (bits + (uint32_t)((int)(bits ^ __float_as_uint(z_rest)) >> 31)) | 1u;  // (cut off, and what was cut)
-  const uint32_t out = z_rest != 0.0f ? odd : bits;
-  return fabsf(pg_rest) < fabsf(pg) ? __uint_as_float(out) : pg;  // (0, Inf, NaN)
+// h root g, rounded to odd: where it is no f32, that neighbour whose last bit is set, so that a
+// further rounding to fewer bits gives what it would give of the exact value.  The products in 64 bits
+// are off by some 2^-51 of it whatever the sizes of h, root and g; above f32's largest it is Inf.
+__device__ __forceinline__ float scaled(float h, double root, float g) {
+  const double y = (double)h * root * (double)g;
+  const float z = (float)y;
+  const double back = (double)z;
+  const uint32_t cut = __float_as_uint(z) - (fabs(back) > fabs(y) ? 1u : 0u);
+  return back == y || fabsf(z) == __builtin_inff() ? z : __uint_as_float(cut | 1u);
 }
 
 // One row by LPR lanes, CH runs of eight entries a lane, so that the row stays in registers between
-// its sum and its scaling: 8191 rows of 4096 with h in and out and e4m3 48.2 us, 4.9 TB/s (46.8 with all in
-// f32, and then now and then an element or a block's scale that is not the formula's).
+// its sum and its scaling: 8191 rows of 4096 with h in and out and e4m3 48.6 us, 4.8 TB/s (46.8 with all in
+// f32, and then now and then an element or a block's scale that is not the formula's; 48.2 with the entries in
+// pairs of f32, which the ends of its range leave without their second half).
 template <int KIND, int LPR, int CH>
 __global__ __launch_bounds__(LPR < QT ? QT : LPR) void add_rmsnorm_kernel(AddRmsnormArgs a) {
   constexpr int WG = LPR < QT ? QT : LPR, ROWS = WG / LPR;
@@ -320,7 +319,6 @@ __global__ __launch_bounds__(LPR < QT ? QT : LPR) void add_rmsnorm_kernel(AddRms
 #pragma unroll
     for (int i = 0; i < 2; ++i) root = root * fma(-0.5 * mean * root, root, 1.5);
   }
-  const float r = (float)root, r_rest = (float)(root - r);
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int k = (c * LPR + t) * 8;
@@ -328,7 +326,7 @@ __global__ __launch_bounds__(LPR < QT ? QT : LPR) void add_rmsnorm_kernel(AddRms
     const f32x4 g0 = *reinterpret_cast<const f32x4 *>(a.g + k), g1 = *reinterpret_cast<const f32x4 *>(a.g + k + 4);
     float z[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = scaled(y[c][e], r, r_rest, e < 4 ? g0[e] : g1[e - 4]);
+    for (int e = 0; e < 8; ++e) z[e] = scaled(y[c][e], root, e < 4 ? g0[e] : g1[e - 4]);
     if constexpr (KIND == kToBf16) {
       *reinterpret_cast<u32x4 *>(a.q + 2 * (row * a.q_stride + k)) = pack_bf16x8(z);
     } else {

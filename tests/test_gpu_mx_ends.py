@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mx_refs as R
-from test_gpu_mx import BF16, F32, SILU_EPS, _check_logprobs, _mx, _np64, _rnd
+from test_gpu_mx import BF16, F32, SILU_EPS, _check_logprobs, _check_norm, _mx, _np64, _rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -103,3 +103,52 @@ def test_quantize_gates_of_all_sizes_together(cuda, kind):
     gate[5, ::2], gate[6], gate[7, 40:60] = -math.inf, -math.inf, float(torch.finfo(BF16).min)
     q, s = _check_gated(x.to(BF16), gate.to(BF16), kind)
     assert not s[6].any() and (R.values(q, s, kind)[6] == 0).all()
+
+
+# ---- rows of the norm at bf16's ends --------------------------------------------------------
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1", "bf16"])
+@pytest.mark.parametrize("power", [-133, -130, -127, -126, -124, -110, 104, 112, 120, 123])
+def test_norm_of_rows_of_any_size(cuda, power, kind):
+    """Rows of subnormals, whose root f32 does not hold, and of the largest numbers: blocks are those of the
+    formula in 64 bits, eps = 0 or not."""
+    x = (_rnd(40, 544, seed=power).clamp(-8, 8) * 2.0 ** power).to(BF16).cuda()
+    assert torch.isfinite(x).all() and x.any(1).all()
+    g = (torch.rand(544, generator=torch.Generator().manual_seed(power)) + 0.5).cuda()
+    _check_norm(x, g, kind, eps=0.0)
+    _check_norm(x, g, kind, eps=1e-30)
+    _check_norm(x, g, kind, delta=(x.float() * 0.5).to(BF16))
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("power", [0, 100, 120, -100, -120])
+def test_norm_of_wide_rows_and_gains(cuda, power, kind):
+    """Rows with entries of all exponents, gains from 2^-140 to 2^118: entries down to f32's least."""
+    g = torch.Generator().manual_seed(power)
+    x = _rnd(20, 4096, seed=power) * 2.0 ** torch.randint(-100, 1, (20, 4096), generator=g) * 2.0 ** min(power, 123)
+    gain = (torch.rand(4096, generator=g) + 0.5) * 2.0 ** torch.randint(-140, 118, (4096 // 32,), generator=g).repeat_interleave(32)
+    _check_norm(x.to(BF16).cuda(), gain.cuda(), kind, eps=0.0)
+
+
+def test_norm_next_to_ties_of_huge_rows(cuda):
+    """Gains that put entries within 2^-23 of half way between two elements, in rows of 2^120: the side on
+    which 64 bits have them."""
+    from npu_amd import groups
+    x = (_rnd(1, 2048, seed=11) * 2.0 ** 120).to(BF16)
+    h = _np64(x)
+    y = h / np.sqrt((h * h).mean(1, keepdims=True))
+    want = np.abs(y).reshape(-1, 32)
+    code = np.random.default_rng(1).integers(8, 120, want.shape)  # (normal elements)
+    tie = (np.array(R.E4M3)[code] + np.array(R.E4M3)[code + 1]) / 2
+    tie[:, 0] = 256.0  # each block's largest, whatever the others': its scale is 1
+    tie[:, 1:] = np.minimum(tie[:, 1:], 248.0)
+    g = torch.from_numpy((tie / np.maximum(want, 2.0 ** -20)).reshape(-1)).float()
+    g[h[0] == 0] = 1.0
+    q, s = _mx(1, 2048, "e4m3")
+    groups.fused_llama_add_rmsnorm(x.cuda(), g.cuda(), q, s, eps=0.0)
+    y = y * g.double().numpy()
+    c, sc = R.quantize(y, "e4m3")
+    # (f64's own roundings, 2^-51 or so, decide where a gain gives a tie to that)
+    t = np.abs(y / np.repeat(np.ldexp(1.0, sc - 127), 32, 1))
+    sure = np.abs(t - tie.reshape(1, -1)) > 2.0 ** -49 * t
+    assert sure.mean() > 0.9 and np.array_equal(s.cpu().numpy(), sc)
+    assert np.array_equal(R.codes(q, "e4m3")[sure], c[sure])
