@@ -14,6 +14,14 @@
 
 namespace {
 
+// The code of a type that an older torch does not name, by what this one calls it; -1: none.
+int32_t newer_dtype(at::ScalarType type) {
+  const char *name = c10::toString(type);
+  if (!std::strcmp(name, "Float8_e4m3fn")) return NPU_E4M3;
+  if (!std::strcmp(name, "Float8_e8m0fnu") || !std::strcmp(name, "Float4_e2m1fn_x2")) return NPU_U8;
+  return -1;
+}
+
 // Descriptor of a tensor on the GPU (None: an operand that is not present, where
 // that is allowed).  False with a Python error set.
 bool describe(PyObject *o, const char *name, bool optional, npu_memref *m) {
@@ -36,11 +44,12 @@ bool describe(PyObject *o, const char *name, bool optional, npu_memref *m) {
     case at::kBFloat16: m->dtype = NPU_BF16; break;
     case at::kChar: m->dtype = NPU_I8; break;
     case at::kInt: m->dtype = NPU_I32; break;
-    case at::kByte:
-    case at::kFloat8_e8m0fnu:
-    case at::kFloat4_e2m1fn_x2: m->dtype = NPU_U8; break;
-    case at::kFloat8_e4m3fn: m->dtype = NPU_E4M3; break;
-    default: PyErr_Format(PyExc_TypeError, "%s: unsupported tensor dtype %s", name, c10::toString(t.scalar_type())); return false;
+    case at::kByte: m->dtype = NPU_U8; break;
+    default:
+      m->dtype = newer_dtype(t.scalar_type());
+      if (m->dtype >= 0) break;
+      PyErr_Format(PyExc_TypeError, "%s: unsupported tensor dtype %s", name, c10::toString(t.scalar_type()));
+      return false;
   }
   if (t.dim() > NPU_MAX_RANK) {
     PyErr_Format(PyExc_ValueError, "%s: npu_memref holds at most rank %d", name, NPU_MAX_RANK);

@@ -16,8 +16,11 @@ def _codes():
     if _DTYPE_CODES is None:
         import torch
         _DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8,
-                        torch.int32: I32, torch.uint8: U8, torch.float8_e8m0fnu: U8,
-                        torch.float4_e2m1fn_x2: U8, torch.float8_e4m3fn: E4M3}
+                        torch.int32: I32, torch.uint8: U8}
+        # (an older torch lacks some of these)
+        for name, code in (("float8_e8m0fnu", U8), ("float4_e2m1fn_x2", U8), ("float8_e4m3fn", E4M3)):
+            if hasattr(torch, name):
+                _DTYPE_CODES[getattr(torch, name)] = code
     return _DTYPE_CODES
 
 
