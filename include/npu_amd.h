@@ -400,9 +400,10 @@ npu_status fused_llama_add_rmsnorm(const npu_memref *x, const npu_memref *delta,
  *   below 2^23 bytes; out bf16 [M, N], M and N up to 2^23, fewer than 2^32 entries, rows at any
  *   stride; workspace f32 [n], n >= npu_mx_matmul_workspace:
  *   scratch that only this call uses while it runs.
- * Products and sums on the scaled matrix instructions: f32 sums in a fixed order, whose
- * terms of 128 k with e4m3 the instruction aligns to the largest (error up
- * to 2^-12 of the terms' magnitudes, 2e-5 of a result of usual rows); one rounding. */
+ * Products and sums on the scaled matrix instructions: f32 sums in a fixed order; one rounding.
+ * With e4m3 the instruction aligns the terms of each eight neighbouring k (from a multiple of 8 on) to
+ * the largest of the eight and cuts off what is less than 2^-13 of it: an error of up to 7 2^-13 of that
+ * term, below 2^-10 of the terms' magnitudes, and 2e-5 of a result of usual rows. */
 npu_status fused_mx_matmul(const npu_memref *a, const npu_memref *a_scale, const npu_memref *w,
                            const npu_memref *w_scale, const npu_memref *out,
                            const npu_memref *workspace, npu_stream stream);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mx_refs as R
-from test_gpu_mx import BF16, F32, SILU_EPS, _check_logprobs, _check_norm, _mx, _np64, _rnd
+from test_gpu_mx import BF16, BF16_HALF_STEP, F32, SILU_EPS, _check_logprobs, _check_norm, _mx, _np64, _product, _rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,56 @@ def test_norm_next_to_ties_of_huge_rows(cuda):
     sure = np.abs(t - tie.reshape(1, -1)) > 2.0 ** -49 * t
     assert sure.mean() > 0.9 and np.array_equal(s.cpu().numpy(), sc)
     assert np.array_equal(R.codes(q, "e4m3")[sure], c[sure])
+
+
+# ---- products of terms far apart -------------------------------------------------------------
+def _check_far_terms(a, sa, w, sw, kind):
+    """A result is off by its rounding to bf16; by the f32 sums' roundings, one for each eight k and each wave or
+    part (64 at most); and with e4m3 by what the instruction cuts off: of each eight neighbouring k
+    less than 2^-13 of the largest term from each of the seven others."""
+    got = _np64(_product(a, sa, w, sw))
+    A, W = R.values(a, sa, kind), R.values(w, sw, "e2m1")
+    exact, mag, cut = A @ W.T, np.abs(A) @ np.abs(W).T, 0.0
+    if kind == "e4m3":
+        for k in range(0, A.shape[1], 8):
+            cut = cut + np.abs(A[:, None, k:k + 8] * W[None, :, k:k + 8]).max(2)
+    off = (A.shape[1] / 8 + 64) * 2.0 ** -24 * mag + 7 * 2.0 ** -13 * cut
+    bad = np.abs(got - exact) > BF16_HALF_STEP * np.abs(exact) + (1 + BF16_HALF_STEP) * off
+    assert not bad.any(), f"{bad.sum()} of {bad.size} outside, first at {np.argwhere(bad)[0].tolist()}"
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("M,N,K", [(5, 40, 544), (17, 64, 128), (48, 96, 4096), (300, 130, 1184), (1030, 100, 1056)])
+def test_product_of_elements_of_all_sizes(cuda, M, N, K, kind):
+    """Every finite element as likely as any other, blocks' scales up to 2^16 apart."""
+    r = np.random.default_rng(M + K)
+    c = r.integers(0, 127, (M, K)) | r.integers(0, 2, (M, K)) << 7 if kind == "e4m3" else r.integers(0, 16, (M, K))
+    a = c.astype(np.uint8) if kind == "e4m3" else (c[:, 0::2] | c[:, 1::2] << 4).astype(np.uint8)
+    a = torch.from_numpy(a).cuda()
+    a = a.view(torch.float8_e4m3fn) if kind == "e4m3" else a
+    sa, sw = (torch.from_numpy(r.integers(119, 136, (n, K // 32)).astype(np.uint8)).cuda() for n in (M, N))
+    w = torch.from_numpy(r.integers(0, 256, (N, K // 2)).astype(np.uint8)).cuda()
+    _check_far_terms(a, sa, w, sw, kind)
+
+
+@pytest.mark.parametrize("M", [1, 20, 200])
+@pytest.mark.parametrize("near", [True, False])
+def test_product_of_small_terms_beside_large_ones(cuda, near, M):
+    """Terms just below what is kept beside a largest one: seven of the same eight, or of other eights, where
+    f32 sums keep them.  A second large term of a later eight takes the first away again."""
+    a = np.zeros((M, 128))
+    a[:, 0] = a[:, 127] = 256.0
+    at = np.arange(1, 8) if near else np.arange(8, 120)
+    # by w = 4 a large term is 2^10; by 1 these are from 2^-3, the least that is kept beside it, down
+    a[:, at] = 1.875 * 2.0 ** -(4 + np.arange(M)[:, None] % 5)
+    w = np.zeros((32, 128))
+    w[:, 0], w[:, 127], w[:, at] = 4.0, -4.0, 1.0
+    ca, cw = R.nearest(a, "e4m3").astype(np.uint8), R.nearest(w, "e2m1").astype(np.uint8)
+    one = lambda n: torch.full((n, 4), 127, dtype=torch.uint8, device="cuda")
+    qa = torch.from_numpy(ca).cuda().view(torch.float8_e4m3fn)
+    qw = torch.from_numpy(cw[:, 0::2] | cw[:, 1::2] << 4).cuda()
+    _check_far_terms(qa, one(M), qw, one(32), "e4m3")
+    if not near:
+        # 2^10 and at most 112 terms in f32: the roundings' steps are 2^-14
+        got, exact = _np64(_product(qa, one(M), qw, one(32))), R.values(qa, one(M), "e4m3") @ w.T
+        assert (np.abs(got - exact) <= BF16_HALF_STEP * np.abs(exact) + 16 * 2.0 ** -14).all()
