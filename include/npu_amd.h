@@ -353,7 +353,8 @@ int64_t npu_sample_workspace(int64_t B, int64_t V);
  *   top_tokens i32 and top_logprobs f32 [T, k], k <= 32, rows at any stride,
  *   both or neither; workspace f32 [n], n >= npu_token_logprobs_workspace:
  *   scratch that only this call uses while it runs.
- * Sums in f32, in a fixed order: the same input gives the same bits. */
+ * Sums in f32, in an order that the shape and the rows' alignment fix: the same call gives the same
+ * bits.  No log probability is above 0 and no entropy below; a token that has all of p has 0 for both. */
 npu_status fused_token_logprobs(const npu_memref *logits, const npu_memref *tokens,
                                 const npu_memref *logprobs, const npu_memref *entropy,
                                 const npu_memref *ranks, const npu_memref *top_tokens,

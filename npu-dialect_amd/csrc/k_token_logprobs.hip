@@ -233,6 +233,11 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   // sums, the rank, the list
   const bool far = !(fabsf(m) < 1e6f);  // summed from x - m below
   const float c = far ? 0.0f : m * LOG2E, rest = far ? 0.0f : fmaf(m, LOG2E, -c);
+  float rest_off;  // 2^-rest, as 1 / what the exponential makes of rest (a step after the instruction's 1 ulp)
+  {
+    const float w = __builtin_amdgcn_exp2f(rest), near = __builtin_amdgcn_rcpf(w);
+    rest_off = fmaf(near, fmaf(-w, near, 1.0f), near);
+  }
   const float at_before = xt > -inf ? below(xt) : -inf;
   float S = 0.0f, W = 0.0f;
   int before = 0;
@@ -365,12 +370,14 @@ __global__ __launch_bounds__(LT) void token_logprobs_kernel(TokenLogprobsArgs a,
   Part out{m, 0.0f, 0.0f, 0};
 #pragma unroll
   for (int w = 0; w < NW; ++w) out.S += wave_a[w], out.W += wave_b[w], out.before += wave_c[w];
-  // S and W of exact exponents: each is off by `rest`
+  // S and W of exact exponents: each is off by `rest`.  The largest entry is 1 of S and 0 of W: divided by
+  // what the exponential makes of `rest`, so that it comes out as 1 (or the number below it), and S is 1 at
+  // least and W 0 at most, no log probability is above 0 and no entropy below.
   if (out.S > 0.0f) {
-    out.W = out.W - rest * out.S;
-    const float f = __builtin_amdgcn_exp2f(-rest);
-    out.S *= f;
-    out.W *= f;
+#pragma clang fp contract(off)
+    const float shift = rest * out.S;
+    out.W = fminf((out.W - shift) * rest_off, 0.0f);
+    out.S = fmaxf(out.S * rest_off, 1.0f);
   }
   if (parts == 1) {
     finish(a, row, tok, out, best, tid);

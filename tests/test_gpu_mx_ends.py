@@ -205,3 +205,29 @@ def test_product_of_small_terms_beside_large_ones(cuda, near, M):
         # 2^10 and at most 112 terms in f32: the roundings' steps are 2^-14
         got, exact = _np64(_product(qa, one(M), qw, one(32))), R.values(qa, one(M), "e4m3") @ w.T
         assert (np.abs(got - exact) <= BF16_HALF_STEP * np.abs(exact) + 16 * 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [50, 4000, 50257])
+def test_logprobs_of_certain_tokens(cuda, V, dtype):
+    """One token far above all others, at any logit: its log probability is 0 and the entropy 0; beside
+    an equal one -ln 2.  No log probability is above 0, no entropy below."""
+    from npu_amd import groups
+    T = 300
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn((T, V), generator=g) - 2000
+    best = torch.randint(0, V, (T,), generator=g)
+    m = torch.randn(T, generator=g) * 40
+    x[torch.arange(T), best] = m
+    x = x.to(dtype).cuda()
+    new = lambda *s, dt=F32: torch.full(s, 55, dtype=dt, device="cuda")
+    lp, en, tt, tl = new(T), new(T), new(T, 2, dt=torch.int32), new(T, 2)
+    groups.fused_token_logprobs(x, best.int().cuda(), lp, groups.token_logprobs_workspace(x, 2), entropy=en, top_tokens=tt,
+                                top_logprobs=tl)
+    # (the others' share is below e^-1700: 0 in f32)
+    assert (lp == 0).all() and (en == 0).all() and (tl[:, 0] == 0).all() and torch.equal(tt[:, 0].cpu(), best.int())
+    near = (torch.randn((T, V), generator=g) * 0.01 - 17).to(dtype).cuda()
+    near[torch.arange(T), best] = torch.rand(T, generator=g).to(dtype).cuda()
+    groups.fused_token_logprobs(near, best.int().cuda(), lp, groups.token_logprobs_workspace(near, 2), entropy=en, top_tokens=tt,
+                                top_logprobs=tl)
+    assert (lp <= 0).all() and (en >= 0).all() and (tl <= 0).all()
