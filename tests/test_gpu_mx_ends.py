@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import mx_refs as R
-from test_gpu_mx import BF16, BF16_HALF_STEP, F32, SILU_EPS, _check_logprobs, _check_norm, _mx, _np64, _product, _rnd
+from test_gpu_mx import (BF16, BF16_HALF_STEP, F32, SILU_EPS, _blocks, _check_logprobs, _check_norm, _exact, _mx, _np64, _product,
+                         _rnd)
 
 pytestmark = pytest.mark.gpu
 
@@ -231,3 +232,68 @@ def test_logprobs_of_certain_tokens(cuda, V, dtype):
     groups.fused_token_logprobs(near, best.int().cuda(), lp, groups.token_logprobs_workspace(near, 2), entropy=en, top_tokens=tt,
                                 top_logprobs=tl)
     assert (lp <= 0).all() and (en >= 0).all() and (tl <= 0).all()
+
+
+# ---- the largest sizes ---------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("M,N", [(3, 40), (40, 64)])
+def test_product_of_the_longest_rows(cuda, M, N, kind):
+    """K = 2^20: sums of few bits come out exact (below 2^24 of the least unit, 2^-4)."""
+    K = 1 << 20
+    (a, sa), (w, sw) = _blocks(M, K, kind, M, small=True), _blocks(N, K, "e2m1", N, small=True)
+    exact, mag = _exact(a, sa, w, sw, kind)
+    got = _product(a, sa, w, sw).cpu()
+    # (where the terms' magnitudes together stay below 2^20 every sum on the way is exact; past it each of 2^17 sums
+    # rounds by half a step of at most 2^22)
+    exact_sums = mag < 2.0 ** 20
+    assert torch.equal(got[exact_sums], exact[exact_sums].float().to(BF16))
+    off = (2.0 ** 17 + 64) * 2.0 ** -24 * mag.clamp(max=2.0 ** 22)
+    assert ((got.double() - exact).abs() <= BF16_HALF_STEP * exact.abs() + (1 + BF16_HALF_STEP) * off).all()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("M,N,K", [(40, 33, 544), (130, 70, 1184), (256, 300, 512)])
+def test_product_of_rows_far_apart(cuda, M, N, K, kind):
+    """Rows nearly 2^23 bytes apart, the most there is: the same bits as side by side."""
+    from npu_amd import groups
+    (a, sa), (w, sw) = _blocks(M, K, kind, 1), _blocks(N, K, "e2m1", 2)
+    want = _product(a, sa, w, sw).clone()
+    step = (1 << 23) - 16
+    wide = torch.zeros((max(M, N), step), dtype=torch.uint8, device="cuda")
+
+    def far(t, at):
+        v = wide[:t.shape[0], at:at + t.shape[1]]
+        v.copy_(t.view(torch.uint8))
+        return v.view(t.dtype)
+
+    got = _product(far(a, 0), far(sa, 1 << 20), far(w, 2 << 20), far(sw, (3 << 20) + 1))
+    assert torch.equal(got, want)
+    with pytest.raises(groups.NpuError, match="at most 2"):
+        far_rows = torch.empty((2, 1 << 23), dtype=torch.uint8, device="cuda")[:, :K // 2]
+        one = torch.zeros((2, K // 32), dtype=torch.uint8, device="cuda")
+        groups.fused_mx_matmul(far_rows, one, w, sw, torch.empty((2, N), dtype=BF16, device="cuda"), torch.empty(1 << 20, device="cuda"))
+
+
+def test_the_most_rows(cuda):
+    """2^23 rows of logits, and of w: the last are those of a call of their own."""
+    from npu_amd import groups
+    T, V = 1 << 23, 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((T, V), generator=g, device="cuda")
+    tok = torch.randint(-1, V, (T,), generator=g, device="cuda").int()
+    lp, rk = torch.full((T,), 5.0, device="cuda"), torch.full((T,), 5, dtype=torch.int32, device="cuda")
+    tt, tl = torch.full((T, 2), 5, dtype=torch.int32, device="cuda"), torch.full((T, 2), 5.0, device="cuda")
+    groups.fused_token_logprobs(x, tok, lp, groups.token_logprobs_workspace(x, 2), ranks=rk, top_tokens=tt, top_logprobs=tl)
+    want = x.double().log_softmax(1)
+    at = tok.long().clamp(min=0)[:, None]
+    # (f32: three terms, their exponentials and logarithm, below 2^-20)
+    assert torch.where(tok < 0, lp.double(), lp.double() - want.gather(1, at)[:, 0]).abs().max() < 2.0 ** -20 * 16
+    best, order = x.sort(dim=1, descending=True, stable=True)
+    assert torch.equal(tt.long(), order[:, :2]) and (tl.double() - want.gather(1, order[:, :2])).abs().max() < 2.0 ** -20 * 16
+    assert torch.equal(rk.long(), torch.where(tok < 0, -1, (x > x.gather(1, at)).sum(1)))
+    del x, want, best, order, tt, tl
+    N, K = 1 << 23, 64
+    (a, sa), (few, s_few) = _blocks(5, K, "e4m3", 1), _blocks(1000, K, "e2m1", 2)
+    w, sw = few.repeat(N // 1000 + 1, 1)[:N].contiguous(), s_few.repeat(N // 1000 + 1, 1)[:N].contiguous()
+    out, some = _product(a, sa, w, sw), _product(a, sa, few, s_few)
+    assert torch.equal(out, some.repeat(1, N // 1000 + 1)[:, :N])
