@@ -11,10 +11,11 @@
 // no other instruction takes e4m3 by e2m1 with the blocks' scales.
 //
 // Few rows are bound by w's bytes and by what a CU's L1 passes on: 48 rows of e4m3 by 14336 x 4096
-// 10.7 us (1 row 7.2, 4.3 TB/s of w), one by 4096 x 4096 4.1, half of it launch.  Many rows are
-// bound by the matrix units and the clock that their power leaves: 8192^3 e2m1 267 us, 4.1 PFLOP/s,
-// without any loads of its operands 228; 4099 rows of e4m3 by 4096 x 14336 177 us, 2.7 PFLOP/s (half of
-// what the same instructions reach on operands that do not change).
+// 10.7 us (1 row 6.9, 4.4 TB/s of w), one by 4096 x 4096 4.1, half of it launch.  These are of w in the last-level
+// cache; where weights change by more than that holds, 14.9, 8.4 and 5.7.  Many rows: 8192^3 e2m1 267 us,
+// 4.1 PFLOP/s, the matrix units busy in 51 % of the clocks, at 1.95 GHz, without any loads of its operands 228;
+// 4099 rows of e4m3 by 4096 x 14336 177 us, 2.7 PFLOP/s, busy in 64 % at 2.1 GHz.  How much of the rest is waits for
+// operands, and how much of the clock power, was not told apart.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -610,9 +611,11 @@ hipError_t matmul_tiles(const MxMatmulArgs &a, int want_parts, hipStream_t s) {
 // ---- which kernel ------------------------------------------------------------------------
 // A call is a few-rows kernel in groups of up to 48 rows by 16 or 32 columns, or tiles of 32 x 64, 64 x 128,
 // 128 x 128 or 256 x 256, with K in one part or in up to eight, by the least of the times that these
-// estimate, in us, from measurements of 480 shapes (M 1 .. 4096, N 512 .. 14336, K 512 .. 14336, both types).
-// The choice takes 4 % more than each shape's fastest of these on average, and these 1.3 % more than
-// the fastest of 22 tried.  In us, e4m3, parts after the slash:
+// estimate, in us, from measurements of 480 shapes (M 1 .. 4096, N 512 .. 14336, K 512 .. 14336, both types;
+// profiles/product_kernels_by_shape.txt).  The choice takes 4 % more than each shape's fastest of these on
+// average, and these 1.3 % more than the fastest of 22 tried.  Past that range it extrapolates: 1, 48 and 128 rows of
+// e4m3 by 128000 x 4096 54, 64 and 98 us with other weights each time, w's bytes 53 of them.
+// In us, e4m3, parts after the slash:
 //   rows      by                  16 cols  32 cols  32 x 64  64 x 128  128 x 128  256 x 256
 //      1   4096 x 14336 (N x K)    9.9/1    10.1/4   10.6/4    12.6/8    14.9/8
 //     48  14336 x 4096            21.2/1    14.5/1   10.8/1    13.3/2    15.1/2
